@@ -20,6 +20,8 @@ LIB_PATH = os.path.join(_HERE, "libctorch_amd.so")
 
 F32, F64, I64, BOOL, F16, BF16 = 0, 1, 2, 3, 4, 5
 CPU, GPU = 0, 1
+ROTARY_INTERLEAVED, ROTARY_HALF = 0, 1
+ROTARY_UNSCALED, ROTARY_LINEAR, ROTARY_BASE, ROTARY_PARTS = 0, 1, 2, 3
 _NP = {F32: np.float32, F64: np.float64, I64: np.int64, BOOL: np.bool_, F16: np.uint16, BF16: np.uint16}
 
 
@@ -46,6 +48,12 @@ class TensorInfo(C.Structure):
 
 class RandomKey(C.Structure):
     _fields_ = [("seed", C.c_uint64), ("stream", C.c_uint64)]
+
+
+class RotaryScaling(C.Structure):
+    """dl_rotary_scaling: how rotary_tables slows its angles for positions beyond the trained ones."""
+    _fields_ = [("kind", C.c_int), ("factor", C.c_double), ("trained", C.c_int64), ("slow_turns", C.c_double),
+                ("fast_turns", C.c_double), ("magnitude", C.c_double)]
 
 
 class MemoryStats(C.Structure):
@@ -150,7 +158,17 @@ SIGNATURES = {
     "dl_transformer_decoder_cache_dtype": (_st, [_p, C.POINTER(C.c_int)]),
     "dl_decoder_cache_state": (_st, [_p, _pp]),
     "dl_decoder_cache_load_state": (_st, [_p, _p, _p]),
+    "dl_rotary_tables": (_st, [_i64, _i64, _f64, C.POINTER(RotaryScaling), Device, _pp, _pp]),
+    "dl_rotary_positions": (_st, [_p, _p, _p, _p, C.c_int, _pp]),
+    "dl_paged_cache_create": (_st, [_i64, _i64, _i64, _i64, _i64, TensorOptions, _pp]),
+    "dl_paged_cache_release": (None, [_p]),
+    "dl_paged_cache_tensors": (_st, [_p, _i64, _pp, _pp]),
+    "dl_paged_batch_create": (_st, [_p, _i64, _i64, _p, _p, _p, _i64, _i64, _pp]),
+    "dl_paged_batch_release": (None, [_p]),
+    "dl_paged_cache_append": (_st, [_p, _i64, _p, _p, _p, _p, _p, _p, C.c_int, _pp]),
+    "dl_paged_attention": (_st, [_p, _i64, _p, _p, _pp]),
     # generate_c_api.h
+    "dl_verify_drafted": (_st, [_p, _p, _p, _f64, _p, _pp, _pp]),
     "dl_decoder_lm_create": (_st, [_p, _p, _p, _pp]),
     "dl_decoder_lm_release": (None, [_p]),
     "dl_decoder_lm_logits": (_st, [_p, _p, _p, _pp]),
@@ -441,6 +459,58 @@ def decode(decoder: Module, x: Tensor, cache: DecoderCache) -> Tensor:
     return Tensor(_new(lib().dl_transformer_decoder_decode, decoder.handle, x.handle, cache.handle))
 
 
+class PagedCache:
+    """dl_paged_cache: pools of pages [pages, kv_heads, page_size, head_dim] for requests of different lengths."""
+
+    def __init__(self, layers: int, pages: int, page_size: int, kv_heads: int, head_dim: int, dtype: int = F32,
+                 dev: Device | None = None):
+        self.handle = None
+        self.handle = _new(lib().dl_paged_cache_create, layers, pages, page_size, kv_heads, head_dim, options(dtype, dev))
+
+    def __del__(self):
+        if getattr(self, "handle", None) and _lib is not None:
+            _lib.dl_paged_cache_release(self.handle)
+            self.handle = None
+
+    def key(self, layer: int) -> Tensor:
+        """The layer's live keys."""
+        out = C.c_void_p()
+        check(lib().dl_paged_cache_tensors(self.handle, layer, C.byref(out), None))
+        return Tensor(out)
+
+    def value(self, layer: int) -> Tensor:
+        out = C.c_void_p()
+        check(lib().dl_paged_cache_tensors(self.handle, layer, None, C.byref(out)))
+        return Tensor(out)
+
+    def append(self, layer: int, batch: "PagedBatch", query: Tensor | None, key: Tensor, value: Tensor, cosine: Tensor,
+               sine: Tensor, layout: int = ROTARY_INTERLEAVED) -> Tensor | None:
+        """dl_paged_cache_append: rotated keys and values into their pages; the rotated queries come back."""
+        out = C.c_void_p()
+        check(lib().dl_paged_cache_append(self.handle, layer, batch.handle, query.handle if query is not None else None,
+                                          key.handle, value.handle, cosine.handle, sine.handle, layout,
+                                          C.byref(out) if query is not None else None))
+        return Tensor(out) if query is not None else None
+
+
+class PagedBatch:
+    """dl_paged_batch: what one step computes.  tables: page ids [sequences, width]."""
+
+    def __init__(self, cache: PagedCache, heads: int, lengths, counts, tables, shared: int = 0):
+        self.handle = None
+        arrays = [np.ascontiguousarray(a, np.int64) for a in (lengths, counts, tables)]
+        if arrays[0].ndim != 1 or arrays[1].shape != arrays[0].shape or arrays[2].ndim != 2 or \
+                len(arrays[2]) != len(arrays[0]):
+            raise ValueError("a paged batch needs lengths [B], counts [B] and tables [B, width]")
+        self.handle = _new(lib().dl_paged_batch_create, cache.handle, heads, len(arrays[0]),
+                           *[a.ctypes.data_as(C.c_void_p) for a in arrays], arrays[2].shape[1], shared)
+
+    def __del__(self):
+        if getattr(self, "handle", None) and _lib is not None:
+            _lib.dl_paged_batch_release(self.handle)
+            self.handle = None
+
+
 class DecoderLM:
     """Embedding -> TransformerDecoder -> head with the whole token step on the GPU."""
 
@@ -511,6 +581,15 @@ def normal(key, shape, scale: float, dtype: int = BF16, dev: Device | None = Non
     return Tensor(_new(lib().dl_normal_with_key, RandomKey(*key), _shape(shape), scale, options(dtype, dev)))
 
 
+def zeros(shape, dtype: int = F32, dev: Device | None = None) -> Tensor:
+    return Tensor(_new(lib().dl_zeros, _shape(shape), options(dtype, dev)))
+
+
+def narrow(x: Tensor, axis: int, start: int, length: int) -> Tensor:
+    """A view of `length` entries of `axis` from `start` on."""
+    return Tensor(_new(lib().dl_narrow, x.handle, axis, start, length))
+
+
 def fold_in(key, label: int) -> tuple[int, int]:
     k = lib().dl_random_fold_in(RandomKey(*key), label)
     return k.seed, k.stream
@@ -549,6 +628,33 @@ def argmax(x: Tensor, axis: int, keepdim: bool = False) -> Tensor:
 
 def sample(logits: Tensor, temperature: float, key) -> Tensor:
     return Tensor(_new(lib().dl_sample, logits.handle, temperature, RandomKey(*key)))
+
+
+def verify_drafted(drafted: Tensor, target: Tensor, draft: Tensor | None, temperature: float,
+                   uniforms: Tensor) -> tuple[Tensor, Tensor]:
+    """dl_verify_drafted: (tokens [B, K + 1], accepted [B])."""
+    tokens, accepted = C.c_void_p(), C.c_void_p()
+    check(lib().dl_verify_drafted(drafted.handle, target.handle, draft.handle if draft is not None else None, temperature,
+                                  uniforms.handle, C.byref(tokens), C.byref(accepted)))
+    return Tensor(tokens), Tensor(accepted)
+
+
+def rotary_tables(dimensions: int, capacity: int, base: float = 10000.0, scaling: RotaryScaling | None = None,
+                  dev: Device | None = None) -> tuple[Tensor, Tensor]:
+    """dl_rotary_tables: (cosine, sine), each [capacity, dimensions / 2] f32."""
+    cosine, sine = C.c_void_p(), C.c_void_p()
+    check(lib().dl_rotary_tables(dimensions, capacity, base, C.byref(scaling) if scaling is not None else None,
+                                 dev if dev is not None else device("gpu"), C.byref(cosine), C.byref(sine)))
+    return Tensor(cosine), Tensor(sine)
+
+
+def rotary_positions(x: Tensor, positions: Tensor, cosine: Tensor, sine: Tensor,
+                     layout: int = ROTARY_INTERLEAVED) -> Tensor:
+    return Tensor(_new(lib().dl_rotary_positions, x.handle, positions.handle, cosine.handle, sine.handle, layout))
+
+
+def paged_attention(cache: PagedCache, layer: int, batch: PagedBatch, query: Tensor) -> Tensor:
+    return Tensor(_new(lib().dl_paged_attention, cache.handle, layer, batch.handle, query.handle))
 
 
 def rotary_embedding(x: Tensor, cosine: Tensor, sine: Tensor) -> Tensor:

@@ -5,6 +5,7 @@
 
 #include "dl/generate_c_api.h"
 #include "dl/decoder.h"
+#include "dl/paged.h"
 #include "nn/language_model.h"
 
 #include <exception>
@@ -15,6 +16,8 @@ struct dl_tensor { dl::Tensor value; };
 struct dl_module { std::shared_ptr<dl::nn::UnaryModule> value; };
 struct dl_state { dl::StateDict value; };
 struct dl_decoder_cache { std::vector<dl::nn::KVCache> value; };
+struct dl_paged_cache { dl::nn::PagedKVCache value; };
+struct dl_paged_batch { dl::nn::PagedBatch value; };
 struct dl_decoder_lm {
     std::shared_ptr<dl::nn::UnaryModule> embedding, decoder, head;
     std::unique_ptr<dl::detail::DecoderLM> value;

@@ -336,4 +336,95 @@ dl_status dl_transformer_decoder_decode(dl_module* decoder, const dl_tensor* inp
     });
 }
 
+dl_status dl_rotary_tables(int64_t dimensions, int64_t capacity, double base, const dl_rotary_scaling* scaling,
+                           dl_device device, dl_tensor** cosine, dl_tensor** sine) {
+    if (cosine) *cosine = nullptr;
+    if (sine) *sine = nullptr;
+    return invoke([&] {
+        require(cosine, "cosine slot");
+        require(sine, "sine slot");
+        dl::RotaryScaling rule;
+        if (scaling)
+            rule = {static_cast<dl::RotaryScaling::Kind>(scaling->kind), scaling->factor, scaling->trained,
+                    scaling->slow_turns, scaling->fast_turns, scaling->magnitude};
+        auto [c, s] = dl::rotary_tables(dimensions, capacity, base, rule, convert(device));
+        auto first = std::make_unique<dl_tensor>(dl_tensor{c}), second = std::make_unique<dl_tensor>(dl_tensor{s});
+        *cosine = first.release();
+        *sine = second.release();
+    });
+}
+
+dl_status dl_rotary_positions(const dl_tensor* input, const dl_tensor* positions, const dl_tensor* cosine,
+                              const dl_tensor* sine, dl_rotary_layout layout, dl_tensor** output) {
+    return make_handle(output, [&] {
+        return dl::rotary_positions(require(input, "input").value, require(positions, "positions").value,
+                                    require(cosine, "cosine").value, require(sine, "sine").value,
+                                    static_cast<dl::RotaryLayout>(layout));
+    });
+}
+
+dl_status dl_paged_cache_create(int64_t layers, int64_t pages, int64_t page_size, int64_t kv_heads, int64_t head_dim,
+                                dl_tensor_options options, dl_paged_cache** output) {
+    return make_handle(output, [&] {
+        return dl::nn::PagedKVCache(layers, pages, page_size, kv_heads, head_dim, convert(options));
+    });
+}
+
+void dl_paged_cache_release(dl_paged_cache* cache) { delete cache; }
+
+dl_status dl_paged_cache_tensors(const dl_paged_cache* cache, int64_t layer, dl_tensor** key, dl_tensor** value) {
+    if (key) *key = nullptr;
+    if (value) *value = nullptr;
+    return invoke([&] {
+        const auto& pages = require(cache, "cache").value;
+        if (layer < 0 || layer >= pages.layers()) throw std::out_of_range("paged cache: layer out of range");
+        auto k = key ? std::make_unique<dl_tensor>(dl_tensor{pages.key(layer).detach()}) : nullptr;
+        auto v = value ? std::make_unique<dl_tensor>(dl_tensor{pages.value(layer).detach()}) : nullptr;
+        if (key) *key = k.release();
+        if (value) *value = v.release();
+    });
+}
+
+dl_status dl_paged_batch_create(const dl_paged_cache* cache, int64_t heads, int64_t sequences, const int64_t* lengths,
+                                const int64_t* counts, const int64_t* tables, int64_t width, int64_t shared,
+                                dl_paged_batch** output) {
+    return make_handle(output, [&] {
+        const auto& pages = require(cache, "cache").value;
+        require(lengths, "lengths");
+        require(counts, "counts");
+        require(tables, "tables");
+        if (sequences <= 0 || width <= 0 || width > INT32_MAX / sequences)
+            throw std::invalid_argument("paged batch: tables must be [sequences, width]");
+        const auto n = static_cast<std::size_t>(sequences);
+        return dl::nn::PagedBatch(pages, heads, {lengths, n}, {counts, n}, {tables, n * static_cast<std::size_t>(width)},
+                                  width, shared);
+    });
+}
+
+void dl_paged_batch_release(dl_paged_batch* batch) { delete batch; }
+
+dl_status dl_paged_cache_append(dl_paged_cache* cache, int64_t layer, const dl_paged_batch* batch, const dl_tensor* query,
+                                const dl_tensor* key, const dl_tensor* value, const dl_tensor* cosine,
+                                const dl_tensor* sine, dl_rotary_layout layout, dl_tensor** rotated) {
+    if (rotated) *rotated = nullptr;
+    return invoke([&] {
+        if ((query == nullptr) != (rotated == nullptr))
+            throw std::invalid_argument("paged_append: query and the slot for the rotated queries go together");
+        dl::Tensor out = dl::paged_append(require(cache, "cache").value, layer, require(batch, "batch").value,
+                                          query ? std::optional<dl::Tensor>{query->value} : std::nullopt,
+                                          require(key, "key").value, require(value, "value").value,
+                                          require(cosine, "cosine").value, require(sine, "sine").value,
+                                          static_cast<dl::RotaryLayout>(layout));
+        if (rotated) *rotated = new dl_tensor{out};
+    });
+}
+
+dl_status dl_paged_attention(const dl_paged_cache* cache, int64_t layer, const dl_paged_batch* batch,
+                             const dl_tensor* query, dl_tensor** output) {
+    return make_handle(output, [&] {
+        return dl::paged_attention(require(cache, "cache").value, layer, require(batch, "batch").value,
+                                   require(query, "query").value);
+    });
+}
+
 } // extern "C"

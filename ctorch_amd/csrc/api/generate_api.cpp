@@ -96,6 +96,22 @@ dl_status dl_sample(const dl_tensor* logits, double temperature, dl_random_key k
     return make_handle(output, [&] { return dl::sample(require(logits, "logits").value, temperature, convert(key)); });
 }
 
+dl_status dl_verify_drafted(const dl_tensor* drafted, const dl_tensor* target, const dl_tensor* draft, double temperature,
+                            const dl_tensor* uniforms, dl_tensor** tokens, dl_tensor** accepted) {
+    if (tokens) *tokens = nullptr;
+    if (accepted) *accepted = nullptr;
+    return invoke([&] {
+        require(tokens, "tokens slot");
+        require(accepted, "accepted slot");
+        auto [t, a] = dl::verify_drafted(require(drafted, "drafted").value, require(target, "target").value,
+                                         draft ? std::optional<dl::Tensor>{draft->value} : std::nullopt, temperature,
+                                         require(uniforms, "uniforms").value);
+        auto first = std::make_unique<dl_tensor>(dl_tensor{t}), second = std::make_unique<dl_tensor>(dl_tensor{a});
+        *tokens = first.release();
+        *accepted = second.release();
+    });
+}
+
 dl_status dl_normal_with_key(dl_random_key key, dl_shape shape, double scale, dl_tensor_options options,
                              dl_tensor** output) {
     return make_handle(output, [&] { return dl::normal(convert(key), convert(shape), scale, convert(options)); });

@@ -246,6 +246,81 @@ int dlk_rms_norm(const float* x, int64_t rows, int64_t width, const void* weight
 /* Interleaved RoPE on contiguous x [outer, L, D] f32 with tables [L, D/2]. */
 int dlk_rope(const float* x, int64_t outer, int64_t length, int64_t dim, const float* cosine, const float* sine,
              float* y, dlh_stream stream);
+/* ------------------------------------------------------------------------------------------------------
+ * Rows at given positions (rotary.hip): the queries, keys and values of `tokens` rows, queries and keys rotated by
+ * the table row of the token's position, keys and values written to the pages of a paged cache.
+ * ---------------------------------------------------------------------------------------------------- */
+typedef struct dlk_row_segment {
+    const void* x;           /* [tokens, heads, dim], last axis contiguous; NULL: the segment is absent */
+    int bf16;                /* bf16 rows, else f32 */
+    int heads;
+    int64_t row, head;       /* element strides of a token and of a head */
+} dlk_row_segment;
+
+typedef struct dlk_rotary_params {
+    dlk_row_segment q, k, v;
+    int64_t tokens;
+    int dim, part;           /* the first `part` (even) of each head's `dim` entries are rotated, the others copied */
+    int half;                /* pairs (i, i + part / 2) instead of (2 i, 2 i + 1) */
+    const int64_t* positions; /* [tokens] */
+    const float* cosine;     /* [capacity, part / 2] */
+    const float* sine;
+    int64_t capacity;        /* a query row whose position lies outside [0, capacity) comes out NaN */
+    float* out;              /* [tokens, q.heads, dim] */
+    void* k_pages;           /* [pages, k.heads, page_size, dim] */
+    void* v_pages;
+    int pages_bf16;
+    int page_shift;          /* log2 of the page size */
+    const int64_t* places;   /* [tokens]: page * page_size + row of the token's place */
+} dlk_rotary_params;
+int dlk_rotary(const dlk_rotary_params* p, dlh_stream stream);
+
+/* ------------------------------------------------------------------------------------------------------
+ * Attention over the pages of a paged cache (attention_paged.hip).  The work of a call is a list of items, made once
+ * for a step's batch: rows of one run of tokens over a range of its keys.  Row r of a run is token r / G and query
+ * head r % G of the KV head's group (G = H / KV).
+ * ---------------------------------------------------------------------------------------------------- */
+typedef struct dlk_paged_item {
+    int32_t token;           /* the run's first token */
+    int32_t row_begin, row_end;
+    int32_t table;           /* where the run's page ids start in `tables` (the page of key 0) */
+    int32_t key_begin, key_end;
+    int32_t first;           /* row r sees the keys up to first + r / G */
+    int32_t slot;            /* partials slot, or -1: the item is all that its rows see, and writes the output */
+} dlk_paged_item;
+
+/* One token whose rows several items share. */
+typedef struct dlk_paged_merge {
+    int32_t token, row;      /* the token, and its first row within its run */
+    int32_t slot, stride;    /* the slot of the run's first row tile, and the slots of each row tile */
+    int32_t count;           /* the first of them that hold keys the row sees */
+    int32_t shared_row;      /* the token's first row within the prefix run */
+} dlk_paged_merge;
+
+typedef struct dlk_paged_params {
+    const void* q;
+    int q_bf16;
+    int64_t q_row, q_head;   /* element strides of a token and of a head; 16-byte aligned rows */
+    const void* k;           /* [pages, KV, page_size, hd] */
+    const void* v;
+    int kv_bf16, page_shift, H, KV, hd;
+    float scale;
+    const int32_t* tables;
+    float* out;              /* [tokens, H, hd] */
+    const dlk_paged_item* items;
+    int item_count, row_tiles; /* 16-row tiles of an item: 1, 2 or 4 */
+    float* partial_o;        /* [slots, KV, 16 * row_tiles, hd] */
+    float* partial_ml;       /* [slots, KV, 16 * row_tiles, 2]: maximum (base 2) and sum */
+    /* the items of a prefix that the whole batch shares: rows of all tokens */
+    const dlk_paged_item* shared_items;
+    int shared_count, shared_row_tiles, shared_splits;
+    float* shared_o;
+    float* shared_ml;
+    const dlk_paged_merge* merges;
+    int merge_count;
+} dlk_paged_params;
+int dlk_paged_attention(const dlk_paged_params* p, dlh_stream stream);
+
 /* First maximum of each row (NaN first); x [rows, n] f32 contiguous -> out i64 [rows]. */
 int dlk_argmax(const float* x, int64_t rows, int64_t n, int64_t* out, dlh_stream stream);
 /* Per-block candidates of a [rows, n] logits matrix (greedy or Gumbel-max), for dlk_sample_finalize. */
@@ -259,6 +334,29 @@ int dlk_sample_blocks(int64_t n);
 int dlk_sample_finalize(const dlk_sample_partial* partial, int64_t rows, int blocks, int64_t* out,
                         int64_t* next_ids, int64_t* tokens, int64_t token_stride, int64_t* step,
                         const void* embedding, int embedding_dtype, int64_t width, float* x, dlh_stream stream);
+/* ------------------------------------------------------------------------------------------------------
+ * Verification of drafted tokens (verify.hip): target [batch, drafts + 1, vocabulary], draft [batch, drafts, vocabulary]
+ * or NULL, uniforms [batch, drafts + 1], all f32 contiguous; drafted [batch, drafts], a negative id ends a row.
+ * inverse = 1 / temperature, or 0: the largest logit decides.
+ * ---------------------------------------------------------------------------------------------------- */
+typedef struct dlk_verify_row { /* one row of logits: its largest, the sum of exp((l - largest) / T), the largest's index */
+    double sum;
+    float largest;
+    int32_t index;
+} dlk_verify_row;
+
+typedef struct dlk_verify_params {
+    const int64_t* drafted;
+    const float* target;
+    const float* draft;
+    const float* uniforms;
+    int64_t batch, drafts, vocabulary;
+    double inverse;
+    dlk_verify_row* rows;    /* [batch, 2 drafts + 1]: the target's, then the draft's */
+    int64_t* tokens;         /* [batch, drafts + 1]: accepted drafts, the drawn token, -1 */
+    int64_t* accepted;       /* [batch] */
+} dlk_verify_params;
+int dlk_verify(const dlk_verify_params* p, dlh_stream stream);
 /* Keyed Philox: mode 0 uniform [low, high), mode 1 standard normal times scale; output f32 or bf16. */
 int dlk_random(uint64_t seed, uint64_t stream_bits, int64_t count, int mode, double low, double high,
                double scale, void* out, int out_dtype, dlh_stream stream);

@@ -80,6 +80,40 @@ void linear_into(const float* x, Index rows, Index k, const Tensor& weight, cons
     hip_check(dlk_gemv(&p, context.stream), "linear");
 }
 
+RotaryTables::RotaryTables(const Tensor& cosine, const Tensor& sine, Index dim, Device device, const char* operation) {
+    const std::string name(operation);
+    if (cosine.ndim() != 2 || cosine.shape() != sine.shape())
+        throw std::invalid_argument(name + ": cosine and sine must be [capacity, R/2] alike");
+    if (cosine.size(0) <= 0 || cosine.size(1) <= 0 || 2 * cosine.size(1) > dim)
+        throw std::invalid_argument(name + ": the tables rotate " + std::to_string(2 * cosine.size(1)) + " of " +
+                                    std::to_string(dim) + " entries");
+    cosine_ = contiguous_f32(cosine.to(device));
+    sine_ = contiguous_f32(sine.to(device));
+}
+
+void RotaryTables::fill(dlk_rotary_params& p, RotaryLayout layout, const char* operation) const {
+    if (layout != RotaryLayout::interleaved && layout != RotaryLayout::half)
+        throw std::invalid_argument(std::string(operation) + ": unknown rotary layout");
+    p.half = layout == RotaryLayout::half;
+    p.part = static_cast<int>(2 * cosine_.size(1));
+    p.cosine = cosine_.data<float>();
+    p.sine = sine_.data<float>();
+    p.capacity = cosine_.size(0);
+}
+
+dlk_row_segment row_segment(const Tensor& t, Tensor& held, Index heads, const char* operation) {
+    if (t.dtype() != DType::f32 && t.dtype() != DType::bf16)
+        throw std::invalid_argument(std::string(operation) + ": rows must be f32 or bf16");
+    held = t.strides()[2] == 1 || t.size(2) <= 1 ? t : t.contiguous();
+    dlk_row_segment s{};
+    s.x = held.data<void>();
+    s.bf16 = held.dtype() == DType::bf16;
+    s.heads = static_cast<int>(heads);
+    s.row = held.strides()[0];
+    s.head = held.strides()[1];
+    return s;
+}
+
 void attention_split(Index batch, Index heads, Index kv_heads, Index head_dim, bool kv_bf16, Index length,
                      Index source, bool causal, int& splits, int& chunk) {
     constexpr Index tile = 64;
@@ -222,6 +256,72 @@ Tensor rotary_embedding(const Tensor& input, const Tensor& cosine, const Tensor&
     return y;
 }
 
+std::pair<Tensor, Tensor> rotary_tables(Index dimensions, Index capacity, double base, const RotaryScaling& scaling,
+                                        Device device) {
+    using Kind = RotaryScaling::Kind;
+    if (dimensions <= 0 || dimensions % 2 != 0 || capacity <= 0 || !(base > 0.0) || !std::isfinite(base))
+        throw std::invalid_argument("rotary_tables: needs an even positive dimension, positive capacity and base");
+    const Kind kind = scaling.kind;
+    if (kind != Kind::none && kind != Kind::linear && kind != Kind::base && kind != Kind::parts)
+        throw std::invalid_argument("rotary_tables: unknown scaling");
+    if (!std::isfinite(scaling.magnitude)) throw std::invalid_argument("rotary_tables: magnitude must be finite");
+    if (kind != Kind::none && !(scaling.factor > 0.0 && std::isfinite(scaling.factor)))
+        throw std::invalid_argument("rotary_tables: the scaling factor must be positive");
+    if (kind == Kind::parts && !(scaling.trained > 0 && scaling.slow_turns < scaling.fast_turns &&
+                                 std::isfinite(scaling.slow_turns) && std::isfinite(scaling.fast_turns)))
+        throw std::invalid_argument("rotary_tables: scaling by parts needs trained positions and slow_turns < fast_turns");
+    if (kind == Kind::base && dimensions < 4)
+        throw std::invalid_argument("rotary_tables: scaling the base needs at least two pairs");
+    const Index half = dimensions / 2;
+    const double width = static_cast<double>(dimensions);
+    if (kind == Kind::base) base *= std::pow(scaling.factor, width / (width - 2.0));
+    std::vector<double> frequencies(static_cast<std::size_t>(half));
+    for (Index i = 0; i < half; ++i) {
+        double f = std::pow(base, -2.0 * static_cast<double>(i) / width);
+        if (kind == Kind::linear) f /= scaling.factor;
+        if (kind == Kind::parts) {
+            const double turns = static_cast<double>(scaling.trained) * f / (2.0 * 3.14159265358979323846);
+            const double keep = std::clamp((turns - scaling.slow_turns) / (scaling.fast_turns - scaling.slow_turns), 0.0, 1.0);
+            f = f * keep + f / scaling.factor * (1.0 - keep);
+        }
+        frequencies[static_cast<std::size_t>(i)] = f;
+    }
+    Tensor c = empty_tensor({capacity, half}, DType::f32, Device::cpu());
+    Tensor s = empty_tensor({capacity, half}, DType::f32, Device::cpu());
+    float* cd = static_cast<float*>(mutable_data(c));
+    float* sd = static_cast<float*>(mutable_data(s));
+    for (Index p = 0; p < capacity; ++p)
+        for (Index i = 0; i < half; ++i) {
+            const double angle = static_cast<double>(p) * frequencies[static_cast<std::size_t>(i)];
+            cd[p * half + i] = static_cast<float>(std::cos(angle) * scaling.magnitude);
+            sd[p * half + i] = static_cast<float>(std::sin(angle) * scaling.magnitude);
+        }
+    return {c.to(device), s.to(device)};
+}
+
+Tensor rotary_positions(const Tensor& input, const Tensor& positions, const Tensor& cosine, const Tensor& sine,
+                        RotaryLayout layout) {
+    GpuContext& context = gpu_of(input, "rotary_positions");
+    if (input.ndim() != 3) throw std::invalid_argument("rotary_positions: input must be [T, H, D]");
+    const Index tokens = input.size(0), heads = input.size(1), dim = input.size(2);
+    if (positions.dtype() != DType::i64 || positions.shape() != Shape{tokens})
+        throw std::invalid_argument("rotary_positions: positions must be i64 [T]");
+    if (!(positions.device() == input.device())) throw std::invalid_argument("rotary_positions: positions on another device");
+    Tensor x, at = positions.contiguous();
+    RotaryTables tables(cosine, sine, dim, input.device(), "rotary_positions");
+    Tensor y = empty_tensor(input.shape(), DType::f32, input.device());
+    if (y.numel() == 0) return y;
+    dlk_rotary_params p{};
+    p.tokens = tokens;
+    p.dim = static_cast<int>(dim);
+    p.q = row_segment(input, x, heads, "rotary_positions");
+    tables.fill(p, layout, "rotary_positions");
+    p.positions = at.data<Index>();
+    p.out = static_cast<float*>(mutable_data(y));
+    hip_check(dlk_rotary(&p, context.stream), "rotary_positions");
+    return y;
+}
+
 Tensor grouped_query_attention(const Tensor& query, const Tensor& key, const Tensor& value,
                                std::optional<Tensor> keep_mask) {
     GpuContext& context = gpu_of(query, "grouped_query_attention");
@@ -342,6 +442,49 @@ Tensor sample(const Tensor& logits, double temperature, RandomKey key) {
                                   nullptr, nullptr, 0, 0, nullptr, context.stream),
               "sample");
     return out;
+}
+
+std::pair<Tensor, Tensor> verify_drafted(const Tensor& drafted, const Tensor& target, const std::optional<Tensor>& draft,
+                                         double temperature, const Tensor& uniforms) {
+    GpuContext& context = gpu_of(target, "verify_drafted");
+    if (drafted.dtype() != DType::i64 || drafted.ndim() != 2)
+        throw std::invalid_argument("verify_drafted: drafted must be i64 [B, K]");
+    const Index batch = drafted.size(0), drafts = drafted.size(1);
+    if (target.ndim() != 3 || target.size(0) != batch || target.size(1) != drafts + 1)
+        throw std::invalid_argument("verify_drafted: target logits must be [B, K + 1, V], got " + shape_string(target.shape()));
+    const Index vocabulary = target.size(2);
+    if (vocabulary <= 0) throw std::invalid_argument("verify_drafted: empty vocabulary");
+    if (draft && draft->shape() != Shape{batch, drafts, vocabulary})
+        throw std::invalid_argument("verify_drafted: draft logits must be [B, K, V], got " + shape_string(draft->shape()));
+    if (uniforms.dtype() != DType::f32 || uniforms.shape() != Shape{batch, drafts + 1})
+        throw std::invalid_argument("verify_drafted: uniforms must be f32 [B, K + 1]");
+    if (!std::isfinite(temperature)) throw std::invalid_argument("verify_drafted: the temperature must be finite");
+    for (const Tensor* t : {&drafted, &uniforms, draft ? &*draft : &target})
+        if (!(t->device() == target.device())) throw std::invalid_argument("verify_drafted: tensors on different devices");
+    for (const Tensor* t : {&target, draft ? &*draft : &target})
+        if (t->dtype() != DType::f32 && t->dtype() != DType::bf16)
+            throw std::invalid_argument("verify_drafted: logits must be f32 or bf16");
+    Tensor ids = drafted.contiguous(), p_logits = contiguous_f32(target), u = uniforms.contiguous();
+    // a greedy verification reads no draft logits
+    Tensor q_logits = draft && temperature > 0.0 ? contiguous_f32(*draft) : Tensor{};
+    Tensor tokens = empty_tensor({batch, drafts + 1}, DType::i64, target.device());
+    Tensor accepted = empty_tensor({batch}, DType::i64, target.device());
+    Tensor rows = empty_tensor({batch * (2 * drafts + 1), 2}, DType::i64, target.device());
+    static_assert(sizeof(dlk_verify_row) == 16);
+    dlk_verify_params p{};
+    p.drafted = ids.data<Index>();
+    p.target = p_logits.data<float>();
+    p.draft = q_logits.defined() && drafts > 0 ? q_logits.data<float>() : nullptr;
+    p.uniforms = u.data<float>();
+    p.batch = batch;
+    p.drafts = drafts;
+    p.vocabulary = vocabulary;
+    p.inverse = temperature > 0.0 ? std::min(1.0 / temperature, 1e300) : 0.0;
+    p.rows = static_cast<dlk_verify_row*>(mutable_data(rows));
+    p.tokens = static_cast<Index*>(mutable_data(tokens));
+    p.accepted = static_cast<Index*>(mutable_data(accepted));
+    hip_check(dlk_verify(&p, context.stream), "verify_drafted");
+    return {tokens, accepted};
 }
 
 } // namespace dl

@@ -20,6 +20,19 @@ dlk_gemv_params gemv_params(const float* x, Index rows, Index k, int epilogue);
 void linear_into(const float* x, Index rows, Index k, const Tensor& weight, const std::optional<Tensor>& bias,
                  float* y, Index ldy, GpuContext& context);
 
+/// The rotation tables of an operator over heads of `dim` entries, on `device`, checked and held for the call.
+class RotaryTables {
+public:
+    RotaryTables(const Tensor& cosine, const Tensor& sine, Index dim, Device device, const char* operation);
+    void fill(dlk_rotary_params& p, RotaryLayout layout, const char* operation) const;
+    Index capacity() const { return cosine_.size(0); }
+
+private:
+    Tensor cosine_, sine_;
+};
+/// Rows [T, heads, D] as a kernel reads them; `held` keeps the tensor (a copy where the last axis has gaps).
+dlk_row_segment row_segment(const Tensor& t, Tensor& held, Index heads, const char* operation);
+
 /// Number of key splits and keys per split for attention of `length` new positions over `source` keys.
 void attention_split(Index batch, Index heads, Index kv_heads, Index head_dim, bool kv_bf16, Index length,
                      Index source, bool causal, int& splits, int& chunk);

@@ -2,7 +2,7 @@
 #define CTORCH_DECODER_C_API_H
 /*
  * Decoder C17 surface: every entry of the reference's include/dl/decoder_c_api.h:13-41 (same names and
- * arguments; bodies in ctorch_amd/csrc/api/decoder.cpp), plus two additive extensions marked below.
+ * arguments; bodies in ctorch_amd/csrc/api/decoder_api.cpp), plus additive extensions marked below.
  * The cache handle belongs to one inference request, holds one K/V store per layer and is released
  * independently of the model.
  */
@@ -87,6 +87,51 @@ DL_API dl_status dl_decoder_cache_load_state(const dl_module* decoder, dl_decode
  * KVCache::append route (include/dl/decoder.h:52) for seeding a prefix.  key/value are [B, KV, n, D]. */
 DL_API dl_status dl_decoder_cache_append(dl_decoder_cache* cache, int64_t layer, const dl_tensor* key,
     const dl_tensor* value);
+
+/* ---- Extensions (no reference counterpart): rows at given positions, and a paged cache for requests of different
+ * lengths.  The rules stand at the C++ entries they call, dl/ops.h and dl/paged.h. ---- */
+typedef enum dl_rotary_layout { DL_ROTARY_INTERLEAVED = 0, DL_ROTARY_HALF = 1 } dl_rotary_layout;
+typedef enum dl_rotary_scaling_kind {
+    DL_ROTARY_UNSCALED = 0, DL_ROTARY_LINEAR = 1, DL_ROTARY_BASE = 2, DL_ROTARY_PARTS = 3
+} dl_rotary_scaling_kind;
+typedef struct dl_rotary_scaling {
+    dl_rotary_scaling_kind kind;
+    double factor;
+    int64_t trained;
+    double slow_turns, fast_turns, magnitude;
+} dl_rotary_scaling;
+/* Cosine and sine tables [capacity, dimensions / 2], f32, on `device`; scaling may be NULL (none, magnitude 1). */
+DL_API dl_status dl_rotary_tables(int64_t dimensions, int64_t capacity, double base, const dl_rotary_scaling* scaling,
+    dl_device device, dl_tensor** cosine, dl_tensor** sine);
+/* input [T, H, D] f32 or bf16, positions [T] i64, tables [capacity, R/2]: the first R entries of each head rotated by
+ * its row's position, the others copied; f32 [T, H, D]. */
+DL_API dl_status dl_rotary_positions(const dl_tensor* input, const dl_tensor* positions, const dl_tensor* cosine,
+    const dl_tensor* sine, dl_rotary_layout layout, dl_tensor** output);
+
+typedef struct dl_paged_cache dl_paged_cache;
+typedef struct dl_paged_batch dl_paged_batch;
+/* options.dtype (f32 or bf16) is the pages' type; options.device a GPU. */
+DL_API dl_status dl_paged_cache_create(int64_t layers, int64_t pages, int64_t page_size, int64_t kv_heads,
+    int64_t head_dim, dl_tensor_options options, dl_paged_cache** output);
+DL_API void dl_paged_cache_release(dl_paged_cache* cache);
+/* Views of a layer's live storage [pages, kv_heads, page_size, head_dim]; either slot may be NULL. */
+DL_API dl_status dl_paged_cache_tensors(const dl_paged_cache* cache, int64_t layer, dl_tensor** key, dl_tensor** value);
+/* A step: sequence b holds lengths[b] positions and gets counts[b] new ones; its position p lies in page
+ * tables[b * width + p / page_size].  `shared` leading positions (whole pages, 0: none) lie in the same pages for all.
+ * The arrays are host memory, read during the call. */
+DL_API dl_status dl_paged_batch_create(const dl_paged_cache* cache, int64_t heads, int64_t sequences,
+    const int64_t* lengths, const int64_t* counts, const int64_t* tables, int64_t width, int64_t shared,
+    dl_paged_batch** output);
+DL_API void dl_paged_batch_release(dl_paged_batch* batch);
+/* The step's keys, rotated, and values, [tokens, kv_heads, head_dim], into their pages of `layer`.  query [tokens, heads,
+ * head_dim] and rotated are both NULL, or rotated receives the queries rotated likewise, f32. */
+DL_API dl_status dl_paged_cache_append(dl_paged_cache* cache, int64_t layer, const dl_paged_batch* batch,
+    const dl_tensor* query, const dl_tensor* key, const dl_tensor* value, const dl_tensor* cosine, const dl_tensor* sine,
+    dl_rotary_layout layout, dl_tensor** rotated);
+/* The step's queries [tokens, heads, head_dim] over the pages of `layer`, each row over the positions up to its own;
+ * f32 [tokens, heads, head_dim]. */
+DL_API dl_status dl_paged_attention(const dl_paged_cache* cache, int64_t layer, const dl_paged_batch* batch,
+    const dl_tensor* query, dl_tensor** output);
 
 #ifdef __cplusplus
 }

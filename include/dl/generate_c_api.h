@@ -76,6 +76,13 @@ DL_API dl_status dl_decoder_lm_set_weight_repack(dl_decoder_lm* lm, int32_t enab
  * evaluated with basic IEEE double operations so that any restatement gives the same index.  [B] i64. */
 DL_API dl_status dl_sample(const dl_tensor* logits, double temperature, dl_random_key key, dl_tensor** output);
 
+/* Verifies drafted tokens [B, K] (i64; a negative id ends a row) against the target's logits [B, K + 1, V], given uniform
+ * numbers [B, K + 1] (f32, from [0, 1)); draft, the draft model's logits [B, K, V], may be NULL (a draft was certain).
+ * tokens [B, K + 1]: the accepted drafts, the token drawn after them, then -1; accepted [B]: how many were.  Both i64.
+ * The rule stands at dl::verify_drafted (dl/ops.h); temperature <= 0 accepts the target's argmax. */
+DL_API dl_status dl_verify_drafted(const dl_tensor* drafted, const dl_tensor* target, const dl_tensor* draft,
+    double temperature, const dl_tensor* uniforms, dl_tensor** tokens, dl_tensor** accepted);
+
 /* scale * N(0, 1) from the keyed Philox normal (dl_randn_with_key's mapping), rounded once to options.dtype
  * (f32 or bf16); for synthesising large seeded weights directly in device memory. */
 DL_API dl_status dl_normal_with_key(dl_random_key key, dl_shape shape, double scale, dl_tensor_options options,
