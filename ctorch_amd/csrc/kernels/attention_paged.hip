@@ -2,317 +2,373 @@
 // keys up to its own position, o = sum_j softmax_j(q k_j / sqrt(hd)) v_j, the keys found through the run's page table.
 // f32 or bf16 pages, head size 16, 32, 64 or 128, page sizes that are powers of two from 16.
 //
-// A work-group takes an item, up to 16 NT rows (token r / G, query head r % G of the KV head's group) over a range of
-// keys, for one KV head; its four waves split the range, stream it in tiles of 32 keys from memory into registers and keep
-// their own online softmax (base 2, log2 e folded into the query's scale), and merge in LDS.  Per tile and 16 rows:
-//   S^T[16 keys][16 rows] = K[16][hd] Q[16][hd]^T    (v_mfma_f32_16x16x32_bf16, A = 16 key rows as they are stored)
-//   O^T[16 d][16 rows]   += V^T[16 d][32 keys] P^T   (A = V^T, transposed through the wave's own LDS tile)
-// so a lane holds the scores of one row, and they are the B operand of the second product as they come.  Queries and
-// probabilities are split into bf16 hi + lo (and f32 keys and values too), which keeps f32 accuracy: two products for
-// bf16 pages, three for f32 ones (the lo * lo term is below 2^-16 of the product).  Row sums come out of one more product
-// whose A operand is all ones.  A tile of 32 keys is two halves of 16, each in one page; keys past the range read as zero
-// from the buffer range and are masked, so that what a page holds behind the sequence never counts, not even a NaN.
-// An item that is all its rows see writes the output, the others (o, max, sum) partials that paged_merge joins.
+// Products are exact to f32 on the matrix cores.  bf16 keys and values go in as they are stored (v_mfma_f32_16x16x32_bf16)
+// against queries and probabilities cut into three bf16 parts of 8 bits each, which hold all 24 bits of an f32: three
+// products (bf16 queries are one part).  (Two parts, 2^-17 off, gave outputs 4e-6 off the 64-bit ones, three 7e-7.)  f32
+// pages take the f32 matrix instruction where memory is the bound, and three by three parts where the products are, the
+// terms below 2^-24 left out: six products, 2.7 times the f32 instruction's rate.
+//   S^T[16 keys][16 rows] = K[16][hd] Q[16][hd]^T    so that a lane holds scores of one row (lane % 16),
+//   O^T[16 d][16 rows]   += V^T[16 d][keys] P^T       and they are the second product's right operand as they come.
+// The softmax runs in base 2 with the running base and sum of each row; keys past a range are masked and their values
+// read as zero, so that what a page holds behind the sequence never counts, not even a NaN.  An item that is all its rows
+// see writes the output, the others (o, maximum, sum) partials that paged_merge joins.
 #include "kernels/device_common.h"
 
 namespace dlk {
 namespace {
 
-constexpr int kTileKeys = 32, kWaves = 4, kThreads = kWaves * kWave;
+constexpr int kWaves = 4, kThreads = kWaves * kWave;
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
 
-// bf16 hi and lo parts of eight f32 values (x = hi + lo to 2^-16; x - hi is exact in f32)
-__device__ __forceinline__ void split8(const f32x8 v, bf16x8& hi, bf16x8& lo) {
-    const u32x4 h = __builtin_bit_cast(u32x4, __builtin_convertvector(v, bf16x8));
-    const f32x8 back = {__uint_as_float(h.x << 16), __uint_as_float(h.x & 0xffff0000u),
-                        __uint_as_float(h.y << 16), __uint_as_float(h.y & 0xffff0000u),
-                        __uint_as_float(h.z << 16), __uint_as_float(h.z & 0xffff0000u),
-                        __uint_as_float(h.w << 16), __uint_as_float(h.w & 0xffff0000u)};
-    hi = __builtin_bit_cast(bf16x8, h);
-    lo = __builtin_convertvector(v - back, bf16x8);
-}
-
-__device__ __forceinline__ void split4(const u32x4 w, u32x2& hi, u32x2& lo) {
-    const f32x4 v = __builtin_bit_cast(f32x4, w);
-    const u32x2 h = __builtin_bit_cast(u32x2, __builtin_convertvector(v, bf16x4));
-    const f32x4 back = {__uint_as_float(h.x << 16), __uint_as_float(h.x & 0xffff0000u),
-                        __uint_as_float(h.y << 16), __uint_as_float(h.y & 0xffff0000u)};
-    hi = h;
-    lo = __builtin_bit_cast(u32x2, __builtin_convertvector(v - back, bf16x4));
-}
-
-// maximum over the four lanes that hold one row's scores (l, l ^ 16, l ^ 32, l ^ 48)
-__device__ __forceinline__ float max_over_row(float x) {
-    const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = fmaxf(__uint_as_float(h[0]), __uint_as_float(h[1]));
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-
-__device__ __forceinline__ bf16x8 load_query(const dlk_paged_params& p, int64_t at, int d, float scale, bf16x8& lo) {
-    f32x8 x;
-    if (p.q_bf16) {
-        const u32x4 w = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p.q) + at + d);
-        x = f32x8{bf16_lo(w.x), bf16_hi(w.x), bf16_lo(w.y), bf16_hi(w.y), bf16_lo(w.z), bf16_hi(w.z), bf16_lo(w.w), bf16_hi(w.w)};
-    } else {
-        const float* row = static_cast<const float*>(p.q) + at + d;
-        const f32x4 a = *reinterpret_cast<const f32x4*>(row), b = *reinterpret_cast<const f32x4*>(row + 4);
-        x = f32x8{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+// The nearest bf16 of each value, and the rest (exact): three parts hold all 24 bits.
+template <int PARTS> __device__ __forceinline__ void cut8(f32x8 v, bf16x8 (&part)[PARTS]) {
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i) {
+        part[i] = __builtin_convertvector(v, bf16x8);
+        const u32x4 h = __builtin_bit_cast(u32x4, part[i]);
+        if (i + 1 < PARTS)
+            v -= f32x8{__uint_as_float(h.x << 16), __uint_as_float(h.x & 0xffff0000u), __uint_as_float(h.y << 16),
+                       __uint_as_float(h.y & 0xffff0000u), __uint_as_float(h.z << 16), __uint_as_float(h.z & 0xffff0000u),
+                       __uint_as_float(h.w << 16), __uint_as_float(h.w & 0xffff0000u)};
     }
-    bf16x8 hi;
-    split8(x * scale, hi, lo);
-    return hi;
 }
 
-template <typename KT, int HD, int NT>
-__global__ __launch_bounds__(kThreads) void paged_stream(const dlk_paged_params p, const dlk_paged_item* items, float* partial_o,
-                                                         float* partial_ml) {
+// The first 8 bits of four values, and the rest: cut off, so that no finite key or value becomes infinite.
+__device__ __forceinline__ u32x2 cut4(f32x4& v) {
+    const u32x4 w = __builtin_bit_cast(u32x4, v);
+    v -= __builtin_bit_cast(f32x4, w & 0xffff0000u);
+    return u32x2{__builtin_amdgcn_perm(w.y, w.x, 0x07060302u), __builtin_amdgcn_perm(w.w, w.z, 0x07060302u)};
+}
+
+// over the four lanes that hold one row's scores (l, l ^ 16, l ^ 32, l ^ 48)
+template <typename Op> __device__ __forceinline__ float over_row(float x, Op op) {
+    const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = op(__uint_as_float(h[0]), __uint_as_float(h[1]));
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float max_over_row(float x) {
+    return over_row(x, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ float sum_over_row(float x) {
+    return over_row(x, [](float a, float b) { return a + b; });
+}
+
+// the compiler keeps LDS accesses of a wave in order across this (the hardware does by itself)
+__device__ __forceinline__ void wave_order() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local"); }
+
+// 8 entries of a query row, unscaled
+__device__ __forceinline__ f32x8 query8(const dlk_paged_params& p, int64_t at) {
+    if (p.q_bf16) {
+        const u32x4 w = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p.q) + at);
+        return f32x8{bf16_lo(w.x), bf16_hi(w.x), bf16_lo(w.y), bf16_hi(w.y), bf16_lo(w.z), bf16_hi(w.z), bf16_lo(w.w), bf16_hi(w.w)};
+    }
+    const float* row = static_cast<const float*>(p.q) + at;
+    const f32x4 a = *reinterpret_cast<const f32x4*>(row), b = *reinterpret_cast<const f32x4*>(row + 4);
+    return f32x8{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+}
+
+// The four values at V[keys at .. +4 rows][d], d = the lane's column of a 16-wide block, out of row-major bf16 LDS rows of
+// STRIDE: the 16 lanes of a group read 4 rows of 16 between them, and each receives a column (ds_read_b64_tr_b16).
+template <int STRIDE> __device__ __forceinline__ u32x2 column4(const uint16_t* block, int col) {
+    typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+    const uint16_t* from = block + (col / 4) * STRIDE + 4 * (col % 4);
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(from)));
+}
+
+// Weights of a row whose base is not set yet: any score sets it.
+constexpr float kNoBase = -1e30f;
+// How far (in powers of two) a score may lie above its row's base before the base follows.
+constexpr float kSlack = 8.0f;
+
+// One row's weights exp2(s c - base) out of 4 N scores of its lane, and the lane's share of their sum.  The base need not be
+// the row's maximum: f32 weights up to 2^8 are as exact, so it moves only when a score passes it by more, mostly once, and
+// the row's lanes do not have to compare their scores before that.  `outputs` are then scaled to the new base.
+template <int N, int D> __device__ __forceinline__ void soften(f32x4 (&s)[N], float& base, float& l, float c, f32x4 (&outputs)[D]) {
+    float top = s[0][0];
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) top = fmaxf(top, s[i][j]);
+    if (__any(top * c > base + kSlack)) {
+        const float next = fmaxf(base, max_over_row(top) * c);
+        const float keep = __builtin_amdgcn_exp2f(base - next);
+        base = next;
+        l *= keep;
+#pragma unroll
+        for (int d = 0; d < D; ++d) outputs[d] *= keep;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            s[i][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][j], c, -base));
+            l += s[i][j];
+        }
+}
+
+// ------------------------------------------------------------------------------------------------ few rows
+// Up to 16 NT rows over a range of keys: the four waves split the range, each streams its run in tiles of 16 NU keys from
+// memory into registers and keeps its own softmax, and they merge in LDS.  Bound by memory: a tile's keys and values are
+// asked for as soon as the registers of the ones before are free, and the waves of a SIMD hide each other's waits.
+//
+// bf16: V goes through the wave's own LDS tile, stored as it comes and read back by columns; the cut queries of two row
+// tiles stay in LDS, where one tile's fit the registers.  f32: no LDS; with the keys of step j of the second product chosen
+// as 4 q + j (q = lane / 16), its right operand is the score register j, and its left one 16 bytes of a V row, whose four
+// entries belong to four output tiles (tile e, row i is head entry 4 i + e).
+template <typename KT, int HD, int NT, int QP>
+__global__ __launch_bounds__(kThreads, 2) void paged_few(const dlk_paged_params p, const dlk_paged_list list) {
     constexpr bool F32 = sizeof(KT) == 4;
-    constexpr int PLANES = F32 ? 2 : 1;               // bf16 planes of the staged V^T
-    constexpr int KS = HD < 32 ? 1 : HD / 32;         // k steps of the score product
-    constexpr int DT = HD / 16;                       // 16-wide head-dim tiles of the output
-    constexpr int KL = F32 ? 2 : 1;                   // 16-byte loads of a K fragment (8 values)
-    constexpr int DPP = 16 / static_cast<int>(sizeof(KT)); // head-dim values of a 16-byte piece
-    constexpr int PIECES = HD / DPP;                  // pieces of a row
-    constexpr int VI = (PIECES + 7) / 8;              // V pieces per lane and key (64 lanes: 8 key pairs x 8 pieces)
-    constexpr int VSTRIDE = kTileKeys + 4;            // bf16 per staged V^T row: 18 words spread the accesses over the banks
+    constexpr int NU = F32 && HD == 128 ? 1 : 2;      // 16-key halves of a tile (f32 heads of 128: registers)
+    constexpr int KEYS = 16 * NU, ROWS = 16 * NT;
+    constexpr int KS = HD < 32 ? 1 : HD / 32;         // bf16: k steps of the score product
+    constexpr int KF = HD / 16;                       // f32: 16-byte pieces of a key per lane
+    constexpr int DT = HD / 16;                       // output tiles
+    constexpr int E = HD >= 64 ? 4 : HD / 16;         // f32: entries of a V row per lane and load
+    constexpr int VL = HD / 16 / E;                   // f32: such loads of a V row
+    constexpr int PIECES = HD / 8;                    // bf16: 16-byte pieces of a row
+    constexpr int VI = (16 * PIECES + kWave - 1) / kWave; // bf16: V pieces per lane and half
+    constexpr int VSTRIDE = HD + 16;                  // bf16 of a staged V row: the column reads hit no bank twice
     constexpr int ROW = HD * static_cast<int>(sizeof(KT));
-    constexpr int ROWS = 16 * NT;
-    constexpr int STAGE = kWaves * PLANES * HD * VSTRIDE * 2, MERGE = kWaves * ROWS * HD * 4;
-    // the staged V^T tiles, and after the last tile the waves' outputs
-    __shared__ __attribute__((aligned(16))) char area[STAGE > MERGE ? STAGE : MERGE];
+    constexpr bool QLDS = !F32 && NT > 1;             // the cut queries, in LDS
+    constexpr int STAGE = F32 ? 0 : kWaves * KEYS * VSTRIDE * 2, QUERIES = QLDS ? QP * ROWS * VSTRIDE * 2 : 0;
+    constexpr int MERGE = kWaves * ROWS * HD * 4;
+    // V tiles and queries, then the waves' outputs
+    __shared__ __attribute__((aligned(16))) char area[STAGE + QUERIES > MERGE ? STAGE + QUERIES : MERGE];
     __shared__ float m_s[kWaves][ROWS], l_s[kWaves][ROWS];
 
     const int t = threadIdx.x, lane = t % kWave, q = lane / 16, col = lane % 16;
     const int wave = __builtin_amdgcn_readfirstlane(t / kWave);
     const int kvh = static_cast<int>(blockIdx.x) % p.KV;
-    const dlk_paged_item item = items[blockIdx.x / p.KV];
+    const dlk_paged_item item = list.items[blockIdx.x / p.KV];
     const int G = p.H / p.KV;
     const int32_t* table = p.tables + item.table;
+    const float c = p.scale * 1.4426950408889634f;
 
     // the item's keys in four runs of whole tiles
-    const int all = (item.key_end - item.key_begin + kTileKeys - 1) / kTileKeys;
+    const int all = (item.key_end - item.key_begin + KEYS - 1) / KEYS;
     const int per_wave = (all + kWaves - 1) / kWaves;
-    const int w_begin = item.key_begin + min(wave * per_wave, all) * kTileKeys;
-    const int w_end = min(item.key_end, w_begin + per_wave * kTileKeys);
-    const int tiles = max(0, (w_end - w_begin + kTileKeys - 1) / kTileKeys);
+    const int w_begin = item.key_begin + min(wave * per_wave, all) * KEYS;
+    const int w_end = min(item.key_end, w_begin + per_wave * KEYS);
+    const int tiles = max(0, (w_end - w_begin + KEYS - 1) / KEYS);
 
-    struct Tile {
-        u32x4 k[2][KS][KL];
-        u32x4 v[2][VI][2];
+    constexpr int kBeyond = INT32_MAX / 2; // an offset past every range: reads as zero
+    const int k_offset = F32 || 8 * q < HD ? col * ROW + 16 * q : kBeyond;
+    // the 16 rows of a half: their place, and how many bytes of them are within the run
+    auto half_of = [&](int tile, int u, int& bytes) {
+        const int key = w_begin + tile * KEYS + 16 * u;
+        bytes = max(0, min(16, w_end - key)) * ROW;
+        const int page = table[min(key, w_end - 1) >> p.page_shift];
+        return (((static_cast<int64_t>(page) * p.KV + kvh) << p.page_shift) + (key & ((1 << p.page_shift) - 1))) * HD;
     };
-    const int kp = lane % 8, piece = lane / 8; // V: keys 2 kp, 2 kp + 1 of a half, pieces piece + 8 i
-    const int k_offset = 8 * q < HD ? col * ROW + 8 * q * static_cast<int>(sizeof(KT)) : INT32_MAX / 2; // (past the range)
-    auto load = [&](int tile, Tile& dst) {
+    u32x4 k[NU][F32 ? KF : KS], v[NU][F32 ? 4 * VL : VI];
+    auto load_keys = [&](int tile) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int key = w_begin + tile * kTileKeys + 16 * u;
-            const int live = max(0, min(16, w_end - key));
-            const int page = table[min(key, w_end - 1) >> p.page_shift];
-            const int64_t at = ((static_cast<int64_t>(page) * p.KV + kvh) << p.page_shift) + (key & ((1 << p.page_shift) - 1));
-            const __amdgpu_buffer_rsrc_t kres = __builtin_amdgcn_make_buffer_rsrc(
-                const_cast<KT*>(static_cast<const KT*>(p.k)) + at * HD, 0, live * ROW, kBufferFlags);
-            const __amdgpu_buffer_rsrc_t vres = __builtin_amdgcn_make_buffer_rsrc(
-                const_cast<KT*>(static_cast<const KT*>(p.v)) + at * HD, 0, live * ROW, kBufferFlags);
+        for (int u = 0; u < NU; ++u) {
+            int bytes;
+            const int64_t at = half_of(tile, u, bytes);
+            const __amdgpu_buffer_rsrc_t rows =
+                __builtin_amdgcn_make_buffer_rsrc(const_cast<KT*>(static_cast<const KT*>(p.k)) + at, 0, bytes, kBufferFlags);
 #pragma unroll
-            for (int st = 0; st < KS; ++st)
-#pragma unroll
-                for (int e = 0; e < KL; ++e)
-                    dst.k[u][st][e] = __builtin_amdgcn_raw_buffer_load_b128(
-                        kres, k_offset + 32 * st * static_cast<int>(sizeof(KT)) + 16 * e, 0, 0);
-#pragma unroll
-            for (int i = 0; i < VI; ++i)
-#pragma unroll
-                for (int e = 0; e < 2; ++e)
-                    dst.v[u][i][e] = __builtin_amdgcn_raw_buffer_load_b128(
-                        vres, (2 * kp + e) * ROW + (min(piece + 8 * i, PIECES - 1)) * 16, 0, 0);
+            for (int st = 0; st < (F32 ? KF : KS); ++st) k[u][st] = __builtin_amdgcn_raw_buffer_load_b128(rows, k_offset + 64 * st, 0, 0);
         }
     };
+    auto load_values = [&](int tile) {
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
+            int bytes;
+            const int64_t at = half_of(tile, u, bytes);
+            const __amdgpu_buffer_rsrc_t rows =
+                __builtin_amdgcn_make_buffer_rsrc(const_cast<KT*>(static_cast<const KT*>(p.v)) + at, 0, bytes, kBufferFlags);
+            if constexpr (F32) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int i = 0; i < VL; ++i) {
+                        const int offset = (4 * q + j) * ROW + (64 * i + E * col) * 4;
+                        u32x4& to = v[u][j * VL + i];
+                        if constexpr (E == 4) to = __builtin_amdgcn_raw_buffer_load_b128(rows, offset, 0, 0);
+                        if constexpr (E == 2) {
+                            const u32x2 two = __builtin_amdgcn_raw_buffer_load_b64(rows, offset, 0, 0);
+                            to = u32x4{two.x, two.y, 0u, 0u};
+                        }
+                        if constexpr (E == 1) to = u32x4{__builtin_amdgcn_raw_buffer_load_b32(rows, offset, 0, 0), 0u, 0u, 0u};
+                    }
+            } else {
+#pragma unroll
+                for (int i = 0; i < VI; ++i) // the half's rows are one piece of memory, read in order
+                    v[u][i] = __builtin_amdgcn_raw_buffer_load_b128(rows, 16 * (lane + kWave * i), 0, 0);
+            }
+        }
+    };
+    if (tiles > 0) {
+        load_keys(0);
+        load_values(0);
+    }
 
-    // the rows as the B operand, in base 2: column col of tile nt is row row_begin + 16 nt + col
-    bf16x8 qh[NT][KS], ql[NT][KS];
+    // the rows as the right operand: column col of tile nt is row row_begin + 16 nt + col
+    bf16x8 qb[QLDS ? 1 : NT][KS][QP];
+    f32x4 qf[NT][KF];
     int limit[NT]; // the last key that the row sees
+    uint16_t* q_s = reinterpret_cast<uint16_t*>(area + STAGE);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         const int row = min(item.row_begin + 16 * nt + col, item.row_end - 1);
         limit[nt] = min(item.first + row / G, w_end - 1);
         const int64_t at = (item.token + row / G) * p.q_row + static_cast<int64_t>(kvh * G + row % G) * p.q_head;
+        if constexpr (F32) {
 #pragma unroll
-        for (int st = 0; st < KS; ++st)
-            qh[nt][st] = load_query(p, at, min(32 * st + 8 * q, HD - 8), p.scale * 1.4426950408889634f, ql[nt][st]);
-    }
-    const int all_see = min(item.first + item.row_begin / G, w_end - 1); // the last key that every row sees
-
-    f32x4 o[NT][DT], l[NT];
-    float m_run[NT];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        m_run[nt] = -INFINITY;
-        l[nt] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int d = 0; d < DT; ++d) o[nt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
-    const bf16x8 ones = __builtin_bit_cast(bf16x8, u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
-    uint16_t* my_vt = reinterpret_cast<uint16_t*>(area) + wave * PLANES * HD * VSTRIDE;
-    uint32_t* vt_words = reinterpret_cast<uint32_t*>(my_vt);
-
-    auto use = [&](int tile, const Tile& cur) {
-        // (a wave's LDS operations complete in order: the fences only keep the compiler from moving them past each other)
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
-        // V^T of the tile into the wave's LDS tile: a word is a key pair of one head-dim row
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int i = 0; i < VI; ++i) {
-                if (PIECES < 8 && piece >= PIECES) continue;
-                const u32x4 a = cur.v[u][i][0], c = cur.v[u][i][1];
-                const int d0 = DPP * (piece + 8 * i), word = 8 * u + kp;
-                if constexpr (F32) {
-                    u32x2 h0, l0, h1, l1;
-                    split4(a, h0, l0);
-                    split4(c, h1, l1);
-                    const uint32_t hw[4] = {(h0.x & 0xffffu) | (h1.x << 16), (h0.x >> 16) | (h1.x & 0xffff0000u),
-                                            (h0.y & 0xffffu) | (h1.y << 16), (h0.y >> 16) | (h1.y & 0xffff0000u)};
-                    const uint32_t lw[4] = {(l0.x & 0xffffu) | (l1.x << 16), (l0.x >> 16) | (l1.x & 0xffff0000u),
-                                            (l0.y & 0xffffu) | (l1.y << 16), (l0.y >> 16) | (l1.y & 0xffff0000u)};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        vt_words[(d0 + e) * (VSTRIDE / 2) + word] = hw[e];
-                        vt_words[(HD + d0 + e) * (VSTRIDE / 2) + word] = lw[e];
-                    }
-                } else {
-                    const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, cw[4] = {c.x, c.y, c.z, c.w};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        vt_words[(d0 + 2 * e) * (VSTRIDE / 2) + word] = (aw[e] & 0xffffu) | (cw[e] << 16);
-                        vt_words[(d0 + 2 * e + 1) * (VSTRIDE / 2) + word] = (aw[e] >> 16) | (cw[e] & 0xffff0000u);
-                    }
-                }
+            for (int st = 0; st < KF; ++st) { // entries 16 st + 4 q .. +4
+                const f32x8 x = query8(p, at + 16 * st + 8 * (q / 2));
+                qf[nt][st] = q % 2 ? f32x4{x[4], x[5], x[6], x[7]} : f32x4{x[0], x[1], x[2], x[3]};
             }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
-        // scores of both halves
-        f32x4 s[NT][2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) s[nt][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+        } else {
 #pragma unroll
             for (int st = 0; st < KS; ++st) {
-                bf16x8 kh, kl;
-                if constexpr (F32)
-                    split8(__builtin_bit_cast(f32x8, __builtin_shufflevector(cur.k[u][st][0], cur.k[u][st][KL - 1], 0, 1, 2, 3,
-                                                                              4, 5, 6, 7)), kh, kl);
-                else kh = __builtin_bit_cast(bf16x8, cur.k[u][st][0]);
+                bf16x8(&parts)[QP] = qb[QLDS ? 0 : nt][st];
+                if (QLDS && wave != nt) continue; // wave nt cuts row tile nt for all
+                cut8<QP>(query8(p, at + min(32 * st + 8 * q, HD - 8)), parts);
+                if (QLDS && 8 * q < HD) {
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    s[nt][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kh, qh[nt][st], s[nt][u], 0, 0, 0);
-                    s[nt][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kh, ql[nt][st], s[nt][u], 0, 0, 0);
-                    if constexpr (F32) s[nt][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kl, qh[nt][st], s[nt][u], 0, 0, 0);
+                    for (int part = 0; part < QP; ++part)
+                        *reinterpret_cast<bf16x8*>(q_s + (part * ROWS + 16 * nt + col) * VSTRIDE + 32 * st + 8 * q) = parts[part];
                 }
             }
         }
-        const int key0 = w_begin + tile * kTileKeys;
-        bf16x8 ph[NT], pl[NT];
+    }
+    if (QLDS) __syncthreads();
+    const int all_see = min(item.first + item.row_begin / G, w_end - 1); // the last key that every row sees
+
+    f32x4 o[NT][DT];
+    float base[NT], l[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        base[nt] = kNoBase;
+        l[nt] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[nt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    uint16_t* my_v = reinterpret_cast<uint16_t*>(area) + wave * KEYS * VSTRIDE;
+
+    for (int tile = 0; tile < tiles; ++tile) {
+        if constexpr (!F32) {
+            wave_order();
+#pragma unroll
+            for (int u = 0; u < NU; ++u)
+#pragma unroll
+                for (int i = 0; i < VI; ++i) {
+                    const int at = lane + kWave * i;
+                    if (16 * PIECES >= kWave || at < 16 * PIECES)
+                        *reinterpret_cast<u32x4*>(my_v + (16 * u + at / PIECES) * VSTRIDE + 8 * (at % PIECES)) = v[u][i];
+                }
+            wave_order();
+            if (tile + 1 < tiles) load_values(tile + 1);
+        }
+        f32x4 s[NT][NU];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int u = 0; u < NU; ++u) s[nt][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int st = 0; st < (F32 ? KF : KS); ++st)
+            if constexpr (F32) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int u = 0; u < NU; ++u)
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+                            s[nt][u] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[u][st][e]), qf[nt][st][e], s[nt][u], 0, 0, 0);
+            } else {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int part = QP - 1; part >= 0; --part) {
+                        bf16x8 x = qb[QLDS ? 0 : nt][st][part];
+                        if constexpr (QLDS)
+                            x = *reinterpret_cast<const bf16x8*>(q_s + (part * ROWS + 16 * nt + col) * VSTRIDE + min(32 * st + 8 * q, HD - 8));
+#pragma unroll
+                        for (int u = 0; u < NU; ++u)
+                            s[nt][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k[u][st]), x, s[nt][u], 0, 0, 0);
+                    }
+            }
+        if (tile + 1 < tiles) load_keys(tile + 1);
+        const int key0 = w_begin + tile * KEYS;
+        bf16x8 pb[NT][3];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            if (key0 + kTileKeys - 1 > all_see) {
+            if (key0 + KEYS - 1 > all_see) {
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
+                for (int u = 0; u < NU; ++u)
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
                         if (key0 + 16 * u + 4 * q + j > limit[nt]) s[nt][u][j] = -INFINITY;
             }
-            float mx = -INFINITY;
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) mx = fmaxf(mx, s[nt][u][j]);
-            const float m_new = fmaxf(m_run[nt], max_over_row(mx));
-            // a row that has seen no key yet (masked so far, or scores of -inf) keeps a finite base: exp2(-inf) = 0
-            const float base = m_new == -INFINITY ? 0.0f : m_new;
-            const float alpha = __builtin_amdgcn_exp2f(m_run[nt] - base);
-            m_run[nt] = m_new;
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) s[nt][u][j] = __builtin_amdgcn_exp2f(s[nt][u][j] - base);
-            if (!__all(alpha == 1.0f)) {
-                l[nt] *= alpha;
-#pragma unroll
-                for (int d = 0; d < DT; ++d) o[nt][d] *= alpha;
-            }
-            split8(f32x8{s[nt][0][0], s[nt][0][1], s[nt][0][2], s[nt][0][3], s[nt][1][0], s[nt][1][1], s[nt][1][2],
-                         s[nt][1][3]}, ph[nt], pl[nt]);
-            l[nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, ph[nt], l[nt], 0, 0, 0);
-            l[nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pl[nt], l[nt], 0, 0, 0);
+            soften(s[nt], base[nt], l[nt], c, o[nt]);
+            if constexpr (!F32)
+                cut8<3>(f32x8{s[nt][0][0], s[nt][0][1], s[nt][0][2], s[nt][0][3], s[nt][NU - 1][0], s[nt][NU - 1][1],
+                              s[nt][NU - 1][2], s[nt][NU - 1][3]}, pb[nt]);
         }
-        // lane (d = 16 dt + col, q) supplies V[keys 4 q .. +4 and 16 + 4 q .. +4][d]
+        if constexpr (F32) {
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-            const int at = (16 * dt + col) * VSTRIDE + 4 * q;
-            const u32x2 lo4 = *reinterpret_cast<const u32x2*>(my_vt + at);
-            const u32x2 hi4 = *reinterpret_cast<const u32x2*>(my_vt + at + 16);
-            const bf16x8 a = __builtin_bit_cast(bf16x8, u32x4{lo4.x, lo4.y, hi4.x, hi4.y});
-            bf16x8 al = a;
-            if constexpr (F32) {
-                const u32x2 llo4 = *reinterpret_cast<const u32x2*>(my_vt + HD * VSTRIDE + at);
-                const u32x2 lhi4 = *reinterpret_cast<const u32x2*>(my_vt + HD * VSTRIDE + at + 16);
-                al = __builtin_bit_cast(bf16x8, u32x4{llo4.x, llo4.y, lhi4.x, lhi4.y});
-            }
+            for (int u = 0; u < NU; ++u)
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                o[nt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, ph[nt], o[nt][dt], 0, 0, 0);
-                o[nt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, pl[nt], o[nt][dt], 0, 0, 0);
-                if constexpr (F32) o[nt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(al, ph[nt], o[nt][dt], 0, 0, 0);
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int i = 0; i < VL; ++i)
+#pragma unroll
+                        for (int e = 0; e < E; ++e)
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+                                o[nt][i * E + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[u][j * VL + i][e]), s[nt][u][j], o[nt][i * E + e], 0, 0, 0);
+            if (tile + 1 < tiles) load_values(tile + 1);
+        } else {
+            // lane (d = 16 dt + col, q) supplies V[keys 4 q .. +4 and 16 + 4 q .. +4][d], as its probabilities lie
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                const u32x2 a = column4<VSTRIDE>(my_v + 4 * q * VSTRIDE + 16 * dt, col);
+                const u32x2 b = column4<VSTRIDE>(my_v + (16 + 4 * q) * VSTRIDE + 16 * dt, col);
+                const bf16x8 columns = __builtin_bit_cast(bf16x8, u32x4{a.x, a.y, b.x, b.y});
+#pragma unroll
+                for (int part = 2; part >= 0; --part)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) o[nt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(columns, pb[nt][part], o[nt][dt], 0, 0, 0);
             }
-        }
-    };
-    if (tiles > 0) {
-        // two tiles a turn, so that the buffers are named statically; the next tile is in flight while one is used
-        Tile a, c;
-        load(0, a);
-        for (int tile = 0;;) {
-            if (tile + 1 >= tiles) { use(tile, a); break; }
-            load(tile + 1, c);
-            use(tile, a);
-            ++tile;
-            if (tile + 1 >= tiles) { use(tile, c); break; }
-            load(tile + 1, a);
-            use(tile, c);
-            ++tile;
         }
     }
 
-    // merge the waves: a lane holds O[row col][d = 16 dt + 4 q + j] and the row's sum in every entry of l
+    // merge the waves
     __syncthreads();
     float* o_s = reinterpret_cast<float*>(area);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
+        const float sum = sum_over_row(l[nt]);
         if (q == 0) {
-            m_s[wave][16 * nt + col] = m_run[nt];
-            l_s[wave][16 * nt + col] = l[nt][0];
+            m_s[wave][16 * nt + col] = base[nt];
+            l_s[wave][16 * nt + col] = sum;
         }
+        float* row = o_s + (wave * ROWS + 16 * nt + col) * HD;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
-            *reinterpret_cast<f32x4*>(o_s + (wave * ROWS + 16 * nt + col) * HD + 16 * dt + 4 * q) = o[nt][dt];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) row[F32 ? 16 * E * (dt / E) + E * (4 * q + j) + dt % E : 16 * dt + 4 * q + j] = o[nt][dt][j];
     }
     __syncthreads();
     const int rows = item.row_end - item.row_begin;
     for (int i = t; i < rows * HD; i += kThreads) {
         const int r = i / HD, d = i % HD;
-        float M = -INFINITY;
+        float M = kNoBase;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) M = fmaxf(M, m_s[w][r]);
-        const float base = M == -INFINITY ? 0.0f : M;
         float L = 0.0f, O = 0.0f;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
-            const float weight = __builtin_amdgcn_exp2f(m_s[w][r] - base);
+            const float weight = __builtin_amdgcn_exp2f(m_s[w][r] - M);
             L += weight * l_s[w][r];
             O += weight * o_s[(w * ROWS + r) * HD + d];
         }
@@ -321,71 +377,286 @@ __global__ __launch_bounds__(kThreads) void paged_stream(const dlk_paged_params 
             p.out[(static_cast<int64_t>(item.token + row / G) * p.H + kvh * G + row % G) * HD + d] = O / L;
         } else {
             const int64_t at = (static_cast<int64_t>(item.slot) * p.KV + kvh) * ROWS + r;
-            partial_o[at * HD + d] = O;
+            list.partial_o[at * HD + d] = O;
             if (d == 0) {
-                partial_ml[2 * at] = M;
-                partial_ml[2 * at + 1] = L;
+                list.partial_ml[2 * at] = M;
+                list.partial_ml[2 * at + 1] = L;
             }
         }
     }
 }
 
-// Joins the partials of a row: those of its own run's splits and those of the prefix that the batch shares.  A wave per
-// (token, query head).
-template <int HD>
-__global__ __launch_bounds__(kThreads) void paged_merge(const dlk_paged_params p) {
-    const int lane = threadIdx.x % kWave;
-    const int unit = static_cast<int>(blockIdx.x) * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    if (unit >= p.merge_count * p.H) return;
-    const dlk_paged_merge merge = p.merges[unit / p.H];
-    const int h = unit % p.H, G = p.H / p.KV, kvh = h / G;
-    const int rows = 16 * p.row_tiles, row = merge.row + h % G;
-    const int shared_rows = 16 * p.shared_row_tiles, shared_row = merge.shared_row + h % G;
-    auto place = [&](int i) { // split i of the row's own run
-        return (static_cast<int64_t>(merge.slot + row / rows * merge.stride + i) * p.KV + kvh) * rows + row % rows;
-    };
-    auto shared_place = [&](int i) {
-        return (static_cast<int64_t>(shared_row / shared_rows * p.shared_splits + i) * p.KV + kvh) * shared_rows +
-               shared_row % shared_rows;
-    };
-    constexpr int PER = HD < kWave ? 1 : HD / kWave;
-    float M = -INFINITY, L = 0.0f, O[PER] = {};
-    auto add = [&](const float* o, const float* ml, int64_t at) {
-        const float m = ml[2 * at], m_new = fmaxf(M, m), base = m_new == -INFINITY ? 0.0f : m_new;
-        const float keep = __builtin_amdgcn_exp2f(M - base), weight = __builtin_amdgcn_exp2f(m - base);
-        M = m_new;
-        L = L * keep + weight * ml[2 * at + 1];
+// ------------------------------------------------------------------------------------------------ many rows
+// 128 rows over a range of keys, 32 a wave, in tiles of 32 keys that pass through LDS for all waves: while one tile is used
+// the next is staged into the other buffer, from the registers that then receive the one after it, so that a tile costs one
+// barrier.  Bound by the matrix cores and the vector ALUs about alike (the weights' parts and the staging).  f32 pages are
+// cut into three bf16 planes as they are staged, once for the 128 rows.
+template <typename KT, int HD, int QP>
+__global__ __launch_bounds__(kThreads, 2) void paged_many(const dlk_paged_params p, const dlk_paged_list list) {
+    constexpr bool F32 = sizeof(KT) == 4;
+    constexpr int PLANES = F32 ? 3 : 1;
+    constexpr int BUFFERS = F32 && HD == 128 ? 1 : 2; // (LDS of two work-groups a CU)
+    constexpr int KEYS = 32, KS = HD < 32 ? 1 : HD / 32, DT = HD / 16;
+    constexpr int STRIDE = HD + 16;                   // bf16 of a staged row
+    constexpr int DPP = 16 / static_cast<int>(sizeof(KT)), PIECES = HD / DPP;
+    constexpr int ROW = HD * static_cast<int>(sizeof(KT)), ROWS = 128;
+    // a half of 16 keys is one piece of memory of BLOCK 16-byte pieces: several passes of all threads, or part of them
+    constexpr int BLOCK = 16 * PIECES, PASSES = BLOCK / kThreads, LOADS = PASSES ? 2 * PASSES : 1;
+    constexpr int TEAM = BLOCK < kWave ? kWave : BLOCK; // threads of a half, where one pass takes both
+    __shared__ __attribute__((aligned(16))) uint16_t ks[BUFFERS][PLANES][KEYS * STRIDE];
+    __shared__ __attribute__((aligned(16))) uint16_t vs[BUFFERS][PLANES][KEYS * STRIDE];
+
+    const int t = threadIdx.x, lane = t % kWave, q = lane / 16, col = lane % 16;
+    const int wave = __builtin_amdgcn_readfirstlane(t / kWave);
+    const int kvh = static_cast<int>(blockIdx.x) % p.KV;
+    const dlk_paged_item item = list.items[blockIdx.x / p.KV];
+    const int G = p.H / p.KV;
+    const int32_t* table = p.tables + item.table;
+    const float c = p.scale * 1.4426950408889634f;
+    const int tiles = (item.key_end - item.key_begin + KEYS - 1) / KEYS;
+
+    auto half_of = [&](int i) { return PASSES ? i / (PASSES ? PASSES : 1) : wave * kWave / TEAM; };
+    auto piece_of = [&](int i) { return PASSES ? t + kThreads * (i % (PASSES ? PASSES : 1)) : t % TEAM; };
+    const bool loads = PASSES || (t / TEAM < 2 && t % TEAM < BLOCK);
+    u32x4 kr[LOADS], vr[LOADS];
+    auto load = [&](int tile) {
 #pragma unroll
-        for (int e = 0; e < PER; ++e) O[e] = O[e] * keep + weight * o[at * HD + min(lane * PER + e, HD - 1)];
+        for (int i = 0; i < LOADS; ++i) {
+            const int key = item.key_begin + tile * KEYS + 16 * half_of(i);
+            const int bytes = loads ? max(0, min(16, item.key_end - key)) * ROW : 0; // what lies behind reads as zero
+            const int page = table[min(key, item.key_end - 1) >> p.page_shift];
+            const int64_t at = (((static_cast<int64_t>(page) * p.KV + kvh) << p.page_shift) + (key & ((1 << p.page_shift) - 1))) * HD;
+            const int whole = __builtin_amdgcn_readfirstlane(bytes);
+            const int offset = loads ? 16 * piece_of(i) : INT32_MAX / 2;
+            kr[i] = __builtin_amdgcn_raw_buffer_load_b128(
+                __builtin_amdgcn_make_buffer_rsrc(const_cast<KT*>(static_cast<const KT*>(p.k)) + at, 0, whole, kBufferFlags), offset, 0, 0);
+            vr[i] = __builtin_amdgcn_raw_buffer_load_b128(
+                __builtin_amdgcn_make_buffer_rsrc(const_cast<KT*>(static_cast<const KT*>(p.v)) + at, 0, whole, kBufferFlags), offset, 0, 0);
+        }
     };
-    for (int i = 0; i < merge.count; ++i) add(p.partial_o, p.partial_ml, place(i));
-    for (int i = 0; i < p.shared_splits; ++i) add(p.shared_o, p.shared_ml, shared_place(i));
-    float* out = p.out + (static_cast<int64_t>(merge.token) * p.H + h) * HD;
+    auto stage = [&](int buffer) {
+        if (!loads) return;
 #pragma unroll
-    for (int e = 0; e < PER; ++e)
-        if (lane * PER + e < HD) out[lane * PER + e] = O[e] / L;
+        for (int i = 0; i < LOADS; ++i) {
+            const int to = (16 * half_of(i) + piece_of(i) / PIECES) * STRIDE + DPP * (piece_of(i) % PIECES);
+            if constexpr (F32) {
+                f32x4 a = __builtin_bit_cast(f32x4, kr[i]), b = __builtin_bit_cast(f32x4, vr[i]);
+#pragma unroll
+                for (int plane = 0; plane < PLANES; ++plane) {
+                    *reinterpret_cast<u32x2*>(&ks[buffer][plane][to]) = cut4(a);
+                    *reinterpret_cast<u32x2*>(&vs[buffer][plane][to]) = cut4(b);
+                }
+            } else {
+                *reinterpret_cast<u32x4*>(&ks[buffer][0][to]) = kr[i];
+                *reinterpret_cast<u32x4*>(&vs[buffer][0][to]) = vr[i];
+            }
+        }
+    };
+    load(0);
+
+    // this lane's two rows: row_begin + 32 wave + 16 nt + col
+    bf16x8 qb[2][KS][QP];
+    int limit[2];
+    const int first_row = item.row_begin + 32 * wave;
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt) {
+        const int row = min(first_row + 16 * nt + col, item.row_end - 1);
+        limit[nt] = min(item.first + row / G, item.key_end - 1);
+        const int64_t at = (item.token + row / G) * p.q_row + static_cast<int64_t>(kvh * G + row % G) * p.q_head;
+#pragma unroll
+        for (int st = 0; st < KS; ++st) cut8<QP>(query8(p, at + min(32 * st + 8 * q, HD - 8)), qb[nt][st]);
+    }
+    // the last key that every row of the wave sees, and the last that any does
+    const int all_see = min(item.first + min(first_row, item.row_end - 1) / G, item.key_end - 1);
+    const int any_sees = first_row < item.row_end ? min(item.first + min(first_row + 31, item.row_end - 1) / G, item.key_end - 1) : -1;
+
+    f32x4 o[2][DT];
+    float base[2] = {kNoBase, kNoBase}, l[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[nt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    auto use = [&](int tile, int buffer) {
+        const int key0 = item.key_begin + tile * KEYS;
+        if (key0 > any_sees) return;
+        f32x4 s[2][2]; // [row tile][16-key half]
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            s[0][u] = s[1][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int st = 0; st < KS; ++st)
+#pragma unroll
+                for (int plane = PLANES - 1; plane >= 0; --plane) {
+                    bf16x8 k = *reinterpret_cast<const bf16x8*>(&ks[buffer][plane][(16 * u + col) * STRIDE + (HD < 32 ? 8 * (q % 2) : 32 * st + 8 * q)]);
+                    if (HD < 32 && q >= 2) k = __builtin_bit_cast(bf16x8, u32x4{0u, 0u, 0u, 0u});
+#pragma unroll
+                    for (int part = QP - 1; part >= 0; --part)
+                        if (part + plane <= 2)
+#pragma unroll
+                            for (int nt = 0; nt < 2; ++nt) s[nt][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, qb[nt][st][part], s[nt][u], 0, 0, 0);
+                }
+        }
+        bf16x8 pb[2][3];
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) {
+            if (key0 + KEYS - 1 > all_see) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (key0 + 16 * u + 4 * q + j > limit[nt]) s[nt][u][j] = -INFINITY;
+            }
+            soften(s[nt], base[nt], l[nt], c, o[nt]);
+            cut8<3>(f32x8{s[nt][0][0], s[nt][0][1], s[nt][0][2], s[nt][0][3], s[nt][1][0], s[nt][1][1], s[nt][1][2], s[nt][1][3]}, pb[nt]);
+        }
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int plane = PLANES - 1; plane >= 0; --plane) {
+                const uint16_t* block = &vs[buffer][plane][4 * q * STRIDE + 16 * dt];
+                const u32x2 a = column4<STRIDE>(block, col), b = column4<STRIDE>(block + 16 * STRIDE, col);
+                const bf16x8 v = __builtin_bit_cast(bf16x8, u32x4{a.x, a.y, b.x, b.y});
+#pragma unroll
+                for (int part = 2; part >= 0; --part)
+                    if (part + plane <= 2)
+#pragma unroll
+                        for (int nt = 0; nt < 2; ++nt) o[nt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pb[nt][part], o[nt][dt], 0, 0, 0);
+            }
+    };
+    stage(0);
+    if (tiles > 1) load(1);
+    __syncthreads();
+    for (int tile = 0; tile < tiles; ++tile) {
+        if constexpr (BUFFERS == 2) {
+            if (tile + 1 < tiles) stage((tile + 1) % 2);
+            if (tile + 2 < tiles) load(tile + 2);
+            use(tile, tile % 2);
+        } else {
+            use(tile, 0);
+            __syncthreads();
+            if (tile + 1 < tiles) stage(0);
+            if (tile + 2 < tiles) load(tile + 2);
+        }
+        __syncthreads();
+    }
+
+    // lane holds O[row col][d = 16 dt + 4 q + j]
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt) {
+        const int row = first_row + 16 * nt + col;
+        const float sum = sum_over_row(l[nt]);
+        if (row >= item.row_end) continue;
+        if (item.slot < 0) {
+            float* out = p.out + (static_cast<int64_t>(item.token + row / G) * p.H + kvh * G + row % G) * HD;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(out + 16 * dt + 4 * q) = o[nt][dt] / sum;
+        } else {
+            const int64_t at = (static_cast<int64_t>(item.slot) * p.KV + kvh) * ROWS + row - item.row_begin;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(list.partial_o + at * HD + 16 * dt + 4 * q) = o[nt][dt];
+            if (q == 0) {
+                list.partial_ml[2 * at] = base[nt];
+                list.partial_ml[2 * at + 1] = sum;
+            }
+        }
+    }
 }
 
-template <typename KT, int HD, int NT>
-int launch_stream(const dlk_paged_params& p, const dlk_paged_item* items, int count, float* o, float* ml, hipStream_t stream) {
-    hipLaunchKernelGGL((paged_stream<KT, HD, NT>), dim3(count * p.KV), dim3(kThreads), 0, stream, p, items, o, ml);
+// ------------------------------------------------------------------------------------------------ the merge
+// Joins the partials of a row: those of the prefix that the batch shares, then those of its own run's splits.  W waves take a
+// (token, query head), each every W-th split, 8 of them asked for at once, rows and sums together.  Bound by the two round
+// trips to memory (the record, the partials), or by the partials' bytes.
+template <int HD, int W>
+__global__ __launch_bounds__(kThreads) void paged_merge(const dlk_paged_params p) {
+    constexpr int PER = HD < kWave ? 1 : HD / kWave, AHEAD = 8;
+    typedef float fragment __attribute__((ext_vector_type(PER)));
+    __shared__ float m_s[kWaves], l_s[kWaves];
+    __shared__ fragment o_s[kWaves][kWave];
+    const int t = threadIdx.x, lane = t % kWave, all = __builtin_amdgcn_readfirstlane(t / kWave), wave = all % W;
+    const int64_t unit = min(static_cast<int64_t>(blockIdx.x) * (kWaves / W) + all / W, static_cast<int64_t>(p.merge_count) * p.H - 1);
+    const dlk_paged_merge merge = p.merges[unit / p.H];
+    const int h = static_cast<int>(unit % p.H), G = p.H / p.KV, kvh = h / G;
+    const dlk_paged_list& own = p.lists[merge.list];
+    const dlk_paged_list& front = p.lists[DLK_PAGED_SHARED];
+    const int row = merge.row + h % G, front_row = merge.shared_row + h % G;
+    const int64_t own_step = static_cast<int64_t>(p.KV) * own.rows, front_step = static_cast<int64_t>(p.KV) * front.rows;
+    const int64_t own_at = (static_cast<int64_t>(merge.slot + row / own.rows * merge.stride) * p.KV + kvh) * own.rows + row % own.rows;
+    const int64_t front_at = (static_cast<int64_t>(front_row / front.rows * p.shared_splits) * p.KV + kvh) * front.rows + front_row % front.rows;
+    const int count = p.shared_splits + merge.count, d = min(lane * PER, HD - PER);
+    float M = kNoBase, L = 0.0f;
+    fragment O = {};
+    for (int begin = wave; begin < count; begin += W * AHEAD) {
+        float m[AHEAD], l[AHEAD];
+        fragment x[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            const int i = min(begin + W * k, count - 1);
+            const bool shared = i < p.shared_splits;
+            const int64_t at = shared ? front_at + i * front_step : own_at + (i - p.shared_splits) * own_step;
+            const float* ml = (shared ? front : own).partial_ml + 2 * at;
+            m[k] = ml[0];
+            l[k] = ml[1];
+            x[k] = *reinterpret_cast<const fragment*>((shared ? front : own).partial_o + at * HD + d);
+        }
+        float top = M;
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) top = fmaxf(top, m[k]); // (repeated ones do not matter)
+        const float keep = __builtin_amdgcn_exp2f(M - top);
+        M = top;
+        L *= keep;
+        O *= keep;
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            if (begin + W * k >= count) break;
+            const float weight = __builtin_amdgcn_exp2f(m[k] - M);
+            L += weight * l[k];
+            O += weight * x[k];
+        }
+    }
+    if constexpr (W > 1) {
+        if (lane == 0) {
+            m_s[wave] = M;
+            l_s[wave] = L;
+        }
+        o_s[wave][lane] = O;
+        __syncthreads();
+        if (wave != 0) return;
+        L = 0.0f;
+        O = fragment{};
+#pragma unroll
+        for (int w = 0; w < W; ++w) M = fmaxf(M, m_s[w]);
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const float weight = __builtin_amdgcn_exp2f(m_s[w] - M);
+            L += weight * l_s[w];
+            O += weight * o_s[w][lane];
+        }
+    }
+    if (lane * PER < HD) *reinterpret_cast<fragment*>(p.out + (static_cast<int64_t>(merge.token) * p.H + h) * HD + d) = O / L;
+}
+
+template <typename KT, int HD, int QP> int launch_list(const dlk_paged_params& p, const dlk_paged_list& list, hipStream_t stream) {
+    if (list.count == 0) return 0;
+    const dim3 grid(static_cast<unsigned>(list.count) * p.KV);
+    constexpr int FQ = sizeof(KT) == 4 ? 1 : QP; // the f32 instruction takes queries as they are
+    if (list.rows == 16) hipLaunchKernelGGL((paged_few<KT, HD, 1, FQ>), grid, dim3(kThreads), 0, stream, p, list);
+    else if (list.rows == 32) hipLaunchKernelGGL((paged_few<KT, HD, 2, FQ>), grid, dim3(kThreads), 0, stream, p, list);
+    else if (list.rows == 128) hipLaunchKernelGGL((paged_many<KT, HD, QP>), grid, dim3(kThreads), 0, stream, p, list);
+    else return static_cast<int>(hipErrorInvalidValue);
     return static_cast<int>(hipGetLastError());
 }
 
-template <typename KT, int HD>
-int launch_rows(const dlk_paged_params& p, const dlk_paged_item* items, int count, int row_tiles, float* o, float* ml,
-                hipStream_t stream) {
-    if (count == 0) return 0;
-    if (row_tiles == 1) return launch_stream<KT, HD, 1>(p, items, count, o, ml, stream);
-    return static_cast<int>(hipErrorInvalidValue);
-}
-
 template <typename KT, int HD> int launch(const dlk_paged_params& p, hipStream_t stream) {
-    int status = launch_rows<KT, HD>(p, p.shared_items, p.shared_count, p.shared_row_tiles, p.shared_o, p.shared_ml, stream);
-    if (status == 0) status = launch_rows<KT, HD>(p, p.items, p.item_count, p.row_tiles, p.partial_o, p.partial_ml, stream);
-    if (status != 0 || p.merge_count == 0) return status;
+    for (const int i : {DLK_PAGED_SHARED, DLK_PAGED_MANY, DLK_PAGED_FEW}) {
+        const int status = p.q_bf16 ? launch_list<KT, HD, 1>(p, p.lists[i], stream) : launch_list<KT, HD, 3>(p, p.lists[i], stream);
+        if (status != 0) return status;
+    }
+    if (p.merge_count == 0) return 0;
     const int64_t units = static_cast<int64_t>(p.merge_count) * p.H;
-    hipLaunchKernelGGL((paged_merge<HD>), dim3((units + kWaves - 1) / kWaves), dim3(kThreads), 0, stream, p);
+    // up to 8 splits are one round trip of one wave (a work-group per row took prompts of 2100 tokens 47 us, this 15)
+    if (p.merge_most <= 8) hipLaunchKernelGGL((paged_merge<HD, 1>), dim3(static_cast<unsigned>((units + kWaves - 1) / kWaves)), dim3(kThreads), 0, stream, p);
+    else hipLaunchKernelGGL((paged_merge<HD, kWaves>), dim3(static_cast<unsigned>(units)), dim3(kThreads), 0, stream, p);
     return static_cast<int>(hipGetLastError());
 }
 

@@ -289,9 +289,21 @@ typedef struct dlk_paged_item {
     int32_t slot;            /* partials slot, or -1: the item is all that its rows see, and writes the output */
 } dlk_paged_item;
 
+/* Items of one kind of work-group, and where their partials go.  rows: the most rows of an item, 16 or 32 (the waves of a
+   work-group split its keys) or 128 (they split its rows). */
+typedef struct dlk_paged_list {
+    const dlk_paged_item* items;
+    int count, rows;
+    float* partial_o;        /* [slots, KV, rows, hd] */
+    float* partial_ml;       /* [slots, KV, rows, 2]: base (a power of two) and sum */
+} dlk_paged_list;
+
+enum { DLK_PAGED_FEW = 0, DLK_PAGED_MANY = 1, DLK_PAGED_SHARED = 2 };
+
 /* One token whose rows several items share. */
 typedef struct dlk_paged_merge {
     int32_t token, row;      /* the token, and its first row within its run */
+    int32_t list;            /* its run's list (DLK_PAGED_FEW or DLK_PAGED_MANY) */
     int32_t slot, stride;    /* the slot of the run's first row tile, and the slots of each row tile */
     int32_t count;           /* the first of them that hold keys the row sees */
     int32_t shared_row;      /* the token's first row within the prefix run */
@@ -307,17 +319,10 @@ typedef struct dlk_paged_params {
     float scale;
     const int32_t* tables;
     float* out;              /* [tokens, H, hd] */
-    const dlk_paged_item* items;
-    int item_count, row_tiles; /* 16-row tiles of an item: 1, 2 or 4 */
-    float* partial_o;        /* [slots, KV, 16 * row_tiles, hd] */
-    float* partial_ml;       /* [slots, KV, 16 * row_tiles, 2]: maximum (base 2) and sum */
-    /* the items of a prefix that the whole batch shares: rows of all tokens */
-    const dlk_paged_item* shared_items;
-    int shared_count, shared_row_tiles, shared_splits;
-    float* shared_o;
-    float* shared_ml;
+    dlk_paged_list lists[3]; /* runs of few rows, of many, and the prefix that the whole batch shares */
+    int shared_splits;       /* slots of each row tile of the prefix (0: none) */
     const dlk_paged_merge* merges;
-    int merge_count;
+    int merge_count, merge_most; /* merges, and the most partials of one */
 } dlk_paged_params;
 int dlk_paged_attention(const dlk_paged_params* p, dlh_stream stream);
 

@@ -33,14 +33,35 @@ PagedKVCache::PagedKVCache(Index layers, Index pages, Index page_size, Index kv_
 
 namespace {
 
-constexpr Index kTileKeys = 32, kWaveTiles = 4 * kTileKeys; // keys of a wave's tile, and of a work-group's four
+// Rows of a work-group for a run of `rows`: 16 or 32, whose waves split the keys, or 128, which they split.
+Index rows_for(Index rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 128; }
 
-Index round_up(Index value, Index to) { return (value + to - 1) / to * to; }
-
-// Keys per item where the row tiles see `total` keys in all: about `wanted` work-groups over the KV heads, of two rounds of
-// the four waves' tiles at least.
-Index chunk_of(Index total, Index kv_heads, Index wanted) {
-    return std::max<Index>(2 * kWaveTiles, round_up((total * kv_heads + wanted - 1) / wanted, kWaveTiles));
+// Keys per item of a list whose row tiles see `seen` keys each, for every KV head.  Times in keys that a work-group
+// takes in while all others run too, about 20 a microsecond for every kernel and type: an item costs its keys and 60
+// to begin; the list ends when the work-groups that fit the device have had their share, half an item later on
+// average; a merge costs 100 for its launch (unless there is one anyway) and its partials' bytes written and read.
+Index chunk_of(const std::vector<Index>& seen, Index kv_heads, Index head_dim, Index rows, Index used_rows, bool merged) {
+    if (seen.empty()) return 256;
+    const double groups = 256.0 * (rows == 128 || head_dim == 128 ? 2 : 4); // work-groups that fit the device
+    const Index longest = *std::max_element(seen.begin(), seen.end());
+    double best = 0.0;
+    Index chosen = 0;
+    for (Index chunk = 128, step = 1;; chunk += 128 * step) {
+        double work = 0.0, items = 0.0, partials = 0.0;
+        for (const Index keys : seen) {
+            const double n = static_cast<double>((keys + chunk - 1) / chunk);
+            work += static_cast<double>(keys);
+            items += n;
+            if (n > 1.0 || merged) partials += n;
+        }
+        const double heads = static_cast<double>(kv_heads), most = static_cast<double>(std::min(chunk, longest));
+        double time = std::max(most + 60.0, (work + 60.0 * items) * heads / groups + most / 2);
+        if (partials > 0.0)
+            time += (merged ? 0.0 : 100.0) + partials * heads * static_cast<double>(used_rows * head_dim * 8) / 4.5e6 * 20.0;
+        if (chosen == 0 || time < best) best = time, chosen = chunk;
+        if (chunk >= longest) return chosen;
+        if (chunk >= 1024 * step) step *= 2;
+    }
 }
 
 } // namespace
@@ -102,14 +123,27 @@ PagedBatch::PagedBatch(const PagedKVCache& cache, Index heads, std::span<const I
     plan->tokens = tokens;
 
     // the runs' rows over their own keys (behind the shared ones), split where that gives more work-groups
-    const Index rows_of = 16 * plan->row_tiles;
-    Index total = 0;
+    auto& lists = plan->lists;
+    lists[DLK_PAGED_FEW].rows = 16;
+    lists[DLK_PAGED_MANY].rows = 128;
+    const auto list_of = [&](Index b) { return rows_for(counts[b] * group) == 128 ? DLK_PAGED_MANY : DLK_PAGED_FEW; };
+    std::vector<Index> seen[2]; // keys of each row tile
+    Index used_rows[2] = {1, 1};
     for (Index b = 0; b < batch; ++b)
-        if (counts[b] > 0) total += (counts[b] * group + rows_of - 1) / rows_of * (lengths[b] + counts[b] - shared);
-    constexpr Index kWanted = 1024; // work-groups
-    const Index chunk = chunk_of(total, cache.kv_heads(), kWanted);
+        if (counts[b] > 0 && list_of(b) == DLK_PAGED_FEW)
+            lists[DLK_PAGED_FEW].rows = std::max(lists[DLK_PAGED_FEW].rows, rows_for(counts[b] * group));
+    for (Index b = 0; b < batch; ++b) {
+        const int kind = list_of(b);
+        const Index rows = counts[b] * group;
+        for (Index row = 0; row < rows; row += lists[kind].rows)
+            seen[kind].push_back(lengths[b] - shared + (std::min(rows, row + lists[kind].rows) - 1) / group + 1);
+        used_rows[kind] = std::max(used_rows[kind], std::min(rows, lists[kind].rows));
+    }
+    Index chunks[2];
+    for (int kind = 0; kind < 2; ++kind)
+        chunks[kind] = chunk_of(seen[kind], cache.kv_heads(), cache.head_dim(), lists[kind].rows, used_rows[kind], shared > 0);
 
-    std::vector<dlk_paged_item> items, shared_items;
+    std::vector<dlk_paged_item> items[3];
     std::vector<dlk_paged_merge> merges;
     std::vector<Index> positions, places;
     positions.reserve(static_cast<std::size_t>(tokens));
@@ -118,50 +152,59 @@ PagedBatch::PagedBatch(const PagedKVCache& cache, Index heads, std::span<const I
     for (Index b = 0; b < batch; ++b) {
         const Index count = counts[b], first = lengths[b] - shared, keys = first + count, rows = count * group;
         if (count == 0) continue;
-        const Index splits = (keys + chunk - 1) / chunk;
+        const int kind = list_of(b);
+        auto& list = lists[kind];
+        const Index chunk = chunks[kind], splits = (keys + chunk - 1) / chunk;
         const bool whole = splits == 1 && shared == 0;
-        for (Index row = 0; row < rows; row += rows_of) {
-            const Index end = std::min(rows, row + rows_of);
-            const Index seen = first + (end - 1) / group + 1; // keys that the tile's last row sees
-            for (Index s = 0; s < splits && s * chunk < seen; ++s)
-                items.push_back({static_cast<int32_t>(token), static_cast<int32_t>(row), static_cast<int32_t>(end),
-                                 static_cast<int32_t>(b * width + shared / page), static_cast<int32_t>(s * chunk),
-                                 static_cast<int32_t>(std::min(seen, (s + 1) * chunk)), static_cast<int32_t>(first),
-                                 whole ? -1 : static_cast<int32_t>(plan->slots + row / rows_of * splits + s)});
+        for (Index row = 0; row < rows; row += list.rows) {
+            const Index end = std::min(rows, row + list.rows);
+            const Index sees = first + (end - 1) / group + 1; // keys of the tile's last row
+            for (Index s = 0; s < splits && s * chunk < sees; ++s)
+                items[kind].push_back({static_cast<int32_t>(token), static_cast<int32_t>(row), static_cast<int32_t>(end),
+                                       static_cast<int32_t>(b * width + shared / page), static_cast<int32_t>(s * chunk),
+                                       static_cast<int32_t>(std::min(sees, (s + 1) * chunk)), static_cast<int32_t>(first),
+                                       whole ? -1 : static_cast<int32_t>(list.slots + row / list.rows * splits + s)});
         }
         for (Index i = 0; i < count; ++i) {
             const Index position = lengths[b] + i;
             positions.push_back(position);
             places.push_back((tables[b * width + position / page] << shift) + position % page);
             if (!whole)
-                merges.push_back({static_cast<int32_t>(token + i), static_cast<int32_t>(i * group),
-                                  static_cast<int32_t>(plan->slots), static_cast<int32_t>(splits),
+                merges.push_back({static_cast<int32_t>(token + i), static_cast<int32_t>(i * group), kind,
+                                  static_cast<int32_t>(list.slots), static_cast<int32_t>(splits),
                                   static_cast<int32_t>((first + i) / chunk + 1), static_cast<int32_t>((token + i) * group)});
         }
-        if (!whole) plan->slots += (rows + rows_of - 1) / rows_of * splits;
+        if (!whole) list.slots += (rows + list.rows - 1) / list.rows * splits;
         token += count;
     }
     if (shared > 0 && tokens > 0) {
         const Index rows = tokens * group;
-        const Index shared_rows = 16 * plan->shared_row_tiles, tiles = (rows + shared_rows - 1) / shared_rows;
-        const Index part = chunk_of(tiles * shared, cache.kv_heads(), kWanted);
-        const Index splits = (shared + part - 1) / part;
-        plan->shared_splits = static_cast<int>(splits);
+        auto& list = lists[DLK_PAGED_SHARED];
+        list.rows = rows_for(rows);
+        const Index tiles = (rows + list.rows - 1) / list.rows;
+        const Index chunk = chunk_of(std::vector<Index>(static_cast<std::size_t>(tiles), shared), cache.kv_heads(),
+                                     cache.head_dim(), list.rows, std::min(rows, list.rows), true);
+        const Index splits = (shared + chunk - 1) / chunk;
+        plan->shared_splits = splits;
         for (Index s = 0; s < splits; ++s)
             for (Index tile = 0; tile < tiles; ++tile)
-                shared_items.push_back({0, static_cast<int32_t>(tile * shared_rows),
-                                        static_cast<int32_t>(std::min(rows, (tile + 1) * shared_rows)),
-                                        static_cast<int32_t>(front * width), static_cast<int32_t>(s * part),
-                                        static_cast<int32_t>(std::min(shared, (s + 1) * part)), 1 << 30,
-                                        static_cast<int32_t>(tile * splits + s)});
-        plan->shared_slots = tiles * splits;
+                items[DLK_PAGED_SHARED].push_back({0, static_cast<int32_t>(tile * list.rows),
+                                                   static_cast<int32_t>(std::min(rows, (tile + 1) * list.rows)),
+                                                   static_cast<int32_t>(front * width), static_cast<int32_t>(s * chunk),
+                                                   static_cast<int32_t>(std::min(shared, (s + 1) * chunk)), 1 << 30,
+                                                   static_cast<int32_t>(tile * splits + s)});
+        list.slots = tiles * splits;
     }
-    if (std::max<Index>({static_cast<Index>(items.size()), static_cast<Index>(shared_items.size()), plan->slots,
-                         plan->shared_slots}) > INT32_MAX / cache.kv_heads())
-        refuse("too many new positions");
-    plan->item_count = static_cast<Index>(items.size());
-    plan->shared_count = static_cast<Index>(shared_items.size());
+    // the longest first, so that the last work-groups to start are short
+    std::stable_sort(items[DLK_PAGED_MANY].begin(), items[DLK_PAGED_MANY].end(), [](const auto& a, const auto& b) {
+        return a.key_end - a.key_begin > b.key_end - b.key_begin;
+    });
+    for (int i = 0; i < 3; ++i) {
+        lists[i].count = static_cast<Index>(items[i].size());
+        if (std::max(lists[i].count, lists[i].slots) > INT32_MAX / cache.kv_heads()) refuse("too many new positions");
+    }
     plan->merge_count = static_cast<Index>(merges.size());
+    for (const auto& merge : merges) plan->merge_most = std::max<Index>(plan->merge_most, merge.count + plan->shared_splits);
 
     // one copy to the device
     std::vector<std::int32_t> ids(tables.size());
@@ -175,8 +218,7 @@ PagedBatch::PagedBatch(const PagedKVCache& cache, Index heads, std::span<const I
         return at;
     };
     plan->tables = put(ids);
-    plan->items = put(items);
-    plan->shared_items = put(shared_items);
+    for (int i = 0; i < 3; ++i) lists[i].items = put(items[i]);
     plan->merges = put(merges);
     plan->positions = put(positions);
     plan->places = put(places);
@@ -291,25 +333,20 @@ Tensor paged_attention(const nn::PagedKVCache& cache, Index layer, const nn::Pag
     p.scale = static_cast<float>(1.0 / std::sqrt(static_cast<double>(dim)));
     p.tables = plan.at<std::int32_t>(plan.tables);
     p.out = static_cast<float*>(mutable_data(out));
-    p.items = plan.at<dlk_paged_item>(plan.items);
-    p.item_count = static_cast<int>(plan.item_count);
-    p.row_tiles = plan.row_tiles;
-    p.shared_items = plan.at<dlk_paged_item>(plan.shared_items);
-    p.shared_count = static_cast<int>(plan.shared_count);
-    p.shared_row_tiles = plan.shared_row_tiles;
-    p.shared_splits = plan.shared_splits;
+    p.shared_splits = static_cast<int>(plan.shared_splits);
     p.merges = plan.at<dlk_paged_merge>(plan.merges);
     p.merge_count = static_cast<int>(plan.merge_count);
+    p.merge_most = static_cast<int>(plan.merge_most);
     // partials, released to the pool in stream order
-    const Index own_rows = plan.slots * kv * 16 * plan.row_tiles;
-    const Index shared_rows = plan.shared_slots * kv * 16 * plan.shared_row_tiles;
-    Tensor partials;
-    if (own_rows + shared_rows > 0) {
-        partials = empty_tensor({(own_rows + shared_rows) * (dim + 2)}, DType::f32, cache.device());
-        p.partial_o = static_cast<float*>(mutable_data(partials));
-        p.shared_o = p.partial_o + own_rows * dim;
-        p.partial_ml = p.shared_o + shared_rows * dim;
-        p.shared_ml = p.partial_ml + 2 * own_rows;
+    Index rows = 0;
+    for (const auto& list : plan.lists) rows += list.slots * kv * list.rows;
+    Tensor partials = rows > 0 ? empty_tensor({rows * (dim + 2)}, DType::f32, cache.device()) : Tensor{};
+    float* o = rows > 0 ? static_cast<float*>(mutable_data(partials)) : nullptr;
+    float* ml = rows > 0 ? o + rows * dim : nullptr;
+    for (int i = 0; i < 3; ++i) {
+        const auto& list = plan.lists[i];
+        p.lists[i] = {plan.at<dlk_paged_item>(list.items), static_cast<int>(list.count), static_cast<int>(list.rows), o, ml};
+        if (rows > 0) o += list.slots * kv * list.rows * dim, ml += 2 * list.slots * kv * list.rows;
     }
     hip_check(dlk_paged_attention(&p, context.stream), name);
     return out;

@@ -14,11 +14,13 @@ struct PagedBatch::Plan {
     Device device;
 
     Index tokens = 0, last = -1; // new positions, and the largest of them
-    int row_tiles = 1, shared_row_tiles = 1, shared_splits = 0;
-    Index slots = 0, shared_slots = 0; // of partials
-    Index item_count = 0, shared_count = 0, merge_count = 0;
+    struct List {
+        Index rows = 16, count = 0, slots = 0; // rows of an item, items, slots of partials
+        std::size_t items = 0;                 // where the items are
+    } lists[3];                                // by DLK_PAGED_FEW, DLK_PAGED_MANY, DLK_PAGED_SHARED
+    Index shared_splits = 0, merge_count = 0, merge_most = 0;
     Tensor blob; // the arrays below, on the device
-    std::size_t tables = 0, items = 0, shared_items = 0, merges = 0, positions = 0, places = 0; // byte offsets
+    std::size_t tables = 0, merges = 0, positions = 0, places = 0; // byte offsets
     template <class T> const T* at(std::size_t offset) const {
         return reinterpret_cast<const T*>(blob.data<char>() + offset);
     }

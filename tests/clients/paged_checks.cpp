@@ -62,14 +62,17 @@ int plan(char** arg) {
     // seen[row]: the keys (positions) that the items give the row, per slot; whole: rows whose output an item writes
     using Keys = std::vector<char>;
     std::map<std::pair<Index, Index>, Keys> whole;                      // (token, g)
-    std::map<std::pair<Index, Index>, std::pair<std::pair<Index, Index>, Keys>> own, prefix; // (slot, r) -> row, keys
-    auto walk = [&](const dlk_paged_item* items, Index count, int row_tiles, Index slots, bool front, auto& partials) {
-        const Index rows = 16 * row_tiles;
-        for (Index n = 0; n < count; ++n) {
+    std::map<std::pair<Index, Index>, std::pair<std::pair<Index, Index>, Keys>> partials[3]; // (slot, r) -> row, keys
+    for (int kind = 0; kind < 3; ++kind) {
+        const auto& list = p.lists[kind];
+        const auto* items = p.at<dlk_paged_item>(list.items);
+        const Index rows = list.rows;
+        const bool front = kind == DLK_PAGED_SHARED;
+        for (Index n = 0; n < list.count; ++n) {
             const dlk_paged_item& i = items[n];
             expect(i.row_begin % rows == 0 && i.row_end > i.row_begin && i.row_end - i.row_begin <= rows, "rows of an item");
             expect(i.key_begin >= 0 && i.key_begin % 32 == 0 && i.key_end > i.key_begin, "keys of an item");
-            expect(i.slot >= -1 && i.slot < slots, "slot");
+            expect(i.slot >= -1 && i.slot < list.slots, "slot");
             for (Index r = i.row_begin; r < i.row_end; ++r) {
                 const Index token = i.token + r / G;
                 expect(token >= 0 && token < T, "token of a row");
@@ -85,7 +88,7 @@ int plan(char** arg) {
                 }
                 const auto row = std::pair(token, r % G);
                 if (i.slot < 0) expect(whole.emplace(row, keys).second, "output written twice");
-                else expect(partials.emplace(std::pair<Index, Index>(i.slot, r % rows), std::pair(row, keys)).second, "slot written twice");
+                else expect(partials[kind].emplace(std::pair<Index, Index>(i.slot, r % rows), std::pair(row, keys)).second, "slot written twice");
             }
             // the pages that the item's loads may touch, to the end of its last tile's live keys
             for (Index key = i.key_begin; key < i.key_end; ++key) {
@@ -93,31 +96,30 @@ int plan(char** arg) {
                 expect(id >= 0 && id < pages, "page of an item");
             }
         }
-    };
-    walk(p.at<dlk_paged_item>(p.items), p.item_count, p.row_tiles, p.slots, false, own);
-    walk(p.at<dlk_paged_item>(p.shared_items), p.shared_count, p.shared_row_tiles, p.shared_slots, true, prefix);
+    }
     const auto* merges = p.at<dlk_paged_merge>(p.merges);
     for (Index n = 0; n < p.merge_count; ++n) {
         const dlk_paged_merge& m = merges[n];
         for (Index g = 0; g < G; ++g) {
             Keys keys(static_cast<std::size_t>(position[m.token]) + 1, 0);
-            auto add = [&](const auto& partials, Index slot, Index r) {
-                const auto found = partials.find({slot, r});
-                expect(found != partials.end(), "merge of a slot that nobody writes");
+            auto add = [&](int kind, Index slot, Index r) {
+                const auto found = partials[kind].find({slot, r});
+                expect(found != partials[kind].end(), "merge of a slot that nobody writes");
                 expect(found->second.first == std::pair<Index, Index>(m.token, g), "merge of another row's slot");
                 for (std::size_t k = 0; k < keys.size(); ++k) keys[k] += found->second.second[k];
             };
-            const Index rows = 16 * p.row_tiles, row = m.row + g, shared_rows = 16 * p.shared_row_tiles, front = m.shared_row + g;
-            for (Index s = 0; s < m.count; ++s) add(own, m.slot + row / rows * m.stride + s, row % rows);
-            for (Index s = 0; s < p.shared_splits; ++s) add(prefix, front / shared_rows * p.shared_splits + s, front % shared_rows);
+            expect(m.list == DLK_PAGED_FEW || m.list == DLK_PAGED_MANY, "list of a merge");
+            const Index rows = p.lists[m.list].rows, row = m.row + g, shared_rows = p.lists[DLK_PAGED_SHARED].rows, front = m.shared_row + g;
+            for (Index s = 0; s < m.count; ++s) add(m.list, m.slot + row / rows * m.stride + s, row % rows);
+            for (Index s = 0; s < p.shared_splits; ++s) add(DLK_PAGED_SHARED, front / shared_rows * p.shared_splits + s, front % shared_rows);
             expect(whole.emplace(std::pair(Index(m.token), g), keys).second, "output written twice");
         }
     }
     expect(static_cast<Index>(whole.size()) == T * G, "row without an output");
     for (const auto& [row, keys] : whole)
         for (char n : keys) expect(n == 1, "key left out or seen twice");
-    std::printf("%lld %lld %lld %lld\n", static_cast<long long>(T), static_cast<long long>(p.item_count),
-                static_cast<long long>(p.shared_count), static_cast<long long>(p.merge_count));
+    std::printf("%lld %lld %lld %lld\n", static_cast<long long>(T), static_cast<long long>(p.lists[0].count + p.lists[1].count),
+                static_cast<long long>(p.lists[2].count), static_cast<long long>(p.merge_count));
     return 0;
 }
 
