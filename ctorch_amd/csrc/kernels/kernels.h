@@ -342,14 +342,15 @@ int dlk_sample_finalize(const dlk_sample_partial* partial, int64_t rows, int blo
 /* ------------------------------------------------------------------------------------------------------
  * Verification of drafted tokens (verify.hip): target [batch, drafts + 1, vocabulary], draft [batch, drafts, vocabulary]
  * or NULL, uniforms [batch, drafts + 1], all f32 contiguous; drafted [batch, drafts], a negative id ends a row.
- * inverse = 1 / temperature, or 0: the largest logit decides.
+ * inverse = 1 / temperature (at most 1e30), or 0: the largest logit decides.
  * ---------------------------------------------------------------------------------------------------- */
-typedef struct dlk_verify_row { /* one row of logits: its largest, the sum of exp((l - largest) / T), the largest's index */
+typedef struct dlk_verify_slice { /* a slice of a row of logits: its largest, and the sum of exp((l - largest) / T) */
     double sum;
     float largest;
-    int32_t index;
-} dlk_verify_row;
+    int32_t index;           /* of the largest (greedy verification only) */
+} dlk_verify_slice;
 
+#define DLK_VERIFY_DRAW 1024
 typedef struct dlk_verify_params {
     const int64_t* drafted;
     const float* target;
@@ -357,10 +358,18 @@ typedef struct dlk_verify_params {
     const float* uniforms;
     int64_t batch, drafts, vocabulary;
     double inverse;
-    dlk_verify_row* rows;    /* [batch, 2 drafts + 1]: the target's, then the draft's */
+    int slices;              /* of a row, dlk_verify_slices */
+    int64_t slice;           /* entries of one: slices * slice >= vocabulary */
+    dlk_verify_slice* rows;  /* [batch, 2 drafts + 1, slices]: the target's rows, then the draft's */
+    double* drawn;           /* [batch, ceil(vocabulary / DLK_VERIFY_DRAW), 2]: of the row that is drawn from, per so many
+                                entries, what the target has over a refused draft, and the target's own */
+    double* decisions;       /* [batch, 4]: the largest logit and one over the sum, of the row that is drawn from and of
+                                the refused draft's (-1: none was refused) */
     int64_t* tokens;         /* [batch, drafts + 1]: accepted drafts, the drawn token, -1 */
     int64_t* accepted;       /* [batch] */
 } dlk_verify_params;
+/* Slices of a row, where `rows` rows of logits are read. */
+int dlk_verify_slices(int64_t rows, int64_t vocabulary);
 int dlk_verify(const dlk_verify_params* p, dlh_stream stream);
 /* Keyed Philox: mode 0 uniform [low, high), mode 1 standard normal times scale; output f32 or bf16. */
 int dlk_random(uint64_t seed, uint64_t stream_bits, int64_t count, int mode, double low, double high,

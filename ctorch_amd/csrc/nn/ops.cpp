@@ -469,8 +469,10 @@ std::pair<Tensor, Tensor> verify_drafted(const Tensor& drafted, const Tensor& ta
     Tensor q_logits = draft && temperature > 0.0 ? contiguous_f32(*draft) : Tensor{};
     Tensor tokens = empty_tensor({batch, drafts + 1}, DType::i64, target.device());
     Tensor accepted = empty_tensor({batch}, DType::i64, target.device());
-    Tensor rows = empty_tensor({batch * (2 * drafts + 1), 2}, DType::i64, target.device());
-    static_assert(sizeof(dlk_verify_row) == 16);
+    const int slices = dlk_verify_slices(batch * (drafts + 1 + (q_logits.defined() ? drafts : 0)), vocabulary);
+    const Index parts = (vocabulary + DLK_VERIFY_DRAW - 1) / DLK_VERIFY_DRAW;
+    static_assert(sizeof(dlk_verify_slice) == 16);
+    Tensor work = empty_tensor({batch * (slices * 2 * (2 * drafts + 1) + 2 * parts + 4)}, DType::f64, target.device());
     dlk_verify_params p{};
     p.drafted = ids.data<Index>();
     p.target = p_logits.data<float>();
@@ -479,8 +481,12 @@ std::pair<Tensor, Tensor> verify_drafted(const Tensor& drafted, const Tensor& ta
     p.batch = batch;
     p.drafts = drafts;
     p.vocabulary = vocabulary;
-    p.inverse = temperature > 0.0 ? std::min(1.0 / temperature, 1e300) : 0.0;
-    p.rows = static_cast<dlk_verify_row*>(mutable_data(rows));
+    p.inverse = temperature > 0.0 ? std::min(1.0 / temperature, 1e30) : 0.0;
+    p.slices = slices;
+    p.slice = (vocabulary + slices - 1) / slices;
+    p.rows = static_cast<dlk_verify_slice*>(mutable_data(work));
+    p.drawn = static_cast<double*>(mutable_data(work)) + 2 * batch * slices * (2 * drafts + 1);
+    p.decisions = p.drawn + 2 * batch * parts;
     p.tokens = static_cast<Index*>(mutable_data(tokens));
     p.accepted = static_cast<Index*>(mutable_data(accepted));
     hip_check(dlk_verify(&p, context.stream), "verify_drafted");
