@@ -21,16 +21,17 @@ constexpr int kWaves = 4, kThreads = kWaves * kWave;
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 
 // The nearest bf16 of each value, and the rest (exact): three parts hold all 24 bits.
-template <int PARTS> __device__ __forceinline__ void cut8(f32x8 v, bf16x8 (&part)[PARTS]) {
+// (Kept as words: vectors of bf16 that cross a branch are taken apart into halves.)
+template <int PARTS> __device__ __forceinline__ void cut8(f32x8 v, u32x4 (&part)[PARTS]) {
 #pragma unroll
     for (int i = 0; i < PARTS; ++i) {
-        part[i] = __builtin_convertvector(v, bf16x8);
-        const u32x4 h = __builtin_bit_cast(u32x4, part[i]);
+        const u32x4 h = part[i] = __builtin_bit_cast(u32x4, __builtin_convertvector(v, bf16x8));
         if (i + 1 < PARTS)
             v -= f32x8{__uint_as_float(h.x << 16), __uint_as_float(h.x & 0xffff0000u), __uint_as_float(h.y << 16),
                        __uint_as_float(h.y & 0xffff0000u), __uint_as_float(h.z << 16), __uint_as_float(h.z & 0xffff0000u),
@@ -45,22 +46,40 @@ __device__ __forceinline__ u32x2 cut4(f32x4& v) {
     return u32x2{__builtin_amdgcn_perm(w.y, w.x, 0x07060302u), __builtin_amdgcn_perm(w.w, w.z, 0x07060302u)};
 }
 
-// over the four lanes that hold one row's scores (l, l ^ 16, l ^ 32, l ^ 48)
-template <typename Op> __device__ __forceinline__ float over_row(float x, Op op) {
+__device__ __forceinline__ f32x4 product(u32x4 a, u32x4 b, f32x4 sum) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), sum, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 product(u32x4 a, u32x4 b, f32x16 sum) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), sum, 0, 0, 0);
+}
+
+// over the lanes that hold one row's scores: l and l ^ 32, and of ROWS = 16 rows a wave l ^ 16 and l ^ 48 too
+template <int ROWS, typename Op> __device__ __forceinline__ float over_row(float x, Op op) {
     const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     x = op(__uint_as_float(h[0]), __uint_as_float(h[1]));
+    if constexpr (ROWS == 32) return x;
     const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return op(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
-__device__ __forceinline__ float max_over_row(float x) {
-    return over_row(x, [](float a, float b) { return fmaxf(a, b); });
+template <int ROWS> __device__ __forceinline__ float max_over_row(float x) {
+    return over_row<ROWS>(x, [](float a, float b) { return fmaxf(a, b); });
 }
-__device__ __forceinline__ float sum_over_row(float x) {
-    return over_row(x, [](float a, float b) { return a + b; });
+template <int ROWS> __device__ __forceinline__ float sum_over_row(float x) {
+    return over_row<ROWS>(x, [](float a, float b) { return a + b; });
 }
 
 // the compiler keeps LDS accesses of a wave in order across this (the hardware does by itself)
 __device__ __forceinline__ void wave_order() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local"); }
+
+// What the host wrote for the step, read through the scalar cache: page ids and items are the same for a whole wave, and a
+// vector load of them would make every buffer descriptor behind it a loop over the lanes.
+template <typename T> using Planned = const __attribute__((address_space(4))) T;
+template <typename T> __device__ __forceinline__ Planned<T>* planned(const T* pointer) { return (Planned<T>*)(pointer); }
+
+__device__ __forceinline__ dlk_paged_item item_of(const dlk_paged_list& list, int n) {
+    Planned<dlk_paged_item>* from = planned(list.items) + n;
+    return {from->token, from->row_begin, from->row_end, from->table, from->key_begin, from->key_end, from->first, from->slot};
+}
 
 // 8 entries of a query row, unscaled
 __device__ __forceinline__ f32x8 query8(const dlk_paged_params& p, int64_t at) {
@@ -86,29 +105,42 @@ constexpr float kNoBase = -1e30f;
 // How far (in powers of two) a score may lie above its row's base before the base follows.
 constexpr float kSlack = 8.0f;
 
-// One row's weights exp2(s c - base) out of 4 N scores of its lane, and the lane's share of their sum.  The base need not be
-// the row's maximum: f32 weights up to 2^8 are as exact, so it moves only when a score passes it by more, mostly once, and
-// the row's lanes do not have to compare their scores before that.  `outputs` are then scaled to the new base.
-template <int N, int D> __device__ __forceinline__ void soften(f32x4 (&s)[N], float& base, float& l, float c, f32x4 (&outputs)[D]) {
-    float top = s[0][0];
+// The softmax of T rows a lane: base[i] is what row i's weights exp2(s c - base) are taken from, l[i] the lane's share of
+// their sum.  The base need not be the row's maximum: f32 weights up to 2^8 are as exact, so it moves only when a score
+// passes it by more, mostly once, and the row's lanes do not have to compare their scores before that.  S: a vector of a
+// row's scores, N of them; O: one of a row's outputs, D of them.
+template <int ROWS, int T, int N, int D, typename S, typename O>
+__device__ __forceinline__ void settle(const S (&s)[T][N], float (&base)[T], float (&l)[T], float c, O (&outputs)[T][D]) {
+    constexpr int LENGTH = sizeof(S) / 4;
+    float top[T];
+    bool passed = false;
 #pragma unroll
-    for (int i = 0; i < N; ++i)
+    for (int i = 0; i < T; ++i) {
+        top[i] = s[i][0][0];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) top = fmaxf(top, s[i][j]);
-    if (__any(top * c > base + kSlack)) {
-        const float next = fmaxf(base, max_over_row(top) * c);
-        const float keep = __builtin_amdgcn_exp2f(base - next);
-        base = next;
-        l *= keep;
+        for (int u = 0; u < N; ++u)
 #pragma unroll
-        for (int d = 0; d < D; ++d) outputs[d] *= keep;
+            for (int j = 0; j < LENGTH; ++j) top[i] = fmaxf(top[i], s[i][u][j]);
+        passed |= top[i] * c > base[i] + kSlack;
     }
+    if (__any(passed)) {
 #pragma unroll
-    for (int i = 0; i < N; ++i)
+        for (int i = 0; i < T; ++i) {
+            const float next = fmaxf(base[i], max_over_row<ROWS>(top[i]) * c), keep = __builtin_amdgcn_exp2f(base[i] - next);
+            base[i] = next;
+            l[i] *= keep;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            s[i][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][j], c, -base));
-            l += s[i][j];
+            for (int d = 0; d < D; ++d) outputs[i][d] *= keep;
+        }
+    }
+}
+template <int N, typename S> __device__ __forceinline__ void soften(S (&s)[N], float base, float& l, float c) {
+#pragma unroll
+    for (int u = 0; u < N; ++u)
+#pragma unroll
+        for (int j = 0; j < static_cast<int>(sizeof(S) / 4); ++j) {
+            s[u][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][j], c, -base));
+            l += s[u][j];
         }
 }
 
@@ -145,9 +177,9 @@ __global__ __launch_bounds__(kThreads, 2) void paged_few(const dlk_paged_params 
     const int t = threadIdx.x, lane = t % kWave, q = lane / 16, col = lane % 16;
     const int wave = __builtin_amdgcn_readfirstlane(t / kWave);
     const int kvh = static_cast<int>(blockIdx.x) % p.KV;
-    const dlk_paged_item item = list.items[blockIdx.x / p.KV];
+    const dlk_paged_item item = item_of(list, static_cast<int>(blockIdx.x) / p.KV);
     const int G = p.H / p.KV;
-    const int32_t* table = p.tables + item.table;
+    Planned<int32_t>* table = planned(p.tables) + item.table;
     const float c = p.scale * 1.4426950408889634f;
 
     // the item's keys in four runs of whole tiles
@@ -162,7 +194,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_few(const dlk_paged_params 
     // the 16 rows of a half: their place, and how many bytes of them are within the run
     auto half_of = [&](int tile, int u, int& bytes) {
         const int key = w_begin + tile * KEYS + 16 * u;
-        bytes = max(0, min(16, w_end - key)) * ROW;
+        bytes = __builtin_amdgcn_readfirstlane(max(0, min(16, w_end - key)) * ROW);
         const int page = table[min(key, w_end - 1) >> p.page_shift];
         return (((static_cast<int64_t>(page) * p.KV + kvh) << p.page_shift) + (key & ((1 << p.page_shift) - 1))) * HD;
     };
@@ -212,7 +244,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_few(const dlk_paged_params 
     }
 
     // the rows as the right operand: column col of tile nt is row row_begin + 16 nt + col
-    bf16x8 qb[QLDS ? 1 : NT][KS][QP];
+    u32x4 qb[QLDS ? 1 : NT][KS][QP];
     f32x4 qf[NT][KF];
     int limit[NT]; // the last key that the row sees
     uint16_t* q_s = reinterpret_cast<uint16_t*>(area + STAGE);
@@ -230,13 +262,13 @@ __global__ __launch_bounds__(kThreads, 2) void paged_few(const dlk_paged_params 
         } else {
 #pragma unroll
             for (int st = 0; st < KS; ++st) {
-                bf16x8(&parts)[QP] = qb[QLDS ? 0 : nt][st];
+                u32x4(&parts)[QP] = qb[QLDS ? 0 : nt][st];
                 if (QLDS && wave != nt) continue; // wave nt cuts row tile nt for all
                 cut8<QP>(query8(p, at + min(32 * st + 8 * q, HD - 8)), parts);
                 if (QLDS && 8 * q < HD) {
 #pragma unroll
                     for (int part = 0; part < QP; ++part)
-                        *reinterpret_cast<bf16x8*>(q_s + (part * ROWS + 16 * nt + col) * VSTRIDE + 32 * st + 8 * q) = parts[part];
+                        *reinterpret_cast<u32x4*>(q_s + (part * ROWS + 16 * nt + col) * VSTRIDE + 32 * st + 8 * q) = parts[part];
                 }
             }
         }
@@ -289,27 +321,30 @@ __global__ __launch_bounds__(kThreads, 2) void paged_few(const dlk_paged_params 
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int part = QP - 1; part >= 0; --part) {
-                        bf16x8 x = qb[QLDS ? 0 : nt][st][part];
+                        u32x4 x = qb[QLDS ? 0 : nt][st][part];
                         if constexpr (QLDS)
-                            x = *reinterpret_cast<const bf16x8*>(q_s + (part * ROWS + 16 * nt + col) * VSTRIDE + min(32 * st + 8 * q, HD - 8));
+                            x = *reinterpret_cast<const u32x4*>(q_s + (part * ROWS + 16 * nt + col) * VSTRIDE + min(32 * st + 8 * q, HD - 8));
 #pragma unroll
                         for (int u = 0; u < NU; ++u)
-                            s[nt][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k[u][st]), x, s[nt][u], 0, 0, 0);
+                            s[nt][u] = product(k[u][st], x, s[nt][u]);
                     }
             }
         if (tile + 1 < tiles) load_keys(tile + 1);
         const int key0 = w_begin + tile * KEYS;
-        bf16x8 pb[NT][3];
+        u32x4 pb[NT][3];
+        if (key0 + KEYS - 1 > all_see) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            if (key0 + KEYS - 1 > all_see) {
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int u = 0; u < NU; ++u)
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
                         if (key0 + 16 * u + 4 * q + j > limit[nt]) s[nt][u][j] = -INFINITY;
-            }
-            soften(s[nt], base[nt], l[nt], c, o[nt]);
+        }
+        settle<16>(s, base, l, c, o);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            soften(s[nt], base[nt], l[nt], c);
             if constexpr (!F32)
                 cut8<3>(f32x8{s[nt][0][0], s[nt][0][1], s[nt][0][2], s[nt][0][3], s[nt][NU - 1][0], s[nt][NU - 1][1],
                               s[nt][NU - 1][2], s[nt][NU - 1][3]}, pb[nt]);
@@ -333,11 +368,11 @@ __global__ __launch_bounds__(kThreads, 2) void paged_few(const dlk_paged_params 
             for (int dt = 0; dt < DT; ++dt) {
                 const u32x2 a = column4<VSTRIDE>(my_v + 4 * q * VSTRIDE + 16 * dt, col);
                 const u32x2 b = column4<VSTRIDE>(my_v + (16 + 4 * q) * VSTRIDE + 16 * dt, col);
-                const bf16x8 columns = __builtin_bit_cast(bf16x8, u32x4{a.x, a.y, b.x, b.y});
+                const u32x4 columns = {a.x, a.y, b.x, b.y};
 #pragma unroll
                 for (int part = 2; part >= 0; --part)
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) o[nt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(columns, pb[nt][part], o[nt][dt], 0, 0, 0);
+                    for (int nt = 0; nt < NT; ++nt) o[nt][dt] = product(columns, pb[nt][part], o[nt][dt]);
             }
         }
     }
@@ -347,7 +382,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_few(const dlk_paged_params 
     float* o_s = reinterpret_cast<float*>(area);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        const float sum = sum_over_row(l[nt]);
+        const float sum = sum_over_row<16>(l[nt]);
         if (q == 0) {
             m_s[wave][16 * nt + col] = base[nt];
             l_s[wave][16 * nt + col] = sum;
@@ -389,15 +424,19 @@ __global__ __launch_bounds__(kThreads, 2) void paged_few(const dlk_paged_params 
 // ------------------------------------------------------------------------------------------------ many rows
 // 128 rows over a range of keys, 32 a wave, in tiles of 32 keys that pass through LDS for all waves: while one tile is used
 // the next is staged into the other buffer, from the registers that then receive the one after it, so that a tile costs one
-// barrier.  Bound by the matrix cores and the vector ALUs about alike (the weights' parts and the staging).  f32 pages are
-// cut into three bf16 planes as they are staged, once for the 128 rows.
+// barrier.  v_mfma_f32_32x32x16_bf16: a lane holds 16 scores of row lane % 32, of the keys 8 (i / 4) + 4 (lane / 32) + i % 4.
+// (The matrix cores and the vector ALUs, which cut the weights and stage the tiles, have about as much to do here, and the
+// 32 x 32 instruction leaves the vector ALUs more room than two of 16 x 16: three vector instructions beside each of the
+// latter cost 26 % of its rate, beside the former 12 %.)  f32 pages are cut into three bf16 planes as they are staged, once
+// for the 128 rows.
 template <typename KT, int HD, int QP>
 __global__ __launch_bounds__(kThreads, 2) void paged_many(const dlk_paged_params p, const dlk_paged_list list) {
     constexpr bool F32 = sizeof(KT) == 4;
     constexpr int PLANES = F32 ? 3 : 1;
     constexpr int BUFFERS = F32 && HD == 128 ? 1 : 2; // (LDS of two work-groups a CU)
-    constexpr int KEYS = 32, KS = HD < 32 ? 1 : HD / 32, DT = HD / 16;
+    constexpr int KEYS = 32, KS = HD / 16, DT = HD < 32 ? 1 : HD / 32; // (heads of 16: half an output tile is left)
     constexpr int STRIDE = HD + 16;                   // bf16 of a staged row
+    constexpr bool EARLY = HD <= 64;                  // a tile's keys are read ahead of the softmax (registers)
     constexpr int DPP = 16 / static_cast<int>(sizeof(KT)), PIECES = HD / DPP;
     constexpr int ROW = HD * static_cast<int>(sizeof(KT)), ROWS = 128;
     // a half of 16 keys is one piece of memory of BLOCK 16-byte pieces: several passes of all threads, or part of them
@@ -406,12 +445,12 @@ __global__ __launch_bounds__(kThreads, 2) void paged_many(const dlk_paged_params
     __shared__ __attribute__((aligned(16))) uint16_t ks[BUFFERS][PLANES][KEYS * STRIDE];
     __shared__ __attribute__((aligned(16))) uint16_t vs[BUFFERS][PLANES][KEYS * STRIDE];
 
-    const int t = threadIdx.x, lane = t % kWave, q = lane / 16, col = lane % 16;
+    const int t = threadIdx.x, lane = t % kWave, half = lane / 32, r = lane % 32;
     const int wave = __builtin_amdgcn_readfirstlane(t / kWave);
     const int kvh = static_cast<int>(blockIdx.x) % p.KV;
-    const dlk_paged_item item = list.items[blockIdx.x / p.KV];
+    const dlk_paged_item item = item_of(list, static_cast<int>(blockIdx.x) / p.KV);
     const int G = p.H / p.KV;
-    const int32_t* table = p.tables + item.table;
+    Planned<int32_t>* table = planned(p.tables) + item.table;
     const float c = p.scale * 1.4426950408889634f;
     const int tiles = (item.key_end - item.key_begin + KEYS - 1) / KEYS;
 
@@ -419,185 +458,255 @@ __global__ __launch_bounds__(kThreads, 2) void paged_many(const dlk_paged_params
     auto piece_of = [&](int i) { return PASSES ? t + kThreads * (i % (PASSES ? PASSES : 1)) : t % TEAM; };
     const bool loads = PASSES || (t / TEAM < 2 && t % TEAM < BLOCK);
     u32x4 kr[LOADS], vr[LOADS];
-    auto load = [&](int tile) {
+    // the pages of a tile's halves: asked for a tile before the loads that need them
+    struct Pages {
+        int of[2];
+    };
+    auto pages_of = [&](int tile) {
+        const int key = item.key_begin + tile * KEYS;
+        return Pages{{table[min(key, item.key_end - 1) >> p.page_shift], table[min(key + 16, item.key_end - 1) >> p.page_shift]}};
+    };
+    auto load = [&](int tile, const Pages& pages, const void* pool, u32x4 (&to)[LOADS]) {
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
             const int key = item.key_begin + tile * KEYS + 16 * half_of(i);
-            const int bytes = loads ? max(0, min(16, item.key_end - key)) * ROW : 0; // what lies behind reads as zero
-            const int page = table[min(key, item.key_end - 1) >> p.page_shift];
+            const int bytes = __builtin_amdgcn_readfirstlane(max(0, min(16, item.key_end - key)) * ROW); // what lies behind reads as zero
+            const int page = half_of(i) == 0 ? pages.of[0] : pages.of[1];
             const int64_t at = (((static_cast<int64_t>(page) * p.KV + kvh) << p.page_shift) + (key & ((1 << p.page_shift) - 1))) * HD;
-            const int whole = __builtin_amdgcn_readfirstlane(bytes);
-            const int offset = loads ? 16 * piece_of(i) : INT32_MAX / 2;
-            kr[i] = __builtin_amdgcn_raw_buffer_load_b128(
-                __builtin_amdgcn_make_buffer_rsrc(const_cast<KT*>(static_cast<const KT*>(p.k)) + at, 0, whole, kBufferFlags), offset, 0, 0);
-            vr[i] = __builtin_amdgcn_raw_buffer_load_b128(
-                __builtin_amdgcn_make_buffer_rsrc(const_cast<KT*>(static_cast<const KT*>(p.v)) + at, 0, whole, kBufferFlags), offset, 0, 0);
+            to[i] = __builtin_amdgcn_raw_buffer_load_b128(
+                __builtin_amdgcn_make_buffer_rsrc(const_cast<KT*>(static_cast<const KT*>(pool)) + at, 0, bytes, kBufferFlags),
+                loads ? 16 * piece_of(i) : INT32_MAX / 2, 0, 0);
         }
     };
-    auto stage = [&](int buffer) {
+    auto stage = [&](const u32x4 (&from)[LOADS], uint16_t (&planes)[PLANES][KEYS * STRIDE]) {
         if (!loads) return;
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
             const int to = (16 * half_of(i) + piece_of(i) / PIECES) * STRIDE + DPP * (piece_of(i) % PIECES);
             if constexpr (F32) {
-                f32x4 a = __builtin_bit_cast(f32x4, kr[i]), b = __builtin_bit_cast(f32x4, vr[i]);
+                f32x4 x = __builtin_bit_cast(f32x4, from[i]);
 #pragma unroll
-                for (int plane = 0; plane < PLANES; ++plane) {
-                    *reinterpret_cast<u32x2*>(&ks[buffer][plane][to]) = cut4(a);
-                    *reinterpret_cast<u32x2*>(&vs[buffer][plane][to]) = cut4(b);
-                }
+                for (int plane = 0; plane < PLANES; ++plane) *reinterpret_cast<u32x2*>(&planes[plane][to]) = cut4(x);
             } else {
-                *reinterpret_cast<u32x4*>(&ks[buffer][0][to]) = kr[i];
-                *reinterpret_cast<u32x4*>(&vs[buffer][0][to]) = vr[i];
+                *reinterpret_cast<u32x4*>(&planes[0][to]) = from[i];
             }
         }
     };
-    load(0);
+    auto load_keys = [&](int tile, const Pages& pages) { load(tile, pages, p.k, kr); };
+    auto load_values = [&](int tile, const Pages& pages) { load(tile, pages, p.v, vr); };
+    auto stage_keys = [&](int buffer) { stage(kr, ks[buffer]); };
+    auto stage_values = [&](int buffer) { stage(vr, vs[buffer]); };
+    Pages pages = pages_of(0);
+    load_keys(0, pages);
+    load_values(0, pages);
+    pages = pages_of(1);
 
-    // this lane's two rows: row_begin + 32 wave + 16 nt + col
-    bf16x8 qb[2][KS][QP];
-    int limit[2];
-    const int first_row = item.row_begin + 32 * wave;
+    // this lane's row
+    u32x4 qb[KS][QP];
+    const int first_row = item.row_begin + 32 * wave, row = min(first_row + r, item.row_end - 1);
+    const int limit = min(item.first + row / G, item.key_end - 1);
+    const int64_t query = (item.token + row / G) * p.q_row + static_cast<int64_t>(kvh * G + row % G) * p.q_head;
 #pragma unroll
-    for (int nt = 0; nt < 2; ++nt) {
-        const int row = min(first_row + 16 * nt + col, item.row_end - 1);
-        limit[nt] = min(item.first + row / G, item.key_end - 1);
-        const int64_t at = (item.token + row / G) * p.q_row + static_cast<int64_t>(kvh * G + row % G) * p.q_head;
-#pragma unroll
-        for (int st = 0; st < KS; ++st) cut8<QP>(query8(p, at + min(32 * st + 8 * q, HD - 8)), qb[nt][st]);
-    }
+    for (int st = 0; st < KS; ++st) cut8<QP>(query8(p, query + 16 * st + 8 * half), qb[st]);
     // the last key that every row of the wave sees, and the last that any does
     const int all_see = min(item.first + min(first_row, item.row_end - 1) / G, item.key_end - 1);
     const int any_sees = first_row < item.row_end ? min(item.first + min(first_row + 31, item.row_end - 1) / G, item.key_end - 1) : -1;
 
-    f32x4 o[2][DT];
-    float base[2] = {kNoBase, kNoBase}, l[2] = {0.0f, 0.0f};
+    f32x16 o[1][DT];
+    float base[1] = {kNoBase}, l[1] = {0.0f};
 #pragma unroll
-    for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-        for (int d = 0; d < DT; ++d) o[nt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int d = 0; d < DT; ++d) o[0][d] = f32x16{};
 
-    auto use = [&](int tile, int buffer) {
-        const int key0 = item.key_begin + tile * KEYS;
-        if (key0 > any_sees) return;
-        f32x4 s[2][2]; // [row tile][16-key half]
+    auto key_of = [&](int buffer, int st, int plane) {
+        return *reinterpret_cast<const u32x4*>(&ks[buffer][plane][r * STRIDE + 16 * st + 8 * half]);
+    };
+    auto read_keys = [&](int buffer, u32x4 (&to)[KS][PLANES]) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            s[0][u] = s[1][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int st = 0; st < KS; ++st)
 #pragma unroll
-            for (int st = 0; st < KS; ++st)
+            for (int plane = 0; plane < PLANES; ++plane) to[st][plane] = key_of(buffer, st, plane);
+    };
+    auto score = [&](int buffer, const u32x4 (&read)[KS][PLANES], f32x16& s) {
+        s = f32x16{};
 #pragma unroll
-                for (int plane = PLANES - 1; plane >= 0; --plane) {
-                    bf16x8 k = *reinterpret_cast<const bf16x8*>(&ks[buffer][plane][(16 * u + col) * STRIDE + (HD < 32 ? 8 * (q % 2) : 32 * st + 8 * q)]);
-                    if (HD < 32 && q >= 2) k = __builtin_bit_cast(bf16x8, u32x4{0u, 0u, 0u, 0u});
+        for (int st = 0; st < KS; ++st)
 #pragma unroll
-                    for (int part = QP - 1; part >= 0; --part)
-                        if (part + plane <= 2)
+            for (int plane = PLANES - 1; plane >= 0; --plane) {
+                const u32x4 k = EARLY ? read[st][plane] : key_of(buffer, st, plane);
 #pragma unroll
-                            for (int nt = 0; nt < 2; ++nt) s[nt][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, qb[nt][st][part], s[nt][u], 0, 0, 0);
-                }
-        }
-        bf16x8 pb[2][3];
-#pragma unroll
-        for (int nt = 0; nt < 2; ++nt) {
-            if (key0 + KEYS - 1 > all_see) {
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (key0 + 16 * u + 4 * q + j > limit[nt]) s[nt][u][j] = -INFINITY;
+                for (int part = QP - 1; part >= 0; --part)
+                    if (part + plane <= 2) s = product(k, qb[st][part], s);
             }
-            soften(s[nt], base[nt], l[nt], c, o[nt]);
-            cut8<3>(f32x8{s[nt][0][0], s[nt][0][1], s[nt][0][2], s[nt][0][3], s[nt][1][0], s[nt][1][1], s[nt][1][2], s[nt][1][3]}, pb[nt]);
-        }
+    };
+    auto hide = [&](int tile, f32x16& s) {
+        const int key0 = item.key_begin + tile * KEYS;
+        if (key0 + KEYS - 1 <= all_see) return;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (key0 + 8 * (i / 4) + 4 * half + i % 4 > limit) s[i] = -INFINITY;
+    };
+    auto weigh = [&](f32x16 (&s)[1], u32x4 (&pb)[2][3]) {
+        soften(s, base[0], l[0], c);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+            cut8<3>(f32x8{s[0][8 * u], s[0][8 * u + 1], s[0][8 * u + 2], s[0][8 * u + 3], s[0][8 * u + 4], s[0][8 * u + 5],
+                          s[0][8 * u + 6], s[0][8 * u + 7]}, pb[u]);
+    };
+    // lane (d = 32 dt + r, half) supplies V[keys 16 u + 4 half .. +4 and 8 behind them][d], as its weights lie
+    auto add = [&](int buffer, const u32x4 (&pb)[2][3]) {
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-            for (int plane = PLANES - 1; plane >= 0; --plane) {
-                const uint16_t* block = &vs[buffer][plane][4 * q * STRIDE + 16 * dt];
-                const u32x2 a = column4<STRIDE>(block, col), b = column4<STRIDE>(block + 16 * STRIDE, col);
-                const bf16x8 v = __builtin_bit_cast(bf16x8, u32x4{a.x, a.y, b.x, b.y});
+            for (int u = 0; u < 2; ++u)
 #pragma unroll
-                for (int part = 2; part >= 0; --part)
-                    if (part + plane <= 2)
+                for (int plane = PLANES - 1; plane >= 0; --plane) {
+                    const uint16_t* block = &vs[buffer][plane][(16 * u + 4 * half) * STRIDE + 32 * dt + 16 * (r / 16)];
+                    const u32x2 a = column4<STRIDE>(block, r % 16), b = column4<STRIDE>(block + 8 * STRIDE, r % 16);
+                    const u32x4 v = {a.x, a.y, b.x, b.y};
 #pragma unroll
-                        for (int nt = 0; nt < 2; ++nt) o[nt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, pb[nt][part], o[nt][dt], 0, 0, 0);
-            }
+                    for (int part = 2; part >= 0; --part)
+                        if (part + plane <= 2) o[0][dt] = product(v, pb[u][part], o[0][dt]);
+                }
     };
-    stage(0);
-    if (tiles > 1) load(1);
-    __syncthreads();
-    for (int tile = 0; tile < tiles; ++tile) {
-        if constexpr (BUFFERS == 2) {
-            if (tile + 1 < tiles) stage((tile + 1) % 2);
-            if (tile + 2 < tiles) load(tile + 2);
-            use(tile, tile % 2);
-        } else {
-            use(tile, 0);
-            __syncthreads();
-            if (tile + 1 < tiles) stage(0);
-            if (tile + 2 < tiles) load(tile + 2);
-        }
+    // tiles that some row of the wave sees
+    const int mine = any_sees < item.key_begin ? 0 : min(tiles, (any_sees - item.key_begin) / KEYS + 1);
+    f32x16 s[1][1];
+    u32x4 keys[KS][PLANES];
+    if constexpr (BUFFERS == 2) {
+        // Tile t's weights are worked out while the products of tile t + 1's scores run, and tile t + 1's values and tile
+        // t + 2's keys are staged while those of its outputs do.  (Loads behind the last tile read nothing.)  The buffers'
+        // numbers are constants, so that the compiler sees that the reads and writes of a step are apart.
+        stage_keys(0);
+        load_keys(1, pages);
+        stage_values(0);
+        load_values(1, pages);
+        pages = pages_of(2); // of tile t + 2
         __syncthreads();
+        stage_keys(1);
+        load_keys(2, pages);
+        if (EARLY) read_keys(0, keys);
+        if (mine > 0) score(0, keys, s[0][0]);
+        __syncthreads();
+        auto step = [&](int tile, auto buffer) {
+            constexpr int B = decltype(buffer)::value;
+            const Pages ahead = pages_of(tile + 3);
+            u32x4 pb[2][3];
+            f32x16 next;
+            if (EARLY) read_keys(1 - B, keys);
+            hide(tile, s[0][0]);
+            settle<32>(s, base, l, c, o);
+            score(1 - B, keys, next); // (of no use behind the last tile)
+            weigh(s[0], pb);
+            stage_keys(B);
+            stage_values(1 - B);
+            load_keys(tile + 3, ahead);
+            load_values(tile + 2, pages);
+            add(B, pb);
+            s[0][0] = next;
+            pages = ahead;
+            __syncthreads();
+        };
+        int tile = 0;
+        for (; tile + 1 < mine; tile += 2) {
+            step(tile, std::integral_constant<int, 0>{});
+            step(tile + 1, std::integral_constant<int, 1>{});
+        }
+        if (tile < mine) step(tile++, std::integral_constant<int, 0>{});
+        for (; tile < tiles; ++tile) { // the other waves' tiles
+            const Pages ahead = pages_of(tile + 3);
+            stage_keys(tile % 2);
+            stage_values((tile + 1) % 2);
+            load_keys(tile + 3, ahead);
+            load_values(tile + 2, pages);
+            pages = ahead;
+            __syncthreads();
+        }
+    } else {
+        stage_keys(0);
+        stage_values(0);
+        load_keys(1, pages);
+        load_values(1, pages);
+        __syncthreads();
+        for (int tile = 0; tile < tiles; ++tile) {
+            pages = pages_of(tile + 2);
+            if (tile < mine) {
+                u32x4 pb[2][3];
+                score(0, keys, s[0][0]);
+                hide(tile, s[0][0]);
+                settle<32>(s, base, l, c, o);
+                weigh(s[0], pb);
+                add(0, pb);
+            }
+            __syncthreads();
+            stage_keys(0);
+            stage_values(0);
+            load_keys(tile + 2, pages);
+            load_values(tile + 2, pages);
+            __syncthreads();
+        }
     }
 
-    // lane holds O[row col][d = 16 dt + 4 q + j]
+    // lane holds O[row r][d = 32 dt + 8 (i / 4) + 4 half + i % 4]
+    const float sum = sum_over_row<32>(l[0]);
+    if (first_row + r >= item.row_end) return;
+    const bool whole = item.slot < 0;
+    const int64_t at = (static_cast<int64_t>(item.slot) * p.KV + kvh) * ROWS + row - item.row_begin;
+    float* out = whole ? p.out + (static_cast<int64_t>(item.token + row / G) * p.H + kvh * G + row % G) * HD : list.partial_o + at * HD;
+    const float scale = whole ? 1.0f / sum : 1.0f;
 #pragma unroll
-    for (int nt = 0; nt < 2; ++nt) {
-        const int row = first_row + 16 * nt + col;
-        const float sum = sum_over_row(l[nt]);
-        if (row >= item.row_end) continue;
-        if (item.slot < 0) {
-            float* out = p.out + (static_cast<int64_t>(item.token + row / G) * p.H + kvh * G + row % G) * HD;
+    for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(out + 16 * dt + 4 * q) = o[nt][dt] / sum;
-        } else {
-            const int64_t at = (static_cast<int64_t>(item.slot) * p.KV + kvh) * ROWS + row - item.row_begin;
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(list.partial_o + at * HD + 16 * dt + 4 * q) = o[nt][dt];
-            if (q == 0) {
-                list.partial_ml[2 * at] = base[nt];
-                list.partial_ml[2 * at + 1] = sum;
-            }
-        }
+        for (int i = 0; i < 4; ++i)
+            if (32 * dt + 8 * i < HD)
+                *reinterpret_cast<f32x4*>(out + 32 * dt + 8 * i + 4 * half) =
+                    f32x4{o[0][dt][4 * i], o[0][dt][4 * i + 1], o[0][dt][4 * i + 2], o[0][dt][4 * i + 3]} * scale;
+    if (!whole && half == 0) {
+        list.partial_ml[2 * at] = base[0];
+        list.partial_ml[2 * at + 1] = sum;
     }
 }
 
 // ------------------------------------------------------------------------------------------------ the merge
-// Joins the partials of a row: those of the prefix that the batch shares, then those of its own run's splits.  W waves take a
-// (token, query head), each every W-th split, 8 of them asked for at once, rows and sums together.  Bound by the two round
-// trips to memory (the record, the partials), or by the partials' bytes.
+// Joins the partials of a token's rows: those of the prefix that the batch shares, then those of its own run's splits.  16
+// bytes a lane, so that a wave takes 256 / HD heads at once; W waves take the splits in turn, AHEAD of them asked for at once,
+// rows and sums together.  Bound by the two round trips to memory (the record, the partials), or by the partials' bytes.
 template <int HD, int W>
 __global__ __launch_bounds__(kThreads) void paged_merge(const dlk_paged_params p) {
-    constexpr int PER = HD < kWave ? 1 : HD / kWave, AHEAD = 8;
-    typedef float fragment __attribute__((ext_vector_type(PER)));
-    __shared__ float m_s[kWaves], l_s[kWaves];
-    __shared__ fragment o_s[kWaves][kWave];
+    constexpr int LANES = HD / 4, HEADS = kWave / LANES, AHEAD = 8;
+    __shared__ float m_s[kWaves][HEADS], l_s[kWaves][HEADS];
+    __shared__ f32x4 o_s[kWaves][kWave];
     const int t = threadIdx.x, lane = t % kWave, all = __builtin_amdgcn_readfirstlane(t / kWave), wave = all % W;
-    const int64_t unit = min(static_cast<int64_t>(blockIdx.x) * (kWaves / W) + all / W, static_cast<int64_t>(p.merge_count) * p.H - 1);
-    const dlk_paged_merge merge = p.merges[unit / p.H];
-    const int h = static_cast<int>(unit % p.H), G = p.H / p.KV, kvh = h / G;
-    const dlk_paged_list& own = p.lists[merge.list];
+    const uint32_t groups = (p.H + HEADS - 1) / HEADS; // of heads
+    const uint32_t unit = min(blockIdx.x * (kWaves / W) + all / W, p.merge_count * groups - 1);
+    Planned<dlk_paged_merge>* merge = planned(p.merges) + unit / groups;
+    const int token = merge->token, splits = merge->count, shared = p.shared_splits, count = shared + splits;
+    const int h = min(static_cast<int>(unit % groups) * HEADS + lane / LANES, p.H - 1), G = p.H / p.KV, kvh = h / G;
+    const bool many = merge->list == DLK_PAGED_MANY;
+    const dlk_paged_list& few_list = p.lists[DLK_PAGED_FEW];
+    const dlk_paged_list& many_list = p.lists[DLK_PAGED_MANY];
     const dlk_paged_list& front = p.lists[DLK_PAGED_SHARED];
-    const int row = merge.row + h % G, front_row = merge.shared_row + h % G;
-    const int64_t own_step = static_cast<int64_t>(p.KV) * own.rows, front_step = static_cast<int64_t>(p.KV) * front.rows;
-    const int64_t own_at = (static_cast<int64_t>(merge.slot + row / own.rows * merge.stride) * p.KV + kvh) * own.rows + row % own.rows;
-    const int64_t front_at = (static_cast<int64_t>(front_row / front.rows * p.shared_splits) * p.KV + kvh) * front.rows + front_row % front.rows;
-    const int count = p.shared_splits + merge.count, d = min(lane * PER, HD - PER);
+    const int rows = many ? many_list.rows : few_list.rows, row = merge->row + h % G, front_row = merge->shared_row + h % G;
+    const float* own_o = many ? many_list.partial_o : few_list.partial_o;
+    const float* own_ml = many ? many_list.partial_ml : few_list.partial_ml;
+    // where the row's first partials are, in rows, and how far apart
+    const int64_t own_step = static_cast<int64_t>(p.KV) * rows, front_step = static_cast<int64_t>(p.KV) * front.rows;
+    const int64_t own_at = (static_cast<int64_t>(merge->slot + row / rows * merge->stride) * p.KV + kvh) * rows + row % rows;
+    const int64_t front_at = (static_cast<int64_t>(front_row / front.rows * shared) * p.KV + kvh) * front.rows + front_row % front.rows;
+    const int d = lane % LANES * 4;
     float M = kNoBase, L = 0.0f;
-    fragment O = {};
+    f32x4 O = {0.f, 0.f, 0.f, 0.f};
     for (int begin = wave; begin < count; begin += W * AHEAD) {
         float m[AHEAD], l[AHEAD];
-        fragment x[AHEAD];
+        f32x4 x[AHEAD];
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k) {
             const int i = min(begin + W * k, count - 1);
-            const bool shared = i < p.shared_splits;
-            const int64_t at = shared ? front_at + i * front_step : own_at + (i - p.shared_splits) * own_step;
-            const float* ml = (shared ? front : own).partial_ml + 2 * at;
+            const bool in_front = i < shared;
+            const int64_t at = in_front ? front_at + i * front_step : own_at + (i - shared) * own_step;
+            const float* ml = (in_front ? front.partial_ml : own_ml) + 2 * at;
             m[k] = ml[0];
             l[k] = ml[1];
-            x[k] = *reinterpret_cast<const fragment*>((shared ? front : own).partial_o + at * HD + d);
+            x[k] = *reinterpret_cast<const f32x4*>((in_front ? front.partial_o : own_o) + at * HD + d);
         }
         float top = M;
 #pragma unroll
@@ -615,25 +724,25 @@ __global__ __launch_bounds__(kThreads) void paged_merge(const dlk_paged_params p
         }
     }
     if constexpr (W > 1) {
-        if (lane == 0) {
-            m_s[wave] = M;
-            l_s[wave] = L;
+        if (d == 0) {
+            m_s[wave][lane / LANES] = M;
+            l_s[wave][lane / LANES] = L;
         }
         o_s[wave][lane] = O;
         __syncthreads();
         if (wave != 0) return;
         L = 0.0f;
-        O = fragment{};
+        O = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < W; ++w) M = fmaxf(M, m_s[w]);
+        for (int w = 0; w < W; ++w) M = fmaxf(M, m_s[w][lane / LANES]);
 #pragma unroll
         for (int w = 0; w < W; ++w) {
-            const float weight = __builtin_amdgcn_exp2f(m_s[w] - M);
-            L += weight * l_s[w];
+            const float weight = __builtin_amdgcn_exp2f(m_s[w][lane / LANES] - M);
+            L += weight * l_s[w][lane / LANES];
             O += weight * o_s[w][lane];
         }
     }
-    if (lane * PER < HD) *reinterpret_cast<fragment*>(p.out + (static_cast<int64_t>(merge.token) * p.H + h) * HD + d) = O / L;
+    *reinterpret_cast<f32x4*>(p.out + (static_cast<int64_t>(token) * p.H + h) * HD + d) = O / L;
 }
 
 template <typename KT, int HD, int QP> int launch_list(const dlk_paged_params& p, const dlk_paged_list& list, hipStream_t stream) {
@@ -653,8 +762,8 @@ template <typename KT, int HD> int launch(const dlk_paged_params& p, hipStream_t
         if (status != 0) return status;
     }
     if (p.merge_count == 0) return 0;
-    const int64_t units = static_cast<int64_t>(p.merge_count) * p.H;
-    // up to 8 splits are one round trip of one wave (a work-group per row took prompts of 2100 tokens 47 us, this 15)
+    const int64_t heads = 256 / HD, units = p.merge_count * ((p.H + heads - 1) / heads);
+    // up to 8 splits are one round trip of one wave
     if (p.merge_most <= 8) hipLaunchKernelGGL((paged_merge<HD, 1>), dim3(static_cast<unsigned>((units + kWaves - 1) / kWaves)), dim3(kThreads), 0, stream, p);
     else hipLaunchKernelGGL((paged_merge<HD, kWaves>), dim3(static_cast<unsigned>(units)), dim3(kThreads), 0, stream, p);
     return static_cast<int>(hipGetLastError());
