@@ -153,11 +153,23 @@ template <int N, typename S> __device__ __forceinline__ void soften(S (&s)[N], f
 // tiles stay in LDS, where one tile's fit the registers.  f32: no LDS; with the keys of step j of the second product chosen
 // as 4 q + j (q = lane / 16), its right operand is the score register j, and its left one 16 bytes of a V row, whose four
 // entries belong to four output tiles (tile e, row i is head entry 4 i + e).
+template <typename KT, int HD, int NT, int QP> struct Few {
+    static constexpr bool F32 = sizeof(KT) == 4;
+    static constexpr int NU = F32 && HD == 128 ? 1 : 2; // 16-key halves of a tile (f32 heads of 128: registers)
+    static constexpr int KEYS = 16 * NU, ROWS = 16 * NT;
+    static constexpr int VSTRIDE = HD + 16;             // bf16 of a staged V row: the column reads hit no bank twice
+    static constexpr bool QLDS = !F32 && NT > 1;        // the cut queries, in LDS
+    // LDS: V tiles and queries, then the waves' outputs; and the waves' bases and sums
+    static constexpr int STAGE = F32 ? 0 : kWaves * KEYS * VSTRIDE * 2, QUERIES = QLDS ? QP * ROWS * VSTRIDE * 2 : 0;
+    static constexpr int MERGE = kWaves * ROWS * HD * 4;
+    static constexpr int AREA = STAGE + QUERIES > MERGE ? STAGE + QUERIES : MERGE, LDS = AREA + 2 * kWaves * ROWS * 4;
+};
+
 template <typename KT, int HD, int NT, int QP>
-__global__ __launch_bounds__(kThreads, 2) void paged_few(const dlk_paged_params p, const dlk_paged_list list) {
-    constexpr bool F32 = sizeof(KT) == 4;
-    constexpr int NU = F32 && HD == 128 ? 1 : 2;      // 16-key halves of a tile (f32 heads of 128: registers)
-    constexpr int KEYS = 16 * NU, ROWS = 16 * NT;
+__device__ __forceinline__ void attend_few(const dlk_paged_params& p, const dlk_paged_list& list, int block, char* area) {
+    using S = Few<KT, HD, NT, QP>;
+    constexpr bool F32 = S::F32, QLDS = S::QLDS;
+    constexpr int NU = S::NU, KEYS = S::KEYS, ROWS = S::ROWS, VSTRIDE = S::VSTRIDE, STAGE = S::STAGE;
     constexpr int KS = HD < 32 ? 1 : HD / 32;         // bf16: k steps of the score product
     constexpr int KF = HD / 16;                       // f32: 16-byte pieces of a key per lane
     constexpr int DT = HD / 16;                       // output tiles
@@ -165,19 +177,14 @@ __global__ __launch_bounds__(kThreads, 2) void paged_few(const dlk_paged_params 
     constexpr int VL = HD / 16 / E;                   // f32: such loads of a V row
     constexpr int PIECES = HD / 8;                    // bf16: 16-byte pieces of a row
     constexpr int VI = (16 * PIECES + kWave - 1) / kWave; // bf16: V pieces per lane and half
-    constexpr int VSTRIDE = HD + 16;                  // bf16 of a staged V row: the column reads hit no bank twice
     constexpr int ROW = HD * static_cast<int>(sizeof(KT));
-    constexpr bool QLDS = !F32 && NT > 1;             // the cut queries, in LDS
-    constexpr int STAGE = F32 ? 0 : kWaves * KEYS * VSTRIDE * 2, QUERIES = QLDS ? QP * ROWS * VSTRIDE * 2 : 0;
-    constexpr int MERGE = kWaves * ROWS * HD * 4;
-    // V tiles and queries, then the waves' outputs
-    __shared__ __attribute__((aligned(16))) char area[STAGE + QUERIES > MERGE ? STAGE + QUERIES : MERGE];
-    __shared__ float m_s[kWaves][ROWS], l_s[kWaves][ROWS];
+    float(*m_s)[ROWS] = reinterpret_cast<float(*)[ROWS]>(area + S::AREA);
+    float(*l_s)[ROWS] = m_s + kWaves;
 
     const int t = threadIdx.x, lane = t % kWave, q = lane / 16, col = lane % 16;
     const int wave = __builtin_amdgcn_readfirstlane(t / kWave);
-    const int kvh = static_cast<int>(blockIdx.x) % p.KV;
-    const dlk_paged_item item = item_of(list, static_cast<int>(blockIdx.x) / p.KV);
+    const int kvh = block % p.KV;
+    const dlk_paged_item item = item_of(list, block / p.KV);
     const int G = p.H / p.KV;
     Planned<int32_t>* table = planned(p.tables) + item.table;
     const float c = p.scale * 1.4426950408889634f;
@@ -429,26 +436,33 @@ __global__ __launch_bounds__(kThreads, 2) void paged_few(const dlk_paged_params 
 // 32 x 32 instruction leaves the vector ALUs more room than two of 16 x 16: three vector instructions beside each of the
 // latter cost 26 % of its rate, beside the former 12 %.)  f32 pages are cut into three bf16 planes as they are staged, once
 // for the 128 rows.
+template <typename KT, int HD> struct Many {
+    static constexpr int PLANES = sizeof(KT) == 4 ? 3 : 1;
+    static constexpr int BUFFERS = sizeof(KT) == 4 && HD == 128 ? 1 : 2; // (LDS of two work-groups a CU)
+    static constexpr int KEYS = 32, STRIDE = HD + 16;                    // bf16 of a staged row
+    static constexpr int LDS = 2 * BUFFERS * PLANES * KEYS * STRIDE * 2;
+};
+
 template <typename KT, int HD, int QP>
-__global__ __launch_bounds__(kThreads, 2) void paged_many(const dlk_paged_params p, const dlk_paged_list list) {
+__device__ __forceinline__ void attend_many(const dlk_paged_params& p, const dlk_paged_list& list, int block, char* area) {
+    using S = Many<KT, HD>;
     constexpr bool F32 = sizeof(KT) == 4;
-    constexpr int PLANES = F32 ? 3 : 1;
-    constexpr int BUFFERS = F32 && HD == 128 ? 1 : 2; // (LDS of two work-groups a CU)
-    constexpr int KEYS = 32, KS = HD / 16, DT = HD < 32 ? 1 : HD / 32; // (heads of 16: half an output tile is left)
-    constexpr int STRIDE = HD + 16;                   // bf16 of a staged row
+    constexpr int PLANES = S::PLANES, BUFFERS = S::BUFFERS, KEYS = S::KEYS, STRIDE = S::STRIDE;
+    constexpr int KS = HD / 16, DT = HD < 32 ? 1 : HD / 32; // (heads of 16: half an output tile is left)
     constexpr bool EARLY = HD <= 64;                  // a tile's keys are read ahead of the softmax (registers)
     constexpr int DPP = 16 / static_cast<int>(sizeof(KT)), PIECES = HD / DPP;
     constexpr int ROW = HD * static_cast<int>(sizeof(KT)), ROWS = 128;
     // a half of 16 keys is one piece of memory of BLOCK 16-byte pieces: several passes of all threads, or part of them
     constexpr int BLOCK = 16 * PIECES, PASSES = BLOCK / kThreads, LOADS = PASSES ? 2 * PASSES : 1;
     constexpr int TEAM = BLOCK < kWave ? kWave : BLOCK; // threads of a half, where one pass takes both
-    __shared__ __attribute__((aligned(16))) uint16_t ks[BUFFERS][PLANES][KEYS * STRIDE];
-    __shared__ __attribute__((aligned(16))) uint16_t vs[BUFFERS][PLANES][KEYS * STRIDE];
+    typedef uint16_t Planes[PLANES][KEYS * STRIDE];
+    Planes* const ks = reinterpret_cast<Planes*>(area);
+    Planes* const vs = ks + BUFFERS;
 
     const int t = threadIdx.x, lane = t % kWave, half = lane / 32, r = lane % 32;
     const int wave = __builtin_amdgcn_readfirstlane(t / kWave);
-    const int kvh = static_cast<int>(blockIdx.x) % p.KV;
-    const dlk_paged_item item = item_of(list, static_cast<int>(blockIdx.x) / p.KV);
+    const int kvh = block % p.KV;
+    const dlk_paged_item item = item_of(list, block / p.KV);
     const int G = p.H / p.KV;
     Planned<int32_t>* table = planned(p.tables) + item.table;
     const float c = p.scale * 1.4426950408889634f;
@@ -478,7 +492,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_many(const dlk_paged_params
                 loads ? 16 * piece_of(i) : INT32_MAX / 2, 0, 0);
         }
     };
-    auto stage = [&](const u32x4 (&from)[LOADS], uint16_t (&planes)[PLANES][KEYS * STRIDE]) {
+    auto stage = [&](const u32x4 (&from)[LOADS], Planes& planes) {
         if (!loads) return;
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
@@ -666,6 +680,28 @@ __global__ __launch_bounds__(kThreads, 2) void paged_many(const dlk_paged_params
     }
 }
 
+// One launch for all items: the ones of many rows first, which take longest, and beside them those of few, which wait for
+// memory where the others wait for the matrix cores.
+template <typename KT, int HD, int NT, int QP, bool FEW, bool MANY>
+__global__ __launch_bounds__(kThreads, 2) void paged_attend(const dlk_paged_params p) {
+    constexpr int FQ = sizeof(KT) == 4 ? 1 : QP; // the f32 instruction takes queries as they are
+    constexpr int A = FEW ? Few<KT, HD, NT, FQ>::LDS : 0, B = MANY ? Many<KT, HD>::LDS : 0;
+    __shared__ __attribute__((aligned(16))) char area[A > B ? A : B];
+    int block = static_cast<int>(blockIdx.x);
+    const int many = p.lists[DLK_PAGED_MANY].count * p.KV, shared = p.lists[DLK_PAGED_SHARED].count * p.KV;
+    const int kind = block < many ? DLK_PAGED_MANY : block < many + shared ? DLK_PAGED_SHARED : DLK_PAGED_FEW;
+    block -= kind == DLK_PAGED_MANY ? 0 : kind == DLK_PAGED_SHARED ? many : many + shared;
+    const dlk_paged_list list = p.lists[kind];
+    if constexpr (FEW && MANY) {
+        if (list.rows == 128) attend_many<KT, HD, QP>(p, list, block, area);
+        else attend_few<KT, HD, NT, FQ>(p, list, block, area);
+    } else if constexpr (MANY) {
+        attend_many<KT, HD, QP>(p, list, block, area);
+    } else {
+        attend_few<KT, HD, NT, FQ>(p, list, block, area);
+    }
+}
+
 // ------------------------------------------------------------------------------------------------ the merge
 // Joins the partials of a token's rows: those of the prefix that the batch shares, then those of its own run's splits.  16
 // bytes a lane, so that a wave takes 256 / HD heads at once; W waves take the splits in turn, AHEAD of them asked for at once,
@@ -745,22 +781,31 @@ __global__ __launch_bounds__(kThreads) void paged_merge(const dlk_paged_params p
     *reinterpret_cast<f32x4*>(p.out + (static_cast<int64_t>(token) * p.H + h) * HD + d) = O / L;
 }
 
-template <typename KT, int HD, int QP> int launch_list(const dlk_paged_params& p, const dlk_paged_list& list, hipStream_t stream) {
-    if (list.count == 0) return 0;
-    const dim3 grid(static_cast<unsigned>(list.count) * p.KV);
-    constexpr int FQ = sizeof(KT) == 4 ? 1 : QP; // the f32 instruction takes queries as they are
-    if (list.rows == 16) hipLaunchKernelGGL((paged_few<KT, HD, 1, FQ>), grid, dim3(kThreads), 0, stream, p, list);
-    else if (list.rows == 32) hipLaunchKernelGGL((paged_few<KT, HD, 2, FQ>), grid, dim3(kThreads), 0, stream, p, list);
-    else if (list.rows == 128) hipLaunchKernelGGL((paged_many<KT, HD, QP>), grid, dim3(kThreads), 0, stream, p, list);
-    else return static_cast<int>(hipErrorInvalidValue);
+template <typename KT, int HD, int QP> int launch_items(const dlk_paged_params& p, hipStream_t stream) {
+    int64_t blocks = 0;
+    int few = 0; // the most rows of the lists of few
+    bool many = false;
+    for (const dlk_paged_list& list : p.lists) {
+        if (list.count == 0) continue;
+        blocks += static_cast<int64_t>(list.count) * p.KV;
+        if (list.rows == 128) many = true;
+        else if (few != 0 && few != list.rows) return static_cast<int>(hipErrorInvalidValue);
+        else few = list.rows;
+    }
+    if (blocks == 0) return 0;
+    if (blocks > INT32_MAX || (few != 0 && few != 16 && few != 32)) return static_cast<int>(hipErrorInvalidValue);
+    const dim3 grid(static_cast<unsigned>(blocks)), threads(kThreads);
+    if (many && few == 32) hipLaunchKernelGGL((paged_attend<KT, HD, 2, QP, true, true>), grid, threads, 0, stream, p);
+    else if (many && few == 16) hipLaunchKernelGGL((paged_attend<KT, HD, 1, QP, true, true>), grid, threads, 0, stream, p);
+    else if (many) hipLaunchKernelGGL((paged_attend<KT, HD, 1, QP, false, true>), grid, threads, 0, stream, p);
+    else if (few == 32) hipLaunchKernelGGL((paged_attend<KT, HD, 2, QP, true, false>), grid, threads, 0, stream, p);
+    else hipLaunchKernelGGL((paged_attend<KT, HD, 1, QP, true, false>), grid, threads, 0, stream, p);
     return static_cast<int>(hipGetLastError());
 }
 
 template <typename KT, int HD> int launch(const dlk_paged_params& p, hipStream_t stream) {
-    for (const int i : {DLK_PAGED_SHARED, DLK_PAGED_MANY, DLK_PAGED_FEW}) {
-        const int status = p.q_bf16 ? launch_list<KT, HD, 1>(p, p.lists[i], stream) : launch_list<KT, HD, 3>(p, p.lists[i], stream);
-        if (status != 0) return status;
-    }
+    const int status = p.q_bf16 ? launch_items<KT, HD, 1>(p, stream) : launch_items<KT, HD, 3>(p, stream);
+    if (status != 0) return status;
     if (p.merge_count == 0) return 0;
     const int64_t heads = 256 / HD, units = p.merge_count * ((p.H + heads - 1) / heads);
     // up to 8 splits are one round trip of one wave

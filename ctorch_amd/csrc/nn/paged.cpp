@@ -36,28 +36,44 @@ namespace {
 // Rows of a work-group for a run of `rows`: 16 or 32, whose waves split the keys, or 128, which they split.
 Index rows_for(Index rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 128; }
 
-// Keys per item of a list whose row tiles see `seen` keys each, for every KV head.  Times in keys that a work-group
-// takes in while all others run too, about 20 a microsecond for every kernel and type: an item costs its keys and 60
-// to begin; the list ends when the work-groups that fit the device have had their share, half an item later on
-// average; a merge costs 100 for its launch (unless there is one anyway) and its partials' bytes written and read.
-Index chunk_of(const std::vector<Index>& seen, Index kv_heads, Index head_dim, Index rows, Index used_rows, bool merged) {
-    if (seen.empty()) return 256;
-    const double groups = 256.0 * (rows == 128 || head_dim == 128 ? 2 : 4); // work-groups that fit the device
-    const Index longest = *std::max_element(seen.begin(), seen.end());
+// A list whose row tiles see `seen` keys each, for every KV head, and what its work-groups take.
+struct Load {
+    std::vector<Index> seen;
+    Index kv_heads, head_dim, rows, used_rows; // used: the most rows that a tile really has
+    bool f32, merged;                          // merged: its rows are merged anyway (with a prefix)
+};
+
+// Keys per item: the split with the smallest time by this account, in microseconds (measured on MI355X):
+// - `slots` work-groups run at once, and take `rate` keys a microsecond each then: of few rows what memory gives (5.4
+//   TB/s), of many what the matrix cores do (8500 / (products of a pair's entry, twice the head size): 19 keys for bf16 pages
+//   and heads of 64, 12 for heads of 128 or f32 pages); fewer of them run faster, until each CU has one;
+// - an item takes 5 more to begin and to end; the last ones run half an item alone, of many rows, where the longest come
+//   first, an eighth; a work-group of many rows runs a third faster as its neighbours end;
+// - a merge takes 6, and its partials, written and read, their bytes at 1.5 TB/s.
+// (8 sequences of 32768 keys: 64 items of 2048 keys a head 133 us, of 768 124, of 256 139; 3000 new rows after 1000: whole
+// 335 us, in 512 keys 366; four prompts of 310 to 809 rows after 321 to 745, 544 work-groups: whole 103 us, in 1024 keys 115.)
+Index chunk_of(const Load& load) {
+    if (load.seen.empty()) return 256;
+    const bool many = load.rows == 128;
+    const double per_cu = many || load.head_dim == 128 ? 2.0 : 4.0, slots = 256.0 * per_cu, heads = static_cast<double>(load.kv_heads);
+    const double rate = many ? 8500.0 / static_cast<double>(load.head_dim * (load.f32 ? 12 : 6))
+                             : 5.4e6 / (slots * static_cast<double>(load.head_dim * (load.f32 ? 8 : 4)));
+    const Index longest = *std::max_element(load.seen.begin(), load.seen.end());
     double best = 0.0;
     Index chosen = 0;
     for (Index chunk = 128, step = 1;; chunk += 128 * step) {
         double work = 0.0, items = 0.0, partials = 0.0;
-        for (const Index keys : seen) {
+        for (const Index keys : load.seen) {
             const double n = static_cast<double>((keys + chunk - 1) / chunk);
             work += static_cast<double>(keys);
             items += n;
-            if (n > 1.0 || merged) partials += n;
+            if (n > 1.0 || load.merged) partials += n;
         }
-        const double heads = static_cast<double>(kv_heads), most = static_cast<double>(std::min(chunk, longest));
-        double time = std::max(most + 60.0, (work + 60.0 * items) * heads / groups + most / 2);
+        const double most = static_cast<double>(std::min(chunk, longest));
+        const double own = rate * std::clamp(slots / (items * heads), many ? 4.0 / 3.0 : 1.0, per_cu); // a work-group's rate
+        double time = std::max(most / own + 5.0, (work / rate + 5.0 * items) * heads / slots + most / rate / (many ? 8.0 : 2.0));
         if (partials > 0.0)
-            time += (merged ? 0.0 : 100.0) + partials * heads * static_cast<double>(used_rows * head_dim * 8) / 4.5e6 * 20.0;
+            time += (load.merged ? 0.0 : 6.0) + partials * heads * static_cast<double>(load.used_rows * load.head_dim * 8) / 1.5e6;
         if (chosen == 0 || time < best) best = time, chosen = chunk;
         if (chunk >= longest) return chosen;
         if (chunk >= 1024 * step) step *= 2;
@@ -127,21 +143,25 @@ PagedBatch::PagedBatch(const PagedKVCache& cache, Index heads, std::span<const I
     lists[DLK_PAGED_FEW].rows = 16;
     lists[DLK_PAGED_MANY].rows = 128;
     const auto list_of = [&](Index b) { return rows_for(counts[b] * group) == 128 ? DLK_PAGED_MANY : DLK_PAGED_FEW; };
-    std::vector<Index> seen[2]; // keys of each row tile
-    Index used_rows[2] = {1, 1};
     for (Index b = 0; b < batch; ++b)
         if (counts[b] > 0 && list_of(b) == DLK_PAGED_FEW)
             lists[DLK_PAGED_FEW].rows = std::max(lists[DLK_PAGED_FEW].rows, rows_for(counts[b] * group));
-    for (Index b = 0; b < batch; ++b) {
-        const int kind = list_of(b);
-        const Index rows = counts[b] * group;
-        for (Index row = 0; row < rows; row += lists[kind].rows)
-            seen[kind].push_back(lengths[b] - shared + (std::min(rows, row + lists[kind].rows) - 1) / group + 1);
-        used_rows[kind] = std::max(used_rows[kind], std::min(rows, lists[kind].rows));
-    }
+    // a prefix of few rows is taken like the runs of few, in row tiles of one size
+    auto& prefix = lists[DLK_PAGED_SHARED];
+    prefix.rows = rows_for(tokens * group);
+    if (shared > 0 && prefix.rows < 128) lists[DLK_PAGED_FEW].rows = prefix.rows = std::max(prefix.rows, lists[DLK_PAGED_FEW].rows);
     Index chunks[2];
-    for (int kind = 0; kind < 2; ++kind)
-        chunks[kind] = chunk_of(seen[kind], cache.kv_heads(), cache.head_dim(), lists[kind].rows, used_rows[kind], shared > 0);
+    for (int kind = 0; kind < 2; ++kind) {
+        Load load{{}, cache.kv_heads(), cache.head_dim(), lists[kind].rows, 1, cache.dtype() == DType::f32, shared > 0};
+        for (Index b = 0; b < batch; ++b) {
+            if (list_of(b) != kind) continue;
+            const Index rows = counts[b] * group;
+            for (Index row = 0; row < rows; row += load.rows)
+                load.seen.push_back(lengths[b] - shared + (std::min(rows, row + load.rows) - 1) / group + 1);
+            load.used_rows = std::max(load.used_rows, std::min(rows, load.rows));
+        }
+        chunks[kind] = chunk_of(load);
+    }
 
     std::vector<dlk_paged_item> items[3];
     std::vector<dlk_paged_merge> merges;
@@ -179,11 +199,10 @@ PagedBatch::PagedBatch(const PagedKVCache& cache, Index heads, std::span<const I
     }
     if (shared > 0 && tokens > 0) {
         const Index rows = tokens * group;
-        auto& list = lists[DLK_PAGED_SHARED];
-        list.rows = rows_for(rows);
+        auto& list = prefix;
         const Index tiles = (rows + list.rows - 1) / list.rows;
-        const Index chunk = chunk_of(std::vector<Index>(static_cast<std::size_t>(tiles), shared), cache.kv_heads(),
-                                     cache.head_dim(), list.rows, std::min(rows, list.rows), true);
+        const Index chunk = chunk_of({std::vector<Index>(static_cast<std::size_t>(tiles), shared), cache.kv_heads(), cache.head_dim(),
+                                      list.rows, std::min(rows, list.rows), cache.dtype() == DType::f32, true});
         const Index splits = (shared + chunk - 1) / chunk;
         plan->shared_splits = splits;
         for (Index s = 0; s < splits; ++s)
