@@ -436,7 +436,7 @@ extern "C" int dlk_verify_slices(int64_t rows, int64_t vocabulary) {
 
 extern "C" int dlk_verify(const dlk_verify_params* params, dlh_stream stream_handle) {
     const dlk_verify_params& p = *params;
-    if (p.batch < 0 || p.drafts < 0 || p.vocabulary <= 0 || p.vocabulary > INT32_MAX || p.drafts > INT32_MAX || p.slices <= 0 ||
+    if (p.batch < 0 || p.drafts < 0 || p.vocabulary <= 0 || p.vocabulary > INT32_MAX || p.drafts > (1 << 20) || p.slices <= 0 ||
         p.slice <= 0 || p.slice > dlk::kThreads * dlk::kHeld || p.slice * p.slices < p.vocabulary)
         return static_cast<int>(hipErrorInvalidValue);
     if (p.batch == 0) return 0;

@@ -304,6 +304,7 @@ Tensor rotary_positions(const Tensor& input, const Tensor& positions, const Tens
     GpuContext& context = gpu_of(input, "rotary_positions");
     if (input.ndim() != 3) throw std::invalid_argument("rotary_positions: input must be [T, H, D]");
     const Index tokens = input.size(0), heads = input.size(1), dim = input.size(2);
+    if (heads > INT32_MAX / 2 || dim > INT32_MAX / 2) throw std::invalid_argument("rotary_positions: too many heads or entries of a head");
     if (positions.dtype() != DType::i64 || positions.shape() != Shape{tokens})
         throw std::invalid_argument("rotary_positions: positions must be i64 [T]");
     if (!(positions.device() == input.device())) throw std::invalid_argument("rotary_positions: positions on another device");
@@ -454,6 +455,7 @@ std::pair<Tensor, Tensor> verify_drafted(const Tensor& drafted, const Tensor& ta
         throw std::invalid_argument("verify_drafted: target logits must be [B, K + 1, V], got " + shape_string(target.shape()));
     const Index vocabulary = target.size(2);
     if (vocabulary <= 0) throw std::invalid_argument("verify_drafted: empty vocabulary");
+    if (drafts > (1 << 20)) throw std::invalid_argument("verify_drafted: more than 2^20 drafts of a sequence");
     if (draft && draft->shape() != Shape{batch, drafts, vocabulary})
         throw std::invalid_argument("verify_drafted: draft logits must be [B, K, V], got " + shape_string(draft->shape()));
     if (uniforms.dtype() != DType::f32 || uniforms.shape() != Shape{batch, drafts + 1})

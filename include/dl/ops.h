@@ -60,9 +60,9 @@ DL_API Tensor sample(const Tensor& logits, double temperature, RandomKey key);
 /// x = drafted[b, i] is accepted while uniforms[b, i] * q_i(x) < p_i(x).  The next token is drawn with uniforms[b, K]: behind
 /// the last draft from p, at the first refused one from max(p - q, 0) (from p where that is zero), as the first index whose
 /// cumulative weight exceeds uniforms[b, K] times the total.  Without draft logits [B, K, V] a draft was certain: q(x) = 1.  A
-/// temperature <= 0 accepts the target's argmax and nothing else.  An id beyond the vocabulary is refused; a row whose
-/// weights have no positive finite sum (NaN logits) takes its argmax.  Returns tokens [B, K + 1] (the accepted drafts, the drawn token, then -1)
-/// and the number accepted [B], both i64.
+/// temperature <= 0 accepts the target's argmax and nothing else.  A draft beyond the vocabulary is not accepted; a row whose
+/// weights have no positive finite sum (NaN logits) takes its argmax.  K is at most 2^20.  Returns tokens [B, K + 1] (the
+/// accepted drafts, the drawn token, then -1) and the number accepted [B], both i64.
 DL_API std::pair<Tensor, Tensor> verify_drafted(const Tensor& drafted, const Tensor& target,
                                                 const std::optional<Tensor>& draft, double temperature,
                                                 const Tensor& uniforms);

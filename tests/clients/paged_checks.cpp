@@ -184,6 +184,7 @@ int call(const std::string& name) {
         {"rotary type", [&] { dl::rotary_positions(tensor({5, 2, 32}, dl::DType::f64), at, c, s); }},
         {"rotary wide tables", [&] { dl::rotary_positions(tensor({5, 2, 30}), at, c, s); }},
         {"rotary layout", [&] { dl::rotary_positions(x, at, c, s, static_cast<RotaryLayout>(2)); }},
+        {"rotary heads", [&] { dl::rotary_positions(tensor({1, Index(1) << 31, 2}, dl::DType::bf16), tensor({1}, dl::DType::i64), c, s); }},
         {"rotary nothing", [&] { dl::rotary_positions(tensor({0, 2, 32}), tensor({0}, dl::DType::i64), c, s); }},
         {"tables odd", [&] { dl::rotary_tables(7, 4); }},
         {"tables empty", [&] { dl::rotary_tables(8, 0); }},
@@ -200,6 +201,10 @@ int call(const std::string& name) {
         {"verify uniforms", [&] { dl::verify_drafted(ids, target, draft, 1.0, tensor({2, 3})); }},
         {"verify uniforms type", [&] { dl::verify_drafted(ids, target, draft, 1.0, tensor({2, 4}, dl::DType::f64)); }},
         {"verify vocabulary", [&] { dl::verify_drafted(ids, tensor({2, 4, 0}), std::nullopt, 1.0, u); }},
+        {"verify drafts", [&] {
+             const Index n = (1 << 20) + 1;
+             dl::verify_drafted(tensor({1, n}, dl::DType::i64), tensor({1, n + 1, 1}), std::nullopt, 1.0, tensor({1, n + 1}));
+         }},
         {"verify temperature", [&] { dl::verify_drafted(ids, target, draft, inf, u); }},
         {"verify temperature nan", [&] { dl::verify_drafted(ids, target, draft, inf - inf, u); }},
         {"verify logits type", [&] { dl::verify_drafted(ids, tensor({2, 4, 10}, dl::DType::f64), std::nullopt, 1.0, u); }},

@@ -154,3 +154,39 @@ def test_views_are_read_as_they_lie():
     tokens, accepted = ct.verify_drafted(d, t, None, 1.0, gu)
     want = verify(ids[:, 2:5], wide[:, :, 7:57], None, 1.0, u[:, 5:])
     assert np.array_equal(tokens.numpy(), want[0]) and np.array_equal(accepted.numpy(), want[1])
+
+
+def test_long_rows_of_nothing_but_few_entries():
+    """A vocabulary of many slices and parts whose weight lies in a few entries far apart, and many drafts of a sequence."""
+    rng = np.random.default_rng(8)
+    V = 200001
+    target = np.full((2, 3, V), -np.inf, np.float32)
+    draft = np.full((2, 2, V), -np.inf, np.float32)
+    for b in range(2):
+        for i in range(3):
+            target[b, i, [70000, 130000 + i, V - 1]] = rng.standard_normal(3)
+        draft[b, :, [70000, 150000]] = 0.5
+    for u in (0.0, 0.3, 0.6, 0.95):
+        numbers = np.full((2, 3), u, np.float32)
+        for given in (draft, None):
+            for ids in ([70000, 150000], [150000, 70000]):
+                drafted = np.array([ids, ids])
+                want = verify(drafted, target, given, 1.0, numbers)
+                got = run(drafted, target, given, 1.0, numbers)
+                assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1]), (u, ids)
+    K = 300  # more than one round of comparisons
+    logits = rng.standard_normal((2, K + 1, 7)).astype(np.float32)
+    drafted = rng.integers(0, 7, (2, K))
+    for numbers in (np.zeros((2, K + 1)), np.where(np.arange(K + 1) == 270, 1 - 2.0 ** -24, 0.0) * np.ones((2, 1))):
+        for given in (logits[:, :K] * np.float32(1.5), None):
+            want = verify(drafted, logits, given, 0.9, numbers.astype(np.float32))
+            got = run(drafted, logits, given, 0.9, numbers)
+            assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
+
+
+def test_a_greedy_verification_takes_a_nan_for_the_largest():
+    target = np.random.default_rng(2).standard_normal((1, 3, 5000)).astype(np.float32)
+    target[0, 0, 4321] = np.nan
+    target[0, 1, :] = -np.inf
+    tokens, accepted = run(np.array([[4321, 0]]), target, None, 0.0, np.zeros((1, 3)))
+    assert accepted[0] == 2 and tokens[0].tolist() == [4321, 0, int(target[0, 2].argmax())]

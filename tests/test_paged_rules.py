@@ -108,7 +108,7 @@ REFUSED = {
     "attend type": "f32 or bf16", "attend host rows": "another device", "rotary rank": "[T, H, D]",
     "rotary positions": "positions must be", "rotary positions type": "positions must be",
     "rotary host positions": "another device", "rotary host rows": "GPU only", "rotary type": "f32 or bf16",
-    "rotary wide tables": "rotate 32 of 30", "rotary layout": "layout", "tables odd": "even", "tables empty": "capacity",
+    "rotary wide tables": "rotate 32 of 30", "rotary layout": "layout", "rotary heads": "too many heads", "verify drafts": "2^20 drafts", "tables odd": "even", "tables empty": "capacity",
     "tables base": "base", "tables kind": "unknown scaling", "tables factor": "factor", "tables trained": "trained",
     "tables turns": "slow_turns", "tables one pair": "two pairs", "tables magnitude": "finite", "verify ids": "drafted must be",
     "verify target": "[B, K + 1, V]", "verify draft": "[B, K, V]", "verify uniforms": "uniforms must be",
