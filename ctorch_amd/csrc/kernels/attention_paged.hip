@@ -100,7 +100,36 @@ template <int STRIDE> __device__ __forceinline__ u32x2 column4(const uint16_t* b
     return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(from)));
 }
 
-// Weights of a row whose base is not set yet: any score sets it.
+// A value that some of a tile's rows do not see must not reach them, and zero times an infinity or a NaN would.  So the
+// tiles that are like that are looked over: what is not finite goes into the products as zero, and if there was any, it is
+// added to the rows that see it in the end, key by key (infinities and NaN add up the same in any order).
+__device__ __forceinline__ bool not_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u; }
+template <typename KT> __device__ __forceinline__ bool clear_not_finite(u32x4& words) {
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const bool high = not_finite(__uint_as_float(words[i])), low = sizeof(KT) == 2 && not_finite(__uint_as_float(words[i] << 16));
+        if (sizeof(KT) == 4) words[i] = high ? 0u : words[i];
+        else words[i] &= (high ? 0xffffu : ~0u) & (low ? 0xffff0000u : ~0u);
+        any |= high || low;
+    }
+    return any;
+}
+// An entry, and four, of a row of values.
+__device__ __forceinline__ float value_of(float x) { return x; }
+__device__ __forceinline__ float value_of(uint16_t x) { return bf16_to_f32(x); }
+__device__ __forceinline__ f32x4 four(const float* from) { return *reinterpret_cast<const f32x4*>(from); }
+__device__ __forceinline__ f32x4 four(const uint16_t* from) {
+    const u32x2 w = *reinterpret_cast<const u32x2*>(from);
+    return f32x4{bf16_lo(w.x), bf16_hi(w.x), bf16_lo(w.y), bf16_hi(w.y)};
+}
+template <typename KT> __device__ __forceinline__ const KT* value_row(const dlk_paged_params& p, Planned<int32_t>* table, int kvh, int key) {
+    const int64_t page = table[key >> p.page_shift];
+    return static_cast<const KT*>(p.v) + (((page * p.KV + kvh) << p.page_shift) + (key & ((1 << p.page_shift) - 1))) * (int64_t(1) * p.hd);
+}
+
+// Weights of a row whose base is not set yet: any score sets it.  (Scores stay below 2^30: s c - base is one fma, off by the
+// rounding of the base, a factor that the weights and their sum share.)
 constexpr float kNoBase = -1e30f;
 // How far (in powers of two) a score may lie above its row's base before the base follows.
 constexpr float kSlack = 8.0f;
@@ -281,7 +310,7 @@ __device__ __forceinline__ void attend_few(const dlk_paged_params& p, const dlk_
         }
     }
     if (QLDS) __syncthreads();
-    const int all_see = min(item.first + item.row_begin / G, w_end - 1); // the last key that every row sees
+    const int every = item.first + item.row_begin / G, all_see = min(every, w_end - 1); // the last key that every row sees
 
     f32x4 o[NT][DT];
     float base[NT], l[NT];
@@ -292,10 +321,19 @@ __device__ __forceinline__ void attend_few(const dlk_paged_params& p, const dlk_
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[nt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
+    auto entry_of = [&](int dt, int j) { return F32 ? 16 * E * (dt / E) + E * (4 * q + j) + dt % E : 16 * dt + 4 * q + j; }; // of o[.][dt][j]
     uint16_t* my_v = reinterpret_cast<uint16_t*>(area) + wave * KEYS * VSTRIDE;
 
+    uint64_t spoiled = 0;
     for (int tile = 0; tile < tiles; ++tile) {
+        const int key0 = w_begin + tile * KEYS;
+        auto look = [&] {
+            if (min(key0 + KEYS, w_end) - 1 <= every) return; // (every row sees all of it)
+            for (auto& half : v)
+                for (u32x4& words : half) spoiled |= __ballot(clear_not_finite<KT>(words));
+        };
         if constexpr (!F32) {
+            look();
             wave_order();
 #pragma unroll
             for (int u = 0; u < NU; ++u)
@@ -337,7 +375,6 @@ __device__ __forceinline__ void attend_few(const dlk_paged_params& p, const dlk_
                     }
             }
         if (tile + 1 < tiles) load_keys(tile + 1);
-        const int key0 = w_begin + tile * KEYS;
         u32x4 pb[NT][3];
         if (key0 + KEYS - 1 > all_see) {
 #pragma unroll
@@ -357,6 +394,7 @@ __device__ __forceinline__ void attend_few(const dlk_paged_params& p, const dlk_
                               s[nt][NU - 1][2], s[nt][NU - 1][3]}, pb[nt]);
         }
         if constexpr (F32) {
+            look();
 #pragma unroll
             for (int u = 0; u < NU; ++u)
 #pragma unroll
@@ -383,6 +421,21 @@ __device__ __forceinline__ void attend_few(const dlk_paged_params& p, const dlk_
             }
         }
     }
+    if (spoiled) {
+#pragma unroll 1
+        for (int key = w_begin + max(0, every + 1 - w_begin) / KEYS * KEYS; key < w_end; ++key) {
+            const KT* row = value_row<KT>(p, table, kvh, key);
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float x = value_of(row[entry_of(dt, j)]);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+                        if (not_finite(x) && key <= limit[nt]) o[nt][dt][j] += x;
+                }
+        }
+    }
 
     // merge the waves
     __syncthreads();
@@ -398,7 +451,7 @@ __device__ __forceinline__ void attend_few(const dlk_paged_params& p, const dlk_
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) row[F32 ? 16 * E * (dt / E) + E * (4 * q + j) + dt % E : 16 * dt + 4 * q + j] = o[nt][dt][j];
+            for (int j = 0; j < 4; ++j) row[entry_of(dt, j)] = o[nt][dt][j];
     }
     __syncthreads();
     const int rows = item.row_end - item.row_begin;
@@ -467,6 +520,10 @@ __device__ __forceinline__ void attend_many(const dlk_paged_params& p, const dlk
     Planned<int32_t>* table = planned(p.tables) + item.table;
     const float c = p.scale * 1.4426950408889634f;
     const int tiles = (item.key_end - item.key_begin + KEYS - 1) / KEYS;
+    // the last key that every row sees; the tiles behind it hold keys that some row does not see
+    const int every = item.first + item.row_begin / G;
+    auto end_of = [&](int tile) { return min(item.key_begin + (tile + 1) * KEYS, item.key_end); };
+    uint64_t spoiled = 0;
 
     auto half_of = [&](int i) { return PASSES ? i / (PASSES ? PASSES : 1) : wave * kWave / TEAM; };
     auto piece_of = [&](int i) { return PASSES ? t + kThreads * (i % (PASSES ? PASSES : 1)) : t % TEAM; };
@@ -509,6 +566,10 @@ __device__ __forceinline__ void attend_many(const dlk_paged_params& p, const dlk
     auto load_keys = [&](int tile, const Pages& pages) { load(tile, pages, p.k, kr); };
     auto load_values = [&](int tile, const Pages& pages) { load(tile, pages, p.v, vr); };
     auto stage_keys = [&](int buffer) { stage(kr, ks[buffer]); };
+    auto look = [&](int tile) {
+        if (end_of(tile) - 1 <= every) return;
+        for (u32x4& words : vr) spoiled |= __ballot(clear_not_finite<KT>(words));
+    };
     auto stage_values = [&](int buffer) { stage(vr, vs[buffer]); };
     Pages pages = pages_of(0);
     load_keys(0, pages);
@@ -592,6 +653,7 @@ __device__ __forceinline__ void attend_many(const dlk_paged_params& p, const dlk
         // numbers are constants, so that the compiler sees that the reads and writes of a step are apart.
         stage_keys(0);
         load_keys(1, pages);
+        look(0);
         stage_values(0);
         load_values(1, pages);
         pages = pages_of(2); // of tile t + 2
@@ -601,7 +663,7 @@ __device__ __forceinline__ void attend_many(const dlk_paged_params& p, const dlk
         if (EARLY) read_keys(0, keys);
         if (mine > 0) score(0, keys, s[0][0]);
         __syncthreads();
-        auto step = [&](int tile, auto buffer) {
+        auto step = [&](int tile, auto buffer, auto looks) {
             constexpr int B = decltype(buffer)::value;
             const Pages ahead = pages_of(tile + 3);
             u32x4 pb[2][3];
@@ -611,6 +673,7 @@ __device__ __forceinline__ void attend_many(const dlk_paged_params& p, const dlk
             settle<32>(s, base, l, c, o);
             score(1 - B, keys, next); // (of no use behind the last tile)
             weigh(s[0], pb);
+            if (decltype(looks)::value) look(tile + 1);
             stage_keys(B);
             stage_values(1 - B);
             load_keys(tile + 3, ahead);
@@ -621,14 +684,20 @@ __device__ __forceinline__ void attend_many(const dlk_paged_params& p, const dlk
             __syncthreads();
         };
         int tile = 0;
-        for (; tile + 1 < mine; tile += 2) {
-            step(tile, std::integral_constant<int, 0>{});
-            step(tile + 1, std::integral_constant<int, 1>{});
-        }
-        if (tile < mine) step(tile++, std::integral_constant<int, 0>{});
+        const auto pairs = [&](int end, auto looks) {
+            for (; tile + 1 < end; tile += 2) {
+                step(tile, std::integral_constant<int, 0>{}, looks);
+                step(tile + 1, std::integral_constant<int, 1>{}, looks);
+            }
+        };
+        // (first the ones that stage tiles that every row sees: a branch in the midst of the products costs 5 %)
+        pairs(min(mine, (every + 1 - item.key_begin) / KEYS - 1), std::false_type{});
+        pairs(mine, std::true_type{});
+        if (tile < mine) step(tile++, std::integral_constant<int, 0>{}, std::true_type{});
         for (; tile < tiles; ++tile) { // the other waves' tiles
             const Pages ahead = pages_of(tile + 3);
             stage_keys(tile % 2);
+            look(tile + 1);
             stage_values((tile + 1) % 2);
             load_keys(tile + 3, ahead);
             load_values(tile + 2, pages);
@@ -637,6 +706,7 @@ __device__ __forceinline__ void attend_many(const dlk_paged_params& p, const dlk
         }
     } else {
         stage_keys(0);
+        look(0);
         stage_values(0);
         load_keys(1, pages);
         load_values(1, pages);
@@ -653,6 +723,7 @@ __device__ __forceinline__ void attend_many(const dlk_paged_params& p, const dlk
             }
             __syncthreads();
             stage_keys(0);
+            look(tile + 1);
             stage_values(0);
             load_keys(tile + 2, pages);
             load_values(tile + 2, pages);
@@ -661,6 +732,22 @@ __device__ __forceinline__ void attend_many(const dlk_paged_params& p, const dlk
     }
 
     // lane holds O[row r][d = 32 dt + 8 (i / 4) + 4 half + i % 4]
+    if (item.key_end - 1 > every && __syncthreads_or(spoiled != 0)) {
+#pragma unroll 1
+        for (int key = item.key_begin + max(0, every + 1 - item.key_begin) / KEYS * KEYS; key < item.key_end; ++key) {
+            const KT* from = value_row<KT>(p, table, kvh, key) + 4 * half;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (32 * dt + 8 * i >= HD) continue;
+                    const f32x4 x = four(from + 32 * dt + 8 * i);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (not_finite(x[j]) && key <= limit) o[0][dt][4 * i + j] += x[j];
+                }
+        }
+    }
     const float sum = sum_over_row<32>(l[0]);
     if (first_row + r >= item.row_end) return;
     const bool whole = item.slot < 0;
@@ -683,7 +770,7 @@ __device__ __forceinline__ void attend_many(const dlk_paged_params& p, const dlk
 // One launch for all items: the ones of many rows first, which take longest, and beside them those of few, which wait for
 // memory where the others wait for the matrix cores.
 template <typename KT, int HD, int NT, int QP, bool FEW, bool MANY>
-__global__ __launch_bounds__(kThreads, 2) void paged_attend(const dlk_paged_params p) {
+__global__ __launch_bounds__(kThreads, MANY || NT > 1 || (sizeof(KT) == 2 && QP > 1) ? 2 : 3) void paged_attend(const dlk_paged_params p) {
     constexpr int FQ = sizeof(KT) == 4 ? 1 : QP; // the f32 instruction takes queries as they are
     constexpr int A = FEW ? Few<KT, HD, NT, FQ>::LDS : 0, B = MANY ? Many<KT, HD>::LDS : 0;
     __shared__ __attribute__((aligned(16))) char area[A > B ? A : B];

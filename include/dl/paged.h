@@ -65,6 +65,8 @@ DL_API Tensor paged_append(const nn::PagedKVCache& cache, Index layer, const nn:
 
 /// Attention of the step's (rotated) queries [tokens, heads, head_dim], f32 or bf16, over the pages of `layer`: the row
 /// at position p sees the positions 0 .. p of its sequence, its own included (append first).  f32 [tokens, heads, head_dim].
+/// What a row does not see may hold anything.  Products are exact to f32: of finite values up to 3e38 and scores q k / sqrt(head_dim) below 2^29;
+/// where a row sees a value that is not finite, that entry of it is not finite either.
 DL_API Tensor paged_attention(const nn::PagedKVCache& cache, Index layer, const nn::PagedBatch& batch, const Tensor& query);
 
 } // namespace dl

@@ -2,9 +2,9 @@
 the pages with and without a shared prefix, and a serving loop of them together.
 
 Tolerances, from the arithmetic.  Rotation: two products and a sum in f32, each rounded by at most 2^-24, of values up to
-|a| + |b| times the tables' entries.  Attention: queries, f32 keys and probabilities are sums of two bf16 parts, each part
-off by half a step, so x = hi + lo within 2^-9 * 2^-9 = 2^-18 of x; of a product of two such values the two parts' errors
-and the dropped lo * lo add up to less than 2^-16 of it, and sums of n products add n * 2^-24.  A score off by e changes its
+|a| + |b| times the tables' entries.  Attention: queries, f32 keys and probabilities may be sums of no fewer than two bf16
+parts, each off by half a step, so x = hi + lo within 2^-9 * 2^-9 = 2^-18 of x; of a product of two such values the parts'
+errors and the dropped lo * lo add up to less than 2^-16 of it, and sums of n products add n * 2^-24.  A score off by e changes its
 weight by a factor of at most exp(2 e), so an output is off by at most (2 e + 2^-16 + n * 2^-24) of sum_j p_j |v_j|."""
 import random
 
@@ -233,6 +233,60 @@ def test_extreme_values(dtype, counts):
     fill(step.cache.key(0), k)
     got = ct.paged_attention(step.cache, 0, step.batch, q).numpy()
     assert np.all(np.abs(got[counts[0]:] - want[counts[0]:]) <= bound[counts[0]:])
+
+
+AHEAD = [([100], [4], 8, 2, 64), ([40], [8], 8, 2, 128), ([90], [150], 8, 2, 64), ([1000], [70], 16, 4, 128), ([33], [3], 4, 1, 16),
+         ([0], [2], 40, 2, 32), ([3000], [6], 8, 2, 32), ([5], [400], 4, 4, 16)]
+
+
+@pytest.mark.parametrize("case", range(len(AHEAD)))
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_what_lies_ahead_of_a_row_does_not_reach_it(case, dtype):
+    """Values and then keys that are not finite at a new position: the rows before it do not see them, and of the others only
+    those entries change."""
+    lengths, counts, heads, kv, dim = AHEAD[case]
+    say(f"case: paged attention {AHEAD[case]} pages {dtype}, not finite ahead")
+    step = Step(lengths, counts, heads, kv, dim, 16, dtype, 0, 50 + case)
+    q, values = give(step.rng.standard_normal((step.tokens, heads, dim)))
+    row, at, group = counts[0] // 2, lengths[0] + counts[0] // 2, heads // kv
+    place = step.tables[0, at // 16], 0, at % 16  # KV head 0
+    marks = {3: np.nan, 5: np.inf, dim - 1: -np.inf}
+    for d in marks:
+        step.value[0][place][d] = 0
+    want, bound = step.attend(values)
+    spoiled = step.value[0].copy()
+    for d, x in marks.items():
+        spoiled[place][d] = x
+    fill(step.cache.value(0), spoiled)
+    got = ct.paged_attention(step.cache, 0, step.batch, q).numpy()
+    sees = np.zeros(got.shape, bool)
+    for d in marks:
+        sees[row:, :group, d] = True
+    assert not np.isfinite(got[sees]).any()
+    assert np.all(np.abs(got - want)[~sees] <= bound[~sees])
+    fill(step.cache.value(0), step.value[0])
+    key = step.key[0].copy()
+    key[place] = np.nan
+    fill(step.cache.key(0), key)
+    got = ct.paged_attention(step.cache, 0, step.batch, q).numpy()
+    sees[row:, :group] = True
+    assert np.isnan(got[sees]).all() and np.all(np.abs(got - want)[~sees] <= bound[~sees])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("counts", [[1, 0], [1, 200], [9, 1]])
+def test_scores_far_below_zero(dtype, counts):
+    """A row's one key, and equal ones, still weigh what they weigh."""
+    step = Step([0, 0], counts, 8, 2, 64, 16, dtype, 0, 8)
+    fill(step.cache.key(0), np.full_like(step.key[0], -2.0 ** 12))
+    q = give(np.full((step.tokens, 8, 64), 1.375 * 2.0 ** 13))[0]  # 64 * 1.375 * 2^25 / 8 = 1.375 * 2^28
+    got, t = ct.paged_attention(step.cache, 0, step.batch, q).numpy(), 0
+    for b, c in enumerate(counts):
+        v = step.held(step.value[0], b, c)
+        for i in range(c):  # the mean of i + 1 values: equal weights that round, their sum in f32, and the quotient
+            want, size = v[:, :i + 1].mean(1), np.abs(v[:, :i + 1]).mean(1)
+            assert np.all(np.abs(got[t + i].reshape(2, 4, 64) - want[:, None]) <= (2 * i + 16) * 2.0 ** -23 * size[:, None])
+        t += c
 
 
 def test_a_nan_stays_in_the_rows_that_see_it():
