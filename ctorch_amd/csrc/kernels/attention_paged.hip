@@ -104,16 +104,37 @@ template <int STRIDE> __device__ __forceinline__ u32x2 column4(const uint16_t* b
 // tiles that are like that are looked over: what is not finite goes into the products as zero, and if there was any, it is
 // added to the rows that see it in the end, key by key (infinities and NaN add up the same in any order).
 __device__ __forceinline__ bool not_finite(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u; }
-template <typename KT> __device__ __forceinline__ bool clear_not_finite(u32x4& words) {
-    bool any = false;
+template <typename KT, int N> __device__ __forceinline__ bool clear_not_finite(u32x4 (&pieces)[N]) {
+    if constexpr (sizeof(KT) == 4) {
+        uint64_t any = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const bool high = not_finite(__uint_as_float(words[i])), low = sizeof(KT) == 2 && not_finite(__uint_as_float(words[i] << 16));
-        if (sizeof(KT) == 4) words[i] = high ? 0u : words[i];
-        else words[i] &= (high ? 0xffffu : ~0u) & (low ? 0xffff0000u : ~0u);
-        any |= high || low;
+        for (int n = 0; n < N; ++n) {
+            bool piece = false;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const bool word = not_finite(__uint_as_float(pieces[n][i]));
+                pieces[n][i] = word ? 0u : pieces[n][i];
+                piece |= word;
+            }
+            any |= __ballot(piece);
+        }
+        return any != 0;
+    } else {
+        uint32_t sum = 0; // (an exponent of ones carries into the sign)
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum |= (pieces[n][i] & 0x7f807f80u) + 0x00800080u;
+        if (!__any((sum & 0x80008000u) != 0)) return false;
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t w = pieces[n][i];
+                pieces[n][i] &= (not_finite(__uint_as_float(w)) ? 0xffffu : ~0u) & (not_finite(__uint_as_float(w << 16)) ? 0xffff0000u : ~0u);
+            }
+        return true;
     }
-    return any;
 }
 // An entry, and four, of a row of values.
 __device__ __forceinline__ float value_of(float x) { return x; }
@@ -195,7 +216,7 @@ template <typename KT, int HD, int NT, int QP> struct Few {
 };
 
 template <typename KT, int HD, int NT, int QP>
-__device__ __forceinline__ void attend_few(const dlk_paged_params& p, const dlk_paged_list& list, int block, char* area) {
+__device__ __forceinline__ void attend_few(const dlk_paged_params& p, int block, char* area) {
     using S = Few<KT, HD, NT, QP>;
     constexpr bool F32 = S::F32, QLDS = S::QLDS;
     constexpr int NU = S::NU, KEYS = S::KEYS, ROWS = S::ROWS, VSTRIDE = S::VSTRIDE, STAGE = S::STAGE;
@@ -213,7 +234,7 @@ __device__ __forceinline__ void attend_few(const dlk_paged_params& p, const dlk_
     const int t = threadIdx.x, lane = t % kWave, q = lane / 16, col = lane % 16;
     const int wave = __builtin_amdgcn_readfirstlane(t / kWave);
     const int kvh = block % p.KV;
-    const dlk_paged_item item = item_of(list, block / p.KV);
+    const dlk_paged_item item = item_of(p.lists[DLK_PAGED_FEW], block / p.KV);
     const int G = p.H / p.KV;
     Planned<int32_t>* table = planned(p.tables) + item.table;
     const float c = p.scale * 1.4426950408889634f;
@@ -324,13 +345,12 @@ __device__ __forceinline__ void attend_few(const dlk_paged_params& p, const dlk_
     auto entry_of = [&](int dt, int j) { return F32 ? 16 * E * (dt / E) + E * (4 * q + j) + dt % E : 16 * dt + 4 * q + j; }; // of o[.][dt][j]
     uint16_t* my_v = reinterpret_cast<uint16_t*>(area) + wave * KEYS * VSTRIDE;
 
-    uint64_t spoiled = 0;
+    bool spoiled = false;
     for (int tile = 0; tile < tiles; ++tile) {
         const int key0 = w_begin + tile * KEYS;
         auto look = [&] {
             if (min(key0 + KEYS, w_end) - 1 <= every) return; // (every row sees all of it)
-            for (auto& half : v)
-                for (u32x4& words : half) spoiled |= __ballot(clear_not_finite<KT>(words));
+            for (auto& half : v) spoiled |= clear_not_finite<KT>(half);
         };
         if constexpr (!F32) {
             look();
@@ -471,11 +491,11 @@ __device__ __forceinline__ void attend_few(const dlk_paged_params& p, const dlk_
             const int row = item.row_begin + r;
             p.out[(static_cast<int64_t>(item.token + row / G) * p.H + kvh * G + row % G) * HD + d] = O / L;
         } else {
-            const int64_t at = (static_cast<int64_t>(item.slot) * p.KV + kvh) * ROWS + r;
-            list.partial_o[at * HD + d] = O;
+            const int64_t at = static_cast<int64_t>(kvh) * p.places + item.slot + r;
+            p.partial_o[at * HD + d] = O;
             if (d == 0) {
-                list.partial_ml[2 * at] = M;
-                list.partial_ml[2 * at + 1] = L;
+                p.partial_ml[2 * at] = M;
+                p.partial_ml[2 * at + 1] = L;
             }
         }
     }
@@ -497,14 +517,14 @@ template <typename KT, int HD> struct Many {
 };
 
 template <typename KT, int HD, int QP>
-__device__ __forceinline__ void attend_many(const dlk_paged_params& p, const dlk_paged_list& list, int block, char* area) {
+__device__ __forceinline__ void attend_many(const dlk_paged_params& p, int block, char* area) {
     using S = Many<KT, HD>;
     constexpr bool F32 = sizeof(KT) == 4;
     constexpr int PLANES = S::PLANES, BUFFERS = S::BUFFERS, KEYS = S::KEYS, STRIDE = S::STRIDE;
     constexpr int KS = HD / 16, DT = HD < 32 ? 1 : HD / 32; // (heads of 16: half an output tile is left)
     constexpr bool EARLY = HD <= 64;                  // a tile's keys are read ahead of the softmax (registers)
     constexpr int DPP = 16 / static_cast<int>(sizeof(KT)), PIECES = HD / DPP;
-    constexpr int ROW = HD * static_cast<int>(sizeof(KT)), ROWS = 128;
+    constexpr int ROW = HD * static_cast<int>(sizeof(KT));
     // a half of 16 keys is one piece of memory of BLOCK 16-byte pieces: several passes of all threads, or part of them
     constexpr int BLOCK = 16 * PIECES, PASSES = BLOCK / kThreads, LOADS = PASSES ? 2 * PASSES : 1;
     constexpr int TEAM = BLOCK < kWave ? kWave : BLOCK; // threads of a half, where one pass takes both
@@ -515,7 +535,7 @@ __device__ __forceinline__ void attend_many(const dlk_paged_params& p, const dlk
     const int t = threadIdx.x, lane = t % kWave, half = lane / 32, r = lane % 32;
     const int wave = __builtin_amdgcn_readfirstlane(t / kWave);
     const int kvh = block % p.KV;
-    const dlk_paged_item item = item_of(list, block / p.KV);
+    const dlk_paged_item item = item_of(p.lists[DLK_PAGED_MANY], block / p.KV);
     const int G = p.H / p.KV;
     Planned<int32_t>* table = planned(p.tables) + item.table;
     const float c = p.scale * 1.4426950408889634f;
@@ -523,7 +543,8 @@ __device__ __forceinline__ void attend_many(const dlk_paged_params& p, const dlk
     // the last key that every row sees; the tiles behind it hold keys that some row does not see
     const int every = item.first + item.row_begin / G;
     auto end_of = [&](int tile) { return min(item.key_begin + (tile + 1) * KEYS, item.key_end); };
-    uint64_t spoiled = 0;
+    __shared__ int spoiled[kWaves]; // what a wave staged behind `every` was not all finite
+    if (lane == 0) spoiled[wave] = 0;
 
     auto half_of = [&](int i) { return PASSES ? i / (PASSES ? PASSES : 1) : wave * kWave / TEAM; };
     auto piece_of = [&](int i) { return PASSES ? t + kThreads * (i % (PASSES ? PASSES : 1)) : t % TEAM; };
@@ -568,7 +589,7 @@ __device__ __forceinline__ void attend_many(const dlk_paged_params& p, const dlk
     auto stage_keys = [&](int buffer) { stage(kr, ks[buffer]); };
     auto look = [&](int tile) {
         if (end_of(tile) - 1 <= every) return;
-        for (u32x4& words : vr) spoiled |= __ballot(clear_not_finite<KT>(words));
+        if (clear_not_finite<KT>(vr)) spoiled[wave] = 1;
     };
     auto stage_values = [&](int buffer) { stage(vr, vs[buffer]); };
     Pages pages = pages_of(0);
@@ -663,8 +684,9 @@ __device__ __forceinline__ void attend_many(const dlk_paged_params& p, const dlk
         if (EARLY) read_keys(0, keys);
         if (mine > 0) score(0, keys, s[0][0]);
         __syncthreads();
-        auto step = [&](int tile, auto buffer, auto looks) {
+        auto step = [&](int tile, auto buffer) {
             constexpr int B = decltype(buffer)::value;
+            look(tile + 1); // (here, where no products are in flight: a branch in the midst of them costs 5 %)
             const Pages ahead = pages_of(tile + 3);
             u32x4 pb[2][3];
             f32x16 next;
@@ -673,7 +695,6 @@ __device__ __forceinline__ void attend_many(const dlk_paged_params& p, const dlk
             settle<32>(s, base, l, c, o);
             score(1 - B, keys, next); // (of no use behind the last tile)
             weigh(s[0], pb);
-            if (decltype(looks)::value) look(tile + 1);
             stage_keys(B);
             stage_values(1 - B);
             load_keys(tile + 3, ahead);
@@ -684,16 +705,11 @@ __device__ __forceinline__ void attend_many(const dlk_paged_params& p, const dlk
             __syncthreads();
         };
         int tile = 0;
-        const auto pairs = [&](int end, auto looks) {
-            for (; tile + 1 < end; tile += 2) {
-                step(tile, std::integral_constant<int, 0>{}, looks);
-                step(tile + 1, std::integral_constant<int, 1>{}, looks);
-            }
-        };
-        // (first the ones that stage tiles that every row sees: a branch in the midst of the products costs 5 %)
-        pairs(min(mine, (every + 1 - item.key_begin) / KEYS - 1), std::false_type{});
-        pairs(mine, std::true_type{});
-        if (tile < mine) step(tile++, std::integral_constant<int, 0>{}, std::true_type{});
+        for (; tile + 1 < mine; tile += 2) {
+            step(tile, std::integral_constant<int, 0>{});
+            step(tile + 1, std::integral_constant<int, 1>{});
+        }
+        if (tile < mine) step(tile++, std::integral_constant<int, 0>{});
         for (; tile < tiles; ++tile) { // the other waves' tiles
             const Pages ahead = pages_of(tile + 3);
             stage_keys(tile % 2);
@@ -732,7 +748,7 @@ __device__ __forceinline__ void attend_many(const dlk_paged_params& p, const dlk
     }
 
     // lane holds O[row r][d = 32 dt + 8 (i / 4) + 4 half + i % 4]
-    if (item.key_end - 1 > every && __syncthreads_or(spoiled != 0)) {
+    if (item.key_end - 1 > every && (spoiled[0] | spoiled[1] | spoiled[2] | spoiled[3])) { // (a barrier ended the last tile)
 #pragma unroll 1
         for (int key = item.key_begin + max(0, every + 1 - item.key_begin) / KEYS * KEYS; key < item.key_end; ++key) {
             const KT* from = value_row<KT>(p, table, kvh, key) + 4 * half;
@@ -751,8 +767,8 @@ __device__ __forceinline__ void attend_many(const dlk_paged_params& p, const dlk
     const float sum = sum_over_row<32>(l[0]);
     if (first_row + r >= item.row_end) return;
     const bool whole = item.slot < 0;
-    const int64_t at = (static_cast<int64_t>(item.slot) * p.KV + kvh) * ROWS + row - item.row_begin;
-    float* out = whole ? p.out + (static_cast<int64_t>(item.token + row / G) * p.H + kvh * G + row % G) * HD : list.partial_o + at * HD;
+    const int64_t at = static_cast<int64_t>(kvh) * p.places + item.slot + row - item.row_begin;
+    float* out = whole ? p.out + (static_cast<int64_t>(item.token + row / G) * p.H + kvh * G + row % G) * HD : p.partial_o + at * HD;
     const float scale = whole ? 1.0f / sum : 1.0f;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
@@ -762,8 +778,8 @@ __device__ __forceinline__ void attend_many(const dlk_paged_params& p, const dlk
                 *reinterpret_cast<f32x4*>(out + 32 * dt + 8 * i + 4 * half) =
                     f32x4{o[0][dt][4 * i], o[0][dt][4 * i + 1], o[0][dt][4 * i + 2], o[0][dt][4 * i + 3]} * scale;
     if (!whole && half == 0) {
-        list.partial_ml[2 * at] = base[0];
-        list.partial_ml[2 * at + 1] = sum;
+        p.partial_ml[2 * at] = base[0];
+        p.partial_ml[2 * at + 1] = sum;
     }
 }
 
@@ -774,18 +790,14 @@ __global__ __launch_bounds__(kThreads, MANY || NT > 1 || (sizeof(KT) == 2 && QP 
     constexpr int FQ = sizeof(KT) == 4 ? 1 : QP; // the f32 instruction takes queries as they are
     constexpr int A = FEW ? Few<KT, HD, NT, FQ>::LDS : 0, B = MANY ? Many<KT, HD>::LDS : 0;
     __shared__ __attribute__((aligned(16))) char area[A > B ? A : B];
-    int block = static_cast<int>(blockIdx.x);
-    const int many = p.lists[DLK_PAGED_MANY].count * p.KV, shared = p.lists[DLK_PAGED_SHARED].count * p.KV;
-    const int kind = block < many ? DLK_PAGED_MANY : block < many + shared ? DLK_PAGED_SHARED : DLK_PAGED_FEW;
-    block -= kind == DLK_PAGED_MANY ? 0 : kind == DLK_PAGED_SHARED ? many : many + shared;
-    const dlk_paged_list list = p.lists[kind];
+    const int block = static_cast<int>(blockIdx.x), many = p.lists[DLK_PAGED_MANY].count * p.KV;
     if constexpr (FEW && MANY) {
-        if (list.rows == 128) attend_many<KT, HD, QP>(p, list, block, area);
-        else attend_few<KT, HD, NT, FQ>(p, list, block, area);
+        if (block < many) attend_many<KT, HD, QP>(p, block, area);
+        else attend_few<KT, HD, NT, FQ>(p, block - many, area);
     } else if constexpr (MANY) {
-        attend_many<KT, HD, QP>(p, list, block, area);
+        attend_many<KT, HD, QP>(p, block, area);
     } else {
-        attend_few<KT, HD, NT, FQ>(p, list, block, area);
+        attend_few<KT, HD, NT, FQ>(p, block, area);
     }
 }
 
@@ -802,19 +814,11 @@ __global__ __launch_bounds__(kThreads) void paged_merge(const dlk_paged_params p
     const uint32_t groups = (p.H + HEADS - 1) / HEADS; // of heads
     const uint32_t unit = min(blockIdx.x * (kWaves / W) + all / W, p.merge_count * groups - 1);
     Planned<dlk_paged_merge>* merge = planned(p.merges) + unit / groups;
-    const int token = merge->token, splits = merge->count, shared = p.shared_splits, count = shared + splits;
-    const int h = min(static_cast<int>(unit % groups) * HEADS + lane / LANES, p.H - 1), G = p.H / p.KV, kvh = h / G;
-    const bool many = merge->list == DLK_PAGED_MANY;
-    const dlk_paged_list& few_list = p.lists[DLK_PAGED_FEW];
-    const dlk_paged_list& many_list = p.lists[DLK_PAGED_MANY];
-    const dlk_paged_list& front = p.lists[DLK_PAGED_SHARED];
-    const int rows = many ? many_list.rows : few_list.rows, row = merge->row + h % G, front_row = merge->shared_row + h % G;
-    const float* own_o = many ? many_list.partial_o : few_list.partial_o;
-    const float* own_ml = many ? many_list.partial_ml : few_list.partial_ml;
-    // where the row's first partials are, in rows, and how far apart
-    const int64_t own_step = static_cast<int64_t>(p.KV) * rows, front_step = static_cast<int64_t>(p.KV) * front.rows;
-    const int64_t own_at = (static_cast<int64_t>(merge->slot + row / rows * merge->stride) * p.KV + kvh) * rows + row % rows;
-    const int64_t front_at = (static_cast<int64_t>(front_row / front.rows * shared) * p.KV + kvh) * front.rows + front_row % front.rows;
+    const int token = merge->token, shared = p.shared_splits, count = shared + merge->count;
+    const int h = min(static_cast<int>(unit % groups) * HEADS + lane / LANES, p.H - 1), G = p.H / p.KV;
+    // where the row's first partials are, and how far apart
+    const int64_t row = static_cast<int64_t>(h / G) * p.places + h % G, own_at = row + merge->slot, front_at = row + merge->shared_slot;
+    const int64_t own_step = merge->stride, front_step = p.shared_stride;
     const int d = lane % LANES * 4;
     float M = kNoBase, L = 0.0f;
     f32x4 O = {0.f, 0.f, 0.f, 0.f};
@@ -826,10 +830,9 @@ __global__ __launch_bounds__(kThreads) void paged_merge(const dlk_paged_params p
             const int i = min(begin + W * k, count - 1);
             const bool in_front = i < shared;
             const int64_t at = in_front ? front_at + i * front_step : own_at + (i - shared) * own_step;
-            const float* ml = (in_front ? front.partial_ml : own_ml) + 2 * at;
-            m[k] = ml[0];
-            l[k] = ml[1];
-            x[k] = *reinterpret_cast<const f32x4*>((in_front ? front.partial_o : own_o) + at * HD + d);
+            m[k] = p.partial_ml[2 * at];
+            l[k] = p.partial_ml[2 * at + 1];
+            x[k] = *reinterpret_cast<const f32x4*>(p.partial_o + at * HD + d);
         }
         float top = M;
 #pragma unroll
@@ -869,18 +872,12 @@ __global__ __launch_bounds__(kThreads) void paged_merge(const dlk_paged_params p
 }
 
 template <typename KT, int HD, int QP> int launch_items(const dlk_paged_params& p, hipStream_t stream) {
-    int64_t blocks = 0;
-    int few = 0; // the most rows of the lists of few
-    bool many = false;
-    for (const dlk_paged_list& list : p.lists) {
-        if (list.count == 0) continue;
-        blocks += static_cast<int64_t>(list.count) * p.KV;
-        if (list.rows == 128) many = true;
-        else if (few != 0 && few != list.rows) return static_cast<int>(hipErrorInvalidValue);
-        else few = list.rows;
-    }
+    const dlk_paged_list &few_list = p.lists[DLK_PAGED_FEW], &many_list = p.lists[DLK_PAGED_MANY];
+    const int64_t blocks = (static_cast<int64_t>(few_list.count) + many_list.count) * p.KV;
+    const int few = few_list.count > 0 ? few_list.rows : 0;
+    const bool many = many_list.count > 0;
     if (blocks == 0) return 0;
-    if (blocks > INT32_MAX || (few != 0 && few != 16 && few != 32)) return static_cast<int>(hipErrorInvalidValue);
+    if (blocks > INT32_MAX || (few != 0 && few != 16 && few != 32) || (many && many_list.rows != 128)) return static_cast<int>(hipErrorInvalidValue);
     const dim3 grid(static_cast<unsigned>(blocks)), threads(kThreads);
     if (many && few == 32) hipLaunchKernelGGL((paged_attend<KT, HD, 2, QP, true, true>), grid, threads, 0, stream, p);
     else if (many && few == 16) hipLaunchKernelGGL((paged_attend<KT, HD, 1, QP, true, true>), grid, threads, 0, stream, p);

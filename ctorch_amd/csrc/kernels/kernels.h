@@ -286,27 +286,23 @@ typedef struct dlk_paged_item {
     int32_t table;           /* where the run's page ids start in `tables` (the page of key 0) */
     int32_t key_begin, key_end;
     int32_t first;           /* row r sees the keys up to first + r / G */
-    int32_t slot;            /* partials slot, or -1: the item is all that its rows see, and writes the output */
+    int32_t slot;            /* the first row's place among the partials, or -1: the item is all that its rows see, and
+                                writes the output */
 } dlk_paged_item;
 
-/* Items of one kind of work-group, and where their partials go.  rows: the most rows of an item, 16 or 32 (the waves of a
-   work-group split its keys) or 128 (they split its rows). */
+/* Items of one kind of work-group.  rows: the most rows of an item, 16 or 32 (the waves of a work-group split its keys) or
+   128 (they split its rows). */
 typedef struct dlk_paged_list {
     const dlk_paged_item* items;
     int count, rows;
-    float* partial_o;        /* [slots, KV, rows, hd] */
-    float* partial_ml;       /* [slots, KV, rows, 2]: base (a power of two) and sum */
 } dlk_paged_list;
 
-enum { DLK_PAGED_FEW = 0, DLK_PAGED_MANY = 1, DLK_PAGED_SHARED = 2 };
+enum { DLK_PAGED_FEW = 0, DLK_PAGED_MANY = 1 };
 
-/* One token whose rows several items share. */
+/* One token whose rows several items share: its first row's place among the partials of its run's first split, how far
+   apart the splits are, and how many of them hold keys that it sees; and the first row's place among the prefix's. */
 typedef struct dlk_paged_merge {
-    int32_t token, row;      /* the token, and its first row within its run */
-    int32_t list;            /* its run's list (DLK_PAGED_FEW or DLK_PAGED_MANY) */
-    int32_t slot, stride;    /* the slot of the run's first row tile, and the slots of each row tile */
-    int32_t count;           /* the first of them that hold keys the row sees */
-    int32_t shared_row;      /* the token's first row within the prefix run */
+    int32_t token, slot, stride, count, shared_slot;
 } dlk_paged_merge;
 
 typedef struct dlk_paged_params {
@@ -319,8 +315,11 @@ typedef struct dlk_paged_params {
     float scale;
     const int32_t* tables;
     float* out;              /* [tokens, H, hd] */
-    dlk_paged_list lists[3]; /* runs of few rows, of many, and the prefix that the whole batch shares */
-    int shared_splits;       /* slots of each row tile of the prefix (0: none) */
+    dlk_paged_list lists[2]; /* items of few rows, and of many */
+    float* partial_o;        /* [KV, places, hd] */
+    float* partial_ml;       /* [KV, places, 2]: base (a power of two) and sum */
+    int places;
+    int shared_splits, shared_stride; /* splits of the prefix that the whole batch shares (0: none), and how far apart */
     const dlk_paged_merge* merges;
     int merge_count, merge_most; /* merges, and the most partials of one */
 } dlk_paged_params;

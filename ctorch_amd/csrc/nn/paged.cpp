@@ -33,9 +33,6 @@ PagedKVCache::PagedKVCache(Index layers, Index pages, Index page_size, Index kv_
 
 namespace {
 
-// Rows of a work-group for a run of `rows`: 16 or 32, whose waves split the keys, or 128, which they split.
-Index rows_for(Index rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 128; }
-
 // A list whose row tiles see `seen` keys each, for every KV head, and what its work-groups take.
 struct Load {
     std::vector<Index> seen;
@@ -45,13 +42,15 @@ struct Load {
 
 // Keys per item: the split with the smallest time by this account, in microseconds (measured on MI355X):
 // - `slots` work-groups run at once, and take `rate` keys a microsecond each then: of few rows what memory gives (5.4
-//   TB/s), of many what the matrix cores do (8500 / (products of a pair's entry, twice the head size): 19 keys for bf16 pages
-//   and heads of 64, 12 for heads of 128 or f32 pages); fewer of them run faster, until each CU has one;
-// - an item takes 5 more to begin and to end; the last ones run half an item alone, of many rows, where the longest come
-//   first, an eighth; a work-group of many rows runs a third faster as its neighbours end;
-// - a merge takes 6, and its partials, written and read, their bytes at 1.5 TB/s.
+//   TB/s), of many what the matrix cores do (8500 / (products of a pair's entry, twice the head size): 22 keys for bf16 pages
+//   and heads of 64, 11 for heads of 128 or f32 pages).  Fewer of them run faster: of few rows in proportion, until each CU
+//   has one; one of many rows that has a CU to itself 1.75 times;
+// - an item takes 5 more to begin and to end; the last ones run alone for half an item, of many rows, where the longest
+//   come first, a sixth;
+// - a merge takes 6, and its partials, written and read, their bytes at 2.5 TB/s, those of few rows or a prefix at 1.5.
 // (8 sequences of 32768 keys: 64 items of 2048 keys a head 133 us, of 768 124, of 256 139; 3000 new rows after 1000: whole
-// 335 us, in 512 keys 366; four prompts of 310 to 809 rows after 321 to 745, 544 work-groups: whole 103 us, in 1024 keys 115.)
+// 335 us, in 512 keys 366; 16 runs of 192 rows after up to 2000 keys, 256 work-groups: whole 58 us, in 1024 keys 44.  Over 36
+// such batches of many rows the choice is 1.5 % off the best of seven sizes in the mean, 12 % at most.)
 Index chunk_of(const Load& load) {
     if (load.seen.empty()) return 256;
     const bool many = load.rows == 128;
@@ -70,10 +69,10 @@ Index chunk_of(const Load& load) {
             if (n > 1.0 || load.merged) partials += n;
         }
         const double most = static_cast<double>(std::min(chunk, longest));
-        const double own = rate * std::clamp(slots / (items * heads), many ? 4.0 / 3.0 : 1.0, per_cu); // a work-group's rate
-        double time = std::max(most / own + 5.0, (work / rate + 5.0 * items) * heads / slots + most / rate / (many ? 8.0 : 2.0));
+        const double own = rate * (many ? 1.75 : std::clamp(slots / (items * heads), 1.0, per_cu)); // a work-group's rate
+        double time = std::max(most / own + 5.0, (work / rate + 5.0 * items) * heads / slots + most / rate / (many ? 6.0 : 2.0));
         if (partials > 0.0)
-            time += (load.merged ? 0.0 : 6.0) + partials * heads * static_cast<double>(load.used_rows * load.head_dim * 8) / 1.5e6;
+            time += (load.merged ? 0.0 : 6.0) + partials * heads * static_cast<double>(load.used_rows * load.head_dim * 8) / (many && !load.merged ? 2.5e6 : 1.5e6);
         if (chosen == 0 || time < best) best = time, chosen = chunk;
         if (chunk >= longest) return chosen;
         if (chunk >= 1024 * step) step *= 2;
@@ -138,90 +137,102 @@ PagedBatch::PagedBatch(const PagedKVCache& cache, Index heads, std::span<const I
     if (tokens > INT32_MAX / heads) refuse("too many new positions");
     plan->tokens = tokens;
 
-    // the runs' rows over their own keys (behind the shared ones), split where that gives more work-groups
+    // Row tiles: of 128 for the waves to split, and what is left, if it is no more than 32, like runs of few rows in one of
+    // 16 or 32, whose keys they split: its 128 would take as long as full ones.  (16 runs of 144 rows after up to 2000 keys,
+    // bf16, heads of 64: 54 us with the last 16 in a tile of 128, 33 in one of 16.  Two tiles of 32 for 33 to 64 rows gain
+    // a tenth where keys are few, and lose up to a third on f32 pages.)  The runs of few rows settle which of the two, 16
+    // where all of them fit: 32 take more registers (32 tokens of 4096 keys: 39 us, 48 us).
     auto& lists = plan->lists;
-    lists[DLK_PAGED_FEW].rows = 16;
     lists[DLK_PAGED_MANY].rows = 128;
-    const auto list_of = [&](Index b) { return rows_for(counts[b] * group) == 128 ? DLK_PAGED_MANY : DLK_PAGED_FEW; };
-    for (Index b = 0; b < batch; ++b)
-        if (counts[b] > 0 && list_of(b) == DLK_PAGED_FEW)
-            lists[DLK_PAGED_FEW].rows = std::max(lists[DLK_PAGED_FEW].rows, rows_for(counts[b] * group));
-    // a prefix of few rows is taken like the runs of few, in row tiles of one size
-    auto& prefix = lists[DLK_PAGED_SHARED];
-    prefix.rows = rows_for(tokens * group);
-    if (shared > 0 && prefix.rows < 128) lists[DLK_PAGED_FEW].rows = prefix.rows = std::max(prefix.rows, lists[DLK_PAGED_FEW].rows);
-    Index chunks[2];
-    for (int kind = 0; kind < 2; ++kind) {
-        Load load{{}, cache.kv_heads(), cache.head_dim(), lists[kind].rows, 1, cache.dtype() == DType::f32, shared > 0};
-        for (Index b = 0; b < batch; ++b) {
-            if (list_of(b) != kind) continue;
-            const Index rows = counts[b] * group;
-            for (Index row = 0; row < rows; row += load.rows)
-                load.seen.push_back(lengths[b] - shared + (std::min(rows, row + load.rows) - 1) / group + 1);
-            load.used_rows = std::max(load.used_rows, std::min(rows, load.rows));
-        }
-        chunks[kind] = chunk_of(load);
-    }
+    Index& few = lists[DLK_PAGED_FEW].rows;
+    few = 0;
+    Index tails = 16;
+    const auto settle = [&](Index rows) {
+        if (rows > 0 && rows <= 32) few = std::max<Index>(few, rows <= 16 ? 16 : 32);
+        if (rows % 128 > 16 && rows % 128 <= 32) tails = 32;
+    };
+    for (Index b = 0; b < batch; ++b) settle(counts[b] * group);
+    if (shared > 0) settle(tokens * group);
+    if (few == 0) few = tails;
+    struct Tile {
+        Index begin, end;
+        int kind;
+    };
+    const auto tiles_of = [&](Index rows) {
+        std::vector<Tile> tiles;
+        for (Index row = 0; row < rows; row += 128)
+            tiles.push_back({row, std::min(rows, row + 128), rows - row <= few ? DLK_PAGED_FEW : DLK_PAGED_MANY});
+        return tiles;
+    };
 
-    std::vector<dlk_paged_item> items[3];
+    // how many keys an item takes: of the runs' own (behind the shared ones), and of the shared ones
+    Load loads[2];
+    const auto load_of = [&](int kind, bool merged) {
+        return Load{{}, cache.kv_heads(), cache.head_dim(), lists[kind].rows, 1, cache.dtype() == DType::f32, merged};
+    };
+    for (int kind = 0; kind < 2; ++kind) loads[kind] = load_of(kind, shared > 0);
+    for (Index b = 0; b < batch; ++b) {
+        const auto tiles = tiles_of(counts[b] * group);
+        for (const Tile& tile : tiles) {
+            if (tile.kind != tiles[0].kind) continue; // (what is left of a run of many goes along)
+            loads[tile.kind].seen.push_back(lengths[b] - shared + (tile.end - 1) / group + 1);
+            loads[tile.kind].used_rows = std::max(loads[tile.kind].used_rows, tile.end - tile.begin);
+        }
+    }
+    const Index chunks[2] = {chunk_of(loads[0]), chunk_of(loads[1])};
+
+    std::vector<dlk_paged_item> items[2];
     std::vector<dlk_paged_merge> merges;
     std::vector<Index> positions, places;
     positions.reserve(static_cast<std::size_t>(tokens));
     places.reserve(static_cast<std::size_t>(tokens));
+    const auto place = [](Index n) { return static_cast<int32_t>(n); }; // (checked below)
+    if (shared > 0 && tokens > 0) {
+        const Index rows = tokens * group;
+        const auto tiles = tiles_of(rows);
+        Load load = load_of(tiles[0].kind, true);
+        for (const Tile& tile : tiles)
+            if (tile.kind == tiles[0].kind) load.seen.push_back(shared), load.used_rows = std::max(load.used_rows, tile.end - tile.begin);
+        const Index chunk = chunk_of(load);
+        plan->shared_splits = (shared + chunk - 1) / chunk;
+        plan->shared_stride = rows;
+        plan->partials = plan->shared_splits * rows;
+        for (Index s = 0; s < plan->shared_splits; ++s)
+            for (const Tile& tile : tiles)
+                items[tile.kind].push_back({0, place(tile.begin), place(tile.end), place(front * width), place(s * chunk),
+                                            place(std::min(shared, (s + 1) * chunk)), 1 << 30, place(s * rows + tile.begin)});
+    }
     Index token = 0;
     for (Index b = 0; b < batch; ++b) {
         const Index count = counts[b], first = lengths[b] - shared, keys = first + count, rows = count * group;
         if (count == 0) continue;
-        const int kind = list_of(b);
-        auto& list = lists[kind];
-        const Index chunk = chunks[kind], splits = (keys + chunk - 1) / chunk;
+        const auto tiles = tiles_of(rows);
+        const Index chunk = chunks[tiles[0].kind], splits = (keys + chunk - 1) / chunk;
         const bool whole = splits == 1 && shared == 0;
-        for (Index row = 0; row < rows; row += list.rows) {
-            const Index end = std::min(rows, row + list.rows);
-            const Index sees = first + (end - 1) / group + 1; // keys of the tile's last row
+        for (const Tile& tile : tiles) {
+            const Index sees = first + (tile.end - 1) / group + 1; // keys of the tile's last row
             for (Index s = 0; s < splits && s * chunk < sees; ++s)
-                items[kind].push_back({static_cast<int32_t>(token), static_cast<int32_t>(row), static_cast<int32_t>(end),
-                                       static_cast<int32_t>(b * width + shared / page), static_cast<int32_t>(s * chunk),
-                                       static_cast<int32_t>(std::min(sees, (s + 1) * chunk)), static_cast<int32_t>(first),
-                                       whole ? -1 : static_cast<int32_t>(list.slots + row / list.rows * splits + s)});
+                items[tile.kind].push_back({place(token), place(tile.begin), place(tile.end), place(b * width + shared / page),
+                                            place(s * chunk), place(std::min(sees, (s + 1) * chunk)), place(first),
+                                            whole ? -1 : place(plan->partials + s * rows + tile.begin)});
         }
         for (Index i = 0; i < count; ++i) {
             const Index position = lengths[b] + i;
             positions.push_back(position);
             places.push_back((tables[b * width + position / page] << shift) + position % page);
             if (!whole)
-                merges.push_back({static_cast<int32_t>(token + i), static_cast<int32_t>(i * group), kind,
-                                  static_cast<int32_t>(list.slots), static_cast<int32_t>(splits),
-                                  static_cast<int32_t>((first + i) / chunk + 1), static_cast<int32_t>((token + i) * group)});
+                merges.push_back({place(token + i), place(plan->partials + i * group), place(rows), place((first + i) / chunk + 1),
+                                  place((token + i) * group)});
         }
-        if (!whole) list.slots += (rows + list.rows - 1) / list.rows * splits;
+        if (!whole) plan->partials += splits * rows;
         token += count;
-    }
-    if (shared > 0 && tokens > 0) {
-        const Index rows = tokens * group;
-        auto& list = prefix;
-        const Index tiles = (rows + list.rows - 1) / list.rows;
-        const Index chunk = chunk_of({std::vector<Index>(static_cast<std::size_t>(tiles), shared), cache.kv_heads(), cache.head_dim(),
-                                      list.rows, std::min(rows, list.rows), cache.dtype() == DType::f32, true});
-        const Index splits = (shared + chunk - 1) / chunk;
-        plan->shared_splits = splits;
-        for (Index s = 0; s < splits; ++s)
-            for (Index tile = 0; tile < tiles; ++tile)
-                items[DLK_PAGED_SHARED].push_back({0, static_cast<int32_t>(tile * list.rows),
-                                                   static_cast<int32_t>(std::min(rows, (tile + 1) * list.rows)),
-                                                   static_cast<int32_t>(front * width), static_cast<int32_t>(s * chunk),
-                                                   static_cast<int32_t>(std::min(shared, (s + 1) * chunk)), 1 << 30,
-                                                   static_cast<int32_t>(tile * splits + s)});
-        list.slots = tiles * splits;
     }
     // the longest first, so that the last work-groups to start are short
     std::stable_sort(items[DLK_PAGED_MANY].begin(), items[DLK_PAGED_MANY].end(), [](const auto& a, const auto& b) {
         return a.key_end - a.key_begin > b.key_end - b.key_begin;
     });
-    for (int i = 0; i < 3; ++i) {
-        lists[i].count = static_cast<Index>(items[i].size());
-        if (std::max(lists[i].count, lists[i].slots) > INT32_MAX / cache.kv_heads()) refuse("too many new positions");
-    }
+    for (int i = 0; i < 2; ++i) lists[i].count = static_cast<Index>(items[i].size());
+    if (std::max(plan->partials, lists[0].count + lists[1].count) > INT32_MAX / cache.kv_heads()) refuse("too many new positions");
     plan->merge_count = static_cast<Index>(merges.size());
     for (const auto& merge : merges) plan->merge_most = std::max<Index>(plan->merge_most, merge.count + plan->shared_splits);
 
@@ -237,7 +248,7 @@ PagedBatch::PagedBatch(const PagedKVCache& cache, Index heads, std::span<const I
         return at;
     };
     plan->tables = put(ids);
-    for (int i = 0; i < 3; ++i) lists[i].items = put(items[i]);
+    for (int i = 0; i < 2; ++i) lists[i].items = put(items[i]);
     plan->merges = put(merges);
     plan->positions = put(positions);
     plan->places = put(places);
@@ -353,20 +364,18 @@ Tensor paged_attention(const nn::PagedKVCache& cache, Index layer, const nn::Pag
     p.tables = plan.at<std::int32_t>(plan.tables);
     p.out = static_cast<float*>(mutable_data(out));
     p.shared_splits = static_cast<int>(plan.shared_splits);
+    p.shared_stride = static_cast<int>(plan.shared_stride);
     p.merges = plan.at<dlk_paged_merge>(plan.merges);
     p.merge_count = static_cast<int>(plan.merge_count);
     p.merge_most = static_cast<int>(plan.merge_most);
     // partials, released to the pool in stream order
-    Index rows = 0;
-    for (const auto& list : plan.lists) rows += list.slots * kv * list.rows;
+    const Index rows = plan.partials * kv;
     Tensor partials = rows > 0 ? empty_tensor({rows * (dim + 2)}, DType::f32, cache.device()) : Tensor{};
-    float* o = rows > 0 ? static_cast<float*>(mutable_data(partials)) : nullptr;
-    float* ml = rows > 0 ? o + rows * dim : nullptr;
-    for (int i = 0; i < 3; ++i) {
-        const auto& list = plan.lists[i];
-        p.lists[i] = {plan.at<dlk_paged_item>(list.items), static_cast<int>(list.count), static_cast<int>(list.rows), o, ml};
-        if (rows > 0) o += list.slots * kv * list.rows * dim, ml += 2 * list.slots * kv * list.rows;
-    }
+    p.partial_o = rows > 0 ? static_cast<float*>(mutable_data(partials)) : nullptr;
+    p.partial_ml = rows > 0 ? p.partial_o + rows * dim : nullptr;
+    p.places = static_cast<int>(plan.partials);
+    for (int i = 0; i < 2; ++i)
+        p.lists[i] = {plan.at<dlk_paged_item>(plan.lists[i].items), static_cast<int>(plan.lists[i].count), static_cast<int>(plan.lists[i].rows)};
     hip_check(dlk_paged_attention(&p, context.stream), name);
     return out;
 }

@@ -15,10 +15,11 @@ struct PagedBatch::Plan {
 
     Index tokens = 0, last = -1; // new positions, and the largest of them
     struct List {
-        Index rows = 16, count = 0, slots = 0; // rows of an item, items, slots of partials
-        std::size_t items = 0;                 // where the items are
-    } lists[3];                                // by DLK_PAGED_FEW, DLK_PAGED_MANY, DLK_PAGED_SHARED
-    Index shared_splits = 0, merge_count = 0, merge_most = 0;
+        Index rows = 16, count = 0; // the most rows of an item, and items
+        std::size_t items = 0;      // where the items are
+    } lists[2];                     // by DLK_PAGED_FEW, DLK_PAGED_MANY
+    Index partials = 0;             // rows of partials
+    Index shared_splits = 0, shared_stride = 0, merge_count = 0, merge_most = 0;
     Tensor blob; // the arrays below, on the device
     std::size_t tables = 0, merges = 0, positions = 0, places = 0; // byte offsets
     template <class T> const T* at(std::size_t offset) const {

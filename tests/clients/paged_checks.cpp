@@ -62,17 +62,20 @@ int plan(char** arg) {
     // seen[row]: the keys (positions) that the items give the row, per slot; whole: rows whose output an item writes
     using Keys = std::vector<char>;
     std::map<std::pair<Index, Index>, Keys> whole;                      // (token, g)
-    std::map<std::pair<Index, Index>, std::pair<std::pair<Index, Index>, Keys>> partials[3]; // (slot, r) -> row, keys
-    for (int kind = 0; kind < 3; ++kind) {
+    std::map<Index, std::pair<std::pair<Index, Index>, Keys>> partials; // place -> row, keys
+    Index fronts = 0;
+    for (int kind = 0; kind < 2; ++kind) {
         const auto& list = p.lists[kind];
         const auto* items = p.at<dlk_paged_item>(list.items);
         const Index rows = list.rows;
-        const bool front = kind == DLK_PAGED_SHARED;
+        expect(kind == DLK_PAGED_MANY ? rows == 128 : rows == 16 || rows == 32, "rows of a list");
         for (Index n = 0; n < list.count; ++n) {
             const dlk_paged_item& i = items[n];
-            expect(i.row_begin % rows == 0 && i.row_end > i.row_begin && i.row_end - i.row_begin <= rows, "rows of an item");
+            const bool front = i.first == 1 << 30;
+            fronts += front;
+            expect(i.row_end > i.row_begin && i.row_end - i.row_begin <= rows, "rows of an item");
             expect(i.key_begin >= 0 && i.key_begin % 32 == 0 && i.key_end > i.key_begin, "keys of an item");
-            expect(i.slot >= -1 && i.slot < list.slots, "slot");
+            expect(i.slot == -1 || (i.slot >= 0 && i.slot + i.row_end - i.row_begin <= p.partials), "slot");
             for (Index r = i.row_begin; r < i.row_end; ++r) {
                 const Index token = i.token + r / G;
                 expect(token >= 0 && token < T, "token of a row");
@@ -88,7 +91,7 @@ int plan(char** arg) {
                 }
                 const auto row = std::pair(token, r % G);
                 if (i.slot < 0) expect(whole.emplace(row, keys).second, "output written twice");
-                else expect(partials[kind].emplace(std::pair<Index, Index>(i.slot, r % rows), std::pair(row, keys)).second, "slot written twice");
+                else expect(partials.emplace(i.slot + r - i.row_begin, std::pair(row, keys)).second, "slot written twice");
             }
             // the pages that the item's loads may touch, to the end of its last tile's live keys
             for (Index key = i.key_begin; key < i.key_end; ++key) {
@@ -102,24 +105,22 @@ int plan(char** arg) {
         const dlk_paged_merge& m = merges[n];
         for (Index g = 0; g < G; ++g) {
             Keys keys(static_cast<std::size_t>(position[m.token]) + 1, 0);
-            auto add = [&](int kind, Index slot, Index r) {
-                const auto found = partials[kind].find({slot, r});
-                expect(found != partials[kind].end(), "merge of a slot that nobody writes");
+            auto add = [&](Index slot) {
+                const auto found = partials.find(slot);
+                expect(found != partials.end(), "merge of a slot that nobody writes");
                 expect(found->second.first == std::pair<Index, Index>(m.token, g), "merge of another row's slot");
                 for (std::size_t k = 0; k < keys.size(); ++k) keys[k] += found->second.second[k];
             };
-            expect(m.list == DLK_PAGED_FEW || m.list == DLK_PAGED_MANY, "list of a merge");
-            const Index rows = p.lists[m.list].rows, row = m.row + g, shared_rows = p.lists[DLK_PAGED_SHARED].rows, front = m.shared_row + g;
-            for (Index s = 0; s < m.count; ++s) add(m.list, m.slot + row / rows * m.stride + s, row % rows);
-            for (Index s = 0; s < p.shared_splits; ++s) add(DLK_PAGED_SHARED, front / shared_rows * p.shared_splits + s, front % shared_rows);
+            for (Index s = 0; s < m.count; ++s) add(m.slot + s * m.stride + g);
+            for (Index s = 0; s < p.shared_splits; ++s) add(m.shared_slot + s * p.shared_stride + g);
             expect(whole.emplace(std::pair(Index(m.token), g), keys).second, "output written twice");
         }
     }
     expect(static_cast<Index>(whole.size()) == T * G, "row without an output");
     for (const auto& [row, keys] : whole)
         for (char n : keys) expect(n == 1, "key left out or seen twice");
-    std::printf("%lld %lld %lld %lld\n", static_cast<long long>(T), static_cast<long long>(p.lists[0].count + p.lists[1].count),
-                static_cast<long long>(p.lists[2].count), static_cast<long long>(p.merge_count));
+    std::printf("%lld %lld %lld %lld\n", static_cast<long long>(T), static_cast<long long>(p.lists[0].count + p.lists[1].count - fronts),
+                static_cast<long long>(fronts), static_cast<long long>(p.merge_count));
     return 0;
 }
 
