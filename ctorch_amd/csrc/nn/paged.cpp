@@ -134,7 +134,7 @@ PagedBatch::PagedBatch(const PagedKVCache& cache, Index heads, std::span<const I
         for (Index i = 0; counts[b] > 0 && i < lengths[b] / page; ++i)
             if (written[static_cast<std::size_t>(tables[b * width + i])])
                 refuse("page " + std::to_string(tables[b * width + i]) + " is written and belongs to another place too");
-    if (tokens > INT32_MAX / heads) refuse("too many new positions");
+    if (tokens > INT32_MAX / heads || tokens >= 1 << 30) refuse("too many new positions");
     plan->tokens = tokens;
 
     // Row tiles: of 128 for the waves to split, and what is left, if it is no more than 32, like runs of few rows in one of

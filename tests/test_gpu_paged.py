@@ -199,6 +199,24 @@ def test_attention_over_pages(case, dtype, query):
         assert np.array_equal(ct.paged_attention(step.cache, 0, step.again(), q).numpy(), got.numpy())
 
 
+@pytest.mark.parametrize("seed", range(10))
+def test_random_batches(seed):
+    """Runs of few rows, of many and what is left of them side by side, with and without a prefix."""
+    order = random.Random(seed)
+    kv, dim, page = order.choice([1, 2, 4]), order.choice([16, 32, 64, 128]), order.choice([16, 32, 128])
+    heads, shared = kv * order.choice([1, 3, 4, 7, 8]), order.choice([0, 0, page, 9 * page])
+    batch = order.randint(1, 9)
+    counts = [order.choice([0, 1, 1, 2, 5, 17, order.randint(20, 180)]) for _ in range(batch)]
+    counts[0] = max(counts[0], 1)
+    lengths = [shared + order.choice([0, 1, 31, order.randint(0, 300), order.randint(0, 1800)]) for _ in range(batch)]
+    for dtype, query in (("f32", "f32"), ("bf16", "f32"), ("bf16", "bf16")):
+        say(f"case: paged attention {lengths} {counts} heads {heads} of {kv}, {dim}, page {page}, shared {shared}, {dtype} {query}")
+        step = Step(lengths, counts, heads, kv, dim, page, dtype, shared, 100 + seed)
+        q, values = spans(step.tokens, heads, dim, query, step.rng, 0)
+        want, bound = step.attend(values)
+        assert np.all(np.abs(ct.paged_attention(step.cache, 0, step.batch, q).numpy() - want) <= bound)
+
+
 def test_a_prefix_shared_or_not_is_the_same_attention():
     step = Step([2048 + 40, 2048, 2048 + 700], [1, 2, 20], 32, 8, 64, 32, "bf16", 2048, 4)
     q, values = spans(step.tokens, 32, 64, "f32", step.rng, 0)
