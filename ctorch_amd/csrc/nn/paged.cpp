@@ -4,6 +4,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <numeric>
 #include <stdexcept>
 
 namespace dl::nn {
@@ -33,46 +34,57 @@ PagedKVCache::PagedKVCache(Index layers, Index pages, Index page_size, Index kv_
 
 namespace {
 
-// A list whose row tiles see `seen` keys each, for every KV head, and what its work-groups take.
+// Row tiles of one kind that see `seen` keys each, for every KV head, and what their work-groups take.
 struct Load {
     std::vector<Index> seen;
     Index kv_heads, head_dim, rows, used_rows; // used: the most rows that a tile really has
-    bool f32, merged;                          // merged: its rows are merged anyway (with a prefix)
+    bool f32;
+    bool merged; // the rows are merged anyway (with a prefix)
+    bool beside; // there are tiles of many rows in the launch
 };
 
-// Keys per item: the split with the smallest time by this account, in microseconds (measured on MI355X):
-// - `slots` work-groups run at once, and take `rate` keys a microsecond each then: of few rows what memory gives (5.4
-//   TB/s), of many what the matrix cores do (8500 / (products of a pair's entry, twice the head size): 22 keys for bf16 pages
-//   and heads of 64, 11 for heads of 128 or f32 pages).  Fewer of them run faster: of few rows in proportion, until each CU
-//   has one; one of many rows that has a CU to itself 1.75 times;
-// - an item takes 5 more to begin and to end; the last ones run alone for half an item, of many rows, where the longest
-//   come first, a sixth;
-// - a merge takes 6, and its partials, written and read, their bytes at 2.5 TB/s, those of few rows or a prefix at 1.5.
-// (8 sequences of 32768 keys: 64 items of 2048 keys a head 133 us, of 768 124, of 256 139; 3000 new rows after 1000: whole
-// 335 us, in 512 keys 366; 16 runs of 192 rows after up to 2000 keys, 256 work-groups: whole 58 us, in 1024 keys 44.  Over 36
-// such batches of many rows the choice is 1.5 % off the best of seven sizes in the mean, 12 % at most.)
+// Keys per item: the split with the smallest time by this account, in microseconds (measured on MI355X).  `slots` work-groups
+// run at once; `rate` is what each takes in a microsecond then, in keys.
+// Few rows: memory gives 5.4 TB/s to all.  The items run in rounds of `slots`; in the last, of fewer, each is faster, up to
+// three times, and the longest counts.  An item takes 4 more to begin and to end, a merge 6, and the partials, written and
+// read, their bytes at 2.5 TB/s.
+// Many rows: 8500 / (products of a pair's entry, twice the head size), what the matrix cores do: 22 keys for bf16 pages and
+// heads of 64, 11 for heads of 128 or f32 pages; a work-group with a CU to itself 1.75 times that.  An item takes 5 more; the
+// last ones, the longest having come first, run a sixth of an item alone.  The bytes of partials go at 2.5 TB/s, of a prefix at 1.5.
+// (8 sequences of 32768 keys, a row each: 64 items of 2048 keys a head 133 us, of 768 124, of 256 139.  64 runs of 5 after up to
+// 1000, f32: items of 256 61 us, whole 48.  3000 new rows after 1000: whole 335 us, in 512 keys 366.  16 runs of 192 rows
+// after up to 2000 keys, 256 work-groups: whole 58 us, in 1024 keys 44.  Over 32 batches of few rows the choice is 2 % off the
+// best of seven sizes in the mean, 11 % at most, over 36 of many 1.5 and 12 %.)
 Index chunk_of(const Load& load) {
     if (load.seen.empty()) return 256;
-    const bool many = load.rows == 128;
-    const double per_cu = many || load.head_dim == 128 ? 2.0 : 4.0, slots = 256.0 * per_cu, heads = static_cast<double>(load.kv_heads);
-    const double rate = many ? 8500.0 / static_cast<double>(load.head_dim * (load.f32 ? 12 : 6))
-                             : 5.4e6 / (slots * static_cast<double>(load.head_dim * (load.f32 ? 8 : 4)));
+    const bool many = load.rows == 128, wide = load.head_dim == 128;
+    // what registers and LDS leave room for
+    const Index per_cu = many || load.beside ? 2 : load.f32 ? (load.rows == 32 ? 2 : wide ? 3 : 4) : wide ? 2 : 4;
+    const double slots = 256.0 * static_cast<double>(per_cu), heads = static_cast<double>(load.kv_heads);
+    const double dim = static_cast<double>(load.head_dim), partial = heads * static_cast<double>(load.used_rows) * dim * 8.0;
+    const double rate = many ? 8500.0 / (dim * (load.f32 ? 12.0 : 6.0)) : 5.4e6 / (slots * dim * (load.f32 ? 8.0 : 4.0));
     const Index longest = *std::max_element(load.seen.begin(), load.seen.end());
+    const double work = static_cast<double>(std::accumulate(load.seen.begin(), load.seen.end(), Index(0)));
     double best = 0.0;
     Index chosen = 0;
     for (Index chunk = 128, step = 1;; chunk += 128 * step) {
-        double work = 0.0, items = 0.0, partials = 0.0;
+        Index items = 0, partials = 0;
         for (const Index keys : load.seen) {
-            const double n = static_cast<double>((keys + chunk - 1) / chunk);
-            work += static_cast<double>(keys);
+            const Index n = (keys + chunk - 1) / chunk;
             items += n;
-            if (n > 1.0 || load.merged) partials += n;
+            if (n > 1 || load.merged) partials += n;
         }
-        const double most = static_cast<double>(std::min(chunk, longest));
-        const double own = rate * (many ? 1.75 : std::clamp(slots / (items * heads), 1.0, per_cu)); // a work-group's rate
-        double time = std::max(most / own + 5.0, (work / rate + 5.0 * items) * heads / slots + most / rate / (many ? 6.0 : 2.0));
-        if (partials > 0.0)
-            time += (load.merged ? 0.0 : 6.0) + partials * heads * static_cast<double>(load.used_rows * load.head_dim * 8) / (many && !load.merged ? 2.5e6 : 1.5e6);
+        const double n = static_cast<double>(items), most = static_cast<double>(std::min(chunk, longest));
+        double time;
+        if (many) {
+            time = std::max(most / rate / 1.75 + 5.0, (work / rate + 5.0 * n) * heads / slots + most / rate / 6.0);
+        } else {
+            const double rounds = std::floor(n * heads / slots), rest = n * heads - rounds * slots;
+            time = rounds * (4.0 + work / n / rate);
+            if (rest > 0.0) time += 4.0 + most / (rate * std::min(slots / rest, 3.0));
+        }
+        if (partials > 0)
+            time += (load.merged ? 0.0 : 6.0) + static_cast<double>(partials) * partial / (many && load.merged ? 1.5e6 : 2.5e6);
         if (chosen == 0 || time < best) best = time, chosen = chunk;
         if (chunk >= longest) return chosen;
         if (chunk >= 1024 * step) step *= 2;
@@ -167,8 +179,10 @@ PagedBatch::PagedBatch(const PagedKVCache& cache, Index heads, std::span<const I
 
     // how many keys an item takes: of the runs' own (behind the shared ones), and of the shared ones
     Load loads[2];
+    bool beside = shared > 0 && tokens * group > few;
+    for (Index b = 0; b < batch; ++b) beside = beside || counts[b] * group > few;
     const auto load_of = [&](int kind, bool merged) {
-        return Load{{}, cache.kv_heads(), cache.head_dim(), lists[kind].rows, 1, cache.dtype() == DType::f32, merged};
+        return Load{{}, cache.kv_heads(), cache.head_dim(), lists[kind].rows, 1, cache.dtype() == DType::f32, merged, beside};
     };
     for (int kind = 0; kind < 2; ++kind) loads[kind] = load_of(kind, shared > 0);
     for (Index b = 0; b < batch; ++b) {
