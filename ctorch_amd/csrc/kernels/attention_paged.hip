@@ -198,7 +198,7 @@ template <int N, typename S> __device__ __forceinline__ void soften(S (&s)[N], f
 // Up to 16 NT rows over a range of keys: the four waves split the range, each streams its run in tiles of 16 NU keys from
 // memory into registers and keeps its own softmax, and they merge in LDS.  Bound by memory: a tile's keys and values are
 // asked for as soon as the registers of the ones before are free, and the waves of a SIMD hide each other's waits.  (32
-// tokens over up to 4096 bf16 keys, 8 heads of 64: 34 us, 4.9 TB/s; 8 over up to 32768, heads of 128: 118 us, 5.5 TB/s.)
+// tokens over up to 4096 bf16 keys, 8 heads of 64: 34 us, 4.9 TB/s; 8 over up to 32768, heads of 128: 122 us, 5.4 TB/s.)
 //
 // bf16: V goes through the wave's own LDS tile, stored as it comes and read back by columns; the cut queries of two row
 // tiles stay in LDS, where one tile's fit the registers.  f32: no LDS; with the keys of step j of the second product chosen
