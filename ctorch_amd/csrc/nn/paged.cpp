@@ -53,13 +53,13 @@ struct Load {
 // last ones, the longest having come first, run a sixth of an item alone.  The bytes of partials go at 2.5 TB/s, of a prefix at 1.5.
 // (8 sequences of 32768 keys, a row each: 64 items of 2048 keys a head 133 us, of 768 124, of 256 139.  64 runs of 5 after up to
 // 1000, f32: items of 256 61 us, whole 48.  3000 new rows after 1000: whole 335 us, in 512 keys 366.  16 runs of 192 rows
-// after up to 2000 keys, 256 work-groups: whole 58 us, in 1024 keys 44.  Over 32 batches of few rows the choice is 2 % off the
-// best of seven sizes in the mean, 11 % at most, over 36 of many 1.5 and 12 %.)
+// after up to 2000 keys, 256 work-groups: whole 58 us, in 1024 keys 44.  Over 120 batches of few rows the choice is 4 % off
+// the best of seven sizes in the mean, a third at most, over 36 of many 1.5 and 12 %.)
 Index chunk_of(const Load& load) {
     if (load.seen.empty()) return 256;
     const bool many = load.rows == 128, wide = load.head_dim == 128;
     // what registers and LDS leave room for
-    const Index per_cu = many || load.beside ? 2 : load.f32 ? (load.rows == 32 ? 2 : wide ? 3 : 4) : wide ? 2 : 4;
+    const Index per_cu = many || load.beside ? 2 : !load.f32 ? (wide ? 2 : 4) : load.rows == 32 && load.head_dim >= 64 ? 2 : wide ? 3 : 4;
     const double slots = 256.0 * static_cast<double>(per_cu), heads = static_cast<double>(load.kv_heads);
     const double dim = static_cast<double>(load.head_dim), partial = heads * static_cast<double>(load.used_rows) * dim * 8.0;
     const double rate = many ? 8500.0 / (dim * (load.f32 ? 12.0 : 6.0)) : 5.4e6 / (slots * dim * (load.f32 ? 8.0 : 4.0));
