@@ -250,8 +250,11 @@ struct Weights {
           draft(d.refused && v.draft ? v.draft + (b * v.drafts + d.kept) * v.vocabulary : nullptr), p(d.p.largest, v.inverse),
           q(d.q.largest, v.inverse), p_scale(d.p.scale), q_scale(d.q.scale),
           out(d.refused && !v.draft ? v.drafted[b * v.drafts + d.kept] : -1) {}
-    // the target's weight of entry i, whose logits are l and, with a draft's row, m, and what it has over the draft's
+    // the target's weight of entry i, whose logits are l and, with a draft's row, m, and what it has over the draft's.  Both
+    // products are rounded before they are subtracted: fused into the subtraction, one would leave the other's rounding where
+    // the two are equal, and rows that agree would be drawn from by that instead of by p.
     __device__ __forceinline__ double of(float l, float m, int64_t i, double& over) const {
+#pragma clang fp contract(off)
         const double w = p(l) * p_scale;
         const double rest = w - (draft ? q(m) * q_scale : i == out ? 1.0 : 0.0);
         over = rest < 0.0 ? 0.0 : rest; // (a NaN stays)

@@ -190,3 +190,22 @@ def test_a_greedy_verification_takes_a_nan_for_the_largest():
     target[0, 1, :] = -np.inf
     tokens, accepted = run(np.array([[4321, 0]]), target, None, 0.0, np.zeros((1, 3)))
     assert accepted[0] == 2 and tokens[0].tolist() == [4321, 0, int(target[0, 2].argmax())]
+
+
+@pytest.mark.parametrize("V", [5, 300, 1024, 5000, 32000])
+@pytest.mark.parametrize("t", [0.7, 1.0, 3.0])
+def test_a_refusal_where_both_models_agree_draws_from_the_target(V, t):
+    """Rows that are the same for both models leave nothing of p - q, not even a rounding: the token comes from p.  (The draft
+    has no weight in either, so that 0 < 0 refuses it.)"""
+    say(f"case: verify, equal rows, V={V} T={t}")
+    rng = np.random.default_rng(V)
+    target = (rng.standard_normal((8, 2, V)) * 3).astype(np.float32)
+    drafted = rng.integers(0, V, (8, 1))
+    for b in range(8):
+        target[b, 0, drafted[b, 0]] = -np.inf if b % 2 else -2400.0  # exp(-800) at most: no number of 64 bits
+    u = rng.random((8, 2)).astype(np.float32)
+    u[0, 1], u[1, 1] = 0.0, 1 - 2.0 ** -24
+    tokens, accepted, near = verify(drafted, target, target[:, :1], t, u)
+    assert near > 1e-12 and not accepted.any()  # (a property of the inputs)
+    got = run(drafted, target, target[:, :1], t, u)
+    assert np.array_equal(got[1], accepted) and np.array_equal(got[0], tokens), (got[0][:, 0], tokens[:, 0])
