@@ -341,7 +341,7 @@ int dlk_sample_finalize(const dlk_sample_partial* partial, int64_t rows, int blo
 /* ------------------------------------------------------------------------------------------------------
  * Verification of drafted tokens (verify.hip): target [batch, drafts + 1, vocabulary], draft [batch, drafts, vocabulary]
  * or NULL, uniforms [batch, drafts + 1], all f32 contiguous; drafted [batch, drafts], a negative id ends a row.
- * inverse = 1 / temperature (at most 1e30), or 0: the largest logit decides.
+ * inverse = 1 / temperature (at most 1e300), or 0: the largest logit decides.
  * ---------------------------------------------------------------------------------------------------- */
 typedef struct dlk_verify_slice { /* a slice of a row of logits: its largest, and the sum of exp((l - largest) / T) */
     double sum;

@@ -56,15 +56,18 @@ __device__ __forceinline__ double fma_constant(double a, double b, double c) {
 // here: (l - largest) inverse = n ln 2 + r, |r| <= ln 2 / 2, and the polynomial of degree 8 through exp at the Chebyshev
 // points of that range.  n is found in f32, where being off by one part in 10^6 only moves r.  A third of the instructions
 // of the library's exp, which bound the pass over the logits.  0 below exp(-700); a NaN stays.
-struct Exponential {
+// WIDE: n is found from the difference in f64, for temperatures whose inverse, or the difference of two logits times it, f32
+// does not hold (-inf times an inverse that became 0 is no number).  An instruction an entry more, so only for those.
+template <bool WIDE> struct Exponential {
     double largest, inverse;
     float largest32, inverse32;
     __device__ __forceinline__ Exponential(double largest_, double inverse_)
         : largest(largest_), inverse(inverse_), largest32(static_cast<float>(largest_)), inverse32(static_cast<float>(inverse_)) {}
     __device__ __forceinline__ double operator()(float l) const {
-        const float about = (l - largest32) * inverse32;
+        const double x = (static_cast<double>(l) - largest) * inverse;
+        const float about = WIDE ? static_cast<float>(x) : (l - largest32) * inverse32;
         const float n = __builtin_rintf(about * 1.44269504f);
-        const double x = (static_cast<double>(l) - largest) * inverse, nd = n;
+        const double nd = n;
         const double r = __builtin_fma(nd, -0x1.62e42fefa39efp-1, x);
         double y = fma_constant(r, 0x1.a15a60062d0e8p-16, 0x1.a1aa939e66a93p-13);
         y = fma_constant(y, r, 0x1.6c164de86c8c8p-10);
@@ -91,7 +94,7 @@ __device__ __forceinline__ const dlk_verify_slice* slices_of(const dlk_verify_pa
     return p.rows + (b * (2 * p.drafts + 1) + row) * p.slices;
 }
 
-template <bool GREEDY>
+template <bool GREEDY, bool WIDE>
 __global__ __launch_bounds__(kThreads) void verify_rows(const dlk_verify_params p) {
     __shared__ double sums[kWaves];
     __shared__ float tops[kWaves];
@@ -136,7 +139,7 @@ __global__ __launch_bounds__(kThreads) void verify_rows(const dlk_verify_params 
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) top = fmaxf(top, tops[w]);
-        const Exponential weight(top == -INFINITY ? 0.0 : top, p.inverse);
+        const Exponential<WIDE> weight(top == -INFINITY ? 0.0 : top, p.inverse);
         double sum = 0.0;
 #pragma unroll
         for (int j = 0; j < kHeld; j += 4)
@@ -177,7 +180,7 @@ struct Decision {
 };
 
 // What is kept of sequence b, by the whole work-group.
-__device__ __forceinline__ Decision decide(const dlk_verify_params& p, int64_t b) {
+template <bool WIDE> __device__ __forceinline__ Decision decide(const dlk_verify_params& p, int64_t b) {
     __shared__ int stop;
     __shared__ Row rows[2][kStep];
     const int t = threadIdx.x, n = static_cast<int>(p.drafts), team = t / kTeam, member = t % kTeam;
@@ -208,7 +211,7 @@ __device__ __forceinline__ Decision decide(const dlk_verify_params& p, int64_t b
 #pragma unroll
             for (int offset = kTeam / 2; offset > 0; offset >>= 1) top = fmaxf(top, __shfl_xor(top, offset, kWave));
             const double next = fmax(largest, static_cast<double>(top));
-            const Exponential weight(next == -INFINITY ? 0.0 : next, p.inverse); // (slices of -inf weigh nothing)
+            const Exponential<WIDE> weight(next == -INFINITY ? 0.0 : next, p.inverse); // (slices of -inf weigh nothing)
             if (begin > 0) sum *= weight(static_cast<float>(largest));
             largest = next;
 #pragma unroll
@@ -223,8 +226,8 @@ __device__ __forceinline__ Decision decide(const dlk_verify_params& p, int64_t b
             bool keep = inside;
             if (keep) {
                 double q = 1.0;
-                if (p.draft) q = Exponential(rows[1][t].largest, p.inverse)(draft_logit) * rows[1][t].scale;
-                keep = uniform * q < Exponential(rows[0][t].largest, p.inverse)(target_logit) * rows[0][t].scale;
+                if (p.draft) q = Exponential<WIDE>(rows[1][t].largest, p.inverse)(draft_logit) * rows[1][t].scale;
+                keep = uniform * q < Exponential<WIDE>(rows[0][t].largest, p.inverse)(target_logit) * rows[0][t].scale;
             }
             if (!keep) atomicMin(&stop, step);
         }
@@ -239,10 +242,10 @@ __device__ __forceinline__ Decision decide(const dlk_verify_params& p, int64_t b
 }
 
 // What the token behind the kept ones is drawn with: p, less q where a draft was refused.
-struct Weights {
+template <bool WIDE> struct Weights {
     const float* target;
     const float* draft; // the refused draft's row, or NULL
-    Exponential p, q;
+    Exponential<WIDE> p, q;
     double p_scale, q_scale;
     int64_t out;        // a certain draft that was refused, or -1
     __device__ __forceinline__ Weights(const dlk_verify_params& v, int64_t b, const Decision& d)
@@ -263,12 +266,12 @@ struct Weights {
 };
 
 // a work-group per 1024 entries of a sequence's row
-__global__ __launch_bounds__(kThreads) void verify_weights(const dlk_verify_params p) {
+template <bool WIDE> __global__ __launch_bounds__(kThreads) void verify_weights(const dlk_verify_params p) {
     __shared__ double sums[2][kWaves];
     const int t = threadIdx.x;
     const uint32_t parts = static_cast<uint32_t>((p.vocabulary + kDraw - 1) / kDraw), part = blockIdx.x % parts;
     const int64_t b = blockIdx.x / parts;
-    const Decision d = decide(p, b);
+    const Decision d = decide<WIDE>(p, b);
     if (part == 0 && t == 0) {
         p.accepted[b] = d.kept;
         p.decisions[4 * b] = d.p.largest;
@@ -276,7 +279,7 @@ __global__ __launch_bounds__(kThreads) void verify_weights(const dlk_verify_para
         p.decisions[4 * b + 2] = d.q.largest;
         p.decisions[4 * b + 3] = d.refused ? d.q.scale : -1.0;
     }
-    const Weights weights(p, b, d);
+    const Weights<WIDE> weights(p, b, d);
     const int64_t begin = static_cast<int64_t>(part) * kDraw;
     float l[kDrawHeld], m[kDrawHeld];
 #pragma unroll
@@ -304,7 +307,7 @@ __global__ __launch_bounds__(kThreads) void verify_weights(const dlk_verify_para
 }
 
 // a work-group per sequence
-__global__ __launch_bounds__(kThreads) void verify_draw(const dlk_verify_params p) {
+template <bool WIDE> __global__ __launch_bounds__(kThreads) void verify_draw(const dlk_verify_params p) {
     __shared__ double sums[kWaves];
     __shared__ int first_index, last_index;
     __shared__ double best_s[kWaves];
@@ -322,7 +325,7 @@ __global__ __launch_bounds__(kThreads) void verify_draw(const dlk_verify_params 
         kept = static_cast<int>(p.accepted[b]);
         const Decision d{kept, !(p.decisions[4 * b + 3] < 0.0), {p.decisions[4 * b], p.decisions[4 * b + 1]},
                          {p.decisions[4 * b + 2], p.decisions[4 * b + 3]}};
-        const Weights weights(p, b, d);
+        const Weights<WIDE> weights(p, b, d);
         // every wave goes over the parts' sums alike, 64 at a time: of max(p - q, 0), or of p where that is zero or nothing
         // was refused
         int of = d.refused ? 0 : 1;
@@ -448,13 +451,20 @@ extern "C" int dlk_verify(const dlk_verify_params* params, dlh_stream stream_han
     const int64_t groups = p.batch * (p.drafts + 1 + (p.draft ? p.drafts : 0)) * p.slices;
     const int64_t parts = p.batch * ((p.vocabulary + dlk::kDraw - 1) / dlk::kDraw);
     if (groups > INT32_MAX || parts > INT32_MAX) return static_cast<int>(hipErrorInvalidValue);
-    const dim3 threads(dlk::kThreads);
-    if (p.inverse > 0.0) {
-        hipLaunchKernelGGL(dlk::verify_rows<false>, dim3(groups), threads, 0, stream, p);
-        hipLaunchKernelGGL(dlk::verify_weights, dim3(parts), threads, 0, stream, p);
+    const dim3 threads(dlk::kThreads), rows(groups), sequences(p.batch);
+    // between 2^-100 and 2^100 f32 holds the inverse, and two logits that are further apart than f32 counts weigh nothing
+    const bool wide = p.inverse < 0x1p-100 || p.inverse > 0x1p100;
+    if (!(p.inverse > 0.0)) {
+        hipLaunchKernelGGL((dlk::verify_rows<true, false>), rows, threads, 0, stream, p);
+        hipLaunchKernelGGL(dlk::verify_draw<false>, sequences, threads, 0, stream, p);
+    } else if (wide) {
+        hipLaunchKernelGGL((dlk::verify_rows<false, true>), rows, threads, 0, stream, p);
+        hipLaunchKernelGGL(dlk::verify_weights<true>, dim3(parts), threads, 0, stream, p);
+        hipLaunchKernelGGL(dlk::verify_draw<true>, sequences, threads, 0, stream, p);
     } else {
-        hipLaunchKernelGGL(dlk::verify_rows<true>, dim3(groups), threads, 0, stream, p);
+        hipLaunchKernelGGL((dlk::verify_rows<false, false>), rows, threads, 0, stream, p);
+        hipLaunchKernelGGL(dlk::verify_weights<false>, dim3(parts), threads, 0, stream, p);
+        hipLaunchKernelGGL(dlk::verify_draw<false>, sequences, threads, 0, stream, p);
     }
-    hipLaunchKernelGGL(dlk::verify_draw, dim3(p.batch), dim3(dlk::kThreads), 0, stream, p);
     return static_cast<int>(hipGetLastError());
 }

@@ -483,7 +483,8 @@ std::pair<Tensor, Tensor> verify_drafted(const Tensor& drafted, const Tensor& ta
     p.batch = batch;
     p.drafts = drafts;
     p.vocabulary = vocabulary;
-    p.inverse = temperature > 0.0 ? std::min(1.0 / temperature, 1e30) : 0.0;
+    // (two logits that differ are 1e-45 apart at least: from 1e300 on the smaller one weighs nothing)
+    p.inverse = temperature > 0.0 ? std::min(1.0 / temperature, 1e300) : 0.0;
     p.slices = slices;
     p.slice = (vocabulary + slices - 1) / slices;
     p.rows = static_cast<dlk_verify_slice*>(mutable_data(work));

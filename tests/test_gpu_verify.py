@@ -209,3 +209,29 @@ def test_a_refusal_where_both_models_agree_draws_from_the_target(V, t):
     assert near > 1e-12 and not accepted.any()  # (a property of the inputs)
     got = run(drafted, target, target[:, :1], t, u)
     assert np.array_equal(got[1], accepted) and np.array_equal(got[0], tokens), (got[0][:, 0], tokens[:, 0])
+
+
+@pytest.mark.parametrize("t", [1e-250, 1e-33, 1e-29, 1e29, 1e31, 1e38, 1e46, 1e300])
+@pytest.mark.parametrize("V", [3, 50, 1500, 5001])
+@pytest.mark.parametrize("kind", ["draft", "certain"])
+def test_temperatures_beyond_32_bits(V, t, kind):
+    """Any finite temperature: masked logits weigh nothing, and logits as far apart as the type holds what they weigh."""
+    say(f"case: verify V={V} T={t} {kind}")
+    rng = np.random.default_rng(V)
+    unit = np.float32(1e38 if t >= 1e37 and V != 50 else np.clip(t, 1e-33, 1.0))  # (V = 50: ordinary logits)
+    target = (np.clip(rng.standard_normal((6, 3, V)), -3, 3)).astype(np.float32) * unit
+    draft = (np.clip(rng.standard_normal((6, 2, V)), -3, 3)).astype(np.float32) * unit
+    target[1::2, :, 0] = draft[1::3, :, 0] = -np.inf
+    target[2::4, :, V // 2] = np.finfo(np.float32).min
+    drafted = rng.integers(0, V, (6, 2))
+    drafted[1::2, 1] = 0
+    drafted[2::4, 0] = V // 2
+    u = rng.random((6, 3)).astype(np.float32)
+    u[4, :2] = 0.0
+    given = draft if kind == "draft" else None
+    tokens, accepted, near = verify(drafted, target, given, t, u)
+    # a property of the inputs (at 1e-250 weights are equal or nothing, and the decisions exact where they meet their border)
+    assert near > 1e-9 or t < 1e-200
+    got = run(drafted, target, given, t, u)
+    assert np.array_equal(got[1], accepted), (got[1], accepted)
+    assert np.array_equal(got[0], tokens), (got[0], tokens)
