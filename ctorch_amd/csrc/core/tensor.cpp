@@ -18,6 +18,19 @@ Shape contiguous_strides(const Shape& shape) {
     return strides;
 }
 
+// (The axes that are not empty count for the limit: strides are made of them, also in a tensor without elements.)
+Index element_count(const Shape& shape) {
+    Index all = 1;
+    bool empty = false;
+    for (Index s : shape) {
+        if (s < 0) throw std::invalid_argument("tensor dimensions must be non-negative");
+        if (s == 0) empty = true;
+        else if (__builtin_mul_overflow(all, s, &all) || all > INT64_MAX / 16)
+            throw std::invalid_argument("a tensor of shape " + shape_string(shape) + " has too many elements");
+    }
+    return empty ? 0 : all;
+}
+
 std::string shape_string(const Shape& shape) {
     std::string out = "[";
     for (std::size_t i = 0; i < shape.size(); ++i) out += (i ? ", " : "") + std::to_string(shape[i]);
@@ -36,13 +49,12 @@ int dlk_dtype(DType dtype) {
 }
 
 Tensor empty_tensor(const Shape& shape, DType dtype, Device device) {
-    for (Index s : shape)
-        if (s < 0) throw std::invalid_argument("tensor dimensions must be non-negative");
+    const Index count = element_count(shape);
     auto impl = std::make_shared<TensorImpl>();
     impl->shape = shape;
     impl->strides = contiguous_strides(shape);
     impl->dtype = dtype;
-    impl->storage = allocate_storage(static_cast<std::size_t>(impl->numel()) * element_size(dtype), device);
+    impl->storage = allocate_storage(static_cast<std::size_t>(count) * element_size(dtype), device);
     return TensorAccess::make(std::move(impl));
 }
 
@@ -174,15 +186,14 @@ Tensor view_of(const detail::TensorImpl& base, Shape shape, Shape strides, Index
     return TensorAccess::make(std::move(impl));
 }
 Shape resolve_shape(Shape shape, Index numel) {
-    Index known = 1, infer = -1;
+    Index infer = -1;
     for (std::size_t i = 0; i < shape.size(); ++i) {
-        if (shape[i] == -1) {
-            if (infer >= 0) throw std::invalid_argument("only one -1 is allowed in a shape");
-            infer = static_cast<Index>(i);
-        } else {
-            known *= shape[i];
-        }
+        if (shape[i] != -1) continue;
+        if (infer >= 0) throw std::invalid_argument("only one -1 is allowed in a shape");
+        infer = static_cast<Index>(i);
+        shape[i] = 1;
     }
+    const Index known = detail::element_count(shape);
     if (infer >= 0) {
         if (known == 0 || numel % known != 0) throw std::invalid_argument("shape does not match the element count");
         shape[static_cast<std::size_t>(infer)] = numel / known;

@@ -34,6 +34,8 @@ struct TensorAccess {
 };
 
 Shape contiguous_strides(const Shape& shape);
+/// The elements of a shape; throws where they, or their bytes, are more than an Index counts.
+Index element_count(const Shape& shape);
 /// A new contiguous tensor with uninitialised (host: zeroed) storage.
 Tensor empty_tensor(const Shape& shape, DType dtype, Device device);
 /// Mutable device/host address of the first element.

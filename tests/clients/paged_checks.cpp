@@ -155,6 +155,8 @@ int call(const std::string& name) {
         {"cache heads", [&] { PagedKVCache(1, 8, 16, 0, 32, f32); }},
         {"cache f64", [&] { PagedKVCache(1, 8, 16, 2, 32, {.dtype = dl::DType::f64, .device = gpu}); }},
         {"cache on the host", [&] { PagedKVCache(1, 8, 16, 2, 32, {}); }},
+        {"cache elements", [&] { PagedKVCache(1, Index(1) << 30, 1024, Index(1) << 20, 128, f32); }},
+        {"cache bytes", [&] { PagedKVCache(1, Index(1) << 30, 1024, Index(1) << 15, 128, f32); }},
         {"append layer", [&] { append(k, v, c, s, 2); }},
         {"append layer below", [&] { append(k, v, c, s, -1); }},
         {"append rows", [&] { append(tensor({4, 2, 32}), v, c, s); }},

@@ -124,6 +124,22 @@ def test_an_operator_refuses(name):
     assert run.returncode == 1 and REFUSED[name] in run.stderr, (run.returncode, run.stdout, run.stderr)
 
 
+@pytest.mark.parametrize("name", ["cache elements", "cache bytes"])
+def test_a_cache_whose_size_wraps_is_refused(name):
+    run = checks("call", name)  # 2^67 elements, 2^64 bytes: both nothing in 64 bits
+    assert run.returncode == 1 and "too many elements" in run.stderr, (run.returncode, run.stdout, run.stderr)
+
+
+def test_sizes_that_wrap_are_refused():
+    cpu = ct.device("cpu")
+    for call in (lambda: ct.rotary_tables(32, 2 ** 60, dev=cpu), lambda: ct.rotary_tables(32, 2 ** 58, dev=cpu),
+                 lambda: ct.zeros((2 ** 32, 2 ** 32), ct.F32, cpu), lambda: ct.zeros((2 ** 32, 0, 2 ** 32), ct.F32, cpu),
+                 lambda: ct.zeros((2 ** 61,), ct.F64, cpu)):
+        with pytest.raises(ct.DLError, match="too many elements"):
+            call()
+    assert ct.zeros((2 ** 30, 0, 2 ** 28), ct.F32, cpu).shape == (2 ** 30, 0, 2 ** 28)  # (strides within 2^59)
+
+
 @pytest.mark.parametrize("name", ["append nothing", "attend nothing", "rotary nothing", "verify nothing"])
 def test_nothing_to_do_launches_nothing(name):
     run = checks("call", name)
