@@ -301,6 +301,14 @@ void check_rows(const Tensor& t, Index tokens, Index heads, Index dim, Device de
     if (!(t.device() == device)) throw std::invalid_argument(std::string(operation) + ": " + what + " on another device");
 }
 
+// What lies in the pages that a call writes would be read while it changes: it is read from a copy.
+Tensor apart_from(const nn::PagedKVCache& cache, Index layer, const Tensor& t) {
+    const auto& storage = TensorAccess::impl(t)->storage;
+    for (const Tensor* pages : {&cache.key(layer), &cache.value(layer)})
+        if (storage == TensorAccess::impl(*pages)->storage) return t.clone();
+    return t;
+}
+
 int page_shift(Index page_size) {
     int shift = 0;
     while ((Index(1) << shift) < page_size) ++shift;
@@ -317,7 +325,7 @@ Tensor paged_append(const nn::PagedKVCache& cache, Index layer, const nn::PagedB
     check_rows(key, plan.tokens, kv, dim, cache.device(), name, "key");
     check_rows(value, plan.tokens, kv, dim, cache.device(), name, "value");
     if (query) check_rows(*query, plan.tokens, plan.heads, dim, cache.device(), name, "query");
-    RotaryTables tables(cosine, sine, dim, cache.device(), name);
+    RotaryTables tables(apart_from(cache, layer, cosine), apart_from(cache, layer, sine), dim, cache.device(), name);
     if (plan.last >= tables.capacity())
         throw std::out_of_range(std::string(name) + ": position " + std::to_string(plan.last) + " lies beyond the tables");
     GpuContext& context = gpu_of(key, name);
@@ -329,11 +337,11 @@ Tensor paged_append(const nn::PagedKVCache& cache, Index layer, const nn::PagedB
     p.tokens = plan.tokens;
     p.dim = static_cast<int>(dim);
     if (query) {
-        p.q = row_segment(*query, q, plan.heads, name);
+        p.q = row_segment(apart_from(cache, layer, *query), q, plan.heads, name);
         p.out = static_cast<float*>(mutable_data(out));
     }
-    p.k = row_segment(key, k, kv, name);
-    p.v = row_segment(value, v, kv, name);
+    p.k = row_segment(apart_from(cache, layer, key), k, kv, name);
+    p.v = row_segment(apart_from(cache, layer, value), v, kv, name);
     p.positions = plan.at<Index>(plan.positions);
     p.places = plan.at<Index>(plan.places);
     p.k_pages = mutable_data(cache.key(layer));

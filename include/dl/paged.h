@@ -58,7 +58,8 @@ namespace dl {
 /// Writes the step's keys (rotated at their positions) and values, [tokens, kv_heads, head_dim], to their pages of
 /// `layer`, and returns the queries [tokens, heads, head_dim] rotated likewise (an undefined tensor when there are none).
 /// All three are f32 or bf16 and may be views of one projection output; cosine and sine as for rotary_positions, with a
-/// row for every position of the step.  A bf16 cache rounds each key and value once.
+/// row for every position of the step.  What of them lies in this layer's pages is taken as it was before the call.  A bf16
+/// cache rounds each key and value once.
 DL_API Tensor paged_append(const nn::PagedKVCache& cache, Index layer, const nn::PagedBatch& batch,
                            const std::optional<Tensor>& query, const Tensor& key, const Tensor& value,
                            const Tensor& cosine, const Tensor& sine, RotaryLayout layout);

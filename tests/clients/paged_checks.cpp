@@ -140,6 +140,8 @@ int call(const std::string& name) {
                       const PagedBatch* step = nullptr, std::optional<dl::Tensor> query = std::nullopt, RotaryLayout layout = RotaryLayout::half) {
         return dl::paged_append(cache, layer, step ? *step : batch, query ? query : std::optional<dl::Tensor>{q}, key, value, cosine, sine, layout);
     };
+    // three rows out of a page
+    auto page_rows = [&](const dl::Tensor& pages) { return pages.select(0, 5).transpose(0, 1).narrow(0, 0, 3); };
     const auto x = tensor({5, 2, 32});
     const auto at = tensor({5}, dl::DType::i64);
     const auto ids = tensor({2, 3}, dl::DType::i64);
@@ -170,6 +172,8 @@ int call(const std::string& name) {
         {"append empty tables", [&] { append(k, v, tensor({64, 0}), tensor({64, 0})); }},
         {"append layout", [&] { append(k, v, c, s, 0, nullptr, std::nullopt, static_cast<RotaryLayout>(7)); }},
         {"append nothing", [&] { append(tensor({0, 2, 32}), tensor({0, 2, 32}), c, s, 0, &idle, tensor({0, 4, 32})); }},
+        {"append rows of the pages", [&] { append(page_rows(cache.key(0)), page_rows(cache.value(0)), c, s); }},
+        {"append rows of another layer", [&] { append(page_rows(cache.key(1)), page_rows(cache.value(1)), c, s); }},
         {"attend other cache", [&] { dl::paged_attention(PagedKVCache(2, 8, 32, 2, 32, f32), 0, batch, q); }},
         {"attend other type", [&] { dl::paged_attention(PagedKVCache(2, 8, 16, 2, 32, {.dtype = dl::DType::bf16, .device = gpu}), 0, batch, q); }},
         {"attend fewer pages", [&] { dl::paged_attention(PagedKVCache(2, 7, 16, 2, 32, f32), 0, batch, q); }},

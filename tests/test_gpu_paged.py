@@ -361,6 +361,52 @@ def test_append_without_queries():
     assert np.array_equal(values_of(step.cache.value(0))[pages, :, rows], v[1])
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("by", [1, 16, -7])
+def test_rows_of_the_pages_that_are_written(dtype, by):
+    """Keys and values that lie in the layer's own pages, a few rows from their new places: what was there before the call."""
+    page, dim, count = 1024, 32, 900
+    cache = ct.PagedCache(2, 1, page, 1, dim, TYPES[dtype])
+    rng = np.random.default_rng(by + 8)
+    held = []
+    for layer in range(2):
+        for view in (cache.key(layer), cache.value(layer)):
+            bits = rng.standard_normal(view.shape).astype(np.float32)
+            held.append(oracle.bf16_decode(oracle.bf16_encode(bits)) if dtype == "bf16" else bits)
+            fill(view, held[-1])
+    start = 40  # the new positions; their rows come from `by` further
+    batch = ct.PagedBatch(cache, 1, [start], [count], [[0]])
+    c, s = give(np.ones((page, dim // 2)))[0], give(np.zeros((page, dim // 2)))[0]
+
+    def rows(view):
+        flat = ct.Tensor(ct._new(ct.lib().dl_reshape, view.handle, ct._shape((page, 1, dim))))
+        return ct.narrow(flat, 0, start + by, count)
+
+    query = cache.append(0, batch, rows(cache.value(0)), rows(cache.key(0)), rows(cache.value(0)), c, s).numpy()
+    key, value = (h.reshape(page, dim) for h in held[:2])
+    moved = slice(start + by, start + by + count)
+    assert np.array_equal(query[:, 0], value[moved])
+    for view, old in ((cache.key(0), key), (cache.value(0), value)):
+        want = old.copy()
+        want[start:start + count] = old[moved]
+        assert np.array_equal(values_of(view).reshape(page, dim), want)
+
+
+def test_tables_in_the_pages_that_are_written():
+    page, dim, count = 1024, 32, 1000
+    cache = ct.PagedCache(1, 1, page, 1, dim)
+    fill(cache.key(0), np.ones((1, 1, page, dim)))
+    fill(cache.value(0), np.zeros((1, 1, page, dim)))
+    c, s = (ct.Tensor(ct._new(ct.lib().dl_reshape, view.handle, ct._shape((2 * page, dim // 2))))
+            for view in (cache.key(0), cache.value(0)))
+    k, v = (give(np.random.default_rng(i).standard_normal((count, 1, dim))) for i in range(2))
+    batch = ct.PagedBatch(cache, 1, [0], [count], [[0]])
+    assert np.array_equal(cache.append(0, batch, k[0], k[0], v[0], c, s).numpy(), k[1])
+    for view, want, rest in ((cache.key(0), k[1], 1), (cache.value(0), v[1], 0)):
+        got = values_of(view).reshape(page, 1, dim)
+        assert np.array_equal(got[:count], want) and np.all(got[count:] == rest)
+
+
 def test_a_pool_beyond_4_gib():
     """Pages whose offset passes 32 bits, in bytes and in elements."""
     kv, dim, page = 8, 128, 1024

@@ -146,6 +146,12 @@ def test_nothing_to_do_launches_nothing(name):
     assert run.returncode == 0 and run.stdout.strip() == "0", (run.stdout, run.stderr)
 
 
+@pytest.mark.parametrize("name,launches", [("append rows of the pages", 3), ("append rows of another layer", 1)])
+def test_what_lies_in_the_pages_that_are_written_is_copied_first(name, launches):
+    run = checks("call", name)
+    assert run.returncode == 0 and run.stdout.strip() == str(launches), (run.stdout, run.stderr)
+
+
 # ------------------------------------------------------------------------------------------------ tables
 def frequencies(dims, base, kind, factor, trained, slow, fast):
     i = np.arange(dims // 2, dtype=np.float64)
