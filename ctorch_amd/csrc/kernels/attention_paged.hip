@@ -6,7 +6,8 @@
 // against queries and probabilities cut into three bf16 parts of 8 bits each, which hold all 24 bits of an f32: three
 // products (bf16 queries are one part).  (Two parts, 2^-17 off, gave outputs 4e-6 off the 64-bit ones, three 7e-7.)  f32
 // pages take the f32 matrix instruction where memory is the bound, and three by three parts where the products are, the
-// terms below 2^-24 left out: six products, 2.7 times the f32 instruction's rate.
+// three terms left out that are 2^-22 of a product at most together (typically 2^-24): six products, 2.7 times the f32
+// instruction's rate.
 //   S^T[16 keys][16 rows] = K[16][hd] Q[16][hd]^T    so that a lane holds scores of one row (lane % 16),
 //   O^T[16 d][16 rows]   += V^T[16 d][keys] P^T       and they are the second product's right operand as they come.
 // The softmax runs in base 2 with the running base and sum of each row; keys past a range are masked and their values

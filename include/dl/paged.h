@@ -66,8 +66,10 @@ DL_API Tensor paged_append(const nn::PagedKVCache& cache, Index layer, const nn:
 
 /// Attention of the step's (rotated) queries [tokens, heads, head_dim], f32 or bf16, over the pages of `layer`: the row
 /// at position p sees the positions 0 .. p of its sequence, its own included (append first).  f32 [tokens, heads, head_dim].
-/// What a row does not see may hold anything.  Products are exact to f32: of finite values up to 3e38 and scores q k / sqrt(head_dim) below 2^29;
-/// where a row sees a value that is not finite, that entry of it is not finite either.
+/// What a row does not see may hold anything.  Products keep all bits of an f32 (of f32 queries and weights by f32 keys and
+/// values down to 2^-22 of each product), for finite scores q k / sqrt(head_dim) whose products' magnitudes sum below 2^29 and
+/// for values up to 1e36 over the number of keys that the row sees: they are summed with weights of up to 2^8 before the division.
+/// Where a row sees a value that is not finite, that entry of it is not finite either.
 DL_API Tensor paged_attention(const nn::PagedKVCache& cache, Index layer, const nn::PagedBatch& batch, const Tensor& query);
 
 } // namespace dl

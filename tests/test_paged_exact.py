@@ -157,6 +157,29 @@ def test_products_keep_all_bits(case, dim, pages, queries):
         assert np.all(off <= bound), (kind, float(np.nanmax(off / bound)), np.argwhere(~(off <= bound))[:3])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("pages", ["f32", "bf16"])
+@pytest.mark.parametrize("counts", [[1], [5], [200]])
+@pytest.mark.parametrize("length", [40, 3000])
+def test_the_largest_values(pages, counts, length):
+    """Values of 1e36 over the number of keys, of one sign: their sum by weights of up to 2^8 still is an f32.  Keys of score 0,
+    then one 5 above them, which leaves the row's base where it is, 2^7 below."""
+    from test_gpu_paged import TYPES, fill, give
+
+    say(f"case: largest values, {length} and {counts} pages {pages}")
+    heads, kv, dim, page, keys = 8, 2, 64, 16, length + counts[0]
+    cache = ct.PagedCache(1, -(-keys // page), page, kv, dim, TYPES[pages])
+    value = np.float32(2.0 ** np.floor(np.log2(1e36 / keys)))
+    key = np.zeros((-(-keys // page), kv, page, dim))
+    key[length // 2 // page, :, length // 2 % page, 0] = 40
+    fill(cache.key(0), key)
+    fill(cache.value(0), np.full(key.shape, value))
+    batch = ct.PagedBatch(cache, heads, [length], counts, [np.arange(len(key))])
+    got = ct.paged_attention(cache, 0, batch, give(np.ones((counts[0], heads, dim)))[0]).numpy()
+    # the mean of equal values: keys are added on both sides, a step each
+    assert np.all(np.abs(got / value - 1) <= (4 * keys + 32) * U)
+
+
 def products(a, b, left_out, cut_a=rounded, cut_b=cut_off):
     """a b from three by three parts without those that are left out."""
     return sum(x * y for i, x in enumerate(parts(a, cut_a)) for j, y in enumerate(parts(b, cut_b)) if (i, j) not in left_out)
