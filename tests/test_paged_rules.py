@@ -9,6 +9,7 @@ import pytest
 
 import ctorch_amd as ct
 
+U = 2.0 ** -24
 PROGRAM = os.path.join(os.path.dirname(os.path.abspath(__file__)), "clients", "_build", "paged_checks")
 
 
@@ -187,3 +188,33 @@ def test_the_scalings_keep_what_they_say():
     assert np.isclose(base[0], plain[0]) and np.isclose(base[-1], plain[-1] / 8)
     parts = at((ct.ROTARY_PARTS, 8.0, 8192, 1.0, 32.0))
     assert parts[0] == plain[0] and parts[-1] == plain[-1] / 8
+
+
+@pytest.mark.parametrize("dims,base", [(64, 10000.0), (128, 500000.0)])
+def test_the_tables_scale_as_they_say(dims, base):
+    """The angles of the first position: which pairs a rule leaves alone, which it slows down by the factor, and by how much
+    the others lie in between.  (sin f of f32, off by 2^-24 of it and less than twice that as an angle below 1.)"""
+    cpu = ct.device("cpu")
+
+    def angles(kind, slow=1.0, fast=32.0, magnitude=1.0):
+        rule = ct.RotaryScaling(kind, 8.0, 8192, slow, fast, magnitude)
+        cosine, sine = ct.rotary_tables(dims, 2, base, rule, cpu)
+        return np.arctan2(sine.numpy()[1].astype(np.float64), cosine.numpy()[1].astype(np.float64))
+
+    i = np.arange(dims // 2)
+    plain = angles(ct.ROTARY_UNSCALED)
+    assert np.allclose(plain, base ** (-2 * i / dims), rtol=4 * U, atol=0)
+    assert np.allclose(angles(ct.ROTARY_LINEAR), plain / 8, rtol=8 * U, atol=0)
+    raised = angles(ct.ROTARY_BASE)
+    assert np.allclose(raised, plain * 8.0 ** (-2 * i / (dims - 2)), rtol=8 * U, atol=0)
+    assert np.isclose(raised[0], plain[0], rtol=8 * U) and np.isclose(raised[-1], plain[-1] / 8, rtol=8 * U)
+    parts, turns = angles(ct.ROTARY_PARTS), 8192 * plain / (2 * np.pi)
+    assert np.allclose(parts[turns >= 32], plain[turns >= 32], rtol=8 * U, atol=0)
+    assert np.allclose(parts[turns <= 1], plain[turns <= 1] / 8, rtol=8 * U, atol=0)
+    between = (turns > 1) & (turns < 32)
+    assert between.any() and np.all(parts[between] < plain[between]) and np.all(parts[between] > plain[between] / 8)
+    assert np.all(np.diff(parts) < 0)
+    # other borders move the pairs that are kept
+    assert np.sum(angles(ct.ROTARY_PARTS, 0.25, 4.0) == plain) > np.sum(parts == plain)
+    # a magnitude leaves the angle
+    assert np.allclose(angles(ct.ROTARY_PARTS, magnitude=1.25), parts, rtol=8 * U, atol=0)
