@@ -881,7 +881,7 @@ template <typename KT, int HD, int QP> int launch_items(const dlk_paged_params& 
     const int few = few_list.count > 0 ? few_list.rows : 0;
     const bool many = many_list.count > 0;
     if (blocks == 0) return 0;
-    if (blocks > INT32_MAX || (few != 0 && few != 16 && few != 32) || (many && many_list.rows != 128)) return static_cast<int>(hipErrorInvalidValue);
+    if (blocks > DLK_MOST_GROUPS || (few != 0 && few != 16 && few != 32) || (many && many_list.rows != 128)) return static_cast<int>(hipErrorInvalidValue);
     const dim3 grid(static_cast<unsigned>(blocks)), threads(kThreads);
     if (many && few == 32) hipLaunchKernelGGL((paged_attend<KT, HD, 2, QP, true, true>), grid, threads, 0, stream, p);
     else if (many && few == 16) hipLaunchKernelGGL((paged_attend<KT, HD, 1, QP, true, true>), grid, threads, 0, stream, p);
@@ -891,13 +891,16 @@ template <typename KT, int HD, int QP> int launch_items(const dlk_paged_params& 
     return static_cast<int>(hipGetLastError());
 }
 
+// waves of a merge
+int64_t merge_units(int64_t merges, int64_t H, int64_t hd) { return merges * ((H + 256 / hd - 1) / (256 / hd)); }
+
 template <typename KT, int HD> int launch(const dlk_paged_params& p, hipStream_t stream) {
     const int status = p.q_bf16 ? launch_items<KT, HD, 1>(p, stream) : launch_items<KT, HD, 3>(p, stream);
     if (status != 0) return status;
     if (p.merge_count == 0) return 0;
-    const int64_t heads = 256 / HD, units = p.merge_count * ((p.H + heads - 1) / heads);
-    // up to 8 splits are one round trip of one wave
-    if (p.merge_most <= 8) hipLaunchKernelGGL((paged_merge<HD, 1>), dim3(static_cast<unsigned>((units + kWaves - 1) / kWaves)), dim3(kThreads), 0, stream, p);
+    const int64_t units = merge_units(p.merge_count, p.H, HD);
+    // up to 8 splits are one round trip of one wave, and more waves than a launch has are not needed
+    if (p.merge_most <= 8 || units > DLK_MOST_GROUPS) hipLaunchKernelGGL((paged_merge<HD, 1>), dim3(static_cast<unsigned>((units + kWaves - 1) / kWaves)), dim3(kThreads), 0, stream, p);
     else hipLaunchKernelGGL((paged_merge<HD, kWaves>), dim3(static_cast<unsigned>(units)), dim3(kThreads), 0, stream, p);
     return static_cast<int>(hipGetLastError());
 }
@@ -915,11 +918,16 @@ template <typename KT> int launch_heads(const dlk_paged_params& p, hipStream_t s
 } // namespace
 } // namespace dlk
 
+extern "C" int dlk_paged_fits(int64_t items, int64_t merges, int H, int KV, int hd) {
+    return items <= DLK_MOST_GROUPS / KV && dlk::merge_units(merges, H, hd) <= static_cast<int64_t>(DLK_MOST_GROUPS) * dlk::kWaves;
+}
+
 extern "C" int dlk_paged_attention(const dlk_paged_params* params, dlh_stream stream_handle) {
     const dlk_paged_params& p = *params;
     const int align = p.q_bf16 ? 8 : 4; // elements of 16 bytes
     if (p.KV <= 0 || p.H <= 0 || p.H % p.KV != 0 || p.page_shift < 4 || p.q_row % align != 0 || p.q_head % align != 0 ||
-        reinterpret_cast<uintptr_t>(p.q) % 16 != 0 || (p.merge_count > 0 && !p.merges))
+        reinterpret_cast<uintptr_t>(p.q) % 16 != 0 || (p.merge_count > 0 && !p.merges) ||
+        !dlk_paged_fits(static_cast<int64_t>(p.lists[0].count) + p.lists[1].count, p.merge_count, p.H, p.KV, p.hd))
         return static_cast<int>(hipErrorInvalidValue);
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_handle);
     return p.kv_bf16 ? dlk::launch_heads<uint16_t>(p, stream) : dlk::launch_heads<float>(p, stream);

@@ -246,6 +246,9 @@ int dlk_rms_norm(const float* x, int64_t rows, int64_t width, const void* weight
 /* Interleaved RoPE on contiguous x [outer, L, D] f32 with tables [L, D/2]. */
 int dlk_rope(const float* x, int64_t outer, int64_t length, int64_t dim, const float* cosine, const float* sine,
              float* y, dlh_stream stream);
+/* A launch has fewer than 2^32 threads: so many work-groups of 256. */
+#define DLK_MOST_GROUPS ((1 << 24) - 1)
+
 /* ------------------------------------------------------------------------------------------------------
  * Rows at given positions (rotary.hip): the queries, keys and values of `tokens` rows, queries and keys rotated by
  * the table row of the token's position, keys and values written to the pages of a paged cache.
@@ -324,6 +327,8 @@ typedef struct dlk_paged_params {
     int merge_count, merge_most; /* merges, and the most partials of one */
 } dlk_paged_params;
 int dlk_paged_attention(const dlk_paged_params* p, dlh_stream stream);
+/* Whether a launch holds `items` of each KV head and `merges`. */
+int dlk_paged_fits(int64_t items, int64_t merges, int H, int KV, int hd);
 
 /* First maximum of each row (NaN first); x [rows, n] f32 contiguous -> out i64 [rows]. */
 int dlk_argmax(const float* x, int64_t rows, int64_t n, int64_t* out, dlh_stream stream);

@@ -450,7 +450,7 @@ extern "C" int dlk_verify(const dlk_verify_params* params, dlh_stream stream_han
     hipStream_t stream = reinterpret_cast<hipStream_t>(stream_handle);
     const int64_t groups = p.batch * (p.drafts + 1 + (p.draft ? p.drafts : 0)) * p.slices;
     const int64_t parts = p.batch * ((p.vocabulary + dlk::kDraw - 1) / dlk::kDraw);
-    if (groups > INT32_MAX || parts > INT32_MAX) return static_cast<int>(hipErrorInvalidValue);
+    if (groups > DLK_MOST_GROUPS || parts > DLK_MOST_GROUPS) return static_cast<int>(hipErrorInvalidValue);
     const dim3 threads(dlk::kThreads), rows(groups), sequences(p.batch);
     // between 2^-100 and 2^100 f32 holds the inverse, and two logits that are further apart than f32 counts weigh nothing
     const bool wide = p.inverse < 0x1p-100 || p.inverse > 0x1p100;

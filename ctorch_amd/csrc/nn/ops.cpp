@@ -471,8 +471,11 @@ std::pair<Tensor, Tensor> verify_drafted(const Tensor& drafted, const Tensor& ta
     Tensor q_logits = draft && temperature > 0.0 ? contiguous_f32(*draft) : Tensor{};
     Tensor tokens = empty_tensor({batch, drafts + 1}, DType::i64, target.device());
     Tensor accepted = empty_tensor({batch}, DType::i64, target.device());
-    const int slices = dlk_verify_slices(batch * (drafts + 1 + (q_logits.defined() ? drafts : 0)), vocabulary);
+    const Index rows = batch * (drafts + 1 + (q_logits.defined() ? drafts : 0));
+    const int slices = dlk_verify_slices(rows, vocabulary);
     const Index parts = (vocabulary + DLK_VERIFY_DRAW - 1) / DLK_VERIFY_DRAW;
+    if (rows > DLK_MOST_GROUPS / slices || batch > DLK_MOST_GROUPS / parts)
+        throw std::invalid_argument("verify_drafted: too many rows of logits");
     static_assert(sizeof(dlk_verify_slice) == 16);
     Tensor work = empty_tensor({batch * (slices * 2 * (2 * drafts + 1) + 2 * parts + 4)}, DType::f64, target.device());
     dlk_verify_params p{};

@@ -98,6 +98,7 @@ PagedBatch::PagedBatch(const PagedKVCache& cache, Index heads, std::span<const I
     const Index batch = static_cast<Index>(lengths.size()), page = cache.page_size();
     const auto refuse = [](const std::string& what) { throw std::invalid_argument("paged batch: " + what); };
     if (heads <= 0 || heads % cache.kv_heads() != 0) refuse("heads must be a multiple of the cache's kv_heads");
+    if (heads > INT32_MAX / 1024) refuse("too many heads");
     if (batch <= 0 || counts.size() != lengths.size()) refuse("needs a length and a count for each of its sequences");
     if (width <= 0 || width > INT32_MAX / batch || tables.size() != static_cast<std::size_t>(batch * width))
         refuse("tables must be [sequences, width]");
@@ -246,8 +247,11 @@ PagedBatch::PagedBatch(const PagedKVCache& cache, Index heads, std::span<const I
         return a.key_end - a.key_begin > b.key_end - b.key_begin;
     });
     for (int i = 0; i < 2; ++i) lists[i].count = static_cast<Index>(items[i].size());
-    if (std::max(plan->partials, lists[0].count + lists[1].count) > INT32_MAX / cache.kv_heads()) refuse("too many new positions");
     plan->merge_count = static_cast<Index>(merges.size());
+    if (plan->partials > INT32_MAX / cache.kv_heads() ||
+        !dlk_paged_fits(lists[0].count + lists[1].count, plan->merge_count, static_cast<int>(heads), static_cast<int>(cache.kv_heads()),
+                        static_cast<int>(cache.head_dim())))
+        refuse("too many new positions");
     for (const auto& merge : merges) plan->merge_most = std::max<Index>(plan->merge_most, merge.count + plan->shared_splits);
 
     // one copy to the device

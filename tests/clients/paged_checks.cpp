@@ -159,6 +159,22 @@ int call(const std::string& name) {
         {"cache on the host", [&] { PagedKVCache(1, 8, 16, 2, 32, {}); }},
         {"cache elements", [&] { PagedKVCache(1, Index(1) << 30, 1024, Index(1) << 20, 128, f32); }},
         {"cache bytes", [&] { PagedKVCache(1, Index(1) << 30, 1024, Index(1) << 15, 128, f32); }},
+        {"batch heads", [&] { PagedBatch(cache, Index(1) << 30, one, none, pages, 4); }},
+        {"batch of too many items", [&] { // (17 million work-groups; the pages are never touched)
+             const Index n = 1 << 14;
+             const PagedKVCache wide(1, n, 16, 1024, 16, {.dtype = dl::DType::bf16, .device = gpu});
+             std::vector<Index> lengths(n, 0), counts(n, 1), own(n);
+             for (Index i = 0; i < n; ++i) own[i] = i;
+             PagedBatch(wide, 1024, lengths, counts, own, 1);
+         }},
+        {"batch of too many merges", [&] { // (its rows are some million work-groups, joined by 17)
+             const Index n = 1 << 22;
+             const PagedKVCache narrow(1, n / 16 + 1, 16, 1, 128, {.dtype = dl::DType::bf16, .device = gpu});
+             std::vector<Index> own(n / 16 + 1);
+             for (std::size_t i = 0; i < own.size(); ++i) own[i] = static_cast<Index>(i);
+             const Index length[] = {16}, count[] = {n};
+             PagedBatch(narrow, 32, length, count, own, n / 16 + 1, 16);
+         }},
         {"append layer", [&] { append(k, v, c, s, 2); }},
         {"append layer below", [&] { append(k, v, c, s, -1); }},
         {"append rows", [&] { append(tensor({4, 2, 32}), v, c, s); }},
@@ -211,6 +227,10 @@ int call(const std::string& name) {
         {"verify drafts", [&] {
              const Index n = (1 << 20) + 1;
              dl::verify_drafted(tensor({1, n}, dl::DType::i64), tensor({1, n + 1, 1}), std::nullopt, 1.0, tensor({1, n + 1}));
+         }},
+        {"verify rows", [&] {
+             const Index n = 1 << 24;
+             dl::verify_drafted(tensor({n, 0}, dl::DType::i64), tensor({n, 1, 1}), std::nullopt, 1.0, tensor({n, 1}));
          }},
         {"verify temperature", [&] { dl::verify_drafted(ids, target, draft, inf, u); }},
         {"verify temperature nan", [&] { dl::verify_drafted(ids, target, draft, inf - inf, u); }},

@@ -131,6 +131,13 @@ def test_a_cache_whose_size_wraps_is_refused(name):
     assert run.returncode == 1 and "too many elements" in run.stderr, (run.returncode, run.stdout, run.stderr)
 
 
+@pytest.mark.parametrize("name,said", [("batch heads", "too many heads"), ("batch of too many items", "too many new positions"),
+                                       ("batch of too many merges", "too many new positions"), ("verify rows", "too many rows")])
+def test_a_launch_has_fewer_than_2_to_the_32_threads(name, said):
+    run = checks("call", name)
+    assert run.returncode == 1 and said in run.stderr, (run.returncode, run.stdout, run.stderr)
+
+
 def test_sizes_that_wrap_are_refused():
     cpu = ct.device("cpu")
     for call in (lambda: ct.rotary_tables(32, 2 ** 60, dev=cpu), lambda: ct.rotary_tables(32, 2 ** 58, dev=cpu),
