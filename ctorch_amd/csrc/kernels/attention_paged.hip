@@ -511,7 +511,8 @@ __device__ __forceinline__ void attend_few(const dlk_paged_params& p, int block,
 // 32 x 32 instruction leaves the vector ALUs more room than two of 16 x 16: three vector instructions beside each of the
 // latter cost 26 % of its rate, beside the former 12 %.)  f32 pages are cut into three bf16 planes as they are staged, once
 // for the 128 rows.  (3000 new rows of 32 heads after 1000: f32 pages, heads of 64 340 us, of 128 645 us; bf16 183 and 330 us:
-// 0.95 to 1.1 PF/s of the products that run, where a large bf16 product reaches 1.2.)
+// 0.95 to 1.1 PF/s of the products that run, where a large bf16 product reaches 1.2.  f32 queries over bf16 pages at heads of 128
+// take all 256 registers and spill 5.)
 template <typename KT, int HD> struct Many {
     static constexpr int PLANES = sizeof(KT) == 4 ? 3 : 1;
     static constexpr int BUFFERS = sizeof(KT) == 4 && HD == 128 ? 1 : 2; // (LDS of two work-groups a CU)

@@ -4,13 +4,14 @@
 // first index whose cumulative weight exceeds u times the total.  Without draft logits a draft is certain (q(x) = 1).
 //
 // A decision compares two products and a draw finds a place in a sum over the vocabulary, so that everything behind the
-// logits is in f64: the decisions are those of the exact probabilities, in any order of summation.
+// logits is in f64, with exponentials off by 1.1e-12: decisions are those of the exact probabilities, in any order of
+// summation, but where a number lies that close to its border.
 //
 // Three launches.  verify_rows reads every logit once, slices of a row as work-groups, and leaves each slice's largest and
 // sum.  verify_weights decides what is kept and sums the weights of the row behind it, 1024 entries a work-group.  verify_draw
-// finds the part of 1024 and in it the index.  The first is bound by memory and the f64 instructions alike (32 runs of 7 drafts
-// over 32000 entries, 61 MB: 19 us), the others by round trips to memory (7 and 8 us).  A greedy verification needs the largest
-// only and no sums.
+// finds the part of 1024 and in it the index.  The first is bound by the read and the f64 instructions, which a work-group does one
+// after the other (32 runs of 7 drafts over 32000 entries, 61 MB: 19 us), the others by round trips to memory (7 and 8 us).  A
+// greedy verification needs the largest only and no sums.
 #include "kernels/device_common.h"
 
 #include <algorithm>

@@ -50,7 +50,8 @@ struct Load {
 // read, their bytes at 2.5 TB/s.
 // Many rows: 8500 / (products of a pair's entry, twice the head size), what the matrix cores do: 22 keys for bf16 pages and
 // heads of 64, 11 for heads of 128 or f32 pages; a work-group with a CU to itself 1.75 times that.  An item takes 5 more; the
-// last ones, the longest having come first, run a sixth of an item alone.  The bytes of partials go at 2.5 TB/s, of a prefix at 1.5.
+// last ones, the longest having come first, run a sixth of an item alone.  The bytes of partials go at 2.5 TB/s, of a prefix at 1.5
+// (fitted: it stands too for the items of few rows of the same launch, which are accounted for apart).
 // (8 sequences of 32768 keys, a row each: 64 items of 2048 keys a head 133 us, of 768 124, of 256 139.  64 runs of 5 after up to
 // 1000, f32: items of 256 61 us, whole 48.  3000 new rows after 1000: whole 335 us, in 512 keys 366.  16 runs of 192 rows
 // after up to 2000 keys, 256 work-groups: whole 58 us, in 1024 keys 44.  Over 120 batches of few rows the choice is 4 % off
@@ -58,7 +59,8 @@ struct Load {
 Index chunk_of(const Load& load) {
     if (load.seen.empty()) return 256;
     const bool many = load.rows == 128, wide = load.head_dim == 128;
-    // what registers and LDS leave room for
+    // fitted: no more than registers and LDS leave room for (up to 8 for f32 heads of 16, 3 for bf16 queries at bf16 heads of 128,
+    // 3 or 4 for heads of 16 and 32 beside items of many rows)
     const Index per_cu = many || load.beside ? 2 : !load.f32 ? (wide ? 2 : 4) : load.rows == 32 && load.head_dim >= 64 ? 2 : wide ? 3 : 4;
     const double slots = 256.0 * static_cast<double>(per_cu), heads = static_cast<double>(load.kv_heads);
     const double dim = static_cast<double>(load.head_dim), partial = heads * static_cast<double>(load.used_rows) * dim * 8.0;

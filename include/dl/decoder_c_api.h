@@ -118,7 +118,8 @@ DL_API void dl_paged_cache_release(dl_paged_cache* cache);
 DL_API dl_status dl_paged_cache_tensors(const dl_paged_cache* cache, int64_t layer, dl_tensor** key, dl_tensor** value);
 /* A step: sequence b holds lengths[b] positions and gets counts[b] new ones; its position p lies in page
  * tables[b * width + p / page_size].  `shared` leading positions (whole pages, 0: none) lie in the same pages for all.
- * The arrays are host memory, read during the call. */
+ * The arrays are host memory, read during the call.  Sequences with a count of 0 are not looked at.  The call waits for the
+ * library's stream. */
 DL_API dl_status dl_paged_batch_create(const dl_paged_cache* cache, int64_t heads, int64_t sequences,
     const int64_t* lengths, const int64_t* counts, const int64_t* tables, int64_t width, int64_t shared,
     dl_paged_batch** output);

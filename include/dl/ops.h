@@ -29,7 +29,7 @@ struct RotaryScaling {
     double magnitude = 1.0;
 };
 /// Cosine and sine tables [capacity, dimensions / 2], f32, the angles taken in 64 bits (RotaryEmbedding's own tables
-/// keep the reference's f32 angles).
+/// keep the reference's f32 angles).  `device` is where they will be used: operators copy tables from elsewhere in each call.
 DL_API std::pair<Tensor, Tensor> rotary_tables(Index dimensions, Index capacity, double base = 10000.0,
                                                const RotaryScaling& scaling = {}, Device device = Device::cpu());
 /// Rotates the first R = 2 * cosine.size(1) entries of each head of input [T, H, D] (f32 or bf16) by row positions[t]
@@ -61,8 +61,9 @@ DL_API Tensor sample(const Tensor& logits, double temperature, RandomKey key);
 /// the last draft from p, at the first refused one from max(p - q, 0) (from p where that is zero), as the first index whose
 /// cumulative weight exceeds uniforms[b, K] times the total.  Without draft logits [B, K, V] a draft was certain: q(x) = 1.  A
 /// temperature <= 0 accepts the target's argmax and nothing else.  A draft beyond the vocabulary is not accepted; a row whose
-/// weights have no positive finite sum (NaN logits) takes its argmax.  K is at most 2^20.  Returns tokens [B, K + 1] (the
-/// accepted drafts, the drawn token, then -1) and the number accepted [B], both i64.
+/// weights have no positive finite sum (NaN logits) takes its argmax.  Probabilities are of 64 bits, off by 2e-12 of their value;
+/// a weight below e^-700 of the row's largest is zero.  The temperature is any finite number, K at most 2^20.  Returns tokens
+/// [B, K + 1] (the accepted drafts, the drawn token, then -1) and the number accepted [B], both i64.
 DL_API std::pair<Tensor, Tensor> verify_drafted(const Tensor& drafted, const Tensor& target,
                                                 const std::optional<Tensor>& draft, double temperature,
                                                 const Tensor& uniforms);

@@ -37,8 +37,9 @@ private:
 /// position p lies in page tables[b * width + p / page_size].  The new positions' rows of a step lie one sequence after
 /// another ([tokens, heads, head_dim], tokens the sum of the counts).  With `shared` > 0 (whole pages) the first `shared`
 /// positions of every sequence with new ones lie in the same pages, and attention reads them once for the whole batch.
-/// A page that the step writes belongs to one place of one sequence.  Made once and used for every layer; the cache may
-/// be another one of the same layout.
+/// A page that the step writes belongs to one place of one sequence with new positions; the pages of the others are not
+/// looked at, so the caller sees to it that a step writes none that they still need.  Made once and used for every layer; the
+/// cache may be another one of the same layout.  Making it copies the plan to the device and waits for the library's stream.
 class DL_API PagedBatch {
 public:
     struct Plan;
@@ -58,8 +59,8 @@ namespace dl {
 /// Writes the step's keys (rotated at their positions) and values, [tokens, kv_heads, head_dim], to their pages of
 /// `layer`, and returns the queries [tokens, heads, head_dim] rotated likewise (an undefined tensor when there are none).
 /// All three are f32 or bf16 and may be views of one projection output; cosine and sine as for rotary_positions, with a
-/// row for every position of the step.  What of them lies in this layer's pages is taken as it was before the call.  A bf16
-/// cache rounds each key and value once.
+/// row for every position of the step (on the cache's device, or they are copied there, and waited for, in each call).  What of
+/// them lies in this layer's pages is taken as it was before the call.  A bf16 cache rounds each key and value once.
 DL_API Tensor paged_append(const nn::PagedKVCache& cache, Index layer, const nn::PagedBatch& batch,
                            const std::optional<Tensor>& query, const Tensor& key, const Tensor& value,
                            const Tensor& cosine, const Tensor& sine, RotaryLayout layout);
