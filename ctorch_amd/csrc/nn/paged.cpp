@@ -309,6 +309,7 @@ void check_rows(const Tensor& t, Index tokens, Index heads, Index dim, Device de
 
 // What lies in the pages that a call writes would be read while it changes: it is read from a copy.
 Tensor apart_from(const nn::PagedKVCache& cache, Index layer, const Tensor& t) {
+    if (!t.defined()) return t; // (its reader refuses it)
     const auto& storage = TensorAccess::impl(t)->storage;
     for (const Tensor* pages : {&cache.key(layer), &cache.value(layer)})
         if (storage == TensorAccess::impl(*pages)->storage) return t.clone();

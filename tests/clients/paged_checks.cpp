@@ -186,6 +186,9 @@ int call(const std::string& name) {
         {"append wide tables", [&] { append(k, v, tensor({64, 17}), tensor({64, 17})); }},
         {"append unequal tables", [&] { append(k, v, c, tensor({64, 8})); }},
         {"append empty tables", [&] { append(k, v, tensor({64, 0}), tensor({64, 0})); }},
+        {"append undefined tables", [&] { append(k, v, dl::Tensor{}, s); }},
+        {"append undefined sines", [&] { append(k, v, c, dl::Tensor{}); }},
+        {"append undefined rows", [&] { append(dl::Tensor{}, v, c, s); }},
         {"append layout", [&] { append(k, v, c, s, 0, nullptr, std::nullopt, static_cast<RotaryLayout>(7)); }},
         {"append nothing", [&] { append(tensor({0, 2, 32}), tensor({0, 2, 32}), c, s, 0, &idle, tensor({0, 4, 32})); }},
         {"append rows of the pages", [&] { append(page_rows(cache.key(0)), page_rows(cache.value(0)), c, s); }},

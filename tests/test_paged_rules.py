@@ -125,6 +125,12 @@ def test_an_operator_refuses(name):
     assert run.returncode == 1 and REFUSED[name] in run.stderr, (run.returncode, run.stdout, run.stderr)
 
 
+@pytest.mark.parametrize("name", ["append undefined tables", "append undefined sines", "append undefined rows"])
+def test_undefined_tensors_are_refused(name):
+    run = checks("call", name)
+    assert run.returncode == 1 and "undefined tensor" in run.stderr, (run.returncode, run.stdout, run.stderr)
+
+
 @pytest.mark.parametrize("name", ["cache elements", "cache bytes"])
 def test_a_cache_whose_size_wraps_is_refused(name):
     run = checks("call", name)  # 2^67 elements, 2^64 bytes: both nothing in 64 bits
