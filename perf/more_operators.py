@@ -84,7 +84,7 @@ def draw(rng):
             count = _log(rng, 10, 6000 // batch)
         return dict(kind="delta", batch=batch, count=count, key_heads=key_heads, heads=heads, key_dim=key_dim,
                     value_dim=value_dim, input=rng.choice(["f32", "bf16"]))
-    layers, kv = rng.choice([(4, 8), (16, 8), (24, 4), (40, 2)])
+    layers, kv = rng.choice([(4, 8), (16, 8), (24, 4), (30, 2)])
     common = dict(layers=layers, kv=kv, head_dim=rng.choice([32, 64, 128]), page=rng.choice([16, 32, 64, 128]),
                   dtype=rng.choice(["f32", "bf16", "bf16"]))
     row = 2 * layers * kv * common["head_dim"] * {"f32": 4, "bf16": 2}[common["dtype"]]  # bytes of a position
