@@ -167,6 +167,26 @@ SIGNATURES = {
     "dl_paged_batch_release": (None, [_p]),
     "dl_paged_cache_append": (_st, [_p, _i64, _p, _p, _p, _p, _p, _p, C.c_int, _pp]),
     "dl_paged_attention": (_st, [_p, _i64, _p, _p, _pp]),
+    "dl_page_pool_create": (_st, [_i64, _pp]),
+    "dl_page_pool_release": (None, [_p]),
+    "dl_page_pool_available": (_st, [_p, C.POINTER(_i64)]),
+    "dl_page_pool_references": (_st, [_p, _i64, C.POINTER(_i64)]),
+    "dl_page_pool_take": (_st, [_p, _i64, _p]),
+    "dl_page_pool_claim": (_st, [_p, _i64, _p]),
+    "dl_page_pool_share": (_st, [_p, _i64, _p]),
+    "dl_page_pool_give_back": (_st, [_p, _i64, _p]),
+    "dl_paged_cache_copy": (_st, [_p, _i64, _p, _p, _p]),
+    "dl_paged_cache_fork": (_st, [_p, _p, _i64, _p, _i64, _p, _i64, _p, _p]),
+    "dl_paged_cache_compact": (_st, [_p, _p, _i64, _p, C.POINTER(_i64)]),
+    "dl_delta_states_create": (_st, [_i64, _i64, _i64, _i64, _i64, Device, _pp]),
+    "dl_delta_states_release": (None, [_p]),
+    "dl_delta_states_tensor": (_st, [_p, _i64, _pp]),
+    "dl_delta_states_copy": (_st, [_p, _i64, _p, _p]),
+    "dl_delta_batch_create": (_st, [_p, _i64, _i64, _p, _p, _p, _pp]),
+    "dl_delta_batch_release": (None, [_p]),
+    "dl_gated_delta": (_st, [_p, _i64, _p, _p, _p, _p, _p, _p, C.POINTER(_f64), _pp]),
+    "dl_expert_mixture": (_st, [_p, _p, _p, _p, _p, _i64, _i32, _pp, _pp, _pp]),
+    "dl_expert_mixture_create": (_st, [_i64, _i64, _i64, _i64, _i32, TensorOptions, _pp]),
     # generate_c_api.h
     "dl_verify_drafted": (_st, [_p, _p, _p, _f64, _p, _pp, _pp]),
     "dl_decoder_lm_create": (_st, [_p, _p, _p, _pp]),
@@ -492,6 +512,84 @@ class PagedCache:
                                           C.byref(out) if query is not None else None))
         return Tensor(out) if query is not None else None
 
+    def copy_pages(self, sources, targets, rows=None) -> None:
+        """dl_paged_cache_copy: page sources[i] to targets[i] in every layer, its first rows[i] positions (None: all)."""
+        sources, targets = _ids(sources), _ids(targets)
+        rows = _ids(rows) if rows is not None else None
+        if sources.ndim != 1 or targets.shape != sources.shape or (rows is not None and rows.shape != sources.shape):
+            raise ValueError("copy_pages needs a target (and, if given, rows) for each source")
+        check(lib().dl_paged_cache_copy(self.handle, len(sources), _at(sources), _at(targets),
+                                        _at(rows) if rows is not None else None))
+
+    def fork(self, pool: "PagePool", tables, lengths, parents) -> np.ndarray:
+        """dl_paged_cache_fork: the tables [len(parents), width] of new requests that go on from those of `parents`."""
+        tables, lengths, parents = _ids(tables), _ids(lengths), _ids(parents)
+        if tables.ndim != 2 or lengths.shape != tables.shape[:1] or parents.ndim != 1:
+            raise ValueError("a fork needs tables [B, width], lengths [B] and parents")
+        out = np.empty((len(parents), tables.shape[1]), np.int64)
+        check(lib().dl_paged_cache_fork(self.handle, pool.handle, len(tables), _at(tables), tables.shape[1], _at(lengths),
+                                        len(parents), _at(parents), _at(out)))
+        return out
+
+    def compact(self, pool: "PagePool", tables) -> np.ndarray:
+        """dl_paged_cache_compact: the held pages moved to the front of the pool; the tables with their new ids."""
+        out = np.array(tables, np.int64)
+        check(lib().dl_paged_cache_compact(self.handle, pool.handle, out.size, _at(out), None))
+        return out
+
+
+def _ids(values) -> np.ndarray:
+    return np.ascontiguousarray(values, np.int64)
+
+
+def _at(array: np.ndarray) -> C.c_void_p:
+    return array.ctypes.data_as(C.c_void_p)
+
+
+class PagePool:
+    """dl_page_pool: which pages of a cache are held, and by how many tables.  Ids below zero are passed over."""
+
+    def __init__(self, pages: int):
+        self.handle = None
+        self.handle = _new(lib().dl_page_pool_create, pages)
+
+    def __del__(self):
+        if getattr(self, "handle", None) and _lib is not None:
+            _lib.dl_page_pool_release(self.handle)
+            self.handle = None
+
+    @property
+    def available(self) -> int:
+        n = C.c_int64()
+        check(lib().dl_page_pool_available(self.handle, C.byref(n)))
+        return n.value
+
+    def references(self, page: int) -> int:
+        n = C.c_int64()
+        check(lib().dl_page_pool_references(self.handle, page, C.byref(n)))
+        return n.value
+
+    def take(self, count: int) -> np.ndarray:
+        """The `count` lowest free pages, held from now on."""
+        out = np.empty(max(0, min(count, self.available)), np.int64)
+        check(lib().dl_page_pool_take(self.handle, count, _at(out)))
+        return out
+
+    def claim(self, pages) -> None:
+        """One more holder of each page, free ones among them."""
+        pages = _ids(pages)
+        check(lib().dl_page_pool_claim(self.handle, pages.size, _at(pages)))
+
+    def share(self, pages) -> None:
+        """One more holder of each page, all of them held."""
+        pages = _ids(pages)
+        check(lib().dl_page_pool_share(self.handle, pages.size, _at(pages)))
+
+    def release(self, pages) -> None:
+        """One holder fewer of each page (dl_page_pool_give_back)."""
+        pages = _ids(pages)
+        check(lib().dl_page_pool_give_back(self.handle, pages.size, _at(pages)))
+
 
 class PagedBatch:
     """dl_paged_batch: what one step computes.  tables: page ids [sequences, width]."""
@@ -508,6 +606,47 @@ class PagedBatch:
     def __del__(self):
         if getattr(self, "handle", None) and _lib is not None:
             _lib.dl_paged_batch_release(self.handle)
+            self.handle = None
+
+
+class DeltaStates:
+    """dl_delta_states: the gated delta rule's states [slots, heads, key_dim, value_dim] of each layer."""
+
+    def __init__(self, layers: int, slots: int, heads: int, key_dim: int, value_dim: int, dev: Device | None = None):
+        self.handle = None
+        self.handle = _new(lib().dl_delta_states_create, layers, slots, heads, key_dim, value_dim,
+                           dev if dev is not None else device("gpu"))
+
+    def __del__(self):
+        if getattr(self, "handle", None) and _lib is not None:
+            _lib.dl_delta_states_release(self.handle)
+            self.handle = None
+
+    def state(self, layer: int) -> Tensor:
+        """The layer's live states."""
+        return Tensor(_new(lib().dl_delta_states_tensor, self.handle, layer))
+
+    def copy(self, sources, targets) -> None:
+        """dl_delta_states_copy: slot sources[i] to targets[i] in every layer."""
+        sources, targets = _ids(sources), _ids(targets)
+        if sources.ndim != 1 or targets.shape != sources.shape:
+            raise ValueError("a copy needs a target for each source")
+        check(lib().dl_delta_states_copy(self.handle, len(sources), _at(sources), _at(targets)))
+
+
+class DeltaBatch:
+    """dl_delta_batch: what one step computes, from slots `sources` (-1: zero) to slots `targets`, counts[b] tokens each."""
+
+    def __init__(self, states: DeltaStates, key_heads: int, sources, targets, counts):
+        self.handle = None
+        arrays = [_ids(a) for a in (sources, targets, counts)]
+        if any(a.ndim != 1 or a.shape != arrays[0].shape for a in arrays):
+            raise ValueError("a delta batch needs a source, a target and a count for each request")
+        self.handle = _new(lib().dl_delta_batch_create, states.handle, key_heads, len(arrays[0]), *map(_at, arrays))
+
+    def __del__(self):
+        if getattr(self, "handle", None) and _lib is not None:
+            _lib.dl_delta_batch_release(self.handle)
             self.handle = None
 
 
@@ -655,6 +794,28 @@ def rotary_positions(x: Tensor, positions: Tensor, cosine: Tensor, sine: Tensor,
 
 def paged_attention(cache: PagedCache, layer: int, batch: PagedBatch, query: Tensor) -> Tensor:
     return Tensor(_new(lib().dl_paged_attention, cache.handle, layer, batch.handle, query.handle))
+
+
+def gated_delta(states: DeltaStates, layer: int, batch: DeltaBatch, query: Tensor, key: Tensor, value: Tensor, decay: Tensor,
+                rate: Tensor, scale: float | None = None) -> Tensor:
+    factor = C.c_double(scale) if scale is not None else None
+    return Tensor(_new(lib().dl_gated_delta, states.handle, layer, batch.handle, query.handle, key.handle, value.handle,
+                       decay.handle, rate.handle, C.byref(factor) if factor is not None else None))
+
+
+def expert_mixture(x: Tensor, router: Tensor, gate: Tensor, up: Tensor, down: Tensor, top: int,
+                   normalise: bool = True) -> tuple[Tensor, Tensor, Tensor]:
+    """dl_expert_mixture: (output [..., d], chosen [..., top], weights [..., top])."""
+    out = [C.c_void_p() for _ in range(3)]
+    check(lib().dl_expert_mixture(x.handle, router.handle, gate.handle, up.handle, down.handle, top, int(normalise),
+                                  *map(C.byref, out)))
+    return tuple(map(Tensor, out))
+
+
+def expert_mixture_module(dimensions: int, hidden: int, experts: int, top: int, normalise: bool = True, dtype: int = F32,
+                          dev: Device | None = None) -> Module:
+    """dl_expert_mixture_create: parameters router, gate, up and down."""
+    return Module(_new(lib().dl_expert_mixture_create, dimensions, hidden, experts, top, int(normalise), options(dtype, dev)))
 
 
 def rotary_embedding(x: Tensor, cosine: Tensor, sine: Tensor) -> Tensor:

@@ -5,6 +5,7 @@
 
 #include "dl/generate_c_api.h"
 #include "dl/decoder.h"
+#include "dl/delta.h"
 #include "dl/paged.h"
 #include "nn/language_model.h"
 
@@ -18,6 +19,9 @@ struct dl_state { dl::StateDict value; };
 struct dl_decoder_cache { std::vector<dl::nn::KVCache> value; };
 struct dl_paged_cache { dl::nn::PagedKVCache value; };
 struct dl_paged_batch { dl::nn::PagedBatch value; };
+struct dl_page_pool { dl::nn::PagePool value; };
+struct dl_delta_states { dl::nn::DeltaStates value; };
+struct dl_delta_batch { dl::nn::DeltaBatch value; };
 struct dl_decoder_lm {
     std::shared_ptr<dl::nn::UnaryModule> embedding, decoder, head;
     std::unique_ptr<dl::detail::DecoderLM> value;

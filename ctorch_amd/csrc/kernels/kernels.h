@@ -330,6 +330,71 @@ int dlk_paged_attention(const dlk_paged_params* p, dlh_stream stream);
 /* Whether a launch holds `items` of each KV head and `merges`. */
 int dlk_paged_fits(int64_t items, int64_t merges, int H, int KV, int hd);
 
+/* ------------------------------------------------------------------------------------------------------
+ * Copies of pages within pools of one layout [pages, heads, page, row] (page_copy.hip): the first `rows` rows of each head
+ * of page `from` to page `to`, in every pool.  A page below zero is page ~from or ~to of the staging memory, which holds
+ * `staged` pages for each pool.  No page of a launch is read and written, nor written twice (the caller sees to it).
+ * ---------------------------------------------------------------------------------------------------- */
+typedef struct dlk_page_pair {
+    int32_t from, to, rows;
+} dlk_page_pair;
+#define DLK_PAGE_PAIRS 240
+#define DLK_PAGE_POOLS 64
+typedef struct dlk_page_copy_params { /* (an argument block of a launch: below 4 KB) */
+    int pool_count, count;
+    int heads, page, row_units; /* a row is row_units * 16 bytes */
+    int staged;
+    void* staging;              /* [pool_count, staged, heads, page, row] or NULL */
+    void* pools[DLK_PAGE_POOLS];
+    dlk_page_pair pairs[DLK_PAGE_PAIRS];
+} dlk_page_copy_params;
+int dlk_page_copy(const dlk_page_copy_params* p, dlh_stream stream);
+
+/* ------------------------------------------------------------------------------------------------------
+ * The gated delta rule over a step's tokens (delta_step.hip).  Rows are 16-byte aligned, also between heads and tokens.
+ * ---------------------------------------------------------------------------------------------------- */
+typedef struct dlk_delta_item { /* a request's new tokens: `count` from `token` on */
+    int32_t source, target;     /* slots of its state before (-1: zero) and after */
+    int32_t token, count;
+} dlk_delta_item;
+
+typedef struct dlk_delta_params {
+    dlk_row_segment q, k, v; /* [tokens, heads / group, key_dim] and [tokens, heads, value_dim] */
+    const float* decay;      /* [tokens, heads] */
+    const float* rate;       /* [tokens, heads] */
+    float* states;           /* [slots, heads, key_dim, value_dim] */
+    float* out;              /* [tokens, heads, value_dim] */
+    int heads, group, key_dim, value_dim;
+    float scale;
+    const dlk_delta_item* items;
+    int item_count;
+} dlk_delta_params;
+int dlk_delta_step(const dlk_delta_params* p, dlh_stream stream);
+
+/* ------------------------------------------------------------------------------------------------------
+ * A layer of experts (experts.hip): for each of `tokens` rows x the `top` experts with the largest router logits, and
+ *   y = sum_j weights_j down[e_j] (silu(gate[e_j] x) * (up[e_j] x))
+ * ---------------------------------------------------------------------------------------------------- */
+#define DLK_EXPERTS_MOST 1024    /* experts */
+#define DLK_EXPERTS_TOP_MOST 64  /* chosen ones of a row */
+typedef struct dlk_experts_params {
+    const void* x;           /* [tokens, dim], x_bf16 or f32 */
+    int x_bf16;
+    const void* router;      /* [experts, dim] */
+    const void* gate;        /* [experts, hidden, dim] */
+    const void* up;
+    const void* down;        /* [experts, dim, hidden] */
+    int router_bf16, weights_bf16;
+    int64_t tokens;
+    int dim, hidden, experts, top;
+    int normalise;           /* the chosen experts' weights are divided by their sum */
+    float* y;                /* [tokens, dim] */
+    int64_t* chosen;         /* [tokens, top] */
+    float* weights;          /* [tokens, top] */
+    float* act;              /* [tokens, top, hidden]: workspace */
+} dlk_experts_params;
+int dlk_experts(const dlk_experts_params* p, dlh_stream stream);
+
 /* First maximum of each row (NaN first); x [rows, n] f32 contiguous -> out i64 [rows]. */
 int dlk_argmax(const float* x, int64_t rows, int64_t n, int64_t* out, dlh_stream stream);
 /* Per-block candidates of a [rows, n] logits matrix (greedy or Gumbel-max), for dlk_sample_finalize. */

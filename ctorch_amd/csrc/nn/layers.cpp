@@ -44,15 +44,13 @@ Tensor host_parameter(const Shape& shape, TensorOptions options, int kind, doubl
     return out;
 }
 
+double linear_bound(Index input_features) { return 1.0 / std::sqrt(static_cast<double>(std::max<Index>(1, input_features))); }
+
 } // namespace
 
 Linear::Linear(Index input_features, Index output_features, bool bias, TensorOptions options)
-    : weight_(register_parameter("weight",
-                                 host_parameter({output_features, input_features}, options, 0,
-                                                1.0 / std::sqrt(static_cast<double>(std::max<Index>(1, input_features)))))) {
-    if (bias)
-        bias_ = register_parameter("bias", host_parameter({output_features}, options, 0,
-                                                          1.0 / std::sqrt(static_cast<double>(std::max<Index>(1, input_features)))));
+    : weight_(register_parameter("weight", host_parameter({output_features, input_features}, options, 0, linear_bound(input_features)))) {
+    if (bias) bias_ = register_parameter("bias", host_parameter({output_features}, options, 0, linear_bound(input_features)));
 }
 
 Linear::Linear(Tensor weight, std::optional<Tensor> bias) : weight_(register_parameter("weight", std::move(weight))) {
@@ -83,3 +81,11 @@ double RMSNorm::epsilon() const {
 Tensor RMSNorm::forward(const Tensor& input) { return rms_norm(input, normalized_shape_, weight_, epsilon_); }
 
 } // namespace dl::nn
+
+namespace dl::detail {
+
+Tensor linear_parameter(const Shape& shape, Index input_features, TensorOptions options) {
+    return nn::host_parameter(shape, options, 0, nn::linear_bound(input_features));
+}
+
+} // namespace dl::detail

@@ -33,6 +33,14 @@ private:
 /// Rows [T, heads, D] as a kernel reads them; `held` keeps the tensor (a copy where the last axis has gaps).
 dlk_row_segment row_segment(const Tensor& t, Tensor& held, Index heads, const char* operation);
 
+/// A parameter drawn as a Linear's is, from U(+-1 / sqrt(input_features)).
+Tensor linear_parameter(const Shape& shape, Index input_features, TensorOptions options);
+
+/// Copies pages between places of pools that share the layout [pages, heads, page, row]: of each head the first rows[i] rows
+/// (`rows` empty: all) of page sources[i] to page targets[i], in every pool.  Sources are taken as they were before the call.
+void copy_pages(const std::vector<void*>& pools, Index pages, Index heads, Index page, Index row_bytes, Device device,
+                std::span<const Index> sources, std::span<const Index> targets, std::span<const Index> rows, const char* operation);
+
 /// Number of key splits and keys per split for attention of `length` new positions over `source` keys.
 void attention_split(Index batch, Index heads, Index kv_heads, Index head_dim, bool kv_bf16, Index length,
                      Index source, bool causal, int& splits, int& chunk);

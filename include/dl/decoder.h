@@ -24,6 +24,26 @@ private:
     std::shared_ptr<Linear> gate_, up_, down_;
 };
 
+/// A layer of `experts` SwiGLU experts behind a router, of which each row takes the `top` best (dl::expert_mixture; no
+/// counterpart in the reference).  Parameters router [E, d], gate and up [E, F, d], down [E, d, F].
+class DL_API ExpertMixture : public UnaryModule {
+public:
+    ExpertMixture(Index dimensions, Index hidden, Index experts, Index top, bool normalise = true, TensorOptions options = {});
+    Tensor forward(const Tensor& input) override { return mix(input).output; }
+    /// The output together with the chosen experts and their weights.
+    Mixture mix(const Tensor& input) const;
+    const Tensor& router() const { return router_; }
+    const Tensor& gate() const { return gate_; }
+    const Tensor& up() const { return up_; }
+    const Tensor& down() const { return down_; }
+    Index top() const { return top_; }
+
+private:
+    Index top_;
+    bool normalise_;
+    Tensor router_, gate_, up_, down_;
+};
+
 /// Frozen copy of a base Linear plus alpha/rank * up(down(x)); up starts at zero.  merged() returns an
 /// independent Linear with W + (alpha/rank) * up.weight @ down.weight rounded to W's dtype.
 class DL_API LoRALinear : public UnaryModule {

@@ -134,6 +134,60 @@ DL_API dl_status dl_paged_cache_append(dl_paged_cache* cache, int64_t layer, con
 DL_API dl_status dl_paged_attention(const dl_paged_cache* cache, int64_t layer, const dl_paged_batch* batch,
     const dl_tensor* query, dl_tensor** output);
 
+/* ---- Extensions (no reference counterpart): who holds which page, forks and compaction; the gated delta rule over states of
+ * fixed size; a layer of experts.  The rules stand at the C++ entries they call, dl/paged.h, dl/delta.h and dl/ops.h.  Arrays
+ * of ids are host memory, read (or written) during the call; a refused call changes nothing. ---- */
+typedef struct dl_page_pool dl_page_pool;
+DL_API dl_status dl_page_pool_create(int64_t pages, dl_page_pool** output);
+DL_API void dl_page_pool_release(dl_page_pool* pool);
+DL_API dl_status dl_page_pool_available(const dl_page_pool* pool, int64_t* available);
+DL_API dl_status dl_page_pool_references(const dl_page_pool* pool, int64_t page, int64_t* references);
+/* `count` free pages, the lowest ones, to `pages`. */
+DL_API dl_status dl_page_pool_take(dl_page_pool* pool, int64_t count, int64_t* pages);
+/* One more holder (claim: of free pages too; share: of held ones), or one fewer, of each page; ids below zero are passed over. */
+DL_API dl_status dl_page_pool_claim(dl_page_pool* pool, int64_t count, const int64_t* pages);
+DL_API dl_status dl_page_pool_share(dl_page_pool* pool, int64_t count, const int64_t* pages);
+DL_API dl_status dl_page_pool_give_back(dl_page_pool* pool, int64_t count, const int64_t* pages);
+/* Page sources[i] to page targets[i] in every layer, the first rows[i] positions of it (rows NULL: all). */
+DL_API dl_status dl_paged_cache_copy(dl_paged_cache* cache, int64_t count, const int64_t* sources, const int64_t* targets,
+    const int64_t* rows);
+/* New requests that go on from request parents[i] at its length: tables [sequences, width], forked [children, width]. */
+DL_API dl_status dl_paged_cache_fork(dl_paged_cache* cache, dl_page_pool* pool, int64_t sequences, const int64_t* tables,
+    int64_t width, const int64_t* lengths, int64_t children, const int64_t* parents, int64_t* forked);
+/* Moves the held pages to the front of the pool and renames them in tables (`count` ids, all that hold pages); *moved (may be
+ * NULL) receives how many. */
+DL_API dl_status dl_paged_cache_compact(dl_paged_cache* cache, dl_page_pool* pool, int64_t count, int64_t* tables,
+    int64_t* moved);
+
+typedef struct dl_delta_states dl_delta_states;
+typedef struct dl_delta_batch dl_delta_batch;
+/* States [slots, heads, key_dim, value_dim], f32, of each layer, zero at first. */
+DL_API dl_status dl_delta_states_create(int64_t layers, int64_t slots, int64_t heads, int64_t key_dim, int64_t value_dim,
+    dl_device device, dl_delta_states** output);
+DL_API void dl_delta_states_release(dl_delta_states* states);
+/* A view of a layer's live storage. */
+DL_API dl_status dl_delta_states_tensor(const dl_delta_states* states, int64_t layer, dl_tensor** output);
+DL_API dl_status dl_delta_states_copy(dl_delta_states* states, int64_t count, const int64_t* sources, const int64_t* targets);
+/* A step: request b goes on from slot sources[b] (-1: from zero) by counts[b] tokens and leaves its state in targets[b].  The
+ * call waits for the library's stream. */
+DL_API dl_status dl_delta_batch_create(const dl_delta_states* states, int64_t key_heads, int64_t requests,
+    const int64_t* sources, const int64_t* targets, const int64_t* counts, dl_delta_batch** output);
+DL_API void dl_delta_batch_release(dl_delta_batch* batch);
+/* query and key [tokens, key_heads, key_dim], value [tokens, heads, value_dim], decay and rate [tokens, heads]; scale may be
+ * NULL (1 / sqrt(key_dim)); f32 [tokens, heads, value_dim]. */
+DL_API dl_status dl_gated_delta(dl_delta_states* states, int64_t layer, const dl_delta_batch* batch, const dl_tensor* query,
+    const dl_tensor* key, const dl_tensor* value, const dl_tensor* decay, const dl_tensor* rate, const double* scale,
+    dl_tensor** output);
+
+/* input [..., d], router [E, d], gate and up [E, F, d], down [E, d, F]: output [..., d] f32, chosen [..., top] i64 and weights
+ * [..., top] f32; the last two slots may be NULL. */
+DL_API dl_status dl_expert_mixture(const dl_tensor* input, const dl_tensor* router, const dl_tensor* gate,
+    const dl_tensor* up, const dl_tensor* down, int64_t top, int32_t normalise, dl_tensor** output, dl_tensor** chosen,
+    dl_tensor** weights);
+/* The module: dl_module_forward gives its output. */
+DL_API dl_status dl_expert_mixture_create(int64_t dimensions, int64_t hidden, int64_t experts, int64_t top,
+    int32_t normalise, dl_tensor_options options, dl_module** output);
+
 #ifdef __cplusplus
 }
 #endif

@@ -2,7 +2,7 @@
 // Free functions on the decode path.  Mirrors include/dl/ops.h:100-101,149-158,191,341 of the reference
 // (argmax, rotary_embedding, grouped_query_attention, linear, embedding, rms_norm); `sample` has no
 // reference counterpart (the reference samples on the host, examples/text_generate.cpp:29-41), nor have `rotary_tables`,
-// `rotary_positions` and `verify_drafted`.
+// `rotary_positions`, `verify_drafted` and `expert_mixture`.
 // All arithmetic runs on the GPU; bf16 storage computes and returns f32.
 
 #include "dl/random.h"
@@ -67,5 +67,19 @@ DL_API Tensor sample(const Tensor& logits, double temperature, RandomKey key);
 DL_API std::pair<Tensor, Tensor> verify_drafted(const Tensor& drafted, const Tensor& target,
                                                 const std::optional<Tensor>& draft, double temperature,
                                                 const Tensor& uniforms);
+
+/// A feed-forward layer of E SwiGLU experts, of which each row x of input [..., d] (f32 or bf16) takes the `top` best: with
+/// z = router x (router [E, d]) and p = softmax(z), those with the largest z, the lowest index first among equals (a NaN wins, the
+/// first NaN first); their weights w are their p, divided by their sum where `normalise` is set; and
+///   y = sum_j w_j down[e_j] (silu(gate[e_j] x) * (up[e_j] x)),   gate and up [E, F, d], down [E, d, F].
+/// All matrices are f32 or bf16, the experts' of one type.  z and p are taken in 64 bits, so that rows choose as the exact
+/// numbers do; the experts' products keep all bits of an f32.  E is at most 1024, `top` at most 64.
+struct Mixture {
+    Tensor output;  ///< f32 [..., d]
+    Tensor chosen;  ///< i64 [..., top], the largest z first
+    Tensor weights; ///< f32 [..., top]
+};
+DL_API Mixture expert_mixture(const Tensor& input, const Tensor& router, const Tensor& gate, const Tensor& up,
+                              const Tensor& down, Index top, bool normalise = true);
 
 } // namespace dl

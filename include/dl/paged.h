@@ -2,12 +2,14 @@
 // A paged key/value cache and the operators of a serving step over it (no counterpart in the reference, whose KVCache
 // holds one batch of one length).  Requests of different lengths share one pool of pages; a step's batch says which new
 // positions of which requests it computes and in which pages they lie.  The caller hands pages out; everything it says
-// about them is checked on the host when the batch is made, before any kernel reads it.
+// about them is checked on the host when the batch is made, before any kernel reads it.  A PagePool counts who holds which
+// page; requests are forked, and what is left of a pool moved to its front, by copies that the operators below queue.
 
 #include "dl/ops.h"
 
 #include <memory>
 #include <span>
+#include <vector>
 
 namespace dl::nn {
 
@@ -52,6 +54,32 @@ private:
     std::shared_ptr<const Plan> plan_;
 };
 
+/// Which pages of a cache are held, and by how many page tables.  Host bookkeeping alone; used by one thread at a time.
+/// Ids below zero (the empty places of a table) are passed over; an id beyond the pool is refused, and a refused call
+/// changes nothing.
+class DL_API PagePool {
+public:
+    explicit PagePool(Index pages);
+    Index pages() const { return static_cast<Index>(holders_.size()); }
+    /// Pages that nobody holds.
+    Index available() const { return available_; }
+    Index references(Index page) const;
+    /// `count` free pages, the lowest ones, each held once from now on.
+    std::vector<Index> take(Index count);
+    /// One more holder of each page, free ones among them (a pool made anew from tables).
+    void claim(std::span<const Index> pages);
+    /// One more holder of each page, all of them held.
+    void share(std::span<const Index> pages);
+    /// One holder fewer of each page; without any it is free.  Work queued that reads it has the old contents still: what
+    /// writes it next is queued behind.
+    void release(std::span<const Index> pages);
+
+private:
+    void check(std::span<const Index> pages) const;
+    std::vector<Index> holders_;
+    Index available_, lowest_ = 0; // no page below `lowest_` is free
+};
+
 } // namespace dl::nn
 
 namespace dl {
@@ -72,5 +100,23 @@ DL_API Tensor paged_append(const nn::PagedKVCache& cache, Index layer, const nn:
 /// for values up to 1e36 over the number of keys that the row sees: they are summed with weights of up to 2^8 before the division.
 /// Where a row sees a value that is not finite, that entry of it is not finite either.
 DL_API Tensor paged_attention(const nn::PagedKVCache& cache, Index layer, const nn::PagedBatch& batch, const Tensor& query);
+
+/// Copies page sources[i] to page targets[i] in every layer, keys and values, of each only the first rows[i] positions (an
+/// empty `rows`: whole pages); what else a target holds stays.  Every source is taken as it was before the call, whichever
+/// order the pairs stand in; no page is a target twice.
+DL_API void paged_copy(const nn::PagedKVCache& cache, std::span<const Index> sources, std::span<const Index> targets,
+                       std::span<const Index> rows = {});
+
+/// Tables [parents, width] of new requests that go on from position lengths[p] of request p = parents[i] (a row of `tables`
+/// [sequences, width], all of its pages up to there held): the whole pages in front are shared, a partly filled last one is
+/// copied, as far as it is filled, to a page taken from the pool, and the rest of a row is -1.  With too few free pages
+/// the call is refused and the pool stays as it was.
+DL_API std::vector<Index> paged_fork(const nn::PagedKVCache& cache, nn::PagePool& pool, std::span<const Index> tables, Index width,
+                                     std::span<const Index> lengths, std::span<const Index> parents);
+
+/// Moves the held pages to the front of the pool: those beyond the first n, n the number of held pages, go to the free ones
+/// among them, in ascending order; their ids in `tables` become the new ones.  The tables are all that holds pages: a page
+/// stands in them as often as the pool counts.  Returns how many pages were moved.
+DL_API Index paged_compact(const nn::PagedKVCache& cache, nn::PagePool& pool, std::span<Index> tables);
 
 } // namespace dl

@@ -6,6 +6,7 @@ decoder.* entries (its RoPE buffers stay the library's own), Linear head from ou
 """
 from __future__ import annotations
 
+import ctypes as C
 import sys
 
 import numpy as np
@@ -76,6 +77,16 @@ def say(msg):
     """Progress lines of the GPU tests (flushed: a long case names itself before it runs)."""
     print(msg, flush=True)
     sys.stdout.flush()
+
+
+def write(tensor, values: np.ndarray) -> None:
+    """Host bytes over a live view's storage (through the HIP runtime that the library is linked with)."""
+    copy = ct.lib().hipMemcpy
+    copy.argtypes, copy.restype = [C.c_void_p, C.c_void_p, C.c_size_t, C.c_int], C.c_int
+    values = np.ascontiguousarray(values)
+    assert tensor.info.contiguous and values.nbytes == ct.lib().dl_tensor_nbytes(tensor.handle)
+    ct.synchronize()
+    assert copy(ct.lib().dl_tensor_data(tensor.handle), values.ctypes.data, values.nbytes, 1) == 0
 
 
 def rel_err(got: np.ndarray, want: np.ndarray) -> float:
