@@ -1,10 +1,17 @@
-// A layer of experts over few rows (see dlk_experts_params in kernels.h).
-#include "kernels/device_common.h"
+// A layer of experts over few rows (see dlk_experts_params in kernels.h): the router in f64, the hidden entries of the chosen
+// experts, their output entries, and the weighted sum.  Bound by memory: a few rows read each chosen expert's matrices once.
+//
+// Products keep all bits of an f32: bf16 matrices go into v_mfma_f32_16x16x32_bf16 as they are, rows as three bf16 parts that
+// hold all 24 bits (bf16 rows are one); f32 matrices and rows go into v_mfma_f32_16x16x4_f32.
+#include "kernels/parts.h"
+
+#include <algorithm>
 
 namespace dlk {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr uint32_t kBeyond = 1u << 31; // an offset behind every buffer's end
+constexpr int kPairs = 8192; // (row, chosen expert) pairs of a launch: the list of an expert's in LDS
 
 __device__ __forceinline__ float entry(const void* x, int bf16, int64_t at) {
     return bf16 ? bf16_to_f32(static_cast<const uint16_t*>(x)[at]) : static_cast<const float*>(x)[at];
@@ -16,57 +23,472 @@ __device__ __forceinline__ double wave_sum_f64(double v) {
     return v;
 }
 
-// A work-group per row: the logits in f64, which hold products of two f32 exactly, so that rows choose as the exact logits do
-// but for ties within 1e-15 of them; then one wave picks the best one after another.
-__global__ __launch_bounds__(kThreads) void experts_route(const dlk_experts_params p) {
-    __shared__ double logits[DLK_EXPERTS_MOST];
-    const int64_t token = blockIdx.x;
-    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    for (int e = wave; e < p.experts; e += kThreads / kWave) {
-        double sum = 0.0;
-        for (int i = lane; i < p.dim; i += kWave)
-            sum = fma(static_cast<double>(entry(p.x, p.x_bf16, token * p.dim + i)),
-                      static_cast<double>(entry(p.router, p.router_bf16, static_cast<int64_t>(e) * p.dim + i)), sum);
-        sum = wave_sum_f64(sum);
-        if (lane == 0) logits[e] = sum;
-    }
-    __syncthreads();
-    if (wave != 0) return;
-    uint32_t taken = 0; // of this lane's experts lane, lane + 64, ...
-    double largest = 0.0, all = 0.0, mine = 0.0, picked = 0.0;
-    int64_t own = 0;
-    for (int j = 0; j < p.top; ++j) {
-        double best = 0.0;
-        int64_t at = p.experts; // none
-        for (int e = lane, n = 0; e < p.experts; e += kWave, ++n)
-            if (!(taken >> n & 1) && (at == p.experts || prefer(logits[e], e, best, at))) best = logits[e], at = e;
+__device__ __forceinline__ void eight(const void* x, int bf16, int64_t at, float (&v)[8]) {
+    if (bf16) {
+        const u32x4 w = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(x) + at);
 #pragma unroll
-        for (int d = 1; d < kWave; d *= 2) {
-            const double other = __shfl_xor(best, d);
-            const int64_t index = __shfl_xor(static_cast<long long>(at), d);
-            if (index < p.experts && (at == p.experts || prefer(other, index, best, at))) best = other, at = index;
-        }
-        if (static_cast<int>(at) % kWave == lane) taken |= 1u << at / kWave;
-        if (j == 0) {
-            largest = best;
-            double sum = 0.0;
-            for (int e = lane; e < p.experts; e += kWave) sum += exp(logits[e] - largest);
-            all = wave_sum_f64(sum);
-        }
-        const double weight = exp(best - largest);
-        picked += weight;
-        if (j == lane) mine = weight, own = at;
-    }
-    if (lane < p.top) {
-        p.chosen[token * p.top + lane] = own;
-        p.weights[token * p.top + lane] = static_cast<float>(mine / (p.normalise ? picked : all));
+        for (int i = 0; i < 4; ++i) v[2 * i] = bf16_lo(w[i]), v[2 * i + 1] = bf16_hi(w[i]);
+    } else {
+        const f32x4* from = reinterpret_cast<const f32x4*>(static_cast<const float*>(x) + at);
+        const f32x4 a = from[0], b = from[1];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
     }
 }
 
-// Any sizes and alignments: a wave per pair (row, chosen expert) and hidden entry.
-__global__ __launch_bounds__(kThreads) void experts_hidden_any(const dlk_experts_params p) {
+struct Plan {          // what a launch's kernels hand on
+    uint16_t* pick;    // [tokens, top]: the chosen experts
+    char* rows;        // x as the products read it (see `planes`), or NULL: p.x itself
+    char* act;         // the hidden entries, likewise
+    float* partial;    // [tokens, top, dim]: outputs of each pair
+    int planes;        // bf16 matrices: parts of a row of x; 0: f32 matrices, f32 rows
+};
+
+// A work-group per row: the logits in f64, which hold products of two f32 exactly, so that rows choose as the exact logits do
+// but for ties within 1e-15 of them; an expert's rank is the number of those that are preferred to it.  On the way the row is
+// laid out for the products.  WIDE: pieces of 8 entries (dim a multiple of 8, 16-byte aligned).
+constexpr int kRoute = 1024, kRouteWaves = kRoute / kWave;
+template <bool WIDE>
+__global__ __launch_bounds__(kRoute) void experts_route(const dlk_experts_params p, const Plan plan) {
+    __shared__ double logits[DLK_EXPERTS_MOST];
+    __shared__ int slots[DLK_EXPERTS_TOP_MOST];
+    const int64_t token = blockIdx.x;
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    if constexpr (WIDE) {
+        if (plan.rows)
+            for (int i = threadIdx.x * 8; i < p.dim; i += kRoute * 8) {
+                float v[8];
+                eight(p.x, p.x_bf16, token * p.dim + i, v);
+                if (plan.planes == 0) {
+                    f32x4* to = reinterpret_cast<f32x4*>(reinterpret_cast<float*>(plan.rows) + token * p.dim + i);
+                    to[0] = f32x4{v[0], v[1], v[2], v[3]}, to[1] = f32x4{v[4], v[5], v[6], v[7]};
+                }
+                for (int part = 0; part < plan.planes; ++part)
+                    *reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(plan.rows) + (part * p.tokens + token) * p.dim + i) = cut(v);
+            }
+        constexpr int N = 4; // experts at a time
+        for (int first = wave * N; first < p.experts; first += kRouteWaves * N) {
+            double sum[N] = {};
+            for (int i = lane * 8; i < p.dim; i += kWave * 8) {
+                float x[8], w[N][8];
+                eight(p.x, p.x_bf16, token * p.dim + i, x);
+#pragma unroll
+                for (int n = 0; n < N; ++n) eight(p.router, p.router_bf16, static_cast<int64_t>(min(first + n, p.experts - 1)) * p.dim + i, w[n]);
+#pragma unroll
+                for (int n = 0; n < N; ++n)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) sum[n] = fma(static_cast<double>(x[j]), static_cast<double>(w[n][j]), sum[n]);
+            }
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                const double z = wave_sum_f64(sum[n]);
+                if (lane == 0 && first + n < p.experts) logits[first + n] = z;
+            }
+        }
+    } else {
+        for (int e = wave; e < p.experts; e += kRouteWaves) {
+            double sum = 0.0;
+            for (int i = lane; i < p.dim; i += kWave)
+                sum = fma(static_cast<double>(entry(p.x, p.x_bf16, token * p.dim + i)),
+                          static_cast<double>(entry(p.router, p.router_bf16, static_cast<int64_t>(e) * p.dim + i)), sum);
+            sum = wave_sum_f64(sum);
+            if (lane == 0) logits[e] = sum;
+        }
+    }
+    __syncthreads();
+    for (int first = 0; first < p.experts; first += kRoute / 16) { // 16 lanes an expert
+        const int e = first + threadIdx.x / 16;
+        int before = 0;
+        if (e < p.experts) {
+            const double z = logits[e];
+            for (int f = threadIdx.x % 16; f < p.experts; f += 16) before += f != e && prefer(logits[f], f, z, e);
+        }
+#pragma unroll
+        for (int d = 1; d < 16; d *= 2) before += __shfl_xor(before, d);
+        if (threadIdx.x % 16 == 0 && e < p.experts && before < p.top) slots[before] = e;
+    }
+    __syncthreads();
+    if (wave != 0) return;
+    const double largest = logits[slots[0]];
+    const int own = slots[min(lane, p.top - 1)];
+    const double mine = lane < p.top ? exp(logits[own] - largest) : 0.0;
+    double all = mine;
+    if (!p.normalise) {
+        all = 0.0;
+        for (int e = lane; e < p.experts; e += kWave) all += exp(logits[e] - largest);
+    }
+    all = wave_sum_f64(all);
+    if (lane < p.top) {
+        p.chosen[token * p.top + lane] = own;
+        plan.pick[token * p.top + lane] = static_cast<uint16_t>(own);
+        p.weights[token * p.top + lane] = static_cast<float>(mine / all);
+    }
+}
+
+// The pairs of expert `e`, in order, to `list`; `counts` is scratch.  Each of the WAVES waves looks through a run of them, twice.
+template <int WAVES> __device__ __forceinline__ int collect(const uint16_t* pick, int pairs, int e, uint16_t* list, int* counts) {
+    constexpr int THREADS = WAVES * kWave;
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    const int run = ((pairs + THREADS - 1) / THREADS) * kWave, begin = wave * run, end = min(pairs, begin + run);
+    int count = 0;
+    for (int i = begin + lane; i - lane < end; i += kWave) count += __popcll(__ballot(i < end && pick[i] == e));
+    if (lane == 0) counts[wave] = count;
+    __syncthreads();
+    int at = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+        at += w < wave ? counts[w] : 0;
+        all += counts[w];
+    }
+    for (int i = begin + lane; i - lane < end; i += kWave) {
+        const bool own = i < end && pick[i] == e;
+        const uint64_t mask = __ballot(own);
+        if (own) list[at + __popcll(mask & ((1ull << lane) - 1))] = static_cast<uint16_t>(i);
+        at += __popcll(mask);
+    }
+    __syncthreads();
+    return all;
+}
+
+// Lanes l and l ^ 8 change places with half of what they hold (see below).
+__device__ __forceinline__ void exchange(u32x4 (&w)[2]) {
+    constexpr int kRotate8 = 0x128; // row_ror:8, of 16 lanes
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int a = static_cast<int>(w[0][j]), b = static_cast<int>(w[1][j]);
+        w[0][j] = __builtin_amdgcn_update_dpp(a, b, kRotate8, 0xf, 0xc, false);
+        w[1][j] = __builtin_amdgcn_update_dpp(b, a, kRotate8, 0xf, 0x3, false);
+    }
+}
+
+// An entry of a pair: a hidden one as the next product reads it, or an output.
+template <bool GATE, bool F32>
+__device__ __forceinline__ void keep(const dlk_experts_params& p, const Plan& plan, int pair, int row, float v, float up) {
+    const int64_t height = GATE ? p.hidden : p.dim, to = pair * height + row;
+    if constexpr (!GATE) plan.partial[to] = v;
+    else {
+        v = v / (1.0f + expf(-v)) * up;
+        if constexpr (F32) reinterpret_cast<float*>(plan.act)[to] = v;
+        else
+#pragma unroll
+            for (int part = 0; part < 3; ++part) reinterpret_cast<uint16_t*>(plan.act)[part * p.tokens * p.top * height + to] = cut(v);
+    }
+}
+
+// One chosen expert's products with the rows that chose it, which are the columns here, 16 NT at a time.  16 R rows of its
+// matrices (GATE: of gate and up, and silu(gate) * up of both; else of down) are a wave's own, or, SPLIT, a work-group's whose
+// waves share the sum's index and join their sums in LDS.  A ring of D steps of 64 bytes a row is on its way from memory.
+// A work-group stands for expert blockIdx.y, or, where there are fewer pairs than experts, for the expert of pair blockIdx.y
+// if that is its first.
+template <bool GATE, bool F32, int PARTS, int R, int NT, bool SPLIT>
+__global__ __launch_bounds__(SPLIT ? 512 : 256) void experts_rows(const dlk_experts_params p, const Plan plan) {
+    constexpr int WAVES = SPLIT ? 8 : 4, THREADS = WAVES * kWave, TILES = GATE ? 2 * R : R;
+    constexpr int ROOM = 15 / (TILES + NT * PARTS), D = SPLIT || ROOM < 2 ? 2 : ROOM > 4 ? 4 : ROOM;
+    constexpr int SIZE = F32 ? 4 : 2, PAD = 20;
+    extern __shared__ uint16_t list[];
+    __shared__ int counts[WAVES];
+    __shared__ float sums[SPLIT ? WAVES : 1][TILES][16][PAD];
+    const int pairs = static_cast<int>(p.tokens) * p.top;
+    const bool few = pairs < p.experts;
+    const int e = few ? plan.pick[blockIdx.y] : blockIdx.y;
+
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, n = lane % 16, g = lane / 16;
+    const int width = GATE ? p.dim : p.hidden, height = GATE ? p.hidden : p.dim;
+    const uint32_t row_bytes = static_cast<uint32_t>(width) * SIZE, matrix = row_bytes * static_cast<uint32_t>(height);
+    const int first_row = (SPLIT ? blockIdx.x : blockIdx.x * WAVES + wave) * 16 * R;
+    const auto resource = [](const void* at, uint32_t bytes) {
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(at), 0, bytes, kBufferFlags);
+    };
+    const auto of_expert = [&](const void* w) { return static_cast<const char*>(w) + static_cast<int64_t>(e) * matrix; };
+    const __amdgpu_buffer_rsrc_t w0 = resource(of_expert(GATE ? p.gate : p.down), matrix), w1 = resource(of_expert(GATE ? p.up : p.down), matrix);
+    const uint32_t x_rows = GATE ? static_cast<uint32_t>(p.tokens) : static_cast<uint32_t>(pairs), plane = x_rows * row_bytes;
+    const __amdgpu_buffer_rsrc_t x = resource(GATE ? (plan.rows ? plan.rows : static_cast<const char*>(p.x)) : plan.act, plane * PARTS);
+    uint32_t w_at[R][2];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int row = first_row + 16 * r + 8 * i + n % 8;
+            w_at[r][i] = row < height ? static_cast<uint32_t>(row) * row_bytes : kBeyond;
+        }
+
+    const int steps = (static_cast<int>(row_bytes) + 127) / 128, per = SPLIT ? (steps + WAVES - 1) / WAVES : steps;
+    const int begin = SPLIT ? wave * per : 0, end = min(steps, begin + per);
+    const int turn = static_cast<int>((blockIdx.x * WAVES + wave + blockIdx.y * 5u) * 7u % static_cast<uint32_t>(steps));
+    struct Held {
+        u32x4 w[TILES][2], x[NT][2][PARTS];
+    };
+    // (what lies behind a row's end or the wave's run is read as zero, from beyond the buffer)
+    const auto of_step = [&](int step) {
+        const int turned = SPLIT ? step : step + turn < steps ? step + turn : step + turn - steps;
+        return static_cast<uint32_t>(step < end ? turned : steps) * 128;
+    };
+    const auto load_weights = [&](int step, Held& to) {
+        const uint32_t k = of_step(step) + g * 32 + n / 8 * 16;
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t at = k < row_bytes ? w_at[r][i] + k : kBeyond;
+                to.w[r][i] = __builtin_amdgcn_raw_buffer_load_b128(w0, at, 0, 0);
+                if constexpr (GATE) to.w[R + r][i] = __builtin_amdgcn_raw_buffer_load_b128(w1, at, 0, 0);
+            }
+    };
+    Held ring[D]; // (the weights' on their way while the rows are looked up)
+#pragma unroll
+    for (int d = 0; d < D; ++d) load_weights(begin + d, ring[d]);
+    const int count = collect<WAVES>(plan.pick, pairs, e, list, counts);
+    if (few && list[0] != blockIdx.y) return;
+    for (int first = 0; first < count; first += 16 * NT) {
+        const int tiles = min(NT, (count - first + 15) / 16); // that hold rows
+        uint32_t x_at[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int i = first + 16 * t + n;
+            x_at[t] = i < count ? static_cast<uint32_t>(GATE ? list[i] / p.top : list[i]) * row_bytes : kBeyond;
+        }
+        f32x4 sum[NT][TILES];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < TILES; ++i) sum[t][i] = 0.0f;
+        const auto load_rows = [&](int step, Held& to) {
+            const uint32_t k = of_step(step) + g * 32;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+                if (t < tiles)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int part = 0; part < PARTS; ++part) // (x_at may lie behind the end by itself)
+                            to.x[t][i][part] = __builtin_amdgcn_raw_buffer_load_b128(
+                                x, k + 16 * i < row_bytes ? x_at[t] + part * plane + k + 16 * i : kBeyond, 0, 0);
+        };
+        const auto multiply = [&](Held& of) {
+#pragma unroll
+            for (int i = 0; i < TILES; ++i) exchange(of.w[i]);
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+                if (t < tiles)
+#pragma unroll
+                    for (int i = 0; i < TILES; ++i)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            if constexpr (F32) {
+#pragma unroll
+                                for (int j = 0; j < 4; ++j)
+                                    sum[t][i] = product(__uint_as_float(of.w[i][h][j]), __uint_as_float(of.x[t][h][0][j]), sum[t][i]);
+                            } else {
+#pragma unroll
+                                for (int part = PARTS - 1; part >= 0; --part) sum[t][i] = product(of.w[i][h], of.x[t][h][part], sum[t][i]);
+                            }
+                        }
+        };
+#pragma unroll
+        for (int d = 0; d < D; ++d) {
+            if (first > 0) load_weights(begin + d, ring[d]);
+            load_rows(begin + d, ring[d]);
+        }
+        for (int step = begin; step < end; step += D)
+#pragma unroll
+            for (int d = 0; d < D; ++d) {
+                multiply(ring[d]);
+                load_weights(step + D + d, ring[d]);
+                load_rows(step + D + d, ring[d]);
+            }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            if (t >= tiles) break;
+            if constexpr (SPLIT) {
+#pragma unroll
+                for (int i = 0; i < TILES; ++i) *reinterpret_cast<f32x4*>(&sums[wave][i][n][4 * g]) = sum[t][i];
+                __syncthreads();
+                for (int i = threadIdx.x; i < 256 * R; i += THREADS) {
+                    const int r = i % 16, tile = i / 16 % R, column = i / (16 * R), row = first_row + 16 * tile + r;
+                    const int at = first + 16 * t + column;
+                    if (row >= height || at >= count) continue;
+                    float v = 0.0f, up = 0.0f;
+#pragma unroll
+                    for (int w = 0; w < WAVES; ++w) {
+                        v += sums[w][tile][column][r];
+                        if constexpr (GATE) up += sums[w][R + tile][column][r];
+                    }
+                    keep<GATE, F32>(p, plan, list[at], row, v, up);
+                }
+                __syncthreads();
+            } else {
+                const int at = first + 16 * t + n;
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int row = first_row + 16 * r + 4 * g + j;
+                        if (row < height && at < count) keep<GATE, F32>(p, plan, list[at], row, sum[t][r][j], GATE ? sum[t][TILES - R + r][j] : 0.0f);
+                    }
+            }
+        }
+    }
+}
+
+// The same for experts that many rows chose: the rows pass through LDS, 128 bytes of up to 16 NT of them at a time, for the
+// work-group's waves, which have 16 R rows of the matrices each.  (Read by each wave for itself they took most of the time: of
+// 25 rows an expert through 32 experts of 768 x 2048, 58 us to the hidden entries and 57 back, through LDS 45 and 31.)
+template <bool GATE, bool F32, int PARTS, int R, int NT, int WAVES>
+__global__ __launch_bounds__(WAVES * kWave) void experts_blocks(const dlk_experts_params p, const Plan plan) {
+    constexpr int THREADS = WAVES * kWave, TILES = GATE ? 2 * R : R, D = TILES > 2 ? 2 : 4;
+    constexpr int SIZE = F32 ? 4 : 2, ROWS = 16 * NT, UNITS = PARTS * ROWS * 8, STAGED = (UNITS + THREADS - 1) / THREADS;
+    extern __shared__ uint16_t list[];
+    __shared__ int counts[WAVES];
+    __shared__ u32x4 held[2][UNITS]; // [part][row][8 pieces of 16 bytes, in an order of the row's own]
+    const int pairs = static_cast<int>(p.tokens) * p.top, e = blockIdx.y;
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, n = lane % 16, g = lane / 16;
+    const int width = GATE ? p.dim : p.hidden, height = GATE ? p.hidden : p.dim;
+    const uint32_t row_bytes = static_cast<uint32_t>(width) * SIZE, matrix = row_bytes * static_cast<uint32_t>(height);
+    const int first_row = (blockIdx.x * WAVES + wave) * 16 * R;
+    const auto resource = [](const void* at, uint32_t bytes) {
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(at), 0, bytes, kBufferFlags);
+    };
+    const auto of_expert = [&](const void* w) { return static_cast<const char*>(w) + static_cast<int64_t>(e) * matrix; };
+    const __amdgpu_buffer_rsrc_t w0 = resource(of_expert(GATE ? p.gate : p.down), matrix), w1 = resource(of_expert(GATE ? p.up : p.down), matrix);
+    const uint32_t x_rows = GATE ? static_cast<uint32_t>(p.tokens) : static_cast<uint32_t>(pairs), plane = x_rows * row_bytes;
+    const __amdgpu_buffer_rsrc_t x = resource(GATE ? (plan.rows ? plan.rows : static_cast<const char*>(p.x)) : plan.act, plane * PARTS);
+    uint32_t w_at[R][2];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int row = first_row + 16 * r + 8 * i + n % 8;
+            w_at[r][i] = row < height ? static_cast<uint32_t>(row) * row_bytes : kBeyond;
+        }
+    const int steps = (static_cast<int>(row_bytes) + 127) / 128;
+    const int turn = static_cast<int>((blockIdx.x + blockIdx.y * 5u) * 7u % static_cast<uint32_t>(steps));
+    const auto turned = [&](int step) { return static_cast<uint32_t>(step >= steps ? steps : step + turn < steps ? step + turn : step + turn - steps) * 128; };
+    struct Weights {
+        u32x4 w[TILES][2];
+    };
+    const auto load = [&](int step, Weights& to) {
+        const uint32_t k = turned(step) + g * 32 + n / 8 * 16;
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t at = k < row_bytes ? w_at[r][i] + k : kBeyond;
+                to.w[r][i] = __builtin_amdgcn_raw_buffer_load_b128(w0, at, 0, 0);
+                if constexpr (GATE) to.w[R + r][i] = __builtin_amdgcn_raw_buffer_load_b128(w1, at, 0, 0);
+            }
+    };
+    Weights ring[D]; // (on its way while the rows are looked up)
+#pragma unroll
+    for (int d = 0; d < D; ++d) load(d, ring[d]);
+    const int count = collect<WAVES>(plan.pick, pairs, e, list, counts);
+    for (int first = 0; first < count; first += ROWS) {
+        const int blocks = min(NT, (count - first + 15) / 16); // of 16 columns, that hold rows
+        uint32_t x_at[STAGED];
+#pragma unroll
+        for (int i = 0; i < STAGED; ++i) {
+            const int unit = threadIdx.x + i * THREADS, row = unit / 8 % ROWS, at = first + row;
+            x_at[i] = unit < UNITS && at < count
+                          ? static_cast<uint32_t>(GATE ? list[at] / p.top : list[at]) * row_bytes + unit / (8 * ROWS) * plane : kBeyond;
+        }
+        f32x4 sum[NT][TILES];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < TILES; ++i) sum[t][i] = 0.0f;
+        u32x4 coming[STAGED];
+        const auto fetch = [&](int step) {
+            const uint32_t k = turned(step);
+#pragma unroll
+            for (int i = 0; i < STAGED; ++i) {
+                const uint32_t at = k + threadIdx.x % 8 * 16;
+                coming[i] = __builtin_amdgcn_raw_buffer_load_b128(x, at < row_bytes ? x_at[i] + at : kBeyond, 0, 0);
+            }
+        };
+        const auto stage = [&](int buffer) {
+#pragma unroll
+            for (int i = 0; i < STAGED; ++i) {
+                const int unit = threadIdx.x + i * THREADS;
+                if (UNITS % THREADS == 0 || unit < UNITS) held[buffer][unit ^ (unit / 8 % 8)] = coming[i];
+            }
+        };
+        const auto multiply = [&](Weights& of, int buffer) {
+#pragma unroll
+            for (int i = 0; i < TILES; ++i) exchange(of.w[i]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    if (t >= blocks) break;
+                    u32x4 rows[PARTS];
+#pragma unroll
+                    for (int part = 0; part < PARTS; ++part) {
+                        const int row = part * ROWS + 16 * t + n;
+                        rows[part] = held[buffer][row * 8 + ((2 * g + h) ^ (row % 8))];
+                    }
+#pragma unroll
+                    for (int i = 0; i < TILES; ++i) {
+                        if constexpr (F32) {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                sum[t][i] = product(__uint_as_float(of.w[i][h][j]), __uint_as_float(rows[0][j]), sum[t][i]);
+                        } else {
+#pragma unroll
+                            for (int part = PARTS - 1; part >= 0; --part) sum[t][i] = product(of.w[i][h], rows[part], sum[t][i]);
+                        }
+                    }
+                }
+        };
+        fetch(0);
+        if (first > 0)
+#pragma unroll
+            for (int d = 0; d < D; ++d) load(d, ring[d]);
+        stage(0);
+        fetch(1);
+        __syncthreads();
+        for (int step = 0; step < steps; step += D)
+#pragma unroll
+            for (int d = 0; d < D; ++d) {
+                static_assert(D % 2 == 0, "a buffer for each other step");
+                stage((d + 1) % 2);
+                fetch(step + d + 2);
+                multiply(ring[d], d % 2);
+                load(step + D + d, ring[d]);
+                __syncthreads();
+            }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int at = first + 16 * t + n;
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int row = first_row + 16 * r + 4 * g + j;
+                    if (row < height && at < count) keep<GATE, F32>(p, plan, list[at], row, sum[t][r][j], GATE ? sum[t][TILES - R + r][j] : 0.0f);
+                }
+        }
+    }
+}
+
+// The weighted sum of a row's outputs, in the order of its choice.  A thread has four neighbouring entries.
+__global__ __launch_bounds__(256) void experts_join(const dlk_experts_params p, const float* partial) {
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, units = p.dim / 4;
+    if (i >= p.tokens * units) return;
+    const int64_t token = i / units;
+    const f32x4* from = reinterpret_cast<const f32x4*>(partial) + token * p.top * units + i % units;
+    f32x4 y = 0.0f;
+    for (int j = 0; j < p.top; ++j) {
+        const f32x4 v = from[j * units];
+        const float w = p.weights[token * p.top + j];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) y[c] = fmaf(w, v[c], y[c]);
+    }
+    reinterpret_cast<f32x4*>(p.y)[i] = y;
+}
+
+// Any sizes and alignments: a wave per pair (row, chosen expert) and hidden entry,
+__global__ __launch_bounds__(256) void experts_hidden_any(const dlk_experts_params p, float* act) {
     const int lane = threadIdx.x % kWave;
-    const int64_t unit = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / kWave, step = static_cast<int64_t>(gridDim.x) * kThreads / kWave;
+    const int64_t unit = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / kWave, step = static_cast<int64_t>(gridDim.x) * 256 / kWave;
     for (int64_t u = unit; u < p.tokens * p.top * p.hidden; u += step) {
         const int64_t pair = u / p.hidden, row = p.chosen[pair] * p.hidden + u % p.hidden;
         float g = 0.0f, h = 0.0f;
@@ -76,39 +498,136 @@ __global__ __launch_bounds__(kThreads) void experts_hidden_any(const dlk_experts
             h = fmaf(x, entry(p.up, p.weights_bf16, row * p.dim + i), h);
         }
         g = wave_sum(g), h = wave_sum(h);
-        if (lane == 0) p.act[u] = g / (1.0f + expf(-g)) * h;
+        if (lane == 0) act[u] = g / (1.0f + expf(-g)) * h;
     }
 }
 
-// and a wave per row and output entry, the chosen experts in order
-__global__ __launch_bounds__(kThreads) void experts_down_any(const dlk_experts_params p) {
+// and a wave per row and output entry, the chosen experts in order.
+__global__ __launch_bounds__(256) void experts_down_any(const dlk_experts_params p, const float* act) {
     const int lane = threadIdx.x % kWave;
-    const int64_t unit = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) / kWave, step = static_cast<int64_t>(gridDim.x) * kThreads / kWave;
+    const int64_t unit = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / kWave, step = static_cast<int64_t>(gridDim.x) * 256 / kWave;
     for (int64_t u = unit; u < p.tokens * p.dim; u += step) {
         float y = 0.0f;
         for (int j = 0; j < p.top; ++j) {
             const int64_t pair = u / p.dim * p.top + j, row = p.chosen[pair] * p.dim + u % p.dim;
             float sum = 0.0f;
             for (int i = lane; i < p.hidden; i += kWave)
-                sum = fmaf(p.act[pair * p.hidden + i], entry(p.down, p.weights_bf16, row * p.hidden + i), sum);
+                sum = fmaf(act[pair * p.hidden + i], entry(p.down, p.weights_bf16, row * p.hidden + i), sum);
             y = fmaf(p.weights[pair], wave_sum(sum), y);
         }
         if (lane == 0) p.y[u] = y;
     }
 }
 
+// Whether the products read whole pieces of 16 bytes at offsets of 32 bits.
+bool pieces(const dlk_experts_params& p) {
+    const int unit = p.weights_bf16 ? 8 : 4, size = p.weights_bf16 ? 2 : 4;
+    const auto aligned = [](const void* at) { return reinterpret_cast<uintptr_t>(at) % 16 == 0; };
+    return p.dim % unit == 0 && p.hidden % unit == 0 && aligned(p.gate) && aligned(p.up) && aligned(p.down) &&
+           static_cast<int64_t>(p.dim) * p.hidden * size <= INT32_MAX;
+}
+bool wide(const dlk_experts_params& p) {
+    const auto aligned = [](const void* at) { return reinterpret_cast<uintptr_t>(at) % 16 == 0; };
+    return p.dim % 8 == 0 && aligned(p.x) && aligned(p.router);
+}
+int64_t up16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
+
+struct Layout {
+    bool fast;
+    int planes; // of x: parts (bf16 matrices) or 0
+    int64_t rows, act, partial, bytes;
+};
+Layout layout(const dlk_experts_params& p) {
+    Layout l{};
+    const int64_t pairs = p.tokens * p.top;
+    // rows are laid out by the router's kernel in pieces of 8
+    const int64_t most = std::max<int64_t>(p.tokens * p.dim, pairs * p.hidden) * (p.weights_bf16 ? 6 : 4);
+    l.fast = pieces(p) && most <= INT32_MAX && (wide(p) || (p.weights_bf16 == p.x_bf16 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0));
+    l.planes = p.weights_bf16 ? (p.x_bf16 ? 1 : 3) : 0;
+    l.rows = up16(pairs * 2); // behind the choice
+    int64_t at = l.rows;
+    if (l.fast && p.weights_bf16 != p.x_bf16) at += up16(p.tokens * p.dim * (p.weights_bf16 ? 6 : 4));
+    l.act = at;
+    at += up16(pairs * p.hidden * (l.fast && p.weights_bf16 ? 6 : 4));
+    l.partial = at;
+    l.bytes = at + (l.fast ? pairs * p.dim * 4 : 0);
+    return l;
+}
+
+template <bool GATE, bool F32, int PARTS> void rows_of(const dlk_experts_params& p, const Plan& plan, hipStream_t at) {
+    const int pairs = static_cast<int>(p.tokens) * p.top, height = GATE ? p.hidden : p.dim;
+    const int active = std::min(pairs, p.experts), tiles = (height + 15) / 16;
+    const auto launch = [&](auto r, auto nt, auto split) {
+        constexpr int R = decltype(r)::value, NT = decltype(nt)::value;
+        constexpr bool SPLIT = decltype(split)::value;
+        const int per = R * (SPLIT ? 1 : 4);
+        experts_rows<GATE, F32, PARTS, R, NT, SPLIT><<<dim3((tiles + per - 1) / per, active), SPLIT ? 512 : 256, pairs * 2, at>>>(p, plan);
+    };
+    using std::integral_constant;
+    const integral_constant<int, 1> one;
+    const integral_constant<int, 2> two;
+    const integral_constant<int, 4> four;
+    const std::true_type split;
+    const std::false_type whole;
+    // fewer than 1024 tiles of 16 rows: the waves share a tile
+    const bool large = static_cast<int64_t>(active) * tiles >= 1024;
+    const auto blocks = [&](auto r, auto nt, auto waves) {
+        constexpr int R = decltype(r)::value, NT = decltype(nt)::value, WAVES = decltype(waves)::value;
+        experts_blocks<GATE, F32, PARTS, R, NT, WAVES><<<dim3((tiles + R * WAVES - 1) / (R * WAVES), p.experts), WAVES * kWave, pairs * 2, at>>>(p, plan);
+    };
+    const integral_constant<int, 8> eight;
+    const integral_constant<int, 6> six;
+    if (!large) launch(one, one, split);
+    else if (p.tokens <= 16) launch(four, one, whole);
+    else {
+        // rows that the CU with most of them has
+        const auto most = [&](int rows) { return (static_cast<int64_t>(p.experts) * ((tiles + rows - 1) / rows) + 255) / 256 * rows; };
+        if (most(6) < most(16) && most(6) < most(8)) blocks(one, four, six);
+        else if (most(8) < most(16)) blocks(one, four, eight);
+        else blocks(two, four, eight);
+    }
+}
+
 } // namespace
 } // namespace dlk
+
+extern "C" int64_t dlk_experts_rows(const dlk_experts_params* p) {
+    // pairs that an expert's list holds, and planes of x and of the hidden entries below 2 GiB
+    const int64_t most = std::max<int64_t>(p->dim, p->top * static_cast<int64_t>(p->hidden)) * 12;
+    return std::max<int64_t>(1, std::min<int64_t>(dlk::kPairs / p->top, INT32_MAX / most));
+}
+
+extern "C" int64_t dlk_experts_workspace(const dlk_experts_params* p) { return dlk::layout(*p).bytes; }
 
 extern "C" int dlk_experts(const dlk_experts_params* p, dlh_stream stream) {
     using namespace dlk;
     if (p->experts <= 0 || p->experts > DLK_EXPERTS_MOST || p->top <= 0 || p->top > p->experts || p->top > DLK_EXPERTS_TOP_MOST ||
-        p->dim <= 0 || p->hidden <= 0 || p->tokens <= 0 || p->tokens > DLK_MOST_GROUPS)
+        p->dim <= 0 || p->hidden <= 0 || p->tokens <= 0 || p->tokens > dlk_experts_rows(p) || !p->workspace)
         return hipErrorInvalidValue;
     hipStream_t at = reinterpret_cast<hipStream_t>(stream);
-    const auto groups = [](int64_t waves) { return static_cast<unsigned>(waves / 4 + 1 < 16384 ? waves / 4 + 1 : 16384); };
-    experts_route<<<static_cast<unsigned>(p->tokens), kThreads, 0, at>>>(*p);
-    experts_hidden_any<<<groups(p->tokens * p->top * p->hidden), kThreads, 0, at>>>(*p);
-    experts_down_any<<<groups(p->tokens * p->dim), kThreads, 0, at>>>(*p);
+    const Layout l = layout(*p);
+    char* space = static_cast<char*>(p->workspace);
+    const Plan plan{reinterpret_cast<uint16_t*>(space), l.act > l.rows ? space + l.rows : nullptr, space + l.act,
+                    reinterpret_cast<float*>(space + l.partial), l.planes};
+    const auto tokens = static_cast<unsigned>(p->tokens);
+    if (wide(*p)) experts_route<true><<<tokens, kRoute, 0, at>>>(*p, plan);
+    else experts_route<false><<<tokens, kRoute, 0, at>>>(*p, plan);
+    if (!l.fast) {
+        const auto groups = [](int64_t waves) { return static_cast<unsigned>(std::min<int64_t>(waves / 4 + 1, 16384)); };
+        float* act = reinterpret_cast<float*>(plan.act);
+        experts_hidden_any<<<groups(p->tokens * p->top * p->hidden), 256, 0, at>>>(*p, act);
+        experts_down_any<<<groups(p->tokens * p->dim), 256, 0, at>>>(*p, act);
+        return hipGetLastError();
+    }
+    if (!p->weights_bf16) {
+        rows_of<true, true, 1>(*p, plan, at);
+        rows_of<false, true, 1>(*p, plan, at);
+    } else {
+        if (p->x_bf16) rows_of<true, false, 1>(*p, plan, at);
+        else rows_of<true, false, 3>(*p, plan, at);
+        rows_of<false, false, 3>(*p, plan, at);
+    }
+    const int64_t units = p->tokens * (p->dim / 4);
+    experts_join<<<static_cast<unsigned>((units + 255) / 256), 256, 0, at>>>(*p, plan.partial);
     return hipGetLastError();
 }

@@ -391,8 +391,11 @@ typedef struct dlk_experts_params {
     float* y;                /* [tokens, dim] */
     int64_t* chosen;         /* [tokens, top] */
     float* weights;          /* [tokens, top] */
-    float* act;              /* [tokens, top, hidden]: workspace */
+    void* workspace;         /* dlk_experts_workspace bytes, 16-byte aligned */
 } dlk_experts_params;
+/* The most rows of a launch, and the bytes of workspace that it takes. */
+int64_t dlk_experts_rows(const dlk_experts_params* p);
+int64_t dlk_experts_workspace(const dlk_experts_params* p);
 int dlk_experts(const dlk_experts_params* p, dlh_stream stream);
 
 /* First maximum of each row (NaN first); x [rows, n] f32 contiguous -> out i64 [rows]. */

@@ -37,23 +37,29 @@ Mixture expert_mixture(const Tensor& input, const Tensor& router, const Tensor& 
     Shape few = input.shape();
     few.back() = top;
     p.tokens = x.numel() / dim;
-    if (p.tokens > INT32_MAX / (16 * top)) refuse("too many rows");
     Mixture out{empty_tensor(input.shape(), DType::f32, input.device()), empty_tensor(few, DType::i64, input.device()),
                 empty_tensor(few, DType::f32, input.device())};
     if (p.tokens == 0) return out;
-    const Tensor act = empty_tensor({p.tokens, top, hidden}, DType::f32, input.device()); // released to the pool in stream order
-    p.x = x.data<void>();
     p.x_bf16 = x.dtype() == DType::bf16;
     p.dim = static_cast<int>(dim);
     p.hidden = static_cast<int>(hidden);
     p.experts = static_cast<int>(experts);
     p.top = static_cast<int>(top);
     p.normalise = normalise;
-    p.y = static_cast<float*>(mutable_data(out.output));
-    p.chosen = static_cast<Index*>(mutable_data(out.chosen));
-    p.weights = static_cast<float*>(mutable_data(out.weights));
-    p.act = static_cast<float*>(mutable_data(act));
-    hip_check(dlk_experts(&p, context.stream), name);
+    // (many rows in parts, over one workspace, released to the pool in stream order)
+    const Index rows = p.tokens, most = std::min<Index>(rows, dlk_experts_rows(&p));
+    p.tokens = most;
+    p.x = x.data<void>();
+    const Tensor workspace = empty_tensor({dlk_experts_workspace(&p) / 4 + 1}, DType::f32, input.device());
+    p.workspace = mutable_data(workspace);
+    for (Index first = 0; first < rows; first += most) {
+        p.tokens = std::min(most, rows - first);
+        p.x = x.data<char>() + first * dim * static_cast<Index>(element_size(x.dtype()));
+        p.y = static_cast<float*>(mutable_data(out.output)) + first * dim;
+        p.chosen = static_cast<Index*>(mutable_data(out.chosen)) + first * top;
+        p.weights = static_cast<float*>(mutable_data(out.weights)) + first * top;
+        hip_check(dlk_experts(&p, context.stream), name);
+    }
     return out;
 }
 
