@@ -1,0 +1,437 @@
+// The gated delta rule over prompts, 64 tokens (a chunk) at a time (see dlk_delta_params in kernels.h).
+//
+// Within a chunk, with G_i the sum of its decays up to token i, b the rates and S the state before it, the writes w_i obey
+//   w_i = b_i (v_i - e^G_i S^T k_i - sum_(j < i) e^(G_i - G_j) (k_i . k_j) w_j),
+// a triangular system whose matrix 1 + A, A_ij = b_i e^(G_i - G_j) (k_i . k_j), knows nothing of the states.  So a first launch takes
+// T = (1 + A)^-1 and P_ij = e^(G_i - G_j) (q_i . k_j), j <= i, of all chunks at once, and a second goes through each request's
+// chunks in order with what is left, for 16 columns of the state a work-group (columns know nothing of one another):
+//   R = b (V - e^G K S);   W = T R;   out = scale (e^G Q S + P W);   S = e^G_64 S + K^T (e^(G_64 - G) W)
+//
+// All exact to f32.  bf16 queries and keys go into the matrix cores as they are, what else is a factor there (S, R, W, T, P, f32
+// queries and keys) as three bf16 parts that hold all 24 bits; of a product of two such, the three smallest of nine part
+// products are left out, below 2^-24 of it.  Sums of decays are of 64 bits, since differences of long sums are taken.  (The
+// f32 instruction would take 2.7 times as long as six bf16 ones.)
+#include "kernels/parts.h"
+
+#include <algorithm>
+
+namespace dlk {
+namespace {
+
+constexpr int kThreads = 256, kWaves = 4, kTile = 256, kTiles = 10; // 16 x 16 tiles on and below the diagonal of 64 x 64
+__device__ __forceinline__ int tile_of(int i, int j) { return i * (i + 1) / 2 + j; }
+
+// the compiler keeps LDS accesses of a wave in order across this (the hardware does by itself)
+__device__ __forceinline__ void wave_order() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local"); }
+
+// The entries of a row as PARTS bf16 parts (one: they are bf16).
+template <int PARTS> __device__ __forceinline__ void eight_of(const dlk_row_segment& s, int64_t at, u32x4 (&to)[PARTS]) {
+    if constexpr (PARTS == 1) {
+        to[0] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(s.x) + at);
+    } else {
+        float v[8];
+        if (s.bf16) {
+            const u32x4 w = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(s.x) + at);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[2 * i] = bf16_lo(w[i]), v[2 * i + 1] = bf16_hi(w[i]);
+        } else {
+            const f32x4* from = reinterpret_cast<const f32x4*>(static_cast<const float*>(s.x) + at);
+            const f32x4 a = from[0], b = from[1];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
+        }
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part) to[part] = cut(v);
+    }
+}
+
+// sum + a b, the smallest part products first
+template <int A, int B> __device__ __forceinline__ f32x4 multiply(const u32x4 (&a)[A], const u32x4 (&b)[B], f32x4 sum) {
+    constexpr int LAST = (A > B ? A : B) - 1;
+#pragma unroll
+    for (int order = LAST; order >= 0; --order)
+#pragma unroll
+        for (int i = 0; i < A; ++i)
+            if (order - i >= 0 && order - i < B) sum = product(a[i], b[order - i], sum);
+    return sum;
+}
+
+// ------------------------------------------------------------------------------------------------ the chunks by themselves
+// A work-group per chunk and key head; wave w has the chunk's tokens 16 w to 16 w + 15 as rows.
+template <int DK, int PARTS> __global__ __launch_bounds__(kThreads) void delta_prepare(const dlk_delta_params p) {
+    constexpr int STEPS = DK / 32, LINE = 64 + 8, WIDE = 64 + 4;
+    __shared__ uint16_t turned[DK][LINE];
+    __shared__ float system[64][WIDE], inverse[4][16][20];
+    __shared__ double reach[kWaves][64];
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, n = lane % 16, g = lane / 16;
+    const int key_heads = p.heads / p.group, key_head = blockIdx.x % key_heads;
+    const int64_t index = blockIdx.x / key_heads;
+    const dlk_delta_chunk chunk = p.chunks[index];
+    const int64_t place = index * key_heads + key_head;
+
+    u32x4 k[STEPS][PARTS], q[STEPS][PARTS];
+    {
+        const int row = 16 * wave + n;
+        const int64_t token = chunk.token + min(row, chunk.count - 1);
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            eight_of<PARTS>(p.k, token * p.k.row + key_head * p.k.head + 32 * s + 8 * g, k[s]);
+            eight_of<PARTS>(p.q, token * p.q.row + key_head * p.q.head + 32 * s + 8 * g, q[s]);
+            if (row >= chunk.count)
+#pragma unroll
+                for (int part = 0; part < PARTS; ++part) k[s][part] = 0, q[s][part] = 0;
+        }
+    }
+    // for the second launch: keys with the tokens side by side, and the parts of f32 ones
+    const int64_t plane = static_cast<int64_t>(p.chunk_count) * key_heads * 64 * DK;
+#pragma unroll
+    for (int part = 0; part < PARTS; ++part) {
+        if constexpr (PARTS > 1)
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) {
+                const int64_t at = part * plane + (place * 64 + 16 * wave + n) * DK + 32 * s + 8 * g;
+                *reinterpret_cast<u32x4*>(p.key_parts + at) = k[s][part];
+                *reinterpret_cast<u32x4*>(p.query_parts + at) = q[s][part];
+            }
+        if (part > 0) __syncthreads();
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                turned[32 * s + 8 * g + i][16 * wave + n] = static_cast<uint16_t>(i % 2 ? k[s][part][i / 2] >> 16 : k[s][part][i / 2]);
+        __syncthreads();
+        for (int i = threadIdx.x; i < DK * 8; i += kThreads)
+            *reinterpret_cast<u32x4*>(p.turned_keys + part * plane + (place * DK + i / 8) * 64 + i % 8 * 8) =
+                *reinterpret_cast<const u32x4*>(&turned[i / 8][i % 8 * 8]);
+    }
+    f32x4 kk[4], qk[4]; // row 16 wave + 4 g + r, column 16 j + n
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        kk[j] = 0.0f, qk[j] = 0.0f;
+        if (j > wave) continue;
+        const int row = 16 * j + n;
+        const int64_t token = chunk.token + min(row, chunk.count - 1);
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            u32x4 column[PARTS];
+            eight_of<PARTS>(p.k, token * p.k.row + key_head * p.k.head + 32 * s + 8 * g, column);
+            kk[j] = multiply(k[s], column, kk[j]);
+            qk[j] = multiply(q[s], column, qk[j]);
+        }
+    }
+    for (int h = 0; h < p.group; ++h) {
+        const int head = key_head * p.group + h;
+        const int64_t own = index * p.heads + head;
+        // lane i: token i
+        const int64_t gate = (chunk.token + min(lane, chunk.count - 1)) * p.heads + head;
+        const float decay = p.decay[gate], rate = lane < chunk.count ? p.rate[gate] : 0.0f;
+        // (e^-1000 is 0; sums with -inf would have no differences)
+        double sum = lane >= chunk.count ? 0.0 : decay < -1000.0f ? -1000.0 : static_cast<double>(decay);
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const double before = __shfl_up(sum, d);
+            if (lane >= d) sum += before;
+        }
+        reach[wave][lane] = sum;
+        wave_order();
+        if (wave == 0) {
+            float* to = p.gates + own * 192;
+            to[lane] = expf(static_cast<float>(sum));
+            to[64 + lane] = expf(static_cast<float>(reach[0][63] - sum));
+            to[128 + lane] = rate;
+        }
+        float* within = p.within + own * kTiles * kTile;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (j > wave) continue;
+            const double to = reach[wave][16 * j + n];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int i = 16 * wave + 4 * g + r, at = 16 * j + n;
+                const float fade = expf(static_cast<float>(reach[wave][i] - to)), factor = __shfl(rate, i) * fade;
+                system[i][at] = i > at ? factor * kk[j][r] : 0.0f;
+                within[tile_of(wave, j) * kTile + (4 * g + r) * 16 + n] = i >= at && at < chunk.count ? fade * qk[j][r] : 0.0f;
+            }
+        }
+        __syncthreads();
+        // The inverse of each diagonal tile by substitution, a column a lane (four times over),
+        float x[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            x[i] = i == n ? 1.0f : 0.0f;
+#pragma unroll
+            for (int j = 0; j < i; ++j) x[i] = fmaf(-system[16 * wave + i][16 * wave + j], x[j], x[i]);
+        }
+        f32x4 solved[4]; // [tile row]: rows 4 g + r, column n
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float own_row = g == 0 ? x[r] : g == 1 ? x[4 + r] : g == 2 ? x[8 + r] : x[12 + r];
+            solved[0][r] = own_row;
+            inverse[wave][4 * g + r][n] = own_row;
+        }
+        __syncthreads();
+        // and the tiles below it, in order: X_ij = -X_ii sum_(j <= k < i) A_ik X_kj; wave j has column j of tiles.
+        // (A result's lane layout is that of the next product's right factor, if its index runs over 4 g + r.)
+        float* solution = p.solution + own * kTiles * kTile;
+#pragma unroll
+        for (int step = 0; step < 4; ++step) {
+            const int i = wave + step;
+            if (i > 3) break;
+            if (step > 0) {
+                f32x4 below = 0.0f;
+#pragma unroll
+                for (int t = 0; t < step; ++t) {
+                    const f32x4 a = *reinterpret_cast<const f32x4*>(&system[16 * i + n][16 * (wave + t) + 4 * g]);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) below = product(a[r], solved[t][r], below);
+                }
+                const f32x4 a = *reinterpret_cast<const f32x4*>(&inverse[i][n][4 * g]);
+                solved[step] = 0.0f;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) solved[step] = product(a[r], -below[r], solved[step]);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) solution[tile_of(i, wave) * kTile + (4 * g + r) * 16 + n] = solved[step][r];
+        }
+        __syncthreads();
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ chunk after chunk
+// A work-group per request, head and 16 columns of the state.  Wave w has rows 16 w to 16 w + 15 of a chunk, and DK / 4 rows of
+// the state (of 32: waves 0 and 1, 16 each).
+template <int DK, int PARTS> __global__ __launch_bounds__(kThreads) void delta_scan(const dlk_delta_params p) {
+    constexpr int STEPS = DK / 32, OWN = DK > 64 ? DK / 64 : 1, LINE_S = DK + 8, LINE = 64 + 8;
+    __shared__ uint16_t state_parts[3][16][LINE_S], right[3][16][LINE], write[3][16][LINE], late[3][16][LINE];
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, n = lane % 16, g = lane / 16;
+    // (work-groups go to the 8 dies in turn; the slices of a head read the same chunks, from the cache of one of them)
+    const int slices = p.value_dim / 16, pairs = p.item_count * p.heads;
+    const int pair = static_cast<int>(blockIdx.x / (8 * slices) * 8 + blockIdx.x % 8);
+    if (pair >= pairs) return;
+    const int column = static_cast<int>(blockIdx.x / 8 % slices) * 16 + n, head = pair % p.heads, key_head = head / p.group, key_heads = p.heads / p.group;
+    const dlk_delta_item item = p.items[pair / p.heads];
+    const int chunks = (item.count + 63) / 64;
+    const bool holds = 16 * OWN * wave < DK;
+
+    f32x4 state[OWN]; // rows 16 (OWN wave + t) + 4 g + r
+    const auto row_of = [&](int t, int r) { return 16 * (OWN * wave + t) + 4 * g + r; };
+    const int64_t size = static_cast<int64_t>(DK) * p.value_dim;
+#pragma unroll
+    for (int t = 0; t < OWN; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            state[t][r] = holds && item.source >= 0
+                              ? p.states[(static_cast<int64_t>(item.source) * p.heads + head) * size + static_cast<int64_t>(row_of(t, r)) * p.value_dim + column]
+                              : 0.0f;
+    // four neighbouring rows of a column, in parts
+    const auto part4 = [&](f32x4 v, uint16_t* to, int line) {
+#pragma unroll
+        for (int part = 0; part < 3; ++part) {
+            uint32_t w[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                w[r] = __float_as_uint(v[r]);
+                v[r] -= __uint_as_float(w[r] & 0xffff0000u);
+            }
+            *reinterpret_cast<u32x2*>(to + part * 16 * line) =
+                u32x2{__builtin_amdgcn_perm(w[1], w[0], 0x07060302u), __builtin_amdgcn_perm(w[3], w[2], 0x07060302u)};
+        }
+    };
+    const auto keep_state = [&] {
+        if (holds)
+#pragma unroll
+            for (int t = 0; t < OWN; ++t) part4(state[t], &state_parts[0][n][row_of(t, 0)], LINE_S);
+    };
+    const auto column_parts = [&](const uint16_t* from, int line, u32x4 (&to)[3]) {
+#pragma unroll
+        for (int part = 0; part < 3; ++part) to[part] = *reinterpret_cast<const u32x4*>(from + part * 16 * line);
+    };
+
+    // what a chunk's products read, asked for as soon as the chunk before has used its own
+    u32x4 k[STEPS][PARTS], q[STEPS][PARTS], keys[OWN][2][PARTS];
+    f32x4 solution[2][2], within[2][2], since, left, rate, v;
+    float whole;
+    const int64_t plane = static_cast<int64_t>(p.chunk_count) * key_heads * 64 * DK;
+    const auto tokens_of = [&](int c) { return min(64, item.count - 64 * c); };
+    const auto load_rows = [&](int c) {
+        const int64_t place = static_cast<int64_t>(item.chunk + c) * key_heads + key_head;
+        const int row = min(16 * wave + n, tokens_of(c) - 1);
+        const int64_t token = item.token + 64 * c + row;
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+            for (int part = 0; part < PARTS; ++part) {
+                if constexpr (PARTS == 1) {
+                    k[s][part] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p.k.x) + token * p.k.row + key_head * p.k.head + 32 * s + 8 * g);
+                    q[s][part] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p.q.x) + token * p.q.row + key_head * p.q.head + 32 * s + 8 * g);
+                } else {
+                    const int64_t at = part * plane + (place * 64 + row) * DK + 32 * s + 8 * g;
+                    k[s][part] = *reinterpret_cast<const u32x4*>(p.key_parts + at);
+                    q[s][part] = *reinterpret_cast<const u32x4*>(p.query_parts + at);
+                }
+            }
+    };
+    const auto load_values = [&](int c) {
+        const float* gates = p.gates + (static_cast<int64_t>(item.chunk + c) * p.heads + head) * 192;
+        since = *reinterpret_cast<const f32x4*>(gates + 16 * wave + 4 * g);
+        left = *reinterpret_cast<const f32x4*>(gates + 64 + 16 * wave + 4 * g);
+        rate = *reinterpret_cast<const f32x4*>(gates + 128 + 16 * wave + 4 * g);
+        whole = gates[63];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int64_t token = item.token + 64 * c + min(16 * wave + 4 * g + r, tokens_of(c) - 1), at = token * p.v.row + head * p.v.head + column;
+            v[r] = p.v.bf16 ? bf16_to_f32(static_cast<const uint16_t*>(p.v.x)[at]) : static_cast<const float*>(p.v.x)[at];
+        }
+    };
+    const auto load_tiles = [&](const float* tiles, int c, f32x4 (&to)[2][2]) { // row 16 wave + n, columns 32 s + 8 g to + 7
+        const float* from = tiles + (static_cast<int64_t>(item.chunk + c) * p.heads + head) * kTiles * kTile;
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            const int tile = 2 * s + g / 2;
+            const f32x4* row = reinterpret_cast<const f32x4*>(from + tile_of(wave, min(tile, wave)) * kTile + n * 16 + g % 2 * 8);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) to[s][i] = row[i];
+            if (tile > wave) to[s][0] = 0.0f, to[s][1] = 0.0f;
+        }
+    };
+    const auto load_keys = [&](int c) {
+        const int64_t place = static_cast<int64_t>(item.chunk + c) * key_heads + key_head;
+        if (holds)
+#pragma unroll
+            for (int t = 0; t < OWN; ++t)
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                    for (int part = 0; part < PARTS; ++part)
+                        keys[t][s][part] = *reinterpret_cast<const u32x4*>(p.turned_keys + part * plane + (place * DK + 16 * (OWN * wave + t) + n) * 64 + 32 * s + 8 * g);
+    };
+    // rows of a triangle times columns in LDS
+    const auto triangle = [&](const f32x4 (&rows)[2][2], const uint16_t (&columns)[3][16][LINE], f32x4 sum) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            if (2 * s > wave) break;
+            float a[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) a[i] = rows[s][i / 4][i % 4];
+            u32x4 part[3], b[3];
+#pragma unroll
+            for (int i = 0; i < 3; ++i) part[i] = cut(a);
+            column_parts(&columns[0][n][32 * s + 8 * g], LINE, b);
+            sum = multiply(part, b, sum);
+        }
+        return sum;
+    };
+
+    load_rows(0);
+    load_values(0);
+    load_tiles(p.solution, 0, solution);
+    load_tiles(p.within, 0, within);
+    load_keys(0);
+    keep_state();
+    __syncthreads();
+    for (int c = 0; c < chunks; ++c) {
+        const int next = min(c + 1, chunks - 1), tokens = tokens_of(c);
+        f32x4 ks = 0.0f, qs = 0.0f;
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+            u32x4 b[3];
+            column_parts(&state_parts[0][n][32 * s + 8 * g], LINE_S, b);
+            ks = multiply(k[s], b, ks);
+            qs = multiply(q[s], b, qs);
+        }
+        load_rows(next);
+        f32x4 r;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = 16 * wave + 4 * g + i < tokens ? rate[i] * (v[i] - since[i] * ks[i]) : 0.0f;
+        part4(r, &right[0][n][16 * wave + 4 * g], LINE);
+        __syncthreads();
+        f32x4 w = triangle(solution, right, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+        load_tiles(p.solution, next, solution);
+        part4(w, &write[0][n][16 * wave + 4 * g], LINE);
+        part4(w * left, &late[0][n][16 * wave + 4 * g], LINE);
+        f32x4 out = qs * since;
+#pragma unroll
+        for (int t = 0; t < OWN; ++t) state[t] *= whole;
+        load_values(next);
+        __syncthreads();
+        if (holds)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                u32x4 b[3];
+                column_parts(&late[0][n][32 * s + 8 * g], LINE, b);
+#pragma unroll
+                for (int t = 0; t < OWN; ++t) state[t] = multiply(keys[t][s], b, state[t]);
+            }
+        load_keys(next);
+        keep_state();
+        out = triangle(within, write, out);
+        load_tiles(p.within, next, within);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = 16 * wave + 4 * g + i;
+            if (row < tokens) p.out[(static_cast<int64_t>(item.token + 64 * c + row) * p.heads + head) * p.value_dim + column] = p.scale * out[i];
+        }
+        __syncthreads();
+    }
+    if (holds)
+#pragma unroll
+        for (int t = 0; t < OWN; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                p.states[(static_cast<int64_t>(item.target) * p.heads + head) * size + static_cast<int64_t>(row_of(t, r)) * p.value_dim + column] = state[t][r];
+}
+
+template <int DK, int PARTS> void launch(const dlk_delta_params& p, hipStream_t at) {
+    const int slices = p.value_dim / 16;
+    delta_prepare<DK, PARTS><<<static_cast<unsigned>(p.chunk_count) * (p.heads / p.group), kThreads, 0, at>>>(p);
+    delta_scan<DK, PARTS><<<(static_cast<unsigned>(p.item_count) * p.heads + 7) / 8 * 8 * slices, kThreads, 0, at>>>(p);
+}
+
+int parts_of(const dlk_delta_params* p) { return p->q.bf16 && p->k.bf16 ? 1 : 3; }
+
+struct Layout {
+    int64_t solution, within, gates, turned, keys, queries, bytes;
+};
+Layout layout(const dlk_delta_params* p) {
+    Layout l{};
+    const int64_t heads = static_cast<int64_t>(p->chunk_count) * p->heads, parts = parts_of(p);
+    const int64_t rows = static_cast<int64_t>(p->chunk_count) * (p->heads / p->group) * 64 * p->key_dim * parts * 2;
+    l.within = heads * kTiles * kTile * 4;
+    l.gates = 2 * l.within;
+    l.turned = l.gates + heads * 192 * 4;
+    l.keys = l.turned + rows;
+    l.queries = l.keys + (parts > 1 ? rows : 0);
+    l.bytes = l.queries + (parts > 1 ? rows : 0);
+    return l;
+}
+
+} // namespace
+} // namespace dlk
+
+extern "C" int64_t dlk_delta_workspace(const dlk_delta_params* p) { return dlk::layout(p).bytes; }
+
+extern "C" int dlk_delta_chunks(const dlk_delta_params* given, void* workspace, dlh_stream stream) {
+    using namespace dlk;
+    dlk_delta_params p = *given;
+    if (p.item_count <= 0 || p.chunk_count <= 0) return 0;
+    const int64_t groups = std::max<int64_t>(static_cast<int64_t>(p.chunk_count) * (p.heads / p.group),
+                                             (static_cast<int64_t>(p.item_count) * p.heads + 7) / 8 * 8 * (p.value_dim / 16));
+    if (p.value_dim <= 0 || p.value_dim % 16 != 0 || p.group <= 0 || groups > DLK_MOST_GROUPS || !workspace) return hipErrorInvalidValue;
+    const Layout l = layout(&p);
+    char* at = static_cast<char*>(workspace);
+    p.solution = reinterpret_cast<float*>(at);
+    p.within = reinterpret_cast<float*>(at + l.within);
+    p.gates = reinterpret_cast<float*>(at + l.gates);
+    p.turned_keys = reinterpret_cast<uint16_t*>(at + l.turned);
+    p.key_parts = reinterpret_cast<uint16_t*>(at + l.keys);
+    p.query_parts = reinterpret_cast<uint16_t*>(at + l.queries);
+    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    const bool bf16 = parts_of(&p) == 1;
+    switch (p.key_dim) {
+    case 32: bf16 ? launch<32, 1>(p, s) : launch<32, 3>(p, s); break;
+    case 64: bf16 ? launch<64, 1>(p, s) : launch<64, 3>(p, s); break;
+    case 128: bf16 ? launch<128, 1>(p, s) : launch<128, 3>(p, s); break;
+    default: return hipErrorInvalidValue;
+    }
+    return hipGetLastError();
+}

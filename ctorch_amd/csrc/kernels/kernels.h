@@ -351,12 +351,17 @@ typedef struct dlk_page_copy_params { /* (an argument block of a launch: below 4
 int dlk_page_copy(const dlk_page_copy_params* p, dlh_stream stream);
 
 /* ------------------------------------------------------------------------------------------------------
- * The gated delta rule over a step's tokens (delta_step.hip).  Rows are 16-byte aligned, also between heads and tokens.
+ * The gated delta rule over a step's tokens, one after the other (delta_step.hip) or in chunks of 64 (delta_chunk.hip).  Rows
+ * are 16-byte aligned, also between heads and tokens.
  * ---------------------------------------------------------------------------------------------------- */
 typedef struct dlk_delta_item { /* a request's new tokens: `count` from `token` on */
     int32_t source, target;     /* slots of its state before (-1: zero) and after */
     int32_t token, count;
+    int32_t chunk, unused;      /* the first of its chunks */
 } dlk_delta_item;
+typedef struct dlk_delta_chunk { /* up to 64 tokens of a request */
+    int32_t token, count;
+} dlk_delta_chunk;
 
 typedef struct dlk_delta_params {
     dlk_row_segment q, k, v; /* [tokens, heads / group, key_dim] and [tokens, heads, value_dim] */
@@ -367,8 +372,19 @@ typedef struct dlk_delta_params {
     int heads, group, key_dim, value_dim;
     float scale;
     const dlk_delta_item* items;
-    int item_count;
+    const dlk_delta_chunk* chunks;
+    int item_count, chunk_count;
+    /* set by dlk_delta_chunks: its workspace */
+    float* solution;         /* [chunks, heads, 10 tiles, 16, 16] */
+    float* within;
+    float* gates;            /* [chunks, heads, 3, 64] */
+    uint16_t* turned_keys;   /* [parts, chunks, key heads, key_dim, 64] */
+    uint16_t* key_parts;     /* [parts, chunks, key heads, 64, key_dim], f32 queries or keys only */
+    uint16_t* query_parts;
 } dlk_delta_params;
+/* Bytes of workspace for the chunks of these parameters. */
+int64_t dlk_delta_workspace(const dlk_delta_params* p);
+int dlk_delta_chunks(const dlk_delta_params* p, void* workspace, dlh_stream stream);
 int dlk_delta_step(const dlk_delta_params* p, dlh_stream stream);
 
 /* ------------------------------------------------------------------------------------------------------

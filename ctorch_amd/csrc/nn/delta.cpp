@@ -1,7 +1,9 @@
 // The states of the gated delta rule, the plan of a step over them, and its operator (include/dl/delta.h).
 #include "nn/delta_plan.h"
 
+#include <algorithm>
 #include <cmath>
+#include <cstring>
 #include <stdexcept>
 
 namespace dl::nn {
@@ -51,7 +53,13 @@ DeltaBatch::DeltaBatch(const DeltaStates& states, Index key_heads, std::span<con
         plan->tokens += counts[b];
     }
     if (plan->tokens > INT32_MAX / states.heads()) refuse("too many new tokens");
-    std::vector<dlk_delta_item> items;
+    // (the rule token by token takes about a microsecond a token; in chunks, three launches of some microseconds and one a chunk)
+    constexpr Index few = 16;
+    // (of chunks and heads: 21 KB of workspace each, and the keys' copies)
+    constexpr Index most = 8192;
+    const Index round_chunks = std::max<Index>(1, most / states.heads());
+    std::vector<dlk_delta_item> items, rest; // rest: requests of many tokens, then what is left of them
+    std::vector<dlk_delta_chunk> chunks;
     Index token = 0;
     for (Index b = 0; b < batch; ++b) {
         if (counts[b] == 0) continue;
@@ -59,13 +67,43 @@ DeltaBatch::DeltaBatch(const DeltaStates& states, Index key_heads, std::span<con
             const Index by = writer[static_cast<std::size_t>(sources[b])];
             if (by >= 0 && by != b) refuse("slot " + std::to_string(sources[b]) + " is written by one request and read by another");
         }
-        items.push_back({static_cast<int32_t>(sources[b]), static_cast<int32_t>(targets[b]), static_cast<int32_t>(token),
-                         static_cast<int32_t>(counts[b])});
+        (counts[b] <= few ? items : rest)
+            .push_back({static_cast<int32_t>(sources[b]), static_cast<int32_t>(targets[b]), static_cast<int32_t>(token),
+                        static_cast<int32_t>(counts[b]), 0, 0});
         token += counts[b];
     }
-    plan->items = static_cast<Index>(items.size());
-    if (plan->items > 0)
-        plan->blob = from_host(items.data(), {plan->items * 2}, DType::i64, false, states.device());
+    plan->few = static_cast<Index>(items.size());
+    while (!rest.empty()) {
+        // the requests side by side, each by as many chunks as leave some for all
+        const Index each = std::max<Index>(1, round_chunks / static_cast<Index>(rest.size()));
+        Plan::Round round{static_cast<Index>(items.size()), 0, static_cast<Index>(chunks.size()), 0};
+        std::vector<dlk_delta_item> left;
+        for (dlk_delta_item& item : rest) {
+            if (round.chunks >= round_chunks) {
+                left.push_back(item);
+                continue;
+            }
+            const Index n = std::min<Index>((item.count + 63) / 64, std::min(each, round_chunks - round.chunks));
+            dlk_delta_item now = item;
+            now.count = static_cast<int32_t>(std::min<Index>(item.count, 64 * n));
+            now.chunk = static_cast<int32_t>(round.chunks);
+            for (Index i = 0; i < n; ++i)
+                chunks.push_back({static_cast<int32_t>(item.token + 64 * i), static_cast<int32_t>(std::min<Index>(64, item.count - 64 * i))});
+            round.chunks += n;
+            round.items += 1;
+            items.push_back(now);
+            if (now.count < item.count) left.push_back({item.target, item.target, item.token + now.count, item.count - now.count, 0, 0});
+        }
+        plan->rounds.push_back(round);
+        rest = std::move(left);
+    }
+    plan->chunks = items.size() * sizeof(dlk_delta_item);
+    std::vector<char> bytes(plan->chunks + chunks.size() * sizeof(dlk_delta_chunk));
+    if (!items.empty()) {
+        std::memcpy(bytes.data(), items.data(), plan->chunks);
+        if (!chunks.empty()) std::memcpy(bytes.data() + plan->chunks, chunks.data(), bytes.size() - plan->chunks);
+        plan->blob = from_host(bytes.data(), {static_cast<Index>(bytes.size() / 8)}, DType::i64, false, states.device());
+    }
     plan_ = std::move(plan);
 }
 
@@ -145,9 +183,25 @@ Tensor gated_delta(const nn::DeltaStates& states, Index layer, const nn::DeltaBa
     p.key_dim = static_cast<int>(plan.key_dim);
     p.value_dim = static_cast<int>(plan.value_dim);
     p.scale = static_cast<float>(scale ? *scale : 1.0 / std::sqrt(static_cast<double>(plan.key_dim)));
-    p.items = reinterpret_cast<const dlk_delta_item*>(plan.blob.data<char>());
-    p.item_count = static_cast<int>(plan.items);
+    const auto* items = reinterpret_cast<const dlk_delta_item*>(plan.blob.data<char>());
+    const auto* chunks = reinterpret_cast<const dlk_delta_chunk*>(plan.blob.data<char>() + plan.chunks);
+    Tensor workspace; // of the largest round; released to the pool in stream order
+    Index most = 0;
+    for (const auto& round : plan.rounds) most = std::max(most, round.chunks);
+    if (most > 0) {
+        p.chunk_count = static_cast<int>(most);
+        workspace = empty_tensor({dlk_delta_workspace(&p) / 4}, DType::f32, states.device());
+    }
+    p.items = items;
+    p.item_count = static_cast<int>(plan.few);
     hip_check(dlk_delta_step(&p, context.stream), name);
+    for (const auto& round : plan.rounds) {
+        p.items = items + round.first;
+        p.item_count = static_cast<int>(round.items);
+        p.chunks = chunks + round.first_chunk;
+        p.chunk_count = static_cast<int>(round.chunks);
+        hip_check(dlk_delta_chunks(&p, mutable_data(workspace), context.stream), name);
+    }
     return out;
 }
 

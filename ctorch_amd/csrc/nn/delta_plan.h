@@ -13,8 +13,15 @@ struct DeltaBatch::Plan {
     Device device;
 
     Index tokens = 0;
-    Index items = 0; // requests with new tokens
-    Tensor blob;     // dlk_delta_item [items], on the device
+    // what a launch goes through: the requests with few new tokens, and, in rounds of so many chunks as a workspace holds, the
+    // others' (a request that goes on in the next round does so from its target)
+    struct Round {
+        Index first = 0, items = 0, first_chunk = 0, chunks = 0;
+    };
+    Index few = 0; // items of few tokens, the first ones
+    std::vector<Round> rounds;
+    Tensor blob; // dlk_delta_item [..], then dlk_delta_chunk [..], on the device
+    std::size_t chunks = 0; // where they begin
 };
 
 } // namespace dl::nn
