@@ -24,22 +24,16 @@ __device__ __forceinline__ int tile_of(int i, int j) { return i * (i + 1) / 2 + 
 // the compiler keeps LDS accesses of a wave in order across this (the hardware does by itself)
 __device__ __forceinline__ void wave_order() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local"); }
 
-// The entries of a row as PARTS bf16 parts (one: they are bf16).
+// The entries of a row as PARTS bf16 parts (one: they are bf16; three: f32).
 template <int PARTS> __device__ __forceinline__ void eight_of(const dlk_row_segment& s, int64_t at, u32x4 (&to)[PARTS]) {
     if constexpr (PARTS == 1) {
         to[0] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(s.x) + at);
     } else {
         float v[8];
-        if (s.bf16) {
-            const u32x4 w = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(s.x) + at);
+        const f32x4* from = reinterpret_cast<const f32x4*>(static_cast<const float*>(s.x) + at);
+        const f32x4 a = from[0], b = from[1];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[2 * i] = bf16_lo(w[i]), v[2 * i + 1] = bf16_hi(w[i]);
-        } else {
-            const f32x4* from = reinterpret_cast<const f32x4*>(static_cast<const float*>(s.x) + at);
-            const f32x4 a = from[0], b = from[1];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
-        }
+        for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
 #pragma unroll
         for (int part = 0; part < PARTS; ++part) to[part] = cut(v);
     }
@@ -66,7 +60,8 @@ template <int DK, int PARTS> __global__ __launch_bounds__(kThreads) void delta_p
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, n = lane % 16, g = lane / 16;
     const int key_heads = p.heads / p.group, key_head = blockIdx.x % key_heads;
     const int64_t index = blockIdx.x / key_heads;
-    const dlk_delta_chunk chunk = p.chunks[index];
+    dlk_delta_chunk chunk = p.chunks[index];
+    chunk.token = __builtin_amdgcn_readfirstlane(chunk.token), chunk.count = __builtin_amdgcn_readfirstlane(chunk.count);
     const int64_t place = index * key_heads + key_head;
 
     u32x4 k[STEPS][PARTS], q[STEPS][PARTS];
@@ -172,7 +167,9 @@ template <int DK, int PARTS> __global__ __launch_bounds__(kThreads) void delta_p
         __syncthreads();
         // and the tiles below it, in order: X_ij = -X_ii sum_(j <= k < i) A_ik X_kj; wave j has column j of tiles.
         // (A result's lane layout is that of the next product's right factor, if its index runs over 4 g + r.)
-        float* solution = p.solution + own * kTiles * kTile;
+        uint16_t* solution = p.solution + own * 3 * (kTiles + 1) * kTile;
+        if (threadIdx.x < 96) // a tile of zeros in each part
+            *reinterpret_cast<u32x4*>(solution + (threadIdx.x / 32 * (kTiles + 1) + kTiles) * kTile + threadIdx.x % 32 * 8) = 0;
 #pragma unroll
         for (int step = 0; step < 4; ++step) {
             const int i = wave + step;
@@ -191,38 +188,178 @@ template <int DK, int PARTS> __global__ __launch_bounds__(kThreads) void delta_p
                 for (int r = 0; r < 4; ++r) solved[step] = product(a[r], -below[r], solved[step]);
             }
 #pragma unroll
-            for (int r = 0; r < 4; ++r) solution[tile_of(i, wave) * kTile + (4 * g + r) * 16 + n] = solved[step][r];
+            for (int r = 0; r < 4; ++r) {
+                float x = solved[step][r];
+#pragma unroll
+                for (int part = 0; part < 3; ++part) solution[(part * (kTiles + 1) + tile_of(i, wave)) * kTile + (4 * g + r) * 16 + n] = cut(x);
+            }
         }
         __syncthreads();
     }
 }
 
 // ------------------------------------------------------------------------------------------------ chunk after chunk
-// A work-group per request, head and 16 columns of the state.  Wave w has rows 16 w to 16 w + 15 of a chunk, and DK / 4 rows of
-// the state (of 32: waves 0 and 1, 16 each).
-template <int DK, int PARTS> __global__ __launch_bounds__(kThreads) void delta_scan(const dlk_delta_params p) {
+// A work-group per request, head and 16 columns of the state.  What counts is how long a chunk takes, not how much there is to
+// do (a prompt's chunks follow one another: 128 x 3 barriers), so the waves share it by what waits for what: waves 0 to 3 hold
+// the state (DK / 4 rows each; of 32: waves 0 and 1, 16 each) and take it to the next chunk by way of R and W, 16 tokens each,
+// and waves 4 to 7 make the outputs of 16 tokens each beside them.  What the next chunk's products read is asked for as soon
+// as this one's have used theirs (and not before: its registers are the same).
+template <int DK, int PARTS, bool V_BF16>
+__global__ __launch_bounds__(2 * kThreads) __attribute__((amdgpu_waves_per_eu(2, PARTS == 1 && DK < 128 ? 4 : 2))) void delta_scan(const dlk_delta_params p) {
     constexpr int STEPS = DK / 32, OWN = DK > 64 ? DK / 64 : 1, LINE_S = DK + 8, LINE = 64 + 8;
     __shared__ uint16_t state_parts[3][16][LINE_S], right[3][16][LINE], write[3][16][LINE], late[3][16][LINE];
-    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, n = lane % 16, g = lane / 16;
+    const int lane = threadIdx.x % kWave, n = lane % 16, g = lane / 16;
+    const int role = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), wave = role % kWaves;
     // (work-groups go to the 8 dies in turn; the slices of a head read the same chunks, from the cache of one of them)
     const int slices = p.value_dim / 16, pairs = p.item_count * p.heads;
     const int pair = static_cast<int>(blockIdx.x / (8 * slices) * 8 + blockIdx.x % 8);
     if (pair >= pairs) return;
-    const int column = static_cast<int>(blockIdx.x / 8 % slices) * 16 + n, head = pair % p.heads, key_head = head / p.group, key_heads = p.heads / p.group;
-    const dlk_delta_item item = p.items[pair / p.heads];
+    const auto shared = [](int x) { return __builtin_amdgcn_readfirstlane(x); }; // (by the whole wave, which the compiler cannot know)
+    const int first_column = shared(blockIdx.x / 8 % slices) * 16, head = shared(pair % p.heads), key_head = shared(head / p.group);
+    const int key_heads = shared(p.heads / p.group);
+    dlk_delta_item item = p.items[shared(pair / p.heads)];
+    item = {shared(item.source), shared(item.target), shared(item.token), shared(item.count), shared(item.chunk), 0};
     const int chunks = (item.count + 63) / 64;
-    const bool holds = 16 * OWN * wave < DK;
+    const auto tokens_of = [&](int c) { return min(64, item.count - 64 * c); };
+    const int64_t plane = static_cast<int64_t>(p.chunk_count) * key_heads * 64 * DK;
+    // the places of chunk c: of its key head, and of its head
+    const auto key_place = [&](int c) { return static_cast<int64_t>(item.chunk + c) * key_heads + key_head; };
+    const auto place = [&](int c) { return static_cast<int64_t>(item.chunk + c) * p.heads + head; };
+    const auto column_parts = [&](const uint16_t* from, int line, u32x4 (&to)[3]) {
+#pragma unroll
+        for (int part = 0; part < 3; ++part) to[part] = *reinterpret_cast<const u32x4*>(from + part * 16 * line);
+    };
+    // Offsets of a lane are the same for all chunks but the last, which may end early: reads behind it take its last row.
+    // (32 bits behind an address that the whole wave shares; a 64-bit product a lane takes as long as a dozen other instructions.)
+    const int last_row = tokens_of(chunks - 1) - 1;
+    const auto at_row = [&](int row, int64_t stride, int c) {
+        return static_cast<uint32_t>(c + 1 < chunks ? row : min(row, last_row)) * static_cast<uint32_t>(stride);
+    };
+    // rows 16 wave + n of the chunk's keys or queries, entries 32 s + 8 g to + 7
+    const auto load_rows = [&](const dlk_row_segment& rows, const uint16_t* parts, int c, u32x4 (&to)[STEPS][PARTS]) {
+        if constexpr (PARTS == 1) {
+            const uint16_t* from = static_cast<const uint16_t*>(rows.x) + (item.token + 64 * static_cast<int64_t>(c)) * rows.row + key_head * rows.head;
+            const uint32_t at = at_row(16 * wave + n, rows.row, c) + 8 * g;
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) to[s][0] = *reinterpret_cast<const u32x4*>(from + at + 32 * s);
+        } else {
+#pragma unroll
+            for (int part = 0; part < PARTS; ++part) {
+                const uint16_t* from = parts + part * plane + key_place(c) * 64 * DK;
+                const uint32_t at = static_cast<uint32_t>((16 * wave + n) * DK + 8 * g);
+#pragma unroll
+                for (int s = 0; s < STEPS; ++s) to[s][part] = *reinterpret_cast<const u32x4*>(from + at + 32 * s);
+            }
+        }
+    };
+    // Those rows times the state's columns, all read from LDS before the first product; two sums, since products that follow
+    // one another wait for each other.
+    const auto times_state = [&](const u32x4 (&rows)[STEPS][PARTS]) {
+        u32x4 b[STEPS][3];
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) column_parts(&state_parts[0][n][32 * s + 8 * g], LINE_S, b[s]);
+        __builtin_amdgcn_sched_barrier(0);
+        f32x4 sum[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int s = 0; s < STEPS; s += 2)
+#pragma unroll
+            for (int order = 2; order >= 0; --order)
+#pragma unroll
+                for (int i = 0; i < PARTS && i <= order; ++i)
+#pragma unroll
+                    for (int t = 0; t < 2 && s + t < STEPS; ++t) sum[t] = product(rows[s + t][i], b[s + t][order - i], sum[t]);
+        return sum[0] + sum[1];
+    };
+    // rows of a triangle, parts [2 steps of 32 columns], times columns in LDS
+    const auto triangle = [&](const u32x4 (&rows)[2][3], const uint16_t (&columns)[3][16][LINE], f32x4 sum) {
+        f32x4 small = 0.0f;
+        u32x4 b[2][3];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) column_parts(&columns[0][n][32 * s + 8 * g], LINE, b[s]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            if (2 * s > wave) break;
+            small = product(rows[s][2], b[s][0], small);
+            sum = product(rows[s][1], b[s][0], sum);
+            small = product(rows[s][1], b[s][1], small);
+            sum = product(rows[s][0], b[s][1], sum);
+            small = product(rows[s][0], b[s][2], small);
+            sum = product(rows[s][0], b[s][0], sum);
+        }
+        return sum + small;
+    };
 
+    if (role >= kWaves) {
+        // Two chunks ahead: a load is waited for together with all stores before it, and a store takes longer than a chunk.
+        // (One ahead: 2.4 us a chunk.)
+        u32x4 q[2][STEPS][PARTS];
+        f32x4 within[2][2][2], since[2]; // rows 16 wave + n, columns 32 s + 8 g to + 7 (behind the triangle: anything)
+        const int out_row = p.heads * p.value_dim;
+        const auto load_queries = [&](int c, int slot) {
+            load_rows(p.q, p.query_parts, c, q[slot]);
+            since[slot] = *reinterpret_cast<const f32x4*>(p.gates + place(c) * 192 + static_cast<uint32_t>(16 * wave + 4 * g));
+        };
+        const auto load_within = [&](int c, int slot) {
+            const float* from = p.within + place(c) * kTiles * kTile;
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    within[slot][s][i] = *reinterpret_cast<const f32x4*>(from + static_cast<uint32_t>(tile_of(wave, min(2 * s + g / 2, wave)) * kTile + n * 16 + g % 2 * 8 + 4 * i));
+        };
+        const auto chunk = [&](int c, auto which) {
+            constexpr int SLOT = decltype(which)::value;
+            const int next = min(c + 2, chunks - 1), tokens = tokens_of(c);
+            f32x4 out = times_state(q[SLOT]) * since[SLOT];
+            __builtin_amdgcn_sched_barrier(0);
+            load_queries(next, SLOT);
+            __syncthreads();
+            u32x4 rows[2][3];
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                float a[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) a[i] = 2 * s + g / 2 > wave ? 0.0f : within[SLOT][s][i / 4][i % 4];
+#pragma unroll
+                for (int part = 0; part < 3; ++part) rows[s][part] = cut(a);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            load_within(next, SLOT);
+            __syncthreads();
+            out = triangle(rows, write, out) * p.scale;
+            // Rows behind the chunk's end lie behind the buffer's.  (Of stores under a condition the compiler could not tell how
+            // many came before a load, and would wait for them all.)
+            float* to = p.out + ((item.token + 64 * static_cast<int64_t>(c)) * p.heads + head) * p.value_dim + first_column;
+            const __amdgpu_buffer_rsrc_t rows_out = __builtin_amdgcn_make_buffer_rsrc(to, 0, ((tokens - 1) * out_row + 16) * 4, kBufferFlags);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(out[i]), rows_out, ((16 * wave + 4 * g + i) * out_row + n) * 4, 0, 0);
+            __syncthreads();
+        };
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            load_queries(min(c, chunks - 1), c);
+            load_within(min(c, chunks - 1), c);
+        }
+        __syncthreads();
+        for (int c = 0; c < chunks; c += 2) {
+            chunk(c, std::integral_constant<int, 0>{});
+            if (c + 1 < chunks) chunk(c + 1, std::integral_constant<int, 1>{});
+        }
+        return;
+    }
+
+    const bool holds = 16 * OWN * kWaves <= DK || 16 * OWN * wave < DK;
     f32x4 state[OWN]; // rows 16 (OWN wave + t) + 4 g + r
     const auto row_of = [&](int t, int r) { return 16 * (OWN * wave + t) + 4 * g + r; };
-    const int64_t size = static_cast<int64_t>(DK) * p.value_dim;
+    const auto state_at = [&](int slot) {
+        return p.states + (static_cast<int64_t>(slot) * p.heads + head) * DK * p.value_dim + first_column;
+    };
 #pragma unroll
     for (int t = 0; t < OWN; ++t)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-            state[t][r] = holds && item.source >= 0
-                              ? p.states[(static_cast<int64_t>(item.source) * p.heads + head) * size + static_cast<int64_t>(row_of(t, r)) * p.value_dim + column]
-                              : 0.0f;
+        for (int r = 0; r < 4; ++r) state[t][r] = holds && item.source >= 0 ? state_at(item.source)[row_of(t, r) * p.value_dim + n] : 0.0f;
     // four neighbouring rows of a column, in parts
     const auto part4 = [&](f32x4 v, uint16_t* to, int line) {
 #pragma unroll
@@ -242,152 +379,110 @@ template <int DK, int PARTS> __global__ __launch_bounds__(kThreads) void delta_s
 #pragma unroll
             for (int t = 0; t < OWN; ++t) part4(state[t], &state_parts[0][n][row_of(t, 0)], LINE_S);
     };
-    const auto column_parts = [&](const uint16_t* from, int line, u32x4 (&to)[3]) {
-#pragma unroll
-        for (int part = 0; part < 3; ++part) to[part] = *reinterpret_cast<const u32x4*>(from + part * 16 * line);
-    };
-
-    // what a chunk's products read, asked for as soon as the chunk before has used its own
-    u32x4 k[STEPS][PARTS], q[STEPS][PARTS], keys[OWN][2][PARTS];
-    f32x4 solution[2][2], within[2][2], since, left, rate, v;
+    u32x4 k[STEPS][PARTS], keys[OWN][2][PARTS], solution[2][3];
+    f32x4 since, left, rate;
     float whole;
-    const int64_t plane = static_cast<int64_t>(p.chunk_count) * key_heads * 64 * DK;
-    const auto tokens_of = [&](int c) { return min(64, item.count - 64 * c); };
-    const auto load_rows = [&](int c) {
-        const int64_t place = static_cast<int64_t>(item.chunk + c) * key_heads + key_head;
-        const int row = min(16 * wave + n, tokens_of(c) - 1);
-        const int64_t token = item.token + 64 * c + row;
-#pragma unroll
-        for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-            for (int part = 0; part < PARTS; ++part) {
-                if constexpr (PARTS == 1) {
-                    k[s][part] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p.k.x) + token * p.k.row + key_head * p.k.head + 32 * s + 8 * g);
-                    q[s][part] = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p.q.x) + token * p.q.row + key_head * p.q.head + 32 * s + 8 * g);
-                } else {
-                    const int64_t at = part * plane + (place * 64 + row) * DK + 32 * s + 8 * g;
-                    k[s][part] = *reinterpret_cast<const u32x4*>(p.key_parts + at);
-                    q[s][part] = *reinterpret_cast<const u32x4*>(p.query_parts + at);
-                }
-            }
-    };
+    uint32_t v[4]; // as they lie in memory
     const auto load_values = [&](int c) {
-        const float* gates = p.gates + (static_cast<int64_t>(item.chunk + c) * p.heads + head) * 192;
-        since = *reinterpret_cast<const f32x4*>(gates + 16 * wave + 4 * g);
-        left = *reinterpret_cast<const f32x4*>(gates + 64 + 16 * wave + 4 * g);
-        rate = *reinterpret_cast<const f32x4*>(gates + 128 + 16 * wave + 4 * g);
+        const float* gates = p.gates + place(c) * 192;
+        const uint32_t row = 16 * wave + 4 * g;
+        since = *reinterpret_cast<const f32x4*>(gates + row);
+        left = *reinterpret_cast<const f32x4*>(gates + 64 + row);
+        rate = *reinterpret_cast<const f32x4*>(gates + 128 + row);
         whole = gates[63];
+        const int64_t from = (item.token + 64 * static_cast<int64_t>(c)) * p.v.row + head * p.v.head + first_column;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int64_t token = item.token + 64 * c + min(16 * wave + 4 * g + r, tokens_of(c) - 1), at = token * p.v.row + head * p.v.head + column;
-            v[r] = p.v.bf16 ? bf16_to_f32(static_cast<const uint16_t*>(p.v.x)[at]) : static_cast<const float*>(p.v.x)[at];
+            const uint32_t at = at_row(row + r, p.v.row, c) + n;
+            if constexpr (V_BF16) v[r] = (static_cast<const uint16_t*>(p.v.x) + from)[at];
+            else v[r] = (static_cast<const uint32_t*>(p.v.x) + from)[at];
         }
     };
-    const auto load_tiles = [&](const float* tiles, int c, f32x4 (&to)[2][2]) { // row 16 wave + n, columns 32 s + 8 g to + 7
-        const float* from = tiles + (static_cast<int64_t>(item.chunk + c) * p.heads + head) * kTiles * kTile;
+    const auto load_solution = [&](int c) { // row 16 wave + n, columns 32 s + 8 g to + 7: behind the triangle, of the tile of zeros
+        const uint16_t* from = p.solution + place(c) * 3 * (kTiles + 1) * kTile;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             const int tile = 2 * s + g / 2;
-            const f32x4* row = reinterpret_cast<const f32x4*>(from + tile_of(wave, min(tile, wave)) * kTile + n * 16 + g % 2 * 8);
+            const uint32_t at = (tile > wave ? kTiles : tile_of(wave, tile)) * kTile + n * 16 + g % 2 * 8;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) to[s][i] = row[i];
-            if (tile > wave) to[s][0] = 0.0f, to[s][1] = 0.0f;
+            for (int part = 0; part < 3; ++part) solution[s][part] = *reinterpret_cast<const u32x4*>(from + part * (kTiles + 1) * kTile + at);
         }
     };
     const auto load_keys = [&](int c) {
-        const int64_t place = static_cast<int64_t>(item.chunk + c) * key_heads + key_head;
         if (holds)
 #pragma unroll
-            for (int t = 0; t < OWN; ++t)
+            for (int part = 0; part < PARTS; ++part) {
+                const uint16_t* from = p.turned_keys + part * plane + key_place(c) * DK * 64;
+                const uint32_t at = static_cast<uint32_t>((16 * OWN * wave + n) * 64 + 8 * g);
 #pragma unroll
-                for (int s = 0; s < 2; ++s)
+                for (int t = 0; t < OWN; ++t)
 #pragma unroll
-                    for (int part = 0; part < PARTS; ++part)
-                        keys[t][s][part] = *reinterpret_cast<const u32x4*>(p.turned_keys + part * plane + (place * DK + 16 * (OWN * wave + t) + n) * 64 + 32 * s + 8 * g);
-    };
-    // rows of a triangle times columns in LDS
-    const auto triangle = [&](const f32x4 (&rows)[2][2], const uint16_t (&columns)[3][16][LINE], f32x4 sum) {
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            if (2 * s > wave) break;
-            float a[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) a[i] = rows[s][i / 4][i % 4];
-            u32x4 part[3], b[3];
-#pragma unroll
-            for (int i = 0; i < 3; ++i) part[i] = cut(a);
-            column_parts(&columns[0][n][32 * s + 8 * g], LINE, b);
-            sum = multiply(part, b, sum);
-        }
-        return sum;
+                    for (int s = 0; s < 2; ++s) keys[t][s][part] = *reinterpret_cast<const u32x4*>(from + at + 16 * t * 64 + 32 * s);
+            }
     };
 
-    load_rows(0);
+    load_rows(p.k, p.key_parts, 0, k);
     load_values(0);
-    load_tiles(p.solution, 0, solution);
-    load_tiles(p.within, 0, within);
+    load_solution(0);
     load_keys(0);
     keep_state();
     __syncthreads();
     for (int c = 0; c < chunks; ++c) {
         const int next = min(c + 1, chunks - 1), tokens = tokens_of(c);
-        f32x4 ks = 0.0f, qs = 0.0f;
-#pragma unroll
-        for (int s = 0; s < STEPS; ++s) {
-            u32x4 b[3];
-            column_parts(&state_parts[0][n][32 * s + 8 * g], LINE_S, b);
-            ks = multiply(k[s], b, ks);
-            qs = multiply(q[s], b, qs);
-        }
-        load_rows(next);
+        const f32x4 ks = times_state(k);
+        __builtin_amdgcn_sched_barrier(0);
+        load_rows(p.k, p.key_parts, next, k);
         f32x4 r;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) r[i] = 16 * wave + 4 * g + i < tokens ? rate[i] * (v[i] - since[i] * ks[i]) : 0.0f;
+        for (int i = 0; i < 4; ++i)
+            r[i] = 16 * wave + 4 * g + i < tokens ? rate[i] * (__uint_as_float(V_BF16 ? v[i] << 16 : v[i]) - since[i] * ks[i]) : 0.0f;
         part4(r, &right[0][n][16 * wave + 4 * g], LINE);
         __syncthreads();
-        f32x4 w = triangle(solution, right, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
-        load_tiles(p.solution, next, solution);
-        part4(w, &write[0][n][16 * wave + 4 * g], LINE);
+        const f32x4 w = triangle(solution, right, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+        __builtin_amdgcn_sched_barrier(0);
+        load_solution(next);
         part4(w * left, &late[0][n][16 * wave + 4 * g], LINE);
-        f32x4 out = qs * since;
+        part4(w, &write[0][n][16 * wave + 4 * g], LINE);
 #pragma unroll
         for (int t = 0; t < OWN; ++t) state[t] *= whole;
+        __builtin_amdgcn_sched_barrier(0);
         load_values(next);
         __syncthreads();
-        if (holds)
+        if (holds) {
+            u32x4 b[2][3];
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                u32x4 b[3];
-                column_parts(&late[0][n][32 * s + 8 * g], LINE, b);
+            for (int s = 0; s < 2; ++s) column_parts(&late[0][n][32 * s + 8 * g], LINE, b[s]);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int t = 0; t < OWN; ++t) state[t] = multiply(keys[t][s], b, state[t]);
-            }
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int order = 2; order >= 0; --order)
+#pragma unroll
+                    for (int i = 0; i < PARTS && i <= order; ++i)
+#pragma unroll
+                        for (int t = 0; t < OWN; ++t) state[t] = product(keys[t][s][i], b[s][order - i], state[t]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
         load_keys(next);
         keep_state();
-        out = triangle(within, write, out);
-        load_tiles(p.within, next, within);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int row = 16 * wave + 4 * g + i;
-            if (row < tokens) p.out[(static_cast<int64_t>(item.token + 64 * c + row) * p.heads + head) * p.value_dim + column] = p.scale * out[i];
-        }
         __syncthreads();
     }
     if (holds)
 #pragma unroll
         for (int t = 0; t < OWN; ++t)
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                p.states[(static_cast<int64_t>(item.target) * p.heads + head) * size + static_cast<int64_t>(row_of(t, r)) * p.value_dim + column] = state[t][r];
+            for (int r = 0; r < 4; ++r) state_at(item.target)[row_of(t, r) * p.value_dim + n] = state[t][r];
 }
 
 template <int DK, int PARTS> void launch(const dlk_delta_params& p, hipStream_t at) {
     const int slices = p.value_dim / 16;
     delta_prepare<DK, PARTS><<<static_cast<unsigned>(p.chunk_count) * (p.heads / p.group), kThreads, 0, at>>>(p);
-    delta_scan<DK, PARTS><<<(static_cast<unsigned>(p.item_count) * p.heads + 7) / 8 * 8 * slices, kThreads, 0, at>>>(p);
+    const unsigned groups = (static_cast<unsigned>(p.item_count) * p.heads + 7) / 8 * 8 * slices;
+    if (p.v.bf16) delta_scan<DK, PARTS, true><<<groups, 2 * kThreads, 0, at>>>(p);
+    else delta_scan<DK, PARTS, false><<<groups, 2 * kThreads, 0, at>>>(p);
 }
 
-int parts_of(const dlk_delta_params* p) { return p->q.bf16 && p->k.bf16 ? 1 : 3; }
+int parts_of(const dlk_delta_params* p) { return p->k.bf16 ? 1 : 3; }
 
 struct Layout {
     int64_t solution, within, gates, turned, keys, queries, bytes;
@@ -396,8 +491,8 @@ Layout layout(const dlk_delta_params* p) {
     Layout l{};
     const int64_t heads = static_cast<int64_t>(p->chunk_count) * p->heads, parts = parts_of(p);
     const int64_t rows = static_cast<int64_t>(p->chunk_count) * (p->heads / p->group) * 64 * p->key_dim * parts * 2;
-    l.within = heads * kTiles * kTile * 4;
-    l.gates = 2 * l.within;
+    l.within = heads * 3 * (kTiles + 1) * kTile * 2;
+    l.gates = l.within + heads * kTiles * kTile * 4;
     l.turned = l.gates + heads * 192 * 4;
     l.keys = l.turned + rows;
     l.queries = l.keys + (parts > 1 ? rows : 0);
@@ -416,10 +511,10 @@ extern "C" int dlk_delta_chunks(const dlk_delta_params* given, void* workspace, 
     if (p.item_count <= 0 || p.chunk_count <= 0) return 0;
     const int64_t groups = std::max<int64_t>(static_cast<int64_t>(p.chunk_count) * (p.heads / p.group),
                                              (static_cast<int64_t>(p.item_count) * p.heads + 7) / 8 * 8 * (p.value_dim / 16));
-    if (p.value_dim <= 0 || p.value_dim % 16 != 0 || p.group <= 0 || groups > DLK_MOST_GROUPS || !workspace) return hipErrorInvalidValue;
+    if (p.value_dim <= 0 || p.value_dim % 16 != 0 || p.group <= 0 || groups > DLK_MOST_GROUPS || !workspace || p.q.bf16 != p.k.bf16) return hipErrorInvalidValue;
     const Layout l = layout(&p);
     char* at = static_cast<char*>(workspace);
-    p.solution = reinterpret_cast<float*>(at);
+    p.solution = reinterpret_cast<uint16_t*>(at);
     p.within = reinterpret_cast<float*>(at + l.within);
     p.gates = reinterpret_cast<float*>(at + l.gates);
     p.turned_keys = reinterpret_cast<uint16_t*>(at + l.turned);

@@ -375,14 +375,14 @@ typedef struct dlk_delta_params {
     const dlk_delta_chunk* chunks;
     int item_count, chunk_count;
     /* set by dlk_delta_chunks: its workspace */
-    float* solution;         /* [chunks, heads, 10 tiles, 16, 16] */
-    float* within;
+    uint16_t* solution;      /* [chunks, heads, 3 parts, 10 tiles and one of zeros, 16, 16] */
+    float* within;           /* [chunks, heads, 10 tiles, 16, 16] */
     float* gates;            /* [chunks, heads, 3, 64] */
     uint16_t* turned_keys;   /* [parts, chunks, key heads, key_dim, 64] */
     uint16_t* key_parts;     /* [parts, chunks, key heads, 64, key_dim], f32 queries or keys only */
     uint16_t* query_parts;
 } dlk_delta_params;
-/* Bytes of workspace for the chunks of these parameters. */
+/* Bytes of workspace for the chunks of these parameters (queries and keys of one type). */
 int64_t dlk_delta_workspace(const dlk_delta_params* p);
 int dlk_delta_chunks(const dlk_delta_params* p, void* workspace, dlh_stream stream);
 int dlk_delta_step(const dlk_delta_params* p, dlh_stream stream);

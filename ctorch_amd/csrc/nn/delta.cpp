@@ -18,7 +18,7 @@ DeltaStates::DeltaStates(Index layers, Index slots, Index heads, Index key_dim, 
         throw std::invalid_argument("delta states: key_dim must be 32, 64 or 128");
     if (value_dim <= 0 || value_dim % 32 != 0 || value_dim > 256)
         throw std::invalid_argument("delta states: value_dim must be a multiple of 32 up to 256");
-    if (slots > INT32_MAX || heads > INT32_MAX / (key_dim * value_dim))
+    if (slots > INT32_MAX || heads > 16384)
         throw std::invalid_argument("delta states: too many slots or heads");
     require_gpu(device, "delta states");
     for (Index layer = 0; layer < layers; ++layer)
@@ -167,8 +167,11 @@ Tensor gated_delta(const nn::DeltaStates& states, Index layer, const nn::DeltaBa
     const Tensor& state = states.state(layer);
     Tensor q, k, v;
     dlk_delta_params p{};
-    p.q = aligned_rows(query, q, plan.tokens, plan.key_heads, plan.key_dim, state, "query");
-    p.k = aligned_rows(key, k, plan.tokens, plan.key_heads, plan.key_dim, state, "key");
+    // (the launches over chunks take queries and keys of one type)
+    const bool mixed = !plan.rounds.empty() && query.dtype() != key.dtype() && is_floating(query.dtype()) && is_floating(key.dtype());
+    const auto alike = [&](const Tensor& t) { return mixed && t.dtype() == DType::bf16 ? t.astype(DType::f32) : t; };
+    p.q = aligned_rows(alike(query), q, plan.tokens, plan.key_heads, plan.key_dim, state, "query");
+    p.k = aligned_rows(alike(key), k, plan.tokens, plan.key_heads, plan.key_dim, state, "key");
     p.v = aligned_rows(value, v, plan.tokens, plan.heads, plan.value_dim, state, "value");
     const Tensor g = gates(decay, plan.tokens, plan.heads, state, "decay"), b = gates(rate, plan.tokens, plan.heads, state, "rate");
     GpuContext& context = gpu_of(state, name);

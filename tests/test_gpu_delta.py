@@ -208,6 +208,20 @@ def test_rows_are_views_of_a_projection(dtype, count):
     assert np.array_equal(got, want)
 
 
+@pytest.mark.parametrize("count", [3, 90])
+@pytest.mark.parametrize("types", [("bf16", "f32", "f32"), ("f32", "bf16", "bf16"), ("bf16", "bf16", "f32"), ("f32", "f32", "bf16")])
+def test_rows_of_different_types(types, count):
+    rng = np.random.default_rng(13)
+    hk, h, dk, dv = 1, 2, 64, 64
+    inputs = draw(rng, count, hk, h, dk, dv)
+    tensors, values = zip(*[give(x, types[i] if i < 3 else "f32") for i, x in enumerate(inputs)])
+    states = ct.DeltaStates(1, 1, h, dk, dv)
+    got = ct.gated_delta(states, 0, ct.DeltaBatch(states, hk, [-1], [0], [count]), *tensors).numpy()
+    q, k = (np.repeat(x, h // hk, 1) for x in values[:2])
+    want, tolerance, _, _ = rule(np.zeros((h, dk, dv)), q, k, *values[2:], dk ** -0.5)
+    assert np.all(np.abs(got - want) <= tolerance)
+
+
 def test_bf16_gates():
     rng = np.random.default_rng(8)
     inputs = draw(rng, 5, 1, 2, 32, 32)
