@@ -167,9 +167,7 @@ template <int DK, int PARTS> __global__ __launch_bounds__(kThreads) void delta_p
         __syncthreads();
         // and the tiles below it, in order: X_ij = -X_ii sum_(j <= k < i) A_ik X_kj; wave j has column j of tiles.
         // (A result's lane layout is that of the next product's right factor, if its index runs over 4 g + r.)
-        uint16_t* solution = p.solution + own * 3 * (kTiles + 1) * kTile;
-        if (threadIdx.x < 96) // a tile of zeros in each part
-            *reinterpret_cast<u32x4*>(solution + (threadIdx.x / 32 * (kTiles + 1) + kTiles) * kTile + threadIdx.x % 32 * 8) = 0;
+        uint16_t* solution = p.solution + own * 3 * kTiles * kTile;
 #pragma unroll
         for (int step = 0; step < 4; ++step) {
             const int i = wave + step;
@@ -191,7 +189,7 @@ template <int DK, int PARTS> __global__ __launch_bounds__(kThreads) void delta_p
             for (int r = 0; r < 4; ++r) {
                 float x = solved[step][r];
 #pragma unroll
-                for (int part = 0; part < 3; ++part) solution[(part * (kTiles + 1) + tile_of(i, wave)) * kTile + (4 * g + r) * 16 + n] = cut(x);
+                for (int part = 0; part < 3; ++part) solution[(part * kTiles + tile_of(i, wave)) * kTile + (4 * g + r) * 16 + n] = cut(x);
             }
         }
         __syncthreads();
@@ -208,6 +206,7 @@ template <int DK, int PARTS, bool V_BF16>
 __global__ __launch_bounds__(2 * kThreads) __attribute__((amdgpu_waves_per_eu(2, PARTS == 1 && DK < 128 ? 4 : 2))) void delta_scan(const dlk_delta_params p) {
     constexpr int STEPS = DK / 32, OWN = DK > 64 ? DK / 64 : 1, LINE_S = DK + 8, LINE = 64 + 8;
     __shared__ uint16_t state_parts[3][16][LINE_S], right[3][16][LINE], write[3][16][LINE], late[3][16][LINE];
+    __shared__ float gates[2][192];
     const int lane = threadIdx.x % kWave, n = lane % 16, g = lane / 16;
     const int role = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), wave = role % kWaves;
     // (work-groups go to the 8 dies in turn; the slices of a head read the same chunks, from the cache of one of them)
@@ -270,6 +269,14 @@ __global__ __launch_bounds__(2 * kThreads) __attribute__((amdgpu_waves_per_eu(2,
                     for (int t = 0; t < 2 && s + t < STEPS; ++t) sum[t] = product(rows[s + t][i], b[s + t][order - i], sum[t]);
         return sum[0] + sum[1];
     };
+    // tiles of a triangle: what lies behind it is read as zero, from beyond the buffer
+    const auto tiles_at = [&](const void* at, int bytes) {
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(at), 0, kTiles * kTile * bytes, kBufferFlags);
+    };
+    const auto tile_offset = [&](int s, int size) {
+        const int tile = 2 * s + g / 2;
+        return tile > wave ? 1u << 30 : static_cast<uint32_t>((tile_of(wave, tile) * kTile + n * 16 + g % 2 * 8) * size);
+    };
     // rows of a triangle, parts [2 steps of 32 columns], times columns in LDS
     const auto triangle = [&](const u32x4 (&rows)[2][3], const uint16_t (&columns)[3][16][LINE], f32x4 sum) {
         f32x4 small = 0.0f;
@@ -294,33 +301,42 @@ __global__ __launch_bounds__(2 * kThreads) __attribute__((amdgpu_waves_per_eu(2,
         // Two chunks ahead: a load is waited for together with all stores before it, and a store takes longer than a chunk.
         // (One ahead: 2.4 us a chunk.)
         u32x4 q[2][STEPS][PARTS];
-        f32x4 within[2][2][2], since[2]; // rows 16 wave + n, columns 32 s + 8 g to + 7 (behind the triangle: anything)
+        float coming[2][3]; // (wave 0) the chunk's gates
+        f32x4 within[2][2][2]; // rows 16 wave + n, columns 32 s + 8 g to + 7; behind the triangle: zeros
         const int out_row = p.heads * p.value_dim;
-        const auto load_queries = [&](int c, int slot) {
-            load_rows(p.q, p.query_parts, c, q[slot]);
-            since[slot] = *reinterpret_cast<const f32x4*>(p.gates + place(c) * 192 + static_cast<uint32_t>(16 * wave + 4 * g));
+        const auto load_gates = [&](int c, int slot) {
+#pragma unroll
+            for (int i = 0; i < 3; ++i) coming[slot][i] = (p.gates + place(c) * 192)[static_cast<uint32_t>(64 * i + lane)];
+        };
+        const auto keep_gates = [&](int slot) {
+            if (wave == 0)
+#pragma unroll
+                for (int i = 0; i < 3; ++i) gates[slot][64 * i + lane] = coming[slot][i];
         };
         const auto load_within = [&](int c, int slot) {
-            const float* from = p.within + place(c) * kTiles * kTile;
+            const __amdgpu_buffer_rsrc_t from = tiles_at(p.within + place(c) * kTiles * kTile, 4);
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
-                    within[slot][s][i] = *reinterpret_cast<const f32x4*>(from + static_cast<uint32_t>(tile_of(wave, min(2 * s + g / 2, wave)) * kTile + n * 16 + g % 2 * 8 + 4 * i));
+                    within[slot][s][i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(from, tile_offset(s, 4) + 16 * i, 0, 0));
         };
         const auto chunk = [&](int c, auto which) {
             constexpr int SLOT = decltype(which)::value;
             const int next = min(c + 2, chunks - 1), tokens = tokens_of(c);
-            f32x4 out = times_state(q[SLOT]) * since[SLOT];
+            f32x4 out = times_state(q[SLOT]) * *reinterpret_cast<const f32x4*>(&gates[SLOT][16 * wave + 4 * g]);
             __builtin_amdgcn_sched_barrier(0);
-            load_queries(next, SLOT);
+            load_rows(p.q, p.query_parts, next, q[SLOT]);
+            keep_gates(1 - SLOT); // the next chunk's
+            __builtin_amdgcn_sched_barrier(0);
+            load_gates(min(c + 3, chunks - 1), 1 - SLOT);
             __syncthreads();
             u32x4 rows[2][3];
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                 float a[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) a[i] = 2 * s + g / 2 > wave ? 0.0f : within[SLOT][s][i / 4][i % 4];
+                for (int i = 0; i < 8; ++i) a[i] = within[SLOT][s][i / 4][i % 4];
 #pragma unroll
                 for (int part = 0; part < 3; ++part) rows[s][part] = cut(a);
             }
@@ -339,9 +355,12 @@ __global__ __launch_bounds__(2 * kThreads) __attribute__((amdgpu_waves_per_eu(2,
         };
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-            load_queries(min(c, chunks - 1), c);
+            load_gates(min(c, chunks - 1), c);
+            load_rows(p.q, p.query_parts, min(c, chunks - 1), q[c]);
             load_within(min(c, chunks - 1), c);
         }
+        keep_gates(0);
+        load_gates(min(2, chunks - 1), 0);
         __syncthreads();
         for (int c = 0; c < chunks; c += 2) {
             chunk(c, std::integral_constant<int, 0>{});
@@ -380,33 +399,23 @@ __global__ __launch_bounds__(2 * kThreads) __attribute__((amdgpu_waves_per_eu(2,
             for (int t = 0; t < OWN; ++t) part4(state[t], &state_parts[0][n][row_of(t, 0)], LINE_S);
     };
     u32x4 k[STEPS][PARTS], keys[OWN][2][PARTS], solution[2][3];
-    f32x4 since, left, rate;
-    float whole;
     uint32_t v[4]; // as they lie in memory
     const auto load_values = [&](int c) {
-        const float* gates = p.gates + place(c) * 192;
-        const uint32_t row = 16 * wave + 4 * g;
-        since = *reinterpret_cast<const f32x4*>(gates + row);
-        left = *reinterpret_cast<const f32x4*>(gates + 64 + row);
-        rate = *reinterpret_cast<const f32x4*>(gates + 128 + row);
-        whole = gates[63];
         const int64_t from = (item.token + 64 * static_cast<int64_t>(c)) * p.v.row + head * p.v.head + first_column;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const uint32_t at = at_row(row + r, p.v.row, c) + n;
+            const uint32_t at = at_row(16 * wave + 4 * g + r, p.v.row, c) + n;
             if constexpr (V_BF16) v[r] = (static_cast<const uint16_t*>(p.v.x) + from)[at];
             else v[r] = (static_cast<const uint32_t*>(p.v.x) + from)[at];
         }
     };
-    const auto load_solution = [&](int c) { // row 16 wave + n, columns 32 s + 8 g to + 7: behind the triangle, of the tile of zeros
-        const uint16_t* from = p.solution + place(c) * 3 * (kTiles + 1) * kTile;
+    const auto load_solution = [&](int c) { // row 16 wave + n, columns 32 s + 8 g to + 7; behind the triangle: zeros
+        const __amdgpu_buffer_rsrc_t from = tiles_at(p.solution + place(c) * 3 * kTiles * kTile, 6);
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            const int tile = 2 * s + g / 2;
-            const uint32_t at = (tile > wave ? kTiles : tile_of(wave, tile)) * kTile + n * 16 + g % 2 * 8;
+        for (int s = 0; s < 2; ++s)
 #pragma unroll
-            for (int part = 0; part < 3; ++part) solution[s][part] = *reinterpret_cast<const u32x4*>(from + part * (kTiles + 1) * kTile + at);
-        }
+            for (int part = 0; part < 3; ++part)
+                solution[s][part] = __builtin_amdgcn_raw_buffer_load_b128(from, tile_offset(s, 2) + part * kTiles * kTile * 2, 0, 0);
     };
     const auto load_keys = [&](int c) {
         if (holds)
@@ -429,6 +438,9 @@ __global__ __launch_bounds__(2 * kThreads) __attribute__((amdgpu_waves_per_eu(2,
     __syncthreads();
     for (int c = 0; c < chunks; ++c) {
         const int next = min(c + 1, chunks - 1), tokens = tokens_of(c);
+        const float* own = &gates[c % 2][16 * wave + 4 * g];
+        const f32x4 since = *reinterpret_cast<const f32x4*>(own), left = *reinterpret_cast<const f32x4*>(own + 64), rate = *reinterpret_cast<const f32x4*>(own + 128);
+        const float whole = gates[c % 2][63];
         const f32x4 ks = times_state(k);
         __builtin_amdgcn_sched_barrier(0);
         load_rows(p.k, p.key_parts, next, k);
@@ -491,7 +503,7 @@ Layout layout(const dlk_delta_params* p) {
     Layout l{};
     const int64_t heads = static_cast<int64_t>(p->chunk_count) * p->heads, parts = parts_of(p);
     const int64_t rows = static_cast<int64_t>(p->chunk_count) * (p->heads / p->group) * 64 * p->key_dim * parts * 2;
-    l.within = heads * 3 * (kTiles + 1) * kTile * 2;
+    l.within = heads * 3 * kTiles * kTile * 2;
     l.gates = l.within + heads * kTiles * kTile * 4;
     l.turned = l.gates + heads * 192 * 4;
     l.keys = l.turned + rows;

@@ -375,7 +375,7 @@ typedef struct dlk_delta_params {
     const dlk_delta_chunk* chunks;
     int item_count, chunk_count;
     /* set by dlk_delta_chunks: its workspace */
-    uint16_t* solution;      /* [chunks, heads, 3 parts, 10 tiles and one of zeros, 16, 16] */
+    uint16_t* solution;      /* [chunks, heads, 3 parts, 10 tiles, 16, 16] */
     float* within;           /* [chunks, heads, 10 tiles, 16, 16] */
     float* gates;            /* [chunks, heads, 3, 64] */
     uint16_t* turned_keys;   /* [parts, chunks, key heads, key_dim, 64] */
