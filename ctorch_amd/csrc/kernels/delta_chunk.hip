@@ -52,10 +52,17 @@ template <int A, int B> __device__ __forceinline__ f32x4 multiply(const u32x4 (&
 
 // ------------------------------------------------------------------------------------------------ the chunks by themselves
 // A work-group per chunk and key head; wave w has the chunk's tokens 16 w to 16 w + 15 as rows.
-template <int DK, int PARTS> __global__ __launch_bounds__(kThreads) void delta_prepare(const dlk_delta_params p) {
+template <int DK, int PARTS> __global__ __launch_bounds__(kThreads, 3) void delta_prepare(const dlk_delta_params p) {
     constexpr int STEPS = DK / 32, LINE = 64 + 8, WIDE = 64 + 4;
-    __shared__ uint16_t turned[DK][LINE];
-    __shared__ float system[64][WIDE], inverse[4][16][20];
+    __shared__ union {
+        uint16_t turned[DK][LINE];
+        struct {
+            float system[64][WIDE], inverse[4][16][20];
+        };
+    } room; // (first the one, then the other)
+    auto& turned = room.turned;
+    auto& system = room.system;
+    auto& inverse = room.inverse;
     __shared__ double reach[kWaves][64];
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, n = lane % 16, g = lane / 16;
     const int key_heads = p.heads / p.group, key_head = blockIdx.x % key_heads;
@@ -114,6 +121,7 @@ template <int DK, int PARTS> __global__ __launch_bounds__(kThreads) void delta_p
             qk[j] = multiply(q[s], column, qk[j]);
         }
     }
+    __syncthreads();
     for (int h = 0; h < p.group; ++h) {
         const int head = key_head * p.group + h;
         const int64_t own = index * p.heads + head;
@@ -153,9 +161,13 @@ template <int DK, int PARTS> __global__ __launch_bounds__(kThreads) void delta_p
         float x[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
+            f32x4 row[4];
+#pragma unroll
+            for (int j = 0; j < (i + 3) / 4; ++j) row[j] = *reinterpret_cast<const f32x4*>(&system[16 * wave + i][16 * wave + 4 * j]);
             x[i] = i == n ? 1.0f : 0.0f;
 #pragma unroll
-            for (int j = 0; j < i; ++j) x[i] = fmaf(-system[16 * wave + i][16 * wave + j], x[j], x[i]);
+            for (int j = 0; j < i; ++j) x[i] = fmaf(-row[j / 4][j % 4], x[j], x[i]);
+            if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0); // (all rows read at once would take the registers of another wave)
         }
         f32x4 solved[4]; // [tile row]: rows 4 g + r, column n
 #pragma unroll
@@ -167,7 +179,6 @@ template <int DK, int PARTS> __global__ __launch_bounds__(kThreads) void delta_p
         __syncthreads();
         // and the tiles below it, in order: X_ij = -X_ii sum_(j <= k < i) A_ik X_kj; wave j has column j of tiles.
         // (A result's lane layout is that of the next product's right factor, if its index runs over 4 g + r.)
-        uint16_t* solution = p.solution + own * 3 * kTiles * kTile;
 #pragma unroll
         for (int step = 0; step < 4; ++step) {
             const int i = wave + step;
@@ -185,12 +196,25 @@ template <int DK, int PARTS> __global__ __launch_bounds__(kThreads) void delta_p
 #pragma unroll
                 for (int r = 0; r < 4; ++r) solved[step] = product(a[r], -below[r], solved[step]);
             }
+        }
+        __syncthreads();
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                float x = solved[step][r];
+        for (int step = 0; step < 4; ++step)
+            if (wave + step < 4)
 #pragma unroll
-                for (int part = 0; part < 3; ++part) solution[(part * kTiles + tile_of(i, wave)) * kTile + (4 * g + r) * 16 + n] = cut(x);
-            }
+                for (int r = 0; r < 4; ++r) system[16 * (wave + step) + 4 * g + r][16 * wave + n] = solved[step][r];
+        __syncthreads();
+        // in parts, 8 entries a thread
+        uint16_t* solution = p.solution + own * 3 * kTiles * kTile;
+        for (int i = threadIdx.x; i < kTiles * 32; i += kThreads) {
+            const int tile = i / 32, row = tile < 1 ? 0 : tile < 3 ? 1 : tile < 6 ? 2 : 3, column = tile - tile_of(row, 0);
+            const f32x4* from = reinterpret_cast<const f32x4*>(&system[16 * row + i / 2 % 16][16 * column + i % 2 * 8]);
+            const f32x4 a = from[0], b = from[1];
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = a[j], v[4 + j] = b[j];
+#pragma unroll
+            for (int part = 0; part < 3; ++part) *reinterpret_cast<u32x4*>(solution + part * kTiles * kTile + i * 8) = cut(v);
         }
         __syncthreads();
     }
