@@ -352,7 +352,7 @@ int dlk_page_copy(const dlk_page_copy_params* p, dlh_stream stream);
 
 /* ------------------------------------------------------------------------------------------------------
  * The gated delta rule over a step's tokens, one after the other (delta_step.hip) or in chunks of 64 (delta_chunk.hip).  Rows
- * are 16-byte aligned, also between heads and tokens.
+ * are 16-byte aligned, also between heads and tokens; queries and keys are of one type.
  * ---------------------------------------------------------------------------------------------------- */
 typedef struct dlk_delta_item { /* a request's new tokens: `count` from `token` on */
     int32_t source, target;     /* slots of its state before (-1: zero) and after */
@@ -382,7 +382,7 @@ typedef struct dlk_delta_params {
     uint16_t* key_parts;     /* [parts, chunks, key heads, 64, key_dim], f32 queries or keys only */
     uint16_t* query_parts;
 } dlk_delta_params;
-/* Bytes of workspace for the chunks of these parameters (queries and keys of one type). */
+/* Bytes of workspace for the chunks of these parameters. */
 int64_t dlk_delta_workspace(const dlk_delta_params* p);
 int dlk_delta_chunks(const dlk_delta_params* p, void* workspace, dlh_stream stream);
 int dlk_delta_step(const dlk_delta_params* p, dlh_stream stream);

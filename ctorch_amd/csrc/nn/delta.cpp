@@ -167,8 +167,8 @@ Tensor gated_delta(const nn::DeltaStates& states, Index layer, const nn::DeltaBa
     const Tensor& state = states.state(layer);
     Tensor q, k, v;
     dlk_delta_params p{};
-    // (the launches over chunks take queries and keys of one type)
-    const bool mixed = !plan.rounds.empty() && query.dtype() != key.dtype() && is_floating(query.dtype()) && is_floating(key.dtype());
+    // (the kernels take queries and keys of one type)
+    const bool mixed = query.dtype() != key.dtype() && is_floating(query.dtype()) && is_floating(key.dtype());
     const auto alike = [&](const Tensor& t) { return mixed && t.dtype() == DType::bf16 ? t.astype(DType::f32) : t; };
     p.q = aligned_rows(alike(query), q, plan.tokens, plan.key_heads, plan.key_dim, state, "query");
     p.k = aligned_rows(alike(key), k, plan.tokens, plan.key_heads, plan.key_dim, state, "key");
