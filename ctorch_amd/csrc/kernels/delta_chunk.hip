@@ -322,50 +322,53 @@ __global__ __launch_bounds__(2 * kThreads) __attribute__((amdgpu_waves_per_eu(2,
     };
 
     if (role >= kWaves) {
-        // Two chunks ahead: a load is waited for together with all stores before it, and a store takes longer than a chunk.
-        // (One ahead: 2.4 us a chunk.)
-        u32x4 q[2][STEPS][PARTS];
-        float coming[2][3]; // (wave 0) the chunk's gates
-        f32x4 within[2][2][2]; // rows 16 wave + n, columns 32 s + 8 g to + 7; behind the triangle: zeros
+        u32x4 q[STEPS][PARTS];
+        float coming[3];       // (wave 0) the next chunk's gates
+        f32x4 within[2][2];    // rows 16 wave + n, columns 32 s + 8 g to + 7; behind the triangle: zeros
         const int out_row = p.heads * p.value_dim;
-        const auto load_gates = [&](int c, int slot) {
+        const auto load_gates = [&](int c) {
 #pragma unroll
-            for (int i = 0; i < 3; ++i) coming[slot][i] = (p.gates + place(c) * 192)[static_cast<uint32_t>(64 * i + lane)];
+            for (int i = 0; i < 3; ++i) coming[i] = (p.gates + place(c) * 192)[static_cast<uint32_t>(64 * i + lane)];
         };
-        const auto keep_gates = [&](int slot) {
+        const auto keep_gates = [&](int c) {
             if (wave == 0)
 #pragma unroll
-                for (int i = 0; i < 3; ++i) gates[slot][64 * i + lane] = coming[slot][i];
+                for (int i = 0; i < 3; ++i) gates[c % 2][64 * i + lane] = coming[i];
         };
-        const auto load_within = [&](int c, int slot) {
+        const auto load_within = [&](int c) {
             const __amdgpu_buffer_rsrc_t from = tiles_at(p.within + place(c) * kTiles * kTile, 4);
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
-                    within[slot][s][i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(from, tile_offset(s, 4) + 16 * i, 0, 0));
+                    within[s][i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(from, tile_offset(s, 4) + 16 * i, 0, 0));
         };
-        const auto chunk = [&](int c, auto which) {
-            constexpr int SLOT = decltype(which)::value;
-            const int next = min(c + 2, chunks - 1), tokens = tokens_of(c);
-            f32x4 out = times_state(q[SLOT]) * *reinterpret_cast<const f32x4*>(&gates[SLOT][16 * wave + 4 * g]);
+        load_gates(0);
+        load_rows(p.q, p.query_parts, 0, q);
+        load_within(0);
+        keep_gates(0);
+        load_gates(min(1, chunks - 1));
+        __syncthreads();
+        for (int c = 0; c < chunks; ++c) {
+            const int next = min(c + 1, chunks - 1), tokens = tokens_of(c);
+            f32x4 out = times_state(q) * *reinterpret_cast<const f32x4*>(&gates[c % 2][16 * wave + 4 * g]);
             __builtin_amdgcn_sched_barrier(0);
-            load_rows(p.q, p.query_parts, next, q[SLOT]);
-            keep_gates(1 - SLOT); // the next chunk's
+            load_rows(p.q, p.query_parts, next, q);
+            keep_gates(c + 1);
             __builtin_amdgcn_sched_barrier(0);
-            load_gates(min(c + 3, chunks - 1), 1 - SLOT);
+            load_gates(min(c + 2, chunks - 1));
             __syncthreads();
             u32x4 rows[2][3];
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                 float a[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) a[i] = within[SLOT][s][i / 4][i % 4];
+                for (int i = 0; i < 8; ++i) a[i] = within[s][i / 4][i % 4];
 #pragma unroll
                 for (int part = 0; part < 3; ++part) rows[s][part] = cut(a);
             }
             __builtin_amdgcn_sched_barrier(0);
-            load_within(next, SLOT);
+            load_within(next);
             __syncthreads();
             out = triangle(rows, write, out) * p.scale;
             // Rows behind the chunk's end lie behind the buffer's.  (Of stores under a condition the compiler could not tell how
@@ -376,19 +379,6 @@ __global__ __launch_bounds__(2 * kThreads) __attribute__((amdgpu_waves_per_eu(2,
             for (int i = 0; i < 4; ++i)
                 __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(out[i]), rows_out, ((16 * wave + 4 * g + i) * out_row + n) * 4, 0, 0);
             __syncthreads();
-        };
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            load_gates(min(c, chunks - 1), c);
-            load_rows(p.q, p.query_parts, min(c, chunks - 1), q[c]);
-            load_within(min(c, chunks - 1), c);
-        }
-        keep_gates(0);
-        load_gates(min(2, chunks - 1), 0);
-        __syncthreads();
-        for (int c = 0; c < chunks; c += 2) {
-            chunk(c, std::integral_constant<int, 0>{});
-            if (c + 1 < chunks) chunk(c + 1, std::integral_constant<int, 1>{});
         }
         return;
     }

@@ -53,9 +53,14 @@ DeltaBatch::DeltaBatch(const DeltaStates& states, Index key_heads, std::span<con
         plan->tokens += counts[b];
     }
     if (plan->tokens > INT32_MAX / states.heads()) refuse("too many new tokens");
-    // (the rule token by token takes about a microsecond a token; in chunks, three launches of some microseconds and one a chunk)
-    constexpr Index few = 16;
-    // (of chunks and heads: 21 KB of workspace each, and the keys' copies)
+    // Up to so many tokens a request's go one after the other, 0.6 to 1 us each; more in chunks, which take two launches and, where
+    // requests, heads and columns make more work-groups than run at once, rounds of 5 us.  Measured on MI355X, us one by one / in
+    // chunks: one request of 32 heads of 128 x 128, 16 tokens 18.7 / 19.8, 24 26.4 / 20.2; 16 such requests, 32 tokens 54 / 99, 64
+    // 88 / 107; one request of 8 heads of 64 x 64 in f32, 24 tokens 18.0 / 19.4, 48 33.5 / 19.5; 16 such 24 tokens 18 / 28, 48 33 / 28.
+    Index busy = 0;
+    for (const Index count : counts) busy += count > 0;
+    const Index few = std::min<Index>(64, 16 + 3 * (busy * states.heads() * (states.value_dim() / 16) / 256));
+    // (of chunks and heads: 26 KB of workspace each, and the keys' copies)
     constexpr Index most = 8192;
     const Index round_chunks = std::max<Index>(1, most / states.heads());
     std::vector<dlk_delta_item> items, rest; // rest: requests of many tokens, then what is left of them
