@@ -39,7 +39,8 @@ __device__ __forceinline__ void eight(const void* x, int bf16, int64_t at, float
 struct Plan {          // what a launch's kernels hand on
     uint16_t* pick;    // [tokens, top]: the chosen experts
     char* rows;        // x as the products read it (see `planes`), or NULL: p.x itself
-    char* act;         // the hidden entries, likewise
+    char* act;         // the hidden entries: f32 (`whole`), or three parts
+    bool whole;
     float* partial;    // [tokens, top, dim]: outputs of each pair
     int planes;        // bf16 matrices: parts of a row of x; 0: f32 matrices, f32 rows
 };
@@ -66,24 +67,39 @@ __global__ __launch_bounds__(kRoute) void experts_route(const dlk_experts_params
                 for (int part = 0; part < plan.planes; ++part)
                     *reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(plan.rows) + (part * p.tokens + token) * p.dim + i) = cut(v);
             }
-        constexpr int N = 4; // experts at a time
+        constexpr int N = 4, U = 2; // experts and steps at a time
         for (int first = wave * N; first < p.experts; first += kRouteWaves * N) {
             double sum[N] = {};
-            for (int i = lane * 8; i < p.dim; i += kWave * 8) {
-                float x[8], w[N][8];
-                eight(p.x, p.x_bf16, token * p.dim + i, x);
+            for (int i = lane * 8; i < p.dim; i += U * kWave * 8) {
+                float x[U][8], w[U][N][8];
 #pragma unroll
-                for (int n = 0; n < N; ++n) eight(p.router, p.router_bf16, static_cast<int64_t>(min(first + n, p.experts - 1)) * p.dim + i, w[n]);
+                for (int u = 0; u < U; ++u) {
+                    const int at = min(i + u * kWave * 8, p.dim - 8);
+                    eight(p.x, p.x_bf16, token * p.dim + at, x[u]);
 #pragma unroll
-                for (int n = 0; n < N; ++n)
+                    for (int n = 0; n < N; ++n) eight(p.router, p.router_bf16, static_cast<int64_t>(min(first + n, p.experts - 1)) * p.dim + at, w[u][n]);
+                }
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) sum[n] = fma(static_cast<double>(x[j]), static_cast<double>(w[n][j]), sum[n]);
+                for (int u = 0; u < U; ++u)
+                    if (i + u * kWave * 8 < p.dim)
+#pragma unroll
+                        for (int n = 0; n < N; ++n)
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) sum[n] = fma(static_cast<double>(x[u][j]), static_cast<double>(w[u][n][j]), sum[n]);
             }
+            // lanes that differ in the lowest two bits share the four sums out; lane l ends with that of expert l % 4
+            const bool odd = lane & 1, high = lane & 2;
+            double two[2];
 #pragma unroll
-            for (int n = 0; n < N; ++n) {
-                const double z = wave_sum_f64(sum[n]);
-                if (lane == 0 && first + n < p.experts) logits[first + n] = z;
+            for (int n = 0; n < 2; ++n) {
+                const double give = odd ? sum[2 * n] : sum[2 * n + 1];
+                two[n] = (odd ? sum[2 * n + 1] : sum[2 * n]) + __shfl_xor(give, 1);
             }
+            const double give = high ? two[0] : two[1];
+            double z = (high ? two[1] : two[0]) + __shfl_xor(give, 2);
+#pragma unroll
+            for (int d = 4; d < kWave; d *= 2) z += __shfl_xor(z, d);
+            if (lane < N && first + lane < p.experts) logits[first + lane] = z;
         }
     } else {
         for (int e = wave; e < p.experts; e += kRouteWaves) {
@@ -162,13 +178,13 @@ __device__ __forceinline__ void exchange(u32x4 (&w)[2]) {
 }
 
 // An entry of a pair: a hidden one as the next product reads it, or an output.
-template <bool GATE, bool F32>
+template <bool GATE>
 __device__ __forceinline__ void keep(const dlk_experts_params& p, const Plan& plan, int pair, int row, float v, float up) {
     const int64_t height = GATE ? p.hidden : p.dim, to = pair * height + row;
     if constexpr (!GATE) plan.partial[to] = v;
     else {
         v = v / (1.0f + expf(-v)) * up;
-        if constexpr (F32) reinterpret_cast<float*>(plan.act)[to] = v;
+        if (plan.whole) reinterpret_cast<float*>(plan.act)[to] = v;
         else
 #pragma unroll
             for (int part = 0; part < 3; ++part) reinterpret_cast<uint16_t*>(plan.act)[part * p.tokens * p.top * height + to] = cut(v);
@@ -313,7 +329,7 @@ __global__ __launch_bounds__(SPLIT ? 512 : 256) void experts_rows(const dlk_expe
                         v += sums[w][tile][column][r];
                         if constexpr (GATE) up += sums[w][R + tile][column][r];
                     }
-                    keep<GATE, F32>(p, plan, list[at], row, v, up);
+                    keep<GATE>(p, plan, list[at], row, v, up);
                 }
                 __syncthreads();
             } else {
@@ -323,7 +339,7 @@ __global__ __launch_bounds__(SPLIT ? 512 : 256) void experts_rows(const dlk_expe
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const int row = first_row + 16 * r + 4 * g + j;
-                        if (row < height && at < count) keep<GATE, F32>(p, plan, list[at], row, sum[t][r][j], GATE ? sum[t][TILES - R + r][j] : 0.0f);
+                        if (row < height && at < count) keep<GATE>(p, plan, list[at], row, sum[t][r][j], GATE ? sum[t][TILES - R + r][j] : 0.0f);
                     }
             }
         }
@@ -463,42 +479,64 @@ __global__ __launch_bounds__(WAVES * kWave) void experts_blocks(const dlk_expert
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int row = first_row + 16 * r + 4 * g + j;
-                    if (row < height && at < count) keep<GATE, F32>(p, plan, list[at], row, sum[t][r][j], GATE ? sum[t][TILES - R + r][j] : 0.0f);
+                    if (row < height && at < count) keep<GATE>(p, plan, list[at], row, sum[t][r][j], GATE ? sum[t][TILES - R + r][j] : 0.0f);
                 }
         }
     }
 }
 
-// The weighted sum of a row's outputs, in the order of its choice.  A thread has four neighbouring entries.
-__global__ __launch_bounds__(256) void experts_join(const dlk_experts_params p, const float* partial) {
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, units = p.dim / 4;
+// The weighted sum of a row's outputs, in the order of its choice.  A thread has N neighbouring entries.
+template <int N> __global__ __launch_bounds__(256) void experts_join(const dlk_experts_params p, const float* partial) {
+    struct alignas(4 * N) Entries {
+        float v[N];
+    };
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, units = p.dim / N;
     if (i >= p.tokens * units) return;
     const int64_t token = i / units;
-    const f32x4* from = reinterpret_cast<const f32x4*>(partial) + token * p.top * units + i % units;
-    f32x4 y = 0.0f;
+    const Entries* from = reinterpret_cast<const Entries*>(partial) + token * p.top * units + i % units;
+    Entries y{};
+#pragma unroll 4
     for (int j = 0; j < p.top; ++j) {
-        const f32x4 v = from[j * units];
+        const Entries x = from[j * units];
         const float w = p.weights[token * p.top + j];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) y[c] = fmaf(w, v[c], y[c]);
+        for (int c = 0; c < N; ++c) y.v[c] = fmaf(w, x.v[c], y.v[c]);
     }
-    reinterpret_cast<f32x4*>(p.y)[i] = y;
+    reinterpret_cast<Entries*>(p.y)[i] = y;
 }
 
-// Any sizes and alignments: a wave per pair (row, chosen expert) and hidden entry,
-__global__ __launch_bounds__(256) void experts_hidden_any(const dlk_experts_params p, float* act) {
-    const int lane = threadIdx.x % kWave;
-    const int64_t unit = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / kWave, step = static_cast<int64_t>(gridDim.x) * 256 / kWave;
-    for (int64_t u = unit; u < p.tokens * p.top * p.hidden; u += step) {
-        const int64_t pair = u / p.hidden, row = p.chosen[pair] * p.hidden + u % p.hidden;
-        float g = 0.0f, h = 0.0f;
+// Any sizes and alignments, entry by entry: a wave per expert and hidden entry, for up to 8 of the rows that chose it at a time.
+__global__ __launch_bounds__(256) void experts_hidden_any(const dlk_experts_params p, const Plan plan) {
+    constexpr int WAVES = 4, N = 8;
+    extern __shared__ uint16_t list[];
+    __shared__ int counts[WAVES];
+    const int pairs = static_cast<int>(p.tokens) * p.top, e = blockIdx.y;
+    const int count = collect<WAVES>(plan.pick, pairs, e, list, counts);
+    const int lane = threadIdx.x % kWave, row = blockIdx.x * WAVES + threadIdx.x / kWave;
+    if (row >= p.hidden) return;
+    const int64_t at = (static_cast<int64_t>(e) * p.hidden + row) * p.dim;
+    for (int first = 0; first < count; first += N) {
+        float g[N] = {}, h[N] = {};
+        int64_t rows[N];
+#pragma unroll
+        for (int n = 0; n < N; ++n) rows[n] = static_cast<int64_t>(list[min(first + n, count - 1)] / p.top) * p.dim;
+#pragma unroll 2
         for (int i = lane; i < p.dim; i += kWave) {
-            const float x = entry(p.x, p.x_bf16, pair / p.top * p.dim + i);
-            g = fmaf(x, entry(p.gate, p.weights_bf16, row * p.dim + i), g);
-            h = fmaf(x, entry(p.up, p.weights_bf16, row * p.dim + i), h);
+            const float wg = entry(p.gate, p.weights_bf16, at + i), wu = entry(p.up, p.weights_bf16, at + i);
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+                if (first + n < count) {
+                    const float x = entry(p.x, p.x_bf16, rows[n] + i);
+                    g[n] = fmaf(x, wg, g[n]);
+                    h[n] = fmaf(x, wu, h[n]);
+                }
         }
-        g = wave_sum(g), h = wave_sum(h);
-        if (lane == 0) act[u] = g / (1.0f + expf(-g)) * h;
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+            if (first + n < count) {
+                const float a = wave_sum(g[n]), b = wave_sum(h[n]);
+                if (lane == 0) keep<true>(p, plan, list[first + n], row, a, b);
+            }
     }
 }
 
@@ -519,38 +557,31 @@ __global__ __launch_bounds__(256) void experts_down_any(const dlk_experts_params
     }
 }
 
-// Whether the products read whole pieces of 16 bytes at offsets of 32 bits.
-bool pieces(const dlk_experts_params& p) {
-    const int unit = p.weights_bf16 ? 8 : 4, size = p.weights_bf16 ? 2 : 4;
-    const auto aligned = [](const void* at) { return reinterpret_cast<uintptr_t>(at) % 16 == 0; };
-    return p.dim % unit == 0 && p.hidden % unit == 0 && aligned(p.gate) && aligned(p.up) && aligned(p.down) &&
-           static_cast<int64_t>(p.dim) * p.hidden * size <= INT32_MAX;
-}
-bool wide(const dlk_experts_params& p) {
-    const auto aligned = [](const void* at) { return reinterpret_cast<uintptr_t>(at) % 16 == 0; };
-    return p.dim % 8 == 0 && aligned(p.x) && aligned(p.router);
-}
+bool aligned(const void* at) { return reinterpret_cast<uintptr_t>(at) % 16 == 0; }
+bool wide(const dlk_experts_params& p) { return p.dim % 8 == 0 && aligned(p.x) && aligned(p.router); }
 int64_t up16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
 
+// Each product by itself takes the matrix cores where it reads whole pieces of 16 bytes, at offsets of 32 bits.
 struct Layout {
-    bool fast;
+    bool gate, down;
     int planes; // of x: parts (bf16 matrices) or 0
     int64_t rows, act, partial, bytes;
 };
 Layout layout(const dlk_experts_params& p) {
     Layout l{};
     const int64_t pairs = p.tokens * p.top;
-    // rows are laid out by the router's kernel in pieces of 8
+    const int unit = p.weights_bf16 ? 8 : 4, size = p.weights_bf16 ? 2 : 4;
     const int64_t most = std::max<int64_t>(p.tokens * p.dim, pairs * p.hidden) * (p.weights_bf16 ? 6 : 4);
-    l.fast = pieces(p) && most <= INT32_MAX && (wide(p) || (p.weights_bf16 == p.x_bf16 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0));
+    const bool fits = most <= INT32_MAX && static_cast<int64_t>(p.dim) * p.hidden * size <= INT32_MAX;
+    // (rows of another type than the matrices' are laid out by the router's kernel, in pieces of 8)
+    const bool laid = p.weights_bf16 != p.x_bf16;
+    l.gate = fits && p.dim % unit == 0 && aligned(p.gate) && aligned(p.up) && (laid ? wide(p) : aligned(p.x));
+    l.down = fits && p.hidden % unit == 0 && aligned(p.down);
     l.planes = p.weights_bf16 ? (p.x_bf16 ? 1 : 3) : 0;
     l.rows = up16(pairs * 2); // behind the choice
-    int64_t at = l.rows;
-    if (l.fast && p.weights_bf16 != p.x_bf16) at += up16(p.tokens * p.dim * (p.weights_bf16 ? 6 : 4));
-    l.act = at;
-    at += up16(pairs * p.hidden * (l.fast && p.weights_bf16 ? 6 : 4));
-    l.partial = at;
-    l.bytes = at + (l.fast ? pairs * p.dim * 4 : 0);
+    l.act = l.rows + (l.gate && laid ? up16(p.tokens * p.dim * (p.weights_bf16 ? 6 : 4)) : 0);
+    l.partial = l.act + up16(pairs * p.hidden * (l.down && p.weights_bf16 ? 6 : 4));
+    l.bytes = l.partial + (l.down ? pairs * p.dim * 4 : 0);
     return l;
 }
 
@@ -607,27 +638,27 @@ extern "C" int dlk_experts(const dlk_experts_params* p, dlh_stream stream) {
     hipStream_t at = reinterpret_cast<hipStream_t>(stream);
     const Layout l = layout(*p);
     char* space = static_cast<char*>(p->workspace);
-    const Plan plan{reinterpret_cast<uint16_t*>(space), l.act > l.rows ? space + l.rows : nullptr, space + l.act,
+    const Plan plan{reinterpret_cast<uint16_t*>(space), l.act > l.rows ? space + l.rows : nullptr, space + l.act, !l.down || !p->weights_bf16,
                     reinterpret_cast<float*>(space + l.partial), l.planes};
     const auto tokens = static_cast<unsigned>(p->tokens);
     if (wide(*p)) experts_route<true><<<tokens, kRoute, 0, at>>>(*p, plan);
     else experts_route<false><<<tokens, kRoute, 0, at>>>(*p, plan);
-    if (!l.fast) {
-        const auto groups = [](int64_t waves) { return static_cast<unsigned>(std::min<int64_t>(waves / 4 + 1, 16384)); };
-        float* act = reinterpret_cast<float*>(plan.act);
-        experts_hidden_any<<<groups(p->tokens * p->top * p->hidden), 256, 0, at>>>(*p, act);
-        experts_down_any<<<groups(p->tokens * p->dim), 256, 0, at>>>(*p, act);
+    if (!l.gate) {
+        const dim3 groups((p->hidden + 3) / 4, p->experts);
+        const int list = static_cast<int>(p->tokens) * p->top * 2;
+        experts_hidden_any<<<groups, 256, list, at>>>(*p, plan);
+    } else if (!p->weights_bf16) rows_of<true, true, 1>(*p, plan, at);
+    else if (p->x_bf16) rows_of<true, false, 1>(*p, plan, at);
+    else rows_of<true, false, 3>(*p, plan, at);
+    if (!l.down) {
+        const int64_t waves = p->tokens * p->dim;
+        experts_down_any<<<static_cast<unsigned>(std::min<int64_t>(waves / 4 + 1, 16384)), 256, 0, at>>>(*p, reinterpret_cast<const float*>(plan.act));
         return hipGetLastError();
     }
-    if (!p->weights_bf16) {
-        rows_of<true, true, 1>(*p, plan, at);
-        rows_of<false, true, 1>(*p, plan, at);
-    } else {
-        if (p->x_bf16) rows_of<true, false, 1>(*p, plan, at);
-        else rows_of<true, false, 3>(*p, plan, at);
-        rows_of<false, false, 3>(*p, plan, at);
-    }
-    const int64_t units = p->tokens * (p->dim / 4);
-    experts_join<<<static_cast<unsigned>((units + 255) / 256), 256, 0, at>>>(*p, plan.partial);
+    if (p->weights_bf16) rows_of<false, false, 3>(*p, plan, at);
+    else rows_of<false, true, 1>(*p, plan, at);
+    const int64_t entries = p->tokens * p->dim;
+    if (p->dim % 4 == 0 && aligned(p->y)) experts_join<4><<<static_cast<unsigned>((entries / 4 + 255) / 256), 256, 0, at>>>(*p, plan.partial);
+    else experts_join<1><<<static_cast<unsigned>((entries + 255) / 256), 256, 0, at>>>(*p, plan.partial);
     return hipGetLastError();
 }

@@ -206,3 +206,9 @@ def test_the_same_call_gives_the_same_bits():
     first = [t.numpy() for t in ct.expert_mixture(*tensors, 4)]
     for _ in range(3):
         assert all(np.array_equal(a, t.numpy()) for a, t in zip(first, ct.expert_mixture(*tensors, 4)))
+
+
+@pytest.mark.parametrize("T,d,F", [(1, 65, 64), (40, 63, 24), (3, 64, 63), (150, 129, 40), (20, 96, 41), (9, 130, 66)])
+@pytest.mark.parametrize("weight,inputs", [("bf16", "f32"), ("bf16", "bf16"), ("f32", "bf16"), ("f32", "f32")])
+def test_one_of_the_products_in_pieces(T, d, F, weight, inputs):
+    check(T, d, F, 6, 3, weight, inputs)
