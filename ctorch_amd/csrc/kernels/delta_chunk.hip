@@ -535,9 +535,11 @@ extern "C" int dlk_delta_chunks(const dlk_delta_params* given, void* workspace, 
     using namespace dlk;
     dlk_delta_params p = *given;
     if (p.item_count <= 0 || p.chunk_count <= 0) return 0;
-    const int64_t groups = std::max<int64_t>(static_cast<int64_t>(p.chunk_count) * (p.heads / p.group),
-                                             (static_cast<int64_t>(p.item_count) * p.heads + 7) / 8 * 8 * (p.value_dim / 16));
-    if (p.value_dim <= 0 || p.value_dim % 16 != 0 || p.group <= 0 || groups > DLK_MOST_GROUPS || !workspace || p.q.bf16 != p.k.bf16) return hipErrorInvalidValue;
+    const int64_t prepared = static_cast<int64_t>(p.chunk_count) * (p.heads / p.group);
+    const int64_t scanned = (static_cast<int64_t>(p.item_count) * p.heads + 7) / 8 * 8 * (p.value_dim / 16);
+    if (p.value_dim <= 0 || p.value_dim % 16 != 0 || p.group <= 0 || prepared > DLK_MOST_GROUPS || 2 * scanned > DLK_MOST_GROUPS || !workspace ||
+        p.q.bf16 != p.k.bf16)
+        return hipErrorInvalidValue;
     const Layout l = layout(&p);
     char* at = static_cast<char*>(workspace);
     p.solution = reinterpret_cast<uint16_t*>(at);

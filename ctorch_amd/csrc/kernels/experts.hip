@@ -11,7 +11,7 @@ namespace dlk {
 namespace {
 
 constexpr uint32_t kBeyond = 1u << 31; // an offset behind every buffer's end
-constexpr int kPairs = 8192; // (row, chosen expert) pairs of a launch: the list of an expert's in LDS
+constexpr int kPairs = 8000; // (row, chosen expert) pairs of a launch: the list of an expert's in LDS, beside 48 KB of rows in 64
 
 __device__ __forceinline__ float entry(const void* x, int bf16, int64_t at) {
     return bf16 ? bf16_to_f32(static_cast<const uint16_t*>(x)[at]) : static_cast<const float*>(x)[at];

@@ -59,6 +59,8 @@ DeltaBatch::DeltaBatch(const DeltaStates& states, Index key_heads, std::span<con
     // 88 / 107; one request of 8 heads of 64 x 64 in f32, 24 tokens 18.0 / 19.4, 48 33.5 / 19.5; 16 such 24 tokens 18 / 28, 48 33 / 28.
     Index busy = 0;
     for (const Index count : counts) busy += count > 0;
+    // (a launch has fewer than 2^32 threads: so many columns of 16)
+    if (busy > (1 << 22) / (states.heads() * (states.value_dim() / 16))) refuse("too many requests at once");
     const Index few = std::min<Index>(64, 16 + 3 * (busy * states.heads() * (states.value_dim() / 16) / 256));
     // (of chunks and heads: 26 KB of workspace each, and the keys' copies)
     constexpr Index most = 8192;
@@ -132,7 +134,8 @@ dlk_row_segment aligned_rows(const Tensor& t, Tensor& held, Index tokens, Index 
     if (!(t.device() == states.device())) throw std::invalid_argument(name + ": " + what + " on another device");
     const Index align = t.dtype() == DType::bf16 ? 8 : 4;
     const auto& strides = t.strides();
-    const bool direct = strides[2] == 1 && strides[0] % align == 0 && strides[1] % align == 0 &&
+    // (64 rows lie within 2^32 entries, which a kernel counts in 32 bits)
+    const bool direct = strides[2] == 1 && strides[0] % align == 0 && strides[1] % align == 0 && strides[0] < (1 << 26) &&
                         reinterpret_cast<std::uintptr_t>(t.data<void>()) % 16 == 0 &&
                         TensorAccess::impl(t)->storage != TensorAccess::impl(states)->storage;
     held = t;

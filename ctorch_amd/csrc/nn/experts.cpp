@@ -21,7 +21,8 @@ Mixture expert_mixture(const Tensor& input, const Tensor& router, const Tensor& 
         refuse("expects input [..., d], router [E, d], gate and up [E, F, d], down [E, d, F]; got " + shape_string(input.shape()) + ", " +
                shape_string(router.shape()) + ", " + shape_string(gate.shape()) + ", " + shape_string(up.shape()) + ", " + shape_string(down.shape()));
     if (dim <= 0 || hidden <= 0 || experts <= 0) refuse("d, F and E must be positive");
-    if (experts > DLK_EXPERTS_MOST || dim > INT32_MAX / 16 || hidden > INT32_MAX / 16) refuse("too many experts or entries");
+    // (a launch has fewer than 2^32 threads)
+    if (experts > DLK_EXPERTS_MOST || std::max(dim, hidden) > (1 << 25) / experts) refuse("too many experts or entries");
     if (top <= 0 || top > std::min<Index>(experts, DLK_EXPERTS_TOP_MOST)) refuse("top must be from 1 to the number of experts, and at most 64");
     if (input.dtype() != DType::f32 && input.dtype() != DType::bf16) refuse("input must be f32 or bf16");
     for (const Tensor* t : {&router, &gate, &up, &down})

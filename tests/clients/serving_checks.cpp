@@ -192,6 +192,14 @@ int call(const std::string& name) {
         {"batch read and written", [&] { batch({0, 1}, {1, 2}, {1, 1}); }},
         {"batch read and written before", [&] { batch({1, 0}, {2, 1}, {1, 1}); }},
         {"batch many", [&] { batch({0, 1}, {2, 3}, {1 << 30, 1}); }},
+        {"batch many requests", [&] {
+             const List none(20, -1), counts(20, 1);
+             List targets(20);
+             for (Index i = 0; i < 20; ++i) targets[static_cast<std::size_t>(i)] = i;
+             DeltaBatch(DeltaStates(1, 20, 16384, 32, 256, gpu), 1, none, targets, counts);
+         }},
+        {"states heads", [&] { DeltaStates(1, 1, 16385, 32, 32, gpu); }},
+        {"experts large", [&] { mix(tensor({1, 1}), tensor({1024, 1}), tensor({1024, 32769, 1}), tensor({1024, 32769, 1}), tensor({1024, 1, 32769}), 1); }},
         {"batch many heads", [&] { batch({0}, {2}, {1 << 29}); }},
         {"delta other states", [&] { dl::gated_delta(DeltaStates(2, 6, 4, 32, 32, gpu), 0, step, q, q, v, g, g); }},
         {"delta fewer slots", [&] { dl::gated_delta(DeltaStates(2, 5, 4, 32, 64, gpu), 0, step, q, q, v, g, g); }},

@@ -212,3 +212,24 @@ def test_the_same_call_gives_the_same_bits():
 @pytest.mark.parametrize("weight,inputs", [("bf16", "f32"), ("bf16", "bf16"), ("f32", "bf16"), ("f32", "f32")])
 def test_one_of_the_products_in_pieces(T, d, F, weight, inputs):
     check(T, d, F, 6, 3, weight, inputs)
+
+
+@pytest.mark.parametrize("T,top", [(1001, 8), (8100, 1), (130, 64)])
+def test_more_rows_than_a_launch_takes(T, top):
+    check(T, 64, 32, max(10, top), top, "bf16", "f32")
+
+
+@pytest.mark.parametrize("T", [1, 12, 90])
+@pytest.mark.parametrize("weight,inputs", [("bf16", "f32"), ("bf16", "bf16"), ("f32", "f32")])
+@pytest.mark.parametrize("d,F", [(256, 128), (511, 128), (256, 129)])
+def test_all_bits_of_an_f32_count(T, weight, inputs, d, F):
+    """Roundings of different sums are independent, so that their number adds up by its root: sums of d and of F products are
+    off by sqrt(d + F) u of their size in the mean over many.  A row or hidden entry whose third part of 8 bits is lost is off
+    by 2^-17 in the mean, always to the same side: five times and more of that."""
+    rng = np.random.default_rng(T)
+    arrays = [rng.standard_normal((T, d))] + [rng.standard_normal(s) * s[-1] ** -0.5 for s in ((4, d), (4, F, d), (4, F, d), (4, d, F))]
+    tensors, values = zip(*[give(a, inputs if i == 0 else weight) for i, a in enumerate(arrays)])
+    chosen, weights = route(values[0], values[1], 2, True)
+    want, _ = mixed(values[0], *values[2:], chosen, weights)
+    error = ct.expert_mixture(*tensors, 2)[0].numpy() - want
+    assert np.linalg.norm(error) <= (d + F) ** 0.5 * U * np.linalg.norm(want)

@@ -166,7 +166,8 @@ REFUSED = {
     "batch no key_heads": "multiple of key_heads", "batch empty": "each of its requests", "batch unequal": "each of its requests",
     "batch count": "below zero", "batch target": "slot 6", "batch no target": "slot -1", "batch source": "slot 6",
     "batch source below": "slot -2", "batch written twice": "two requests", "batch read and written": "read by another",
-    "batch read and written before": "read by another", "batch many": "too many", "batch many heads": "too many",
+    "batch read and written before": "read by another", "batch many": "too many", "batch many heads": "too many", "batch many requests": "too many requests", "states heads": "too many",
+    "experts large": "too many experts",
     "delta other states": "another layout", "delta fewer slots": "another layout", "delta layer": "layer out of range",
     "delta layer below": "layer out of range", "delta query": "query must be", "delta key heads": "key must be",
     "delta value": "value must be", "delta type": "f32 or bf16", "delta host": "another device", "delta decay": "decay must be",
