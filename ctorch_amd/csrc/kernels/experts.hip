@@ -645,20 +645,32 @@ template <bool GATE, bool F32, int PARTS, bool LOOSE> void rows_of(const dlk_exp
     const integral_constant<int, 4> four;
     const std::true_type split;
     const std::false_type whole;
-    // fewer than 1024 tiles of 16 rows: the waves share a tile
-    const bool large = static_cast<int64_t>(active) * tiles >= 1024;
     const auto blocks = [&](auto r, auto nt, auto waves) {
         constexpr int R = decltype(r)::value, NT = decltype(nt)::value, WAVES = decltype(waves)::value;
         experts_blocks<GATE, F32, PARTS, R, NT, WAVES, LOOSE><<<dim3((tiles + R * WAVES - 1) / (R * WAVES), p.experts), WAVES * kWave, pairs * 2, at>>>(p, plan);
     };
     const integral_constant<int, 8> eight;
     const integral_constant<int, 6> six;
-    if (!large) launch(one, one, split);
-    // (loads off their alignment take the longer path: 16 rows through 4 of 32 experts of 704 x 2047: 272 us in
-    // tiles of four a wave, 143 here)
-    else if (p.tokens <= 16 && !(LOOSE && pairs >= p.experts)) launch(four, one, whole);
-    else {
-        // rows that the CU with most of them has
+    // What fills the chip: 16 rows of a matrix a work-group whose waves share the sum, until the chosen experts have a tile for each
+    // of 1024 waves, and then as many tiles a wave as leave 1024 waves busy, so that what a wave reads of the rows serves more of
+    // them.  Measured on MI355X, us a call (both products and the rest), bf16 matrices of 2048 x 1024, by what the gates' product takes,
+    // shared / 1 / 2 / 4 tiles a wave: 8 experts (512 tiles) 61 / 67 / 83 / 113; 16 78 / 70 / 85 / 116; 32 117 / 105 / 99 / 129; 64 170 /
+    // 159 / 154 / 149.  f32 matrices take twice the registers and one tile: 32 experts 165 / 161 / 165 / 221.
+    // Through LDS where all experts are read anyway: 16 rows through 4 of 64 experts of 512 x 1024 58 / 55 / 51 / 68, through LDS 51; through
+    // 4 of 32 of 704 x 2048 79 / 87 / 78 / 107 and 67; where many rows share an expert from fewer tiles on: 100 rows through 4 of 16
+    // of 704 x 1024 64 shared, 56 through LDS, 30 rows through 2 of them 37 and 40.  Loads off their alignment take longer, less so
+    // where each is made once (16 rows through 4 of 32 experts of 704 x 2047: 272 with four tiles a wave, 143 through LDS), and
+    // f32 rows are twice as long (8 rows through 8 of 64 experts of 1024 x 2048: 255 and 237).
+    const int64_t all = static_cast<int64_t>(active) * tiles;
+    if (all < (pairs >= 8 * p.experts ? 512 : 1024)) launch(one, one, split);
+    else if (pairs < p.experts || (!LOOSE && !F32 && p.tokens <= 16 && all >= 4096)) {
+        if constexpr (F32) launch(one, one, whole);
+        else if (all < 2048) launch(one, one, whole);
+        else if (all < 4096) launch(two, one, whole);
+        else launch(four, one, whole);
+    } else {
+        // 6, 8 or 16 tiles a work-group, by what the CU with most of them has (48 tiles of each of 32 experts: 102 us a call with 6, 109 and
+        // 142 with the others; 32 of each of 64: 63, 51 and 64; 64 of each of 64: 174, 157 and 148)
         const auto most = [&](int rows) { return (static_cast<int64_t>(p.experts) * ((tiles + rows - 1) / rows) + 255) / 256 * rows; };
         if (most(6) < most(16) && most(6) < most(8)) blocks(one, four, six);
         else if (most(8) < most(16)) blocks(one, four, eight);
