@@ -1,11 +1,14 @@
 // A layer of experts over few rows (see dlk_experts_params in kernels.h): the router in f64, the hidden entries of the chosen
-// experts, their output entries, and the weighted sum.  Bound by memory: a few rows read each chosen expert's matrices once.
+// experts, their output entries, and the weighted sum.  Bound by memory: a few rows read each chosen expert's matrices once.  16 rows
+// through 8 of 64 bf16 experts of 1024 x 2048: router 11 us, hidden entries 87 (5.6 TB/s), outputs 48 (5.0 TB/s), sum 4.7; 200 rows
+// through 4 of 32 of 768 x 2048: 8, 46, 31 and 4.7; one row through 2 of 16 of 704 x 1024: 4.8, 7.0, 4.8 and 2.
 //
 // Products keep all bits of an f32: bf16 matrices go into v_mfma_f32_16x16x32_bf16 as they are, rows as three bf16 parts that
 // hold all 24 bits (bf16 rows are one); f32 matrices and rows go into v_mfma_f32_16x16x4_f32.
 #include "kernels/parts.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace dlk {
 namespace {
@@ -38,6 +41,7 @@ __device__ __forceinline__ void eight(const void* x, int bf16, int64_t at, float
 
 struct Plan {          // what a launch's kernels hand on
     uint16_t* pick;    // [tokens, top]: the chosen experts
+    double* logits;    // [tokens, experts], or NULL: the router's kernel takes them
     char* rows;        // x as the products read it (see `planes` and laid_place), or NULL: p.x itself
     char* act;         // the hidden entries: f32 (`whole`), or three parts
     bool whole, laid;  // laid: in pieces, see laid_place
@@ -53,30 +57,15 @@ __device__ __forceinline__ int laid_place(int i, int width, int unit) {
     return i < whole ? i : whole + i - (width - unit);
 }
 
-// A work-group per row: the logits in f64, which hold products of two f32 exactly, so that rows choose as the exact logits do
-// but for ties within 1e-15 of them; an expert's rank is the number of those that are preferred to it.  On the way the row is
-// laid out for the products.  WIDE: pieces of 8 entries (dim a multiple of 8, 16-byte aligned).
-constexpr int kRoute = 1024, kRouteWaves = kRoute / kWave;
+// A row's logits in f64, which hold products of two f32 exactly, so that rows choose as the exact logits do but for ties within
+// 1e-15 of them: two experts at a time for wave `wave` of `waves`.  Bound by the conversions to f64 and, for few rows, by one way to
+// memory, so all of a wave's loads of 2048 entries are made at once.  WIDE: pieces of 8 entries (dim a multiple of 8, 16-byte aligned).
 template <bool WIDE>
-__global__ __launch_bounds__(kRoute) void experts_route(const dlk_experts_params p, const Plan plan) {
-    __shared__ double logits[DLK_EXPERTS_MOST];
-    __shared__ int slots[DLK_EXPERTS_TOP_MOST];
-    const int64_t token = blockIdx.x;
-    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    if constexpr (WIDE) {
-        if (plan.rows)
-            for (int i = threadIdx.x * 8; i < p.dim; i += kRoute * 8) {
-                float v[8];
-                eight(p.x, p.x_bf16, token * p.dim + i, v);
-                if (plan.planes == 0) {
-                    f32x4* to = reinterpret_cast<f32x4*>(reinterpret_cast<float*>(plan.rows) + token * p.dim + i);
-                    to[0] = f32x4{v[0], v[1], v[2], v[3]}, to[1] = f32x4{v[4], v[5], v[6], v[7]};
-                }
-                for (int part = 0; part < plan.planes; ++part)
-                    *reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(plan.rows) + (part * p.tokens + token) * p.dim + i) = cut(v);
-            }
-        constexpr int N = 4, U = 2; // experts and steps at a time
-        for (int first = wave * N; first < p.experts; first += kRouteWaves * N) {
+__device__ __forceinline__ void take_logits(const dlk_experts_params& p, int64_t token, int wave, int waves, double* logits) {
+    const int lane = threadIdx.x % kWave;
+    for (int first = 2 * wave; first < p.experts; first += 2 * waves) {
+        if constexpr (WIDE) {
+            constexpr int N = 2, U = 4; // experts, and steps at a time
             double sum[N] = {};
             for (int i = lane * 8; i < p.dim; i += U * kWave * 8) {
                 float x[U][8], w[U][N][8];
@@ -95,39 +84,94 @@ __global__ __launch_bounds__(kRoute) void experts_route(const dlk_experts_params
 #pragma unroll
                             for (int j = 0; j < 8; ++j) sum[n] = fma(static_cast<double>(x[u][j]), static_cast<double>(w[u][n][j]), sum[n]);
             }
-            // lanes that differ in the lowest two bits share the four sums out; lane l ends with that of expert l % 4
-            const bool odd = lane & 1, high = lane & 2;
-            double two[2];
+            // lanes that differ in the lowest bit share the two sums out
+            const bool odd = lane & 1;
+            double z = (odd ? sum[1] : sum[0]) + __shfl_xor(odd ? sum[0] : sum[1], 1);
+#pragma unroll
+            for (int d = 2; d < kWave; d *= 2) z += __shfl_xor(z, d);
+            if (lane < N && first + lane < p.experts) logits[first + lane] = z;
+        } else {
+            constexpr int U = 16;
+            double sum[2] = {};
+            const int64_t row[2] = {static_cast<int64_t>(first) * p.dim, static_cast<int64_t>(min(first + 1, p.experts - 1)) * p.dim};
+            const auto entries = [&](auto x_bf16, auto router_bf16) { // (a type looked up at each load would have each waited for)
+                for (int i = lane; i < p.dim; i += U * kWave) {
+                    float x[U], w[U][2];
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        const int at = min(i + u * kWave, p.dim - 1);
+                        x[u] = entry(p.x, x_bf16, token * p.dim + at);
+#pragma unroll
+                        for (int n = 0; n < 2; ++n) w[u][n] = entry(p.router, router_bf16, row[n] + at);
+                    }
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+                        if (i + u * kWave < p.dim)
+#pragma unroll
+                            for (int n = 0; n < 2; ++n) sum[n] = fma(static_cast<double>(x[u]), static_cast<double>(w[u][n]), sum[n]);
+                }
+            };
+            const std::true_type yes;
+            const std::false_type no;
+            if (p.x_bf16) p.router_bf16 ? entries(yes, yes) : entries(yes, no);
+            else p.router_bf16 ? entries(no, yes) : entries(no, no);
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
-                const double give = odd ? sum[2 * n] : sum[2 * n + 1];
-                two[n] = (odd ? sum[2 * n + 1] : sum[2 * n]) + __shfl_xor(give, 1);
+                const double z = wave_sum_f64(sum[n]);
+                if (lane == 0 && first + n < p.experts) logits[first + n] = z;
             }
-            const double give = high ? two[0] : two[1];
-            double z = (high ? two[1] : two[0]) + __shfl_xor(give, 2);
-#pragma unroll
-            for (int d = 4; d < kWave; d *= 2) z += __shfl_xor(z, d);
-            if (lane < N && first + lane < p.experts) logits[first + lane] = z;
+        }
+    }
+}
+
+// A row as the products read it, by `threads` threads.
+template <bool WIDE> __device__ __forceinline__ void lay_row(const dlk_experts_params& p, const Plan& plan, int64_t token, int thread, int threads) {
+    if (!plan.rows) return;
+    if constexpr (WIDE) {
+        for (int i = thread * 8; i < p.dim; i += threads * 8) {
+            float v[8];
+            eight(p.x, p.x_bf16, token * p.dim + i, v);
+            if (plan.planes == 0) {
+                f32x4* to = reinterpret_cast<f32x4*>(reinterpret_cast<float*>(plan.rows) + token * p.dim + i);
+                to[0] = f32x4{v[0], v[1], v[2], v[3]}, to[1] = f32x4{v[4], v[5], v[6], v[7]};
+            }
+            for (int part = 0; part < plan.planes; ++part)
+                *reinterpret_cast<u32x4*>(reinterpret_cast<uint16_t*>(plan.rows) + (part * p.tokens + token) * p.dim + i) = cut(v);
         }
     } else {
-        if (plan.rows) {
-            const int unit = p.weights_bf16 ? 8 : 4, line = laid_width(p.dim, unit), whole = p.dim / unit * unit;
-            for (int i = threadIdx.x; i < line; i += kRoute) {
-                const int from = i < whole ? i : i - whole + p.dim - unit;
-                float v = i < whole || from >= whole ? entry(p.x, p.x_bf16, token * p.dim + from) : 0.0f;
-                if (plan.planes == 0) reinterpret_cast<float*>(plan.rows)[token * line + i] = v;
-                for (int part = 0; part < plan.planes; ++part)
-                    reinterpret_cast<uint16_t*>(plan.rows)[(part * p.tokens + token) * line + i] = cut(v);
-            }
+        const int unit = p.weights_bf16 ? 8 : 4, line = laid_width(p.dim, unit), whole = p.dim / unit * unit;
+        for (int i = thread; i < line; i += threads) {
+            const int from = i < whole ? i : i - whole + p.dim - unit;
+            float v = i < whole || from >= whole ? entry(p.x, p.x_bf16, token * p.dim + from) : 0.0f;
+            if (plan.planes == 0) reinterpret_cast<float*>(plan.rows)[token * line + i] = v;
+            for (int part = 0; part < plan.planes; ++part)
+                reinterpret_cast<uint16_t*>(plan.rows)[(part * p.tokens + token) * line + i] = cut(v);
         }
-        for (int e = wave; e < p.experts; e += kRouteWaves) {
-            double sum = 0.0;
-            for (int i = lane; i < p.dim; i += kWave)
-                sum = fma(static_cast<double>(entry(p.x, p.x_bf16, token * p.dim + i)),
-                          static_cast<double>(entry(p.router, p.router_bf16, static_cast<int64_t>(e) * p.dim + i)), sum);
-            sum = wave_sum_f64(sum);
-            if (lane == 0) logits[e] = sum;
-        }
+    }
+}
+
+// Work-groups that share a row's logits, where one would take long.
+constexpr int kLogits = 256, kLogitsExperts = kLogits / kWave * 2;
+template <bool WIDE>
+__global__ __launch_bounds__(kLogits) void experts_logits(const dlk_experts_params p, const Plan plan) {
+    const int64_t token = blockIdx.y;
+    take_logits<WIDE>(p, token, blockIdx.x * (kLogits / kWave) + threadIdx.x / kWave, gridDim.x * (kLogits / kWave), plan.logits + token * p.experts);
+    lay_row<WIDE>(p, plan, token, blockIdx.x * kLogits + threadIdx.x, gridDim.x * kLogits);
+}
+
+// A work-group per row: an expert's rank is the number of those that are preferred to it.  OWN: it takes the logits by itself.
+constexpr int kRoute = 1024;
+template <bool WIDE, bool OWN>
+__global__ __launch_bounds__(kRoute) void experts_route(const dlk_experts_params p, const Plan plan) {
+    __shared__ double logits[DLK_EXPERTS_MOST];
+    __shared__ int slots[DLK_EXPERTS_TOP_MOST];
+    const int64_t token = blockIdx.x;
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    if constexpr (OWN) {
+        lay_row<WIDE>(p, plan, token, threadIdx.x, kRoute);
+        take_logits<WIDE>(p, token, wave, kRoute / kWave, logits);
+    } else {
+        if (static_cast<int>(threadIdx.x) < p.experts) logits[threadIdx.x] = plan.logits[token * p.experts + threadIdx.x];
     }
     __syncthreads();
     for (int first = 0; first < p.experts; first += kRoute / 16) { // 16 lanes an expert
@@ -601,6 +645,10 @@ __global__ __launch_bounds__(256) void experts_down_any(const dlk_experts_params
 
 bool aligned(const void* at) { return reinterpret_cast<uintptr_t>(at) % 16 == 0; }
 bool wide(const dlk_experts_params& p) { return p.dim % 8 == 0 && aligned(p.x) && aligned(p.router); }
+// A work-group takes a row's logits by itself unless they are many: 16 rows and 64 experts of 2048 entries 13.9 us, by several
+// work-groups 6.7 and 4.7 with the launch behind it (4 rows and 128 experts, the whole call: 102 and 88 us); but 1 row and 16 experts of
+// 1024 4.8, or 3.8 and 2.5, and the small call's 24 us become 27.
+bool shared_logits(const dlk_experts_params& p) { return static_cast<int64_t>(p.experts) * p.dim >= 1 << 17; }
 int64_t up16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
 
 // Each product takes the matrix cores where its rows have a piece of 16 bytes at least, at offsets of 32 bits; loose: where
@@ -608,7 +656,7 @@ int64_t up16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
 struct Layout {
     bool gate, down, loose_gate, loose_down;
     int planes; // of x: parts (bf16 matrices) or 0
-    int64_t rows, act, partial, bytes;
+    int64_t logits, rows, act, partial, bytes;
 };
 Layout layout(const dlk_experts_params& p) {
     Layout l{};
@@ -623,7 +671,8 @@ Layout layout(const dlk_experts_params& p) {
     // (x as it is where its rows are what the products read; else laid out by the router's kernel)
     const bool laid = p.weights_bf16 != p.x_bf16 || p.dim % unit != 0 || !aligned(p.x);
     l.planes = p.weights_bf16 ? (p.x_bf16 ? 1 : 3) : 0;
-    l.rows = up16(pairs * 2); // behind the choice
+    l.logits = up16(pairs * 2); // behind the choice
+    l.rows = l.logits + (shared_logits(p) ? up16(p.tokens * p.experts * 8) : 0);
     l.act = l.rows + (l.gate && laid ? up16(p.tokens * x_line * held) : 0);
     l.partial = l.act + up16(l.down ? pairs * act_line * held : pairs * p.hidden * 4);
     l.bytes = l.partial + (l.down ? pairs * p.dim * 4 : 0);
@@ -659,7 +708,7 @@ template <bool GATE, bool F32, int PARTS, bool LOOSE> void rows_of(const dlk_exp
     // Through LDS where all experts are read anyway: 16 rows through 4 of 64 experts of 512 x 1024 58 / 55 / 51 / 68, through LDS 51; through
     // 4 of 32 of 704 x 2048 79 / 87 / 78 / 107 and 67; where many rows share an expert from fewer tiles on: 100 rows through 4 of 16
     // of 704 x 1024 64 shared, 56 through LDS, 30 rows through 2 of them 37 and 40.  Loads off their alignment take longer, less so
-    // where each is made once (16 rows through 4 of 32 experts of 704 x 2047: 272 with four tiles a wave, 143 through LDS), and
+    // where each is made once (16 rows through 4 of 32 experts of 704 x 2047: 129 us a call more with four tiles a wave than through LDS), and
     // f32 rows are twice as long (8 rows through 8 of 64 experts of 1024 x 2048: 255 and 237).
     const int64_t all = static_cast<int64_t>(active) * tiles;
     if (all < (pairs >= 8 * p.experts ? 512 : 1024)) launch(one, one, split);
@@ -702,11 +751,16 @@ extern "C" int dlk_experts(const dlk_experts_params* p, dlh_stream stream) {
     hipStream_t at = reinterpret_cast<hipStream_t>(stream);
     const Layout l = layout(*p);
     char* space = static_cast<char*>(p->workspace);
-    const Plan plan{reinterpret_cast<uint16_t*>(space), l.act > l.rows ? space + l.rows : nullptr, space + l.act, !l.down || !p->weights_bf16, l.down,
+    const Plan plan{reinterpret_cast<uint16_t*>(space), reinterpret_cast<double*>(space + l.logits), l.act > l.rows ? space + l.rows : nullptr, space + l.act, !l.down || !p->weights_bf16, l.down,
                     reinterpret_cast<float*>(space + l.partial), l.planes};
     const auto tokens = static_cast<unsigned>(p->tokens);
-    if (wide(*p)) experts_route<true><<<tokens, kRoute, 0, at>>>(*p, plan);
-    else experts_route<false><<<tokens, kRoute, 0, at>>>(*p, plan);
+    if (shared_logits(*p)) {
+        const dim3 groups((p->experts + kLogitsExperts - 1) / kLogitsExperts, tokens);
+        if (wide(*p)) experts_logits<true><<<groups, kLogits, 0, at>>>(*p, plan);
+        else experts_logits<false><<<groups, kLogits, 0, at>>>(*p, plan);
+        experts_route<true, false><<<tokens, kRoute, 0, at>>>(*p, plan);
+    } else if (wide(*p)) experts_route<true, true><<<tokens, kRoute, 0, at>>>(*p, plan);
+    else experts_route<false, true><<<tokens, kRoute, 0, at>>>(*p, plan);
     if (!l.gate) {
         const dim3 groups((p->hidden + 3) / 4, p->experts);
         const int list = static_cast<int>(p->tokens) * p->top * 2;
