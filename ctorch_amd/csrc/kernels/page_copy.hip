@@ -1,6 +1,7 @@
 // Copies of pages within pools that share one layout (see dlk_page_copy_params in kernels.h): the keys and values of every
 // layer of a paged cache, or the states of every layer.  Bound by memory: each byte is read and written once, 16 of them a
-// thread's step.  What a launch needs to know comes with its arguments, so that a call copies nothing to the device first
+// thread's step: 229 MB moved in 16 layers' pages of 64 KB 87 us, 5.3 TB/s read and written; 157 MB to four copies of each page
+// 49 us; three copies of 8 rows of a 16 KB page in 16 layers 3.2 us, of a call's 13.  What a launch needs to know comes with its arguments, so that a call copies nothing to the device first
 // and waits for nothing.
 #include "kernels/device_common.h"
 
