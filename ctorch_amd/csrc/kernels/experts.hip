@@ -571,6 +571,53 @@ __global__ __launch_bounds__(WAVES * kWave) void experts_blocks(const dlk_expert
     }
 }
 
+// The outputs of single rows, and their weighted sums with them: a column of a matrix product's sixteen would be all that is used, and
+// its partial sums would need another launch.  A wave has R outputs of a row and goes through the chosen experts' entries 16 bytes of a
+// matrix a lane, all of them side by side.  (f32 hidden entries, which it reads once for R outputs.)
+template <bool F32> __global__ __launch_bounds__(256) void experts_down_single(const dlk_experts_params p, const float* act) {
+    constexpr int N = F32 ? 4 : 8, R = 2, U = 4;
+    const int lane = threadIdx.x % kWave;
+    const int64_t token = blockIdx.y;
+    const int row = __builtin_amdgcn_readfirstlane(static_cast<int>(blockIdx.x * 4 + threadIdx.x / kWave) * R);
+    if (row >= p.dim) return;
+    const int pieces = p.hidden / N, all = p.top * pieces;
+    const char* down = static_cast<const char*>(p.down);
+    float y[R] = {};
+    for (int first = lane; first < all; first += U * kWave) {
+        u32x4 w[U][R];
+        f32x4 a[U][N / 4];
+        float weight[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = min(first + u * kWave, all - 1), j = i / pieces, at = i % pieces;
+            const int64_t pair = token * p.top + j, expert = p.chosen[pair];
+            weight[u] = first + u * kWave < all ? p.weights[pair] : 0.0f;
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+                w[u][r] = *reinterpret_cast<const u32x4*>(down + ((expert * p.dim + min(row + r, p.dim - 1)) * pieces + at) * 16);
+#pragma unroll
+            for (int c = 0; c < N / 4; ++c) a[u][c] = *reinterpret_cast<const f32x4*>(act + pair * p.hidden + at * N + 4 * c);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                float sum = 0.0f;
+#pragma unroll
+                for (int c = 0; c < N; ++c) {
+                    const float v = F32 ? __uint_as_float(w[u][r][c % 4]) : c % 2 ? bf16_hi(w[u][r][c / 2]) : bf16_lo(w[u][r][c / 2]);
+                    sum = fmaf(a[u][c / 4][c % 4], v, sum);
+                }
+                if (first + u * kWave < all) y[r] = fmaf(weight[u], sum, y[r]);
+            }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        y[r] = wave_sum(y[r]);
+        if (lane == 0 && row + r < p.dim) p.y[token * p.dim + row + r] = y[r];
+    }
+}
+
 // The weighted sum of a row's outputs, in the order of its choice.  A thread has N neighbouring entries.
 template <int N> __global__ __launch_bounds__(256) void experts_join(const dlk_experts_params p, const float* partial) {
     struct alignas(4 * N) Entries {
@@ -653,8 +700,16 @@ int64_t up16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
 
 // Each product takes the matrix cores where its rows have a piece of 16 bytes at least, at offsets of 32 bits; loose: where
 // its matrices' rows do not begin at multiples of 16 bytes.
+// Up to 32 rows take their outputs one by one where their experts are others or their matrices stay in the last cache (128 MB, each
+// row's counted): of 8 rows through 2 of 16 experts of 704 x 1024 the call takes 34 us with matrix products and 27 one by one, 1 row
+// through 8 of 64 of 1024 x 2048 41 and 38, 16 rows through 8 of 128 of them 252 and 245, 20 rows through 2 of 8 of 256 x 512 25 and 21; but 16
+// rows through 8 of 64 of 1024 x 2048 (537 MB) 150 and 172, 60 rows through 2 of 16 of 704 x 1024 37 and 45.
+bool single_rows(const dlk_experts_params& p) {
+    const int64_t pairs = p.tokens * p.top, matrix = static_cast<int64_t>(p.dim) * p.hidden * (p.weights_bf16 ? 2 : 4);
+    return p.tokens <= 32 && (pairs <= p.experts || pairs * matrix <= 1 << 27);
+}
 struct Layout {
-    bool gate, down, loose_gate, loose_down;
+    bool gate, down, single, loose_gate, loose_down;
     int planes; // of x: parts (bf16 matrices) or 0
     int64_t logits, rows, act, partial, bytes;
 };
@@ -668,6 +723,8 @@ Layout layout(const dlk_experts_params& p) {
     l.down = fits && p.hidden >= unit;
     l.loose_gate = p.dim % unit != 0 || !aligned(p.gate) || !aligned(p.up);
     l.loose_down = p.hidden % unit != 0 || !aligned(p.down);
+    l.single = l.down && !l.loose_down && single_rows(p);
+    if (l.single) l.down = false;
     // (x as it is where its rows are what the products read; else laid out by the router's kernel)
     const bool laid = p.weights_bf16 != p.x_bf16 || p.dim % unit != 0 || !aligned(p.x);
     l.planes = p.weights_bf16 ? (p.x_bf16 ? 1 : 3) : 0;
@@ -768,6 +825,13 @@ extern "C" int dlk_experts(const dlk_experts_params* p, dlh_stream stream) {
     } else if (!p->weights_bf16) rows_of<true, true, 1>(*p, plan, l.loose_gate, at);
     else if (p->x_bf16) rows_of<true, false, 1>(*p, plan, l.loose_gate, at);
     else rows_of<true, false, 3>(*p, plan, l.loose_gate, at);
+    if (l.single) {
+        const dim3 groups((p->dim + 7) / 8, tokens);
+        const float* act = reinterpret_cast<const float*>(plan.act);
+        if (p->weights_bf16) experts_down_single<false><<<groups, 256, 0, at>>>(*p, act);
+        else experts_down_single<true><<<groups, 256, 0, at>>>(*p, act);
+        return hipGetLastError();
+    }
     if (!l.down) {
         const int64_t waves = p->tokens * p->dim;
         experts_down_any<<<static_cast<unsigned>(std::min<int64_t>(waves / 4 + 1, 16384)), 256, 0, at>>>(*p, reinterpret_cast<const float*>(plan.act));

@@ -102,13 +102,20 @@ def test_many_experts(E, top):
 
 
 @pytest.mark.parametrize("T,E,top,narrow,long", [(4, 64, 4, 32, 1032), (8, 64, 4, 40, 1064), (8, 128, 8, 24, 1040), (16, 64, 4, 32, 1040),
-                                                 (64, 16, 2, 72, 520), (4, 64, 4, 39, 1031), (8, 64, 4, 41, 1063), (16, 64, 4, 33, 1039)])
+                                                 (64, 16, 2, 72, 520), (34, 64, 1, 32, 520), (40, 64, 1, 32, 1040), (60, 64, 1, 24, 1104),
+                                                 (4, 64, 4, 39, 1031), (8, 64, 4, 41, 1063), (16, 64, 4, 33, 1039)])
 @pytest.mark.parametrize("weight", ["f32", "bf16"])
 @pytest.mark.parametrize("inputs", ["f32", "bf16"])
 def test_long_matrices_of_few_and_of_many_experts(T, E, top, narrow, long, weight, inputs):
     """Each product with 512 to 4200 tiles of 16 rows, by itself: as many go to a wave as leave waves enough."""
     check(T, narrow, long, E, top, weight, inputs)
     check(T, long, narrow, E, top, weight, inputs, seed=1)
+
+
+@pytest.mark.parametrize("weight", ["f32", "bf16"])
+def test_many_pairs_of_few_rows(weight):
+    check(16, 1024, 72, 64, 64, weight)
+    check(32, 256, 24, 32, 32, weight)
 
 
 @pytest.mark.parametrize("T,E,long", [(20, 64, 16400), (40, 64, 32776), (60, 64, 65544)])
