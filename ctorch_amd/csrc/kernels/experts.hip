@@ -1,7 +1,7 @@
 // A layer of experts over few rows (see dlk_experts_params in kernels.h): the router in f64, the hidden entries of the chosen
 // experts, their output entries, and the weighted sum.  Bound by memory: a few rows read each chosen expert's matrices once.  16 rows
 // through 8 of 64 bf16 experts of 1024 x 2048: router 11 us, hidden entries 87 (5.6 TB/s), outputs 48 (5.0 TB/s), sum 4.7; 200 rows
-// through 4 of 32 of 768 x 2048: 8, 46, 31 and 4.7; one row through 2 of 16 of 704 x 1024: 4.8, 7.0, 4.8 and 2.
+// through 4 of 32 of 768 x 2048: 8, 46, 31 and 4.7; one row through 2 of 16 of 704 x 1024: 4.5, 4.2, and 3.7 for outputs and sum.
 //
 // Products keep all bits of an f32: bf16 matrices go into v_mfma_f32_16x16x32_bf16 as they are, rows as three bf16 parts that
 // hold all 24 bits (bf16 rows are one); f32 matrices and rows go into v_mfma_f32_16x16x4_f32.
@@ -571,9 +571,73 @@ __global__ __launch_bounds__(WAVES * kWave) void experts_blocks(const dlk_expert
     }
 }
 
+// The hidden entries of single rows (see below): a wave has R of a pair's, and reads their rows of both matrices side by side, x from
+// where it lies.  1 row through 8 of 64 bf16 experts of 1024 x 2048: 13.1 us, 5.1 TB/s, where matrix products took 19.8.
+template <bool F32, bool X_BF16> __global__ __launch_bounds__(256) void experts_hidden_single(const dlk_experts_params p, const Plan plan) {
+    constexpr int N = F32 ? 4 : 8, R = 2, U = 4;
+    const int lane = threadIdx.x % kWave, pair = blockIdx.y;
+    const int row = __builtin_amdgcn_readfirstlane(static_cast<int>(blockIdx.x * 4 + threadIdx.x / kWave) * R);
+    if (row >= p.hidden) return;
+    const int pieces = p.dim / N;
+    const char* x = static_cast<const char*>(p.x) + static_cast<int64_t>(pair / p.top) * p.dim * (X_BF16 ? 2 : 4);
+    const int64_t matrix = static_cast<int64_t>(plan.pick[pair]) * p.hidden;
+    const u32x4* from[2][R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int64_t at = (matrix + min(row + r, p.hidden - 1)) * pieces;
+        from[0][r] = static_cast<const u32x4*>(p.gate) + at;
+        from[1][r] = static_cast<const u32x4*>(p.up) + at;
+    }
+    float sum[2][R] = {};
+    for (int first = lane; first < pieces; first += U * kWave) {
+        u32x4 w[U][2][R];
+        uint32_t held[U][X_BF16 ? N / 2 : N];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = min(first + u * kWave, pieces - 1);
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int r = 0; r < R; ++r) w[u][m][r] = from[m][r][i];
+            if constexpr (X_BF16 && F32) {
+                const u32x2 a = reinterpret_cast<const u32x2*>(x)[i];
+                held[u][0] = a.x, held[u][1] = a.y;
+            } else {
+                constexpr int WORDS = X_BF16 ? N / 2 : N;
+#pragma unroll
+                for (int c = 0; c < WORDS / 4; ++c) {
+                    const u32x4 a = reinterpret_cast<const u32x4*>(x)[i * (WORDS / 4) + c];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) held[u][4 * c + j] = a[j];
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (first + u * kWave < pieces)
+#pragma unroll
+                for (int c = 0; c < N; ++c) {
+                    const float a = !X_BF16 ? __uint_as_float(held[u][c]) : c % 2 ? bf16_hi(held[u][c / 2]) : bf16_lo(held[u][c / 2]);
+#pragma unroll
+                    for (int m = 0; m < 2; ++m)
+#pragma unroll
+                        for (int r = 0; r < R; ++r) {
+                            const u32x4 v = w[u][m][r];
+                            sum[m][r] = fmaf(a, F32 ? __uint_as_float(v[c % 4]) : c % 2 ? bf16_hi(v[c / 2]) : bf16_lo(v[c / 2]), sum[m][r]);
+                        }
+                }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const float gate = wave_sum(sum[0][r]), up = wave_sum(sum[1][r]);
+        if (lane == 0 && row + r < p.hidden) keep<true>(p, plan, pair, row + r, gate, up);
+    }
+}
+
 // The outputs of single rows, and their weighted sums with them: a column of a matrix product's sixteen would be all that is used, and
 // its partial sums would need another launch.  A wave has R outputs of a row and goes through the chosen experts' entries 16 bytes of a
-// matrix a lane, all of them side by side.  (f32 hidden entries, which it reads once for R outputs.)
+// matrix a lane, all of them side by side.  (f32 hidden entries, which it reads once for R outputs.)  1 row through 8 of 64 bf16 experts
+// of 1024 x 2048: 10.6 us, 3.2 TB/s.
 template <bool F32> __global__ __launch_bounds__(256) void experts_down_single(const dlk_experts_params p, const float* act) {
     constexpr int N = F32 ? 4 : 8, R = 2, U = 4;
     const int lane = threadIdx.x % kWave;
@@ -700,16 +764,17 @@ int64_t up16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
 
 // Each product takes the matrix cores where its rows have a piece of 16 bytes at least, at offsets of 32 bits; loose: where
 // its matrices' rows do not begin at multiples of 16 bytes.
-// Up to 32 rows take their outputs one by one where their experts are others or their matrices stay in the last cache (128 MB, each
-// row's counted): of 8 rows through 2 of 16 experts of 704 x 1024 the call takes 34 us with matrix products and 27 one by one, 1 row
-// through 8 of 64 of 1024 x 2048 41 and 38, 16 rows through 8 of 128 of them 252 and 245, 20 rows through 2 of 8 of 256 x 512 25 and 21; but 16
-// rows through 8 of 64 of 1024 x 2048 (537 MB) 150 and 172, 60 rows through 2 of 16 of 704 x 1024 37 and 45.
-bool single_rows(const dlk_experts_params& p) {
-    const int64_t pairs = p.tokens * p.top, matrix = static_cast<int64_t>(p.dim) * p.hidden * (p.weights_bf16 ? 2 : 4);
-    return p.tokens <= 32 && (pairs <= p.experts || pairs * matrix <= 1 << 27);
+// Up to 32 rows go one by one through a product where their experts are others or its matrices stay in the last cache (128 MB, each
+// row's counted).  Measured on MI355X, us a call with matrix products / outputs one by one / both: 1 row through 8 of 64 experts of 1024 x
+// 2048 41 / 38 / 32, 4 rows 79 / 73 / 69, 16 rows through 8 of 128 of them 252 / 244 / 242, 4 rows through 4 of 16 of 704 x 1024 34 / 28 / 21, 8
+// rows through 2 of them 34 / 27 / 22, 20 rows through 2 of 8 of 256 x 512 25 / 21 / 21; but 4 rows through 8 of 8 of 1024 x 2048 41 / 38 / 53,
+// 16 rows through 8 of 64 of them (537 MB) 150 / 172, 60 rows through 2 of 16 of 704 x 1024 37 / 45.
+bool single_rows(const dlk_experts_params& p, int matrices) {
+    const int64_t pairs = p.tokens * p.top, bytes = static_cast<int64_t>(p.dim) * p.hidden * (p.weights_bf16 ? 2 : 4) * matrices;
+    return p.tokens <= 32 && (pairs <= p.experts || pairs * bytes <= 1 << 27);
 }
 struct Layout {
-    bool gate, down, single, loose_gate, loose_down;
+    bool gate, down, single_gate, single, loose_gate, loose_down;
     int planes; // of x: parts (bf16 matrices) or 0
     int64_t logits, rows, act, partial, bytes;
 };
@@ -723,10 +788,11 @@ Layout layout(const dlk_experts_params& p) {
     l.down = fits && p.hidden >= unit;
     l.loose_gate = p.dim % unit != 0 || !aligned(p.gate) || !aligned(p.up);
     l.loose_down = p.hidden % unit != 0 || !aligned(p.down);
-    l.single = l.down && !l.loose_down && single_rows(p);
+    l.single = l.down && !l.loose_down && single_rows(p, 1);
     if (l.single) l.down = false;
     // (x as it is where its rows are what the products read; else laid out by the router's kernel)
-    const bool laid = p.weights_bf16 != p.x_bf16 || p.dim % unit != 0 || !aligned(p.x);
+    l.single_gate = l.gate && !l.loose_gate && aligned(p.x) && single_rows(p, 2);
+    const bool laid = !l.single_gate && (p.weights_bf16 != p.x_bf16 || p.dim % unit != 0 || !aligned(p.x));
     l.planes = p.weights_bf16 ? (p.x_bf16 ? 1 : 3) : 0;
     l.logits = up16(pairs * 2); // behind the choice
     l.rows = l.logits + (shared_logits(p) ? up16(p.tokens * p.experts * 8) : 0);
@@ -818,7 +884,16 @@ extern "C" int dlk_experts(const dlk_experts_params* p, dlh_stream stream) {
         experts_route<true, false><<<tokens, kRoute, 0, at>>>(*p, plan);
     } else if (wide(*p)) experts_route<true, true><<<tokens, kRoute, 0, at>>>(*p, plan);
     else experts_route<false, true><<<tokens, kRoute, 0, at>>>(*p, plan);
-    if (!l.gate) {
+    if (l.single_gate) {
+        const dim3 groups((p->hidden + 7) / 8, tokens * p->top);
+        if (p->weights_bf16) {
+            if (p->x_bf16) experts_hidden_single<false, true><<<groups, 256, 0, at>>>(*p, plan);
+            else experts_hidden_single<false, false><<<groups, 256, 0, at>>>(*p, plan);
+        } else {
+            if (p->x_bf16) experts_hidden_single<true, true><<<groups, 256, 0, at>>>(*p, plan);
+            else experts_hidden_single<true, false><<<groups, 256, 0, at>>>(*p, plan);
+        }
+    } else if (!l.gate) {
         const dim3 groups((p->hidden + 3) / 4, p->experts);
         const int list = static_cast<int>(p->tokens) * p->top * 2;
         experts_hidden_any<<<groups, 256, list, at>>>(*p, plan);
