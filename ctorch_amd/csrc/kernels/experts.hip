@@ -573,40 +573,43 @@ __global__ __launch_bounds__(WAVES * kWave) void experts_blocks(const dlk_expert
 
 // The hidden entries of single rows (see below): a wave has R of a pair's, and reads their rows of both matrices side by side, x from
 // where it lies.  1 row through 8 of 64 bf16 experts of 1024 x 2048: 13.1 us, 5.1 TB/s, where matrix products took 19.8.
-template <bool F32, bool X_BF16> __global__ __launch_bounds__(256) void experts_hidden_single(const dlk_experts_params p, const Plan plan) {
+template <bool F32, bool X_BF16, bool LOOSE> __global__ __launch_bounds__(256) void experts_hidden_single(const dlk_experts_params p, const Plan plan) {
     constexpr int N = F32 ? 4 : 8, R = 2, U = 4;
     const int lane = threadIdx.x % kWave, pair = blockIdx.y;
     const int row = __builtin_amdgcn_readfirstlane(static_cast<int>(blockIdx.x * 4 + threadIdx.x / kWave) * R);
     if (row >= p.hidden) return;
-    const int pieces = p.dim / N;
-    const char* x = static_cast<const char*>(p.x) + static_cast<int64_t>(pair / p.top) * p.dim * (X_BF16 ? 2 : 4);
+    const int pieces = LOOSE ? (p.dim + N - 1) / N : p.dim / N;
+    constexpr int SIZE = F32 ? 4 : 2, X_SIZE = X_BF16 ? 2 : 4, WORDS = X_BF16 ? N / 2 : N;
+    const char* x = static_cast<const char*>(p.x) + static_cast<int64_t>(pair / p.top) * p.dim * X_SIZE;
     const int64_t matrix = static_cast<int64_t>(plan.pick[pair]) * p.hidden;
-    const u32x4* from[2][R];
+    const char* from[2][R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        const int64_t at = (matrix + min(row + r, p.hidden - 1)) * pieces;
-        from[0][r] = static_cast<const u32x4*>(p.gate) + at;
-        from[1][r] = static_cast<const u32x4*>(p.up) + at;
+        const int64_t at = (matrix + min(row + r, p.hidden - 1)) * p.dim * SIZE;
+        from[0][r] = static_cast<const char*>(p.gate) + at;
+        from[1][r] = static_cast<const char*>(p.up) + at;
     }
+    const auto four = [](const char* at) { return LOOSE ? load_loose(at) : *reinterpret_cast<const u32x4*>(at); };
     float sum[2][R] = {};
     for (int first = lane; first < pieces; first += U * kWave) {
         u32x4 w[U][2][R];
-        uint32_t held[U][X_BF16 ? N / 2 : N];
+        uint32_t held[U][WORDS];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int i = min(first + u * kWave, pieces - 1);
+            const int i = min(first + u * kWave, pieces - 1), at = LOOSE ? min(i * N, p.dim - N) : i * N;
 #pragma unroll
             for (int m = 0; m < 2; ++m)
 #pragma unroll
-                for (int r = 0; r < R; ++r) w[u][m][r] = from[m][r][i];
-            if constexpr (X_BF16 && F32) {
-                const u32x2 a = reinterpret_cast<const u32x2*>(x)[i];
+                for (int r = 0; r < R; ++r) w[u][m][r] = four(from[m][r] + at * SIZE);
+            if constexpr (WORDS == 2) {
+                typedef u32x2 __attribute__((aligned(2))) Loose;
+                const char* own = x + at * X_SIZE;
+                const u32x2 a = LOOSE ? *reinterpret_cast<const Loose*>(own) : *reinterpret_cast<const u32x2*>(own);
                 held[u][0] = a.x, held[u][1] = a.y;
             } else {
-                constexpr int WORDS = X_BF16 ? N / 2 : N;
 #pragma unroll
                 for (int c = 0; c < WORDS / 4; ++c) {
-                    const u32x4 a = reinterpret_cast<const u32x4*>(x)[i * (WORDS / 4) + c];
+                    const u32x4 a = four(x + at * X_SIZE + 16 * c);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) held[u][4 * c + j] = a[j];
                 }
@@ -617,7 +620,8 @@ template <bool F32, bool X_BF16> __global__ __launch_bounds__(256) void experts_
             if (first + u * kWave < pieces)
 #pragma unroll
                 for (int c = 0; c < N; ++c) {
-                    const float a = !X_BF16 ? __uint_as_float(held[u][c]) : c % 2 ? bf16_hi(held[u][c / 2]) : bf16_lo(held[u][c / 2]);
+                    float a = !X_BF16 ? __uint_as_float(held[u][c]) : c % 2 ? bf16_hi(held[u][c / 2]) : bf16_lo(held[u][c / 2]);
+                    if (LOOSE && c < (first + u * kWave + 1) * N - p.dim) a = 0.0f; // (the last piece holds what the one before it does)
 #pragma unroll
                     for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -791,7 +795,7 @@ Layout layout(const dlk_experts_params& p) {
     l.single = l.down && !l.loose_down && single_rows(p, 1);
     if (l.single) l.down = false;
     // (x as it is where its rows are what the products read; else laid out by the router's kernel)
-    l.single_gate = l.gate && !l.loose_gate && aligned(p.x) && single_rows(p, 2);
+    l.single_gate = l.gate && single_rows(p, 2);
     const bool laid = !l.single_gate && (p.weights_bf16 != p.x_bf16 || p.dim % unit != 0 || !aligned(p.x));
     l.planes = p.weights_bf16 ? (p.x_bf16 ? 1 : 3) : 0;
     l.logits = up16(pairs * 2); // behind the choice
@@ -885,14 +889,15 @@ extern "C" int dlk_experts(const dlk_experts_params* p, dlh_stream stream) {
     } else if (wide(*p)) experts_route<true, true><<<tokens, kRoute, 0, at>>>(*p, plan);
     else experts_route<false, true><<<tokens, kRoute, 0, at>>>(*p, plan);
     if (l.single_gate) {
-        const dim3 groups((p->hidden + 7) / 8, tokens * p->top);
-        if (p->weights_bf16) {
-            if (p->x_bf16) experts_hidden_single<false, true><<<groups, 256, 0, at>>>(*p, plan);
-            else experts_hidden_single<false, false><<<groups, 256, 0, at>>>(*p, plan);
-        } else {
-            if (p->x_bf16) experts_hidden_single<true, true><<<groups, 256, 0, at>>>(*p, plan);
-            else experts_hidden_single<true, false><<<groups, 256, 0, at>>>(*p, plan);
-        }
+        const auto launch = [&](auto f32, auto x_bf16) {
+            const dim3 groups((p->hidden + 7) / 8, tokens * p->top);
+            if (l.loose_gate || !aligned(p->x)) experts_hidden_single<f32.value, x_bf16.value, true><<<groups, 256, 0, at>>>(*p, plan);
+            else experts_hidden_single<f32.value, x_bf16.value, false><<<groups, 256, 0, at>>>(*p, plan);
+        };
+        const std::true_type yes;
+        const std::false_type no;
+        if (p->weights_bf16) p->x_bf16 ? launch(no, yes) : launch(no, no);
+        else p->x_bf16 ? launch(yes, yes) : launch(yes, no);
     } else if (!l.gate) {
         const dim3 groups((p->hidden + 3) / 4, p->experts);
         const int list = static_cast<int>(p->tokens) * p->top * 2;
