@@ -768,13 +768,18 @@ int64_t up16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
 
 // Each product takes the matrix cores where its rows have a piece of 16 bytes at least, at offsets of 32 bits; loose: where
 // its matrices' rows do not begin at multiples of 16 bytes.
-// Up to 32 rows go one by one through a product where their experts are others or its matrices stay in the last cache (128 MB, each
+// Few rows go one by one through a product where their experts are others or its matrices stay in the last cache (128 MB, each
 // row's counted).  Measured on MI355X, us a call with matrix products / outputs one by one / both: 1 row through 8 of 64 experts of 1024 x
 // 2048 41 / 38 / 32, 4 rows 79 / 73 / 69, 16 rows through 8 of 128 of them 252 / 244 / 242, 4 rows through 4 of 16 of 704 x 1024 34 / 28 / 21, 8
 // rows through 2 of them 34 / 27 / 22, 20 rows through 2 of 8 of 256 x 512 25 / 21 / 21; but 4 rows through 8 of 8 of 1024 x 2048 41 / 38 / 53,
-// 16 rows through 8 of 64 of them (537 MB) 150 / 172, 60 rows through 2 of 16 of 704 x 1024 37 / 45.
-bool single_rows(const dlk_experts_params& p, int matrices) {
+// 16 rows through 8 of 64 of them (537 MB) 150 / 172, 60 rows through 2 of 16 of 704 x 1024 37 / 45.  Of bf16 matrices off their alignment
+// a wave's 1024 bytes in a row take one line more, the matrix products' 8 rows of 128 bytes eight: 16 rows through 8 of 64 of 1024 x 2047
+// 289 / 227 (first the hidden entries with matrix products, then one by one), 16 rows through 4 of 32 of 704 x 2047 124 / 76, 64 rows through
+// 2 of 64 of 1024 x 2047 290 / 222, 8 rows through 8 of 8 of them 114 / 87; but 32 rows through 8 of 64 295 / 371, 64 rows through 2 of 32 of 704 x
+// 1023 75 / 87.
+bool single_rows(const dlk_experts_params& p, int matrices, bool loose) {
     const int64_t pairs = p.tokens * p.top, bytes = static_cast<int64_t>(p.dim) * p.hidden * (p.weights_bf16 ? 2 : 4) * matrices;
+    if (loose && p.weights_bf16) return (p.tokens <= 64 && pairs <= 2 * p.experts) || (p.tokens <= 32 && pairs * bytes <= 1 << 29);
     return p.tokens <= 32 && (pairs <= p.experts || pairs * bytes <= 1 << 27);
 }
 struct Layout {
@@ -792,10 +797,10 @@ Layout layout(const dlk_experts_params& p) {
     l.down = fits && p.hidden >= unit;
     l.loose_gate = p.dim % unit != 0 || !aligned(p.gate) || !aligned(p.up);
     l.loose_down = p.hidden % unit != 0 || !aligned(p.down);
-    l.single = l.down && !l.loose_down && single_rows(p, 1);
+    l.single = l.down && !l.loose_down && single_rows(p, 1, false);
     if (l.single) l.down = false;
     // (x as it is where its rows are what the products read; else laid out by the router's kernel)
-    l.single_gate = l.gate && single_rows(p, 2);
+    l.single_gate = l.gate && single_rows(p, 2, l.loose_gate);
     const bool laid = !l.single_gate && (p.weights_bf16 != p.x_bf16 || p.dim % unit != 0 || !aligned(p.x));
     l.planes = p.weights_bf16 ? (p.x_bf16 ? 1 : 3) : 0;
     l.logits = up16(pairs * 2); // behind the choice

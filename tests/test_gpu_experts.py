@@ -118,6 +118,13 @@ def test_many_pairs_of_few_rows(weight):
     check(32, 256, 24, 32, 32, weight)
 
 
+@pytest.mark.parametrize("T,d,F,E,top", [(40, 65, 40, 32, 1), (64, 127, 33, 64, 2), (65, 127, 33, 64, 2), (33, 63, 64, 8, 8), (32, 2047, 24, 8, 3)])
+@pytest.mark.parametrize("weight", ["f32", "bf16"])
+@pytest.mark.parametrize("inputs", ["f32", "bf16"])
+def test_odd_rows_one_by_one_and_together(T, d, F, E, top, weight, inputs):
+    check(T, d, F, E, top, weight, inputs)
+
+
 @pytest.mark.parametrize("T,E,long", [(20, 64, 16400), (40, 64, 32776), (60, 64, 65544)])
 def test_more_rows_than_a_tile_through_one_of_many_experts(T, E, long):
     def change(a):
