@@ -311,3 +311,21 @@ def test_rows_of_one_head_for_all_tokens():
         views.append(ct.Tensor(ct._new(ct.lib().dl_reshape, part.handle, ct._shape(x.shape))))
         at += x.shape[1] * 32
     assert np.array_equal(ct.gated_delta(states, 0, batch, *views, *tensors[3:]).numpy(), want)
+
+
+def test_states_beyond_4_gib():
+    """The same tokens through the last slots of a large pool and through a small one, bit for bit."""
+    h, d, results = 32, 128, []
+    rng = np.random.default_rng(3)
+    steps = [(n, [give(x)[0] for x in draw(rng, n, 16, h, d, d)]) for n in (1, 100, 1, 100)]
+    for slots in (3, 2200):
+        say(f"case: delta {slots} slots of {h} x {d} x {d}")
+        states, last = ct.DeltaStates(1, slots, h, d, d), slots - 1
+        run = lambda i, source, target: ct.gated_delta(states, 0, ct.DeltaBatch(states, 16, [source], [target], [steps[i][0]]), *steps[i][1]).numpy()
+        out = [run(0, -1, last), run(1, last, last - 1)]
+        states.copy([last - 1], [last])
+        out += [run(2, last, 0), run(3, last, last)]
+        states.copy([last], [0])
+        results.append(out + [run(0, 0, 1)])
+    for small, large in zip(*results):
+        assert np.array_equal(small, large)
