@@ -5,6 +5,7 @@
 //
 // Products keep all bits of an f32: bf16 matrices go into v_mfma_f32_16x16x32_bf16 as they are, rows as three bf16 parts that
 // hold all 24 bits (bf16 rows are one); f32 matrices and rows go into v_mfma_f32_16x16x4_f32.
+#include "kernels/experts_layout.h"
 #include "kernels/parts.h"
 
 #include <algorithm>
@@ -42,20 +43,12 @@ __device__ __forceinline__ void eight(const void* x, int bf16, int64_t at, float
 struct Plan {          // what a launch's kernels hand on
     uint16_t* pick;    // [tokens, top]: the chosen experts
     double* logits;    // [tokens, experts], or NULL: the router's kernel takes them
-    char* rows;        // x as the products read it (see `planes` and laid_place), or NULL: p.x itself
+    char* rows;        // x as the products read it (see `planes` and experts_layout.h), or NULL: p.x itself
     char* act;         // the hidden entries: f32 (`whole`), or three parts
-    bool whole, laid;  // laid: in pieces, see laid_place
+    bool whole, laid;  // laid: in pieces, see experts_layout.h
     float* partial;    // [tokens, top, dim]: outputs of each pair
     int planes;        // bf16 matrices: parts of a row of x; 0: f32 matrices, f32 rows
 };
-
-// Rows of a width that is no multiple of a piece's U entries (8 of bf16, 4 of f32), as the products read them: whole pieces, and then
-// the row's last U entries, of which those that a piece holds already are zeros.  (The matrices' last piece is read so too.)
-__host__ __device__ __forceinline__ int laid_width(int width, int unit) { return (width + unit - 1) / unit * unit; }
-__device__ __forceinline__ int laid_place(int i, int width, int unit) {
-    const int whole = width / unit * unit;
-    return i < whole ? i : whole + i - (width - unit);
-}
 
 // A row's logits in f64, which hold products of two f32 exactly, so that rows choose as the exact logits do but for ties within
 // 1e-15 of them: two experts at a time for wave `wave` of `waves`.  Bound by the conversions to f64 and, for few rows, by one way to
@@ -250,16 +243,16 @@ __device__ __forceinline__ void keep(const dlk_experts_params& p, const Plan& pl
     else {
         const int unit = p.weights_bf16 ? 8 : 4;
         const bool laid = plan.laid;
-        const int64_t line = laid ? laid_width(p.hidden, unit) : p.hidden, from = pair * line;
+        const int64_t line = hidden_line(p.hidden, unit, laid), from = pair * line;
         const auto put = [&](int at, float x) {
             if (plan.whole) reinterpret_cast<float*>(plan.act)[from + at] = x;
             else
 #pragma unroll
                 for (int part = 0; part < 3; ++part) reinterpret_cast<uint16_t*>(plan.act)[part * p.tokens * p.top * line + from + at] = cut(x);
         };
-        put(laid ? laid_place(row, p.hidden, unit) : row, v / (1.0f + expf(-v)) * up);
-        const int whole = p.hidden / unit * unit;
-        if (line > whole && row >= p.hidden - unit && row < whole) put(whole + row - (p.hidden - unit), 0.0f);
+        put(hidden_place(row, p.hidden, unit, laid), v / (1.0f + expf(-v)) * up);
+        const int zero = hidden_zero(row, p.hidden, unit, laid);
+        if (zero >= 0) put(zero, 0.0f);
     }
 }
 

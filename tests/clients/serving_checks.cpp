@@ -8,6 +8,7 @@
 //       checked against the copy from the pools as they were
 //   serving_checks fork PAGES PAGE WIDTH TABLES LENGTHS PARENTS      the tables of the new requests, then the holders of each page
 //   serving_checks compact PAGES PAGE TABLES                         the tables, the pages moved
+//   serving_checks hidden ENTRIES UNIT LAID      the room of a pair's hidden entries; each one's place, and what is zeroed with it
 //   serving_checks call CASE    an operator called with arguments that it refuses (its error), or with nothing to do (launches)
 #define main host_checks_main
 #include "host_checks.cpp"
@@ -15,6 +16,7 @@
 
 #include "dl/delta.h"
 #include "dl/paged.h"
+#include "kernels/experts_layout.h"
 #include "nn/ops_internal.h"
 
 #include <functional>
@@ -96,6 +98,20 @@ int compact(char** arg) {
     const Index moved = dl::paged_compact(cache_of(pages, page), pool, tables);
     print(tables);
     print({moved});
+    return 0;
+}
+
+int hidden(char** arg) {
+    const int entries = std::atoi(arg[0]), unit = std::atoi(arg[1]);
+    const bool laid = std::atoi(arg[2]) != 0;
+    List places, zeros;
+    for (int i = 0; i < entries; ++i) {
+        places.push_back(dlk::hidden_place(i, entries, unit, laid));
+        zeros.push_back(dlk::hidden_zero(i, entries, unit, laid));
+    }
+    print({dlk::hidden_line(entries, unit, laid)});
+    print(places);
+    print(zeros);
     return 0;
 }
 
@@ -273,6 +289,7 @@ int main(int argc, char** argv) {
         if (argc == 10 && std::strcmp(argv[1], "copy") == 0) return copy(argv + 2);
         if (argc == 8 && std::strcmp(argv[1], "fork") == 0) return fork(argv + 2);
         if (argc == 5 && std::strcmp(argv[1], "compact") == 0) return compact(argv + 2);
+        if (argc == 5 && std::strcmp(argv[1], "hidden") == 0) return hidden(argv + 2);
         if (argc == 3 && std::strcmp(argv[1], "call") == 0) return call(argv[2]);
     } catch (const std::exception& error) {
         std::fprintf(stderr, "%s\n", error.what());

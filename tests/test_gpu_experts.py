@@ -9,7 +9,7 @@ import pytest
 
 import ctorch_amd as ct
 import oracle
-from common import say
+from common import say, write
 
 pytestmark = pytest.mark.gpu
 GPU = ct.device("gpu")
@@ -266,3 +266,39 @@ def test_all_bits_of_an_f32_count(T, weight, inputs, d, F):
     want, _ = mixed(values[0], *values[2:], chosen, weights)
     error = ct.expert_mixture(*tensors, 2)[0].numpy() - want
     assert np.linalg.norm(error) <= (d + F) ** 0.5 * U * np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("weight,F", [("bf16", (1 << 24) + 1), ("bf16", (1 << 24) + 15), ("f32", (1 << 23) + 1), ("f32", (1 << 23) + 3)])
+@pytest.mark.parametrize("T", [1, 3, 12])
+def test_matrices_beyond_2_gib(weight, F, T):
+    """Zero but for the hidden entries at both ends: what a row's last ones write must not reach its own or the next row's first.
+    (A zero adds nothing to a sum, whose tolerance counts the others.)"""
+    d, ends = 64, [8, 17]
+    say(f"case: experts T={T} d={d} F={F} {weight}")
+    rng = np.random.default_rng(T)
+    n = sum(ends)
+    x, rows = give(rng.standard_normal((T, d)))
+    router, _ = give(np.ones((1, d)), weight)
+    coded = lambda a: oracle.bf16_encode(np.ascontiguousarray(a, np.float32)) if weight == "bf16" else np.ascontiguousarray(a, np.float32)  # noqa: E731
+    gate, up, down = (rng.standard_normal(s) * s[-1] ** -0.5 for s in ((n, d), (n, d), (d, n)))
+    values = [give(a, weight)[1][None] for a in (gate, up, down)]
+
+    def flat(shape):
+        whole = ct.zeros(shape, TYPES[weight])
+        return whole, ct.Tensor(ct._new(ct.lib().dl_reshape, whole.handle, ct._shape((F * d,))))
+
+    matrices = []
+    for a in (gate, up):
+        whole, line = flat((1, F, d))
+        write(ct.narrow(line, 0, 0, ends[0] * d), coded(a[:ends[0]]).ravel())
+        write(ct.narrow(line, 0, (F - ends[1]) * d, ends[1] * d), coded(a[ends[0]:]).ravel())
+        matrices.append(whole)
+    whole, line = flat((1, d, F))
+    for i in range(d):
+        write(ct.narrow(line, 0, i * F, ends[0]), coded(down[i, :ends[0]]))
+        write(ct.narrow(line, 0, (i + 1) * F - ends[1], ends[1]), coded(down[i, ends[0]:]))
+    matrices.append(whole)
+    y, chosen, weights = (t.numpy() for t in ct.expert_mixture(x, router, *matrices, 1))
+    assert not chosen.any() and np.all(weights == 1.0)
+    want, tolerance = mixed(rows, *values, chosen, weights.astype(np.float64))
+    assert np.all(np.abs(y - want) <= tolerance), np.max(np.abs(y - want) / tolerance)

@@ -153,6 +153,27 @@ def test_compaction_moves_what_lies_behind_to_the_front(seed):
     assert list(map(int, lines[0].split())) == [moved.get(i, i) for i in tables] and int(lines[1]) == len(far)
 
 
+# ------------------------------------------------------------------------------------------------ hidden entries of experts
+@pytest.mark.parametrize("unit", [4, 8])  # entries of a 16-byte piece: f32, bf16
+@pytest.mark.parametrize("laid", [0, 1])
+@pytest.mark.parametrize("hidden", [1, 3, 4, 5, 7, 8, 9, 12, 15, 16, 17, 33, 63, 64, 1025])
+def test_hidden_entries_and_zeros_share_a_pairs_room(hidden, unit, laid):
+    """Each place of a pair's room is written once, and nothing beside it: side by side the entries fill it, in pieces the last
+    piece holds the last `unit` ones, those of them that stand in a piece before it as zeros."""
+    if laid and hidden < unit:
+        return  # (no piece: such products go entry by entry)
+    run = checks("hidden", hidden, unit, laid)
+    assert run.returncode == 0, run.stderr
+    (room,), places, zeros = (list(map(int, line.split())) for line in run.stdout.splitlines())
+    whole = hidden // unit * unit
+    assert room == (-(-hidden // unit) * unit if laid else hidden)
+    want = list(range(hidden))
+    if laid and hidden > whole:
+        want = list(range(whole)) + [i - (hidden - unit) + whole for i in range(whole, hidden)]
+    assert places == want
+    assert sorted(places + [z for z in zeros if z >= 0]) == list(range(room))
+
+
 # ------------------------------------------------------------------------------------------------ refusals
 REFUSED = {
     "pool empty": "positive", "pool large": "2^31", "copy unequal": "target", "copy rows unequal": "rows", "copy source": "not one of",
