@@ -11,6 +11,11 @@
 // queries and keys) as three bf16 parts that hold all 24 bits; of a product of two such, the three smallest of nine part
 // products are left out, below 2^-24 of it.  Sums of decays are of 64 bits, since differences of long sums are taken.  (The
 // f32 instruction would take 2.7 times as long as six bf16 ones.)
+//
+// What is not finite stays behind its token: a matrix product would take it to the tokens before as well, by way of the zeros behind a
+// triangle.  So entries of the products' right factors that are not finite (R, W, and in the inverse A) go in as zeros, and the
+// tokens' outputs from the first of them on, and the state, become NaN.  (1 to 2 % of a prompt's time.)
+//
 // A bf16 prompt of 8191 tokens through 32 heads of 128 x 128 takes 67 us in the first launch and 290 in the second; 6 f32 ones of 6725
 // in all through 16 heads of 64 x 128 43 and 155.
 #include "kernels/parts.h"
@@ -41,6 +46,14 @@ template <int PARTS> __device__ __forceinline__ void eight_of(const dlk_row_segm
     }
 }
 
+__device__ __forceinline__ bool not_finite(float x) { return !(fabsf(x) <= 3.4028234664e38f); }
+// x, or, where it is not finite, zero; `first` goes down to `row` then.
+__device__ __forceinline__ float finite_of(float x, int row, int& first) {
+    const bool bad = not_finite(x);
+    first = bad ? min(first, row) : first;
+    return bad ? 0.0f : x;
+}
+
 // sum + a b, the smallest part products first
 template <int A, int B> __device__ __forceinline__ f32x4 multiply(const u32x4 (&a)[A], const u32x4 (&b)[B], f32x4 sum) {
     constexpr int LAST = (A > B ? A : B) - 1;
@@ -66,6 +79,7 @@ template <int DK, int PARTS> __global__ __launch_bounds__(kThreads, 3) void delt
     auto& system = room.system;
     auto& inverse = room.inverse;
     __shared__ double reach[kWaves][64];
+    __shared__ int first_bad[2]; // the first token whose row of A is not finite (of every other head)
     const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, n = lane % 16, g = lane / 16;
     const int key_heads = p.heads / p.group, key_head = blockIdx.x % key_heads;
     const int64_t index = blockIdx.x / key_heads;
@@ -123,6 +137,7 @@ template <int DK, int PARTS> __global__ __launch_bounds__(kThreads, 3) void delt
             qk[j] = multiply(q[s], column, qk[j]);
         }
     }
+    if (threadIdx.x == 0) first_bad[0] = 64;
     __syncthreads();
     for (int h = 0; h < p.group; ++h) {
         const int head = key_head * p.group + h;
@@ -145,6 +160,7 @@ template <int DK, int PARTS> __global__ __launch_bounds__(kThreads, 3) void delt
             to[64 + lane] = expf(static_cast<float>(reach[0][63] - sum));
             to[128 + lane] = rate;
         }
+        int bad = 64; // of the rows that this lane has entries of, the first that is not finite, from 16 wave + 4 g on
         float* within = p.within + own * kTiles * kTile;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -154,10 +170,11 @@ template <int DK, int PARTS> __global__ __launch_bounds__(kThreads, 3) void delt
             for (int r = 0; r < 4; ++r) {
                 const int i = 16 * wave + 4 * g + r, at = 16 * j + n;
                 const float fade = expf(static_cast<float>(reach[wave][i] - to)), factor = __shfl(rate, i) * fade;
-                system[i][at] = i > at ? factor * kk[j][r] : 0.0f;
+                system[i][at] = finite_of(i > at ? factor * kk[j][r] : 0.0f, r, bad);
                 within[tile_of(wave, j) * kTile + (4 * g + r) * 16 + n] = i >= at && at < chunk.count ? fade * qk[j][r] : 0.0f;
             }
         }
+        if (threadIdx.x == 0) first_bad[(h + 1) % 2] = 64;
         __syncthreads();
         // The inverse of each diagonal tile by substitution, a column a lane (four times over),
         float x[16];
@@ -193,12 +210,15 @@ template <int DK, int PARTS> __global__ __launch_bounds__(kThreads, 3) void delt
 #pragma unroll
                     for (int r = 0; r < 4; ++r) below = product(a[r], solved[t][r], below);
                 }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) below[r] = finite_of(below[r], 16 * step + r, bad);
                 const f32x4 a = *reinterpret_cast<const f32x4*>(&inverse[i][n][4 * g]);
                 solved[step] = 0.0f;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) solved[step] = product(a[r], -below[r], solved[step]);
             }
         }
+        if (bad < 64) atomicMin(&first_bad[h % 2], 16 * wave + 4 * g + bad);
         __syncthreads();
 #pragma unroll
         for (int step = 0; step < 4; ++step)
@@ -206,6 +226,7 @@ template <int DK, int PARTS> __global__ __launch_bounds__(kThreads, 3) void delt
 #pragma unroll
                 for (int r = 0; r < 4; ++r) system[16 * (wave + step) + 4 * g + r][16 * wave + n] = solved[step][r];
         __syncthreads();
+        if (wave == 0 && lane >= first_bad[h % 2]) p.gates[own * 192 + lane] = __builtin_nanf("");
         // in parts, 8 entries a thread
         uint16_t* solution = p.solution + own * 3 * kTiles * kTile;
         for (int i = threadIdx.x; i < kTiles * 32; i += kThreads) {
@@ -235,6 +256,7 @@ __global__ __launch_bounds__(2 * kThreads) __attribute__((amdgpu_waves_per_eu(2,
     constexpr int STEPS = DK / 32, OWN = DK > 64 ? DK / 64 : 1, LINE_S = DK + 8, LINE = 64 + 8;
     __shared__ uint16_t state_parts[3][16][LINE_S], right[3][16][LINE], write[3][16][LINE], late[3][16][LINE];
     __shared__ float gates[2][192];
+    __shared__ int first_bad[16]; // of a column, the first token whose write is not finite (since then of every chunk: the state is not)
     const int lane = threadIdx.x % kWave, n = lane % 16, g = lane / 16;
     const int role = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), wave = role % kWaves;
     // (work-groups go to the 8 dies in turn; the slices of a head read the same chunks, from the cache of one of them)
@@ -351,6 +373,7 @@ __global__ __launch_bounds__(2 * kThreads) __attribute__((amdgpu_waves_per_eu(2,
         load_rows(p.q, p.query_parts, 0, q);
         load_within(0);
         keep_gates(0);
+        if (role == kWaves && lane < 16) first_bad[lane] = 64;
         load_gates(min(1, chunks - 1));
         __syncthreads();
         for (int c = 0; c < chunks; ++c) {
@@ -374,7 +397,10 @@ __global__ __launch_bounds__(2 * kThreads) __attribute__((amdgpu_waves_per_eu(2,
             __builtin_amdgcn_sched_barrier(0);
             load_within(next);
             __syncthreads();
+            const int bad = first_bad[n];
             out = triangle(rows, write, out) * p.scale;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) out[i] = 16 * wave + 4 * g + i < bad ? out[i] : __builtin_nanf("");
             // Rows behind the chunk's end lie behind the buffer's.  (Of stores under a condition the compiler could not tell how
             // many came before a load, and would wait for them all.)
             float* to = p.out + ((item.token + 64 * static_cast<int64_t>(c)) * p.heads + head) * p.value_dim + first_column;
@@ -415,6 +441,17 @@ __global__ __launch_bounds__(2 * kThreads) __attribute__((amdgpu_waves_per_eu(2,
         if (holds)
 #pragma unroll
             for (int t = 0; t < OWN; ++t) part4(state[t], &state_parts[0][n][row_of(t, 0)], LINE_S);
+    };
+    // entries of four neighbouring tokens' rows, zero where they are not finite
+    const auto finite_rows = [&](f32x4 v) {
+        if (not_finite(v[0]) || not_finite(v[1]) || not_finite(v[2]) || not_finite(v[3]))
+#pragma unroll
+            for (int i = 3; i >= 0; --i)
+                if (not_finite(v[i])) {
+                    atomicMin(&first_bad[n], 16 * wave + 4 * g + i);
+                    v[i] = 0.0f;
+                }
+        return v;
     };
     u32x4 k[STEPS][PARTS], keys[OWN][2][PARTS], solution[2][3];
     uint32_t v[4]; // as they lie in memory
@@ -466,9 +503,9 @@ __global__ __launch_bounds__(2 * kThreads) __attribute__((amdgpu_waves_per_eu(2,
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             r[i] = 16 * wave + 4 * g + i < tokens ? rate[i] * (__uint_as_float(V_BF16 ? v[i] << 16 : v[i]) - since[i] * ks[i]) : 0.0f;
-        part4(r, &right[0][n][16 * wave + 4 * g], LINE);
+        part4(finite_rows(r), &right[0][n][16 * wave + 4 * g], LINE);
         __syncthreads();
-        const f32x4 w = triangle(solution, right, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+        const f32x4 w = finite_rows(triangle(solution, right, f32x4{0.0f, 0.0f, 0.0f, 0.0f}));
         __builtin_amdgcn_sched_barrier(0);
         load_solution(next);
         part4(w * left, &late[0][n][16 * wave + 4 * g], LINE);
@@ -482,6 +519,7 @@ __global__ __launch_bounds__(2 * kThreads) __attribute__((amdgpu_waves_per_eu(2,
             u32x4 b[2][3];
 #pragma unroll
             for (int s = 0; s < 2; ++s) column_parts(&late[0][n][32 * s + 8 * g], LINE, b[s]);
+            const bool bad = first_bad[n] < 64;
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int s = 0; s < 2; ++s)
@@ -491,6 +529,9 @@ __global__ __launch_bounds__(2 * kThreads) __attribute__((amdgpu_waves_per_eu(2,
                     for (int i = 0; i < PARTS && i <= order; ++i)
 #pragma unroll
                         for (int t = 0; t < OWN; ++t) state[t] = product(keys[t][s][i], b[s][order - i], state[t]);
+            if (bad)
+#pragma unroll
+                for (int t = 0; t < OWN; ++t) state[t] = __builtin_nanf("");
         }
         __builtin_amdgcn_sched_barrier(0);
         load_keys(next);

@@ -329,3 +329,73 @@ def test_states_beyond_4_gib():
         results.append(out + [run(0, 0, 1)])
     for small, large in zip(*results):
         assert np.array_equal(small, large)
+
+
+WHERE = [(9, 0), (9, 4), (9, 8), (150, 0), (150, 13), (150, 16), (150, 63), (150, 64), (150, 100), (150, 127), (150, 149)]  # (new tokens, which)
+
+
+def step_of(inputs, dtype, begin, counts, sources, key_heads):
+    tensors = [give(x, dtype if i < 3 else "f32")[0] for i, x in enumerate(inputs)]
+    h, dk, dv = begin.shape[1:]
+    states = ct.DeltaStates(1, len(begin), h, dk, dv)
+    put(states, 0, begin)
+    batch = ct.DeltaBatch(states, key_heads, sources, list(range(len(counts))), counts)
+    return ct.gated_delta(states, 0, batch, *tensors).numpy(), states.state(0).numpy()
+
+
+@pytest.mark.parametrize("dk,dv", [(64, 64), (32, 32), (128, 96)])
+@pytest.mark.parametrize("of", ["value", "key", "decay", "rate", "query", "state"])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_what_is_not_finite_reaches_what_follows_it_alone(of, bad, dtype, dk, dv):
+    """Of the same request, and of its column (a value), its heads (a key or a gate) or its row (a query); all else is the same
+    to the bit as without it.  A later decay of -inf does not take it back."""
+    if of == "decay" and bad < 0:
+        return  # (forgets: a number like others)
+    hk, h = 2, 4
+    rng = np.random.default_rng(21)
+    for count, t in WHERE:
+        say(f"case: delta {of} {bad} at {t} of {count} {dk}x{dv} {dtype}")
+        counts = [70, count, 40]  # (the second request is looked at; the first and the last must not know)
+        first, end = 70 + t, 70 + count
+        inputs = draw(rng, sum(counts), hk, h, dk, dv)
+        begin = rng.standard_normal((3, h, dk, dv)).astype(np.float32)
+        if t + 1 < count:
+            inputs[3][first + 1] = -np.inf
+        whole, state = step_of(inputs, dtype, begin, counts, [0, 1, 2], hk)
+        assert np.isfinite(whole).all() and np.isfinite(state).all()
+        reached, left = np.zeros(whole.shape, bool), np.zeros(state.shape, bool)
+        if of == "value":
+            inputs[2][first, 1, 7] = bad
+            reached[first:end, 1, 7], left[1, 1, :, 7] = True, True
+        elif of in ("key", "query"):
+            inputs[1 if of == "key" else 0][first, 1, 21] = bad
+            if of == "key":
+                reached[first:end, 2:], left[1, 2:] = True, True
+            else:
+                reached[first, 2:] = True
+        elif of in ("decay", "rate"):
+            inputs[3 if of == "decay" else 4][first, 1] = bad
+            reached[first:end, 1], left[1, 1] = True, True
+        else:
+            begin[1, 1, 5, 7] = bad
+            reached[70:end, 1, 7], left[1, 1, :, 7] = True, True
+        got, after = step_of(inputs, dtype, begin, counts, [0, 1, 2], hk)
+        assert not np.isfinite(got[reached]).any() and np.array_equal(got[~reached], whole[~reached])
+        assert not np.isfinite(after[left]).any() and np.array_equal(after[~left], state[~left])
+
+
+@pytest.mark.parametrize("count,t,other", [(9, 3, 7), (150, 0, 1), (150, 17, 18), (150, 50, 63), (150, 70, 140)])
+def test_what_f32_does_not_hold_reaches_what_follows_it_alone(count, t, other):
+    """Two long keys that are alike: their product is 1e50.  (The first one's own write is so too, but for a state of zero.)"""
+    rng = np.random.default_rng(22)
+    hk, h, dk, dv = 1, 2, 64, 32
+    inputs = draw(rng, count, hk, h, dk, dv)
+    inputs[3][:] = -1e-3
+    begin = np.zeros((1, h, dk, dv), np.float32)
+    whole, _ = step_of(inputs, "f32", begin, [count], [-1], hk)
+    inputs[1][t] *= 1e25
+    inputs[1][other] = inputs[1][t]
+    got, after = step_of(inputs, "f32", begin, [count], [-1], hk)
+    assert np.array_equal(got[:t], whole[:t]) and (t > 0 or np.isfinite(got[0]).all())
+    assert not np.isfinite(got[other:]).any() and not np.isfinite(after).any()
