@@ -4,6 +4,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <limits>
 #include <stdexcept>
 
 namespace dl::nn {
@@ -171,7 +172,8 @@ Tensor gated_delta(const nn::DeltaStates& states, Index layer, const nn::DeltaBa
         plan.slots != states.slots() || !(plan.device == states.device()))
         throw std::invalid_argument(std::string(name) + ": the batch was made for states of another layout");
     if (layer < 0 || layer >= states.layers()) throw std::out_of_range(std::string(name) + ": layer out of range");
-    if (scale && !std::isfinite(*scale)) throw std::invalid_argument(std::string(name) + ": the scale must be finite");
+    if (scale && !(std::abs(*scale) <= std::numeric_limits<float>::max()))
+        throw std::invalid_argument(std::string(name) + ": the scale must be finite in f32");
     const Tensor& state = states.state(layer);
     Tensor q, k, v;
     dlk_delta_params p{};

@@ -229,6 +229,7 @@ int call(const std::string& name) {
         {"delta decay", [&] { delta(q, q, v, tensor({3, 2}), g); }},
         {"delta rate type", [&] { delta(q, q, v, g, tensor({3, 4}, DType::i64)); }},
         {"delta host decay", [&] { delta(q, q, v, host({3, 4}), g); }},
+        {"delta scale beyond f32", [&] { delta(q, q, v, g, g, 0, -1e39); }},
         {"delta scale", [&] { delta(q, q, v, g, g, 0, std::numeric_limits<double>::infinity()); }},
         {"delta undefined", [&] { delta(Tensor{}, q, v, g, g); }},
         {"delta undefined rate", [&] { delta(q, q, v, g, Tensor{}); }},

@@ -192,7 +192,7 @@ REFUSED = {
     "delta other states": "another layout", "delta fewer slots": "another layout", "delta layer": "layer out of range",
     "delta layer below": "layer out of range", "delta query": "query must be", "delta key heads": "key must be",
     "delta value": "value must be", "delta type": "f32 or bf16", "delta host": "another device", "delta decay": "decay must be",
-    "delta rate type": "f32 or bf16", "delta host decay": "another device", "delta scale": "finite", "delta undefined": "undefined tensor",
+    "delta rate type": "f32 or bf16", "delta host decay": "another device", "delta scale": "finite", "delta scale beyond f32": "finite in f32", "delta undefined": "undefined tensor",
     "delta undefined rate": "undefined tensor", "states copy twice": "written twice", "states copy beyond": "not one of",
     "experts router": "router [E, d]", "experts router rank": "router [E, d]", "experts gate": "gate and up", "experts up": "gate and up",
     "experts down": "down [E, d, F]", "experts top": "top must be", "experts no top": "top must be", "experts top beyond": "top must be",
