@@ -58,10 +58,12 @@ namespace dl {
 ///   S = e^decay S;   S = S + k (rate (v - S^T k))^T;   out = scale S^T q
 /// query and key [tokens, key_heads, key_dim] and value [tokens, heads, value_dim] are f32 or bf16 and may be views of one
 /// projection output; decay and rate [tokens, heads], f32 or bf16.  A decay of -inf forgets everything before the token.  The
-/// default scale is 1 / sqrt(key_dim), and one beyond f32 is refused.  f32 [tokens, heads, value_dim].  The arithmetic is of f32: keys of length 1 and rates up
-/// to 2 keep a state bounded; longer ones let it grow as the rule does.  A number that is not finite makes its token's output and what
-/// follows it in its request not finite: of its column from a value or a state, of its heads from a key or a gate, and from a query its own
-/// row of its heads alone.  A later decay of -inf does not take that back, and nothing before the token knows of it.
+/// default scale is 1 / sqrt(key_dim), and one beyond f32 is refused.  f32 [tokens, heads, value_dim].  The arithmetic is of
+/// f32: keys of length 1, rates up to 2 and decays up to 0 keep a state bounded; others let it grow as the rule does (decays of 64
+/// tokens in a row that add up to more than 88 may overflow although the state would not).  A number that is not finite makes its
+/// token's output and what follows it in its request not finite: of its column from a value or a state, of its heads from a key
+/// or a gate, and from a query its own row of its heads alone.  A later decay of -inf does not take that back, and nothing before
+/// the token knows of it.
 DL_API Tensor gated_delta(const nn::DeltaStates& states, Index layer, const nn::DeltaBatch& batch, const Tensor& query,
                           const Tensor& key, const Tensor& value, const Tensor& decay, const Tensor& rate,
                           std::optional<double> scale = std::nullopt);

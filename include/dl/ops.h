@@ -74,7 +74,7 @@ DL_API std::pair<Tensor, Tensor> verify_drafted(const Tensor& drafted, const Ten
 ///   y = sum_j w_j down[e_j] (silu(gate[e_j] x) * (up[e_j] x)),   gate and up [E, F, d], down [E, d, F].
 /// All matrices are f32 or bf16, the experts' of one type.  z and p are taken in 64 bits, so that rows choose as the exact
 /// numbers do; the experts' products keep all bits of an f32.  An output that a number which is not finite takes part in is not finite
-/// either, and no other row's.  E is at most 1024, `top` at most 64, and E times the larger of d and F at most 2^25.
+/// either, and no other row's (a logit of -inf takes part with p = 0, unless all of a row's are).  E is at most 1024, `top` at most 64, and E times the larger of d and F at most 2^25.
 struct Mixture {
     Tensor output;  ///< f32 [..., d]
     Tensor chosen;  ///< i64 [..., top], the largest z first

@@ -165,6 +165,14 @@ def test_decays_whose_sums_are_long():
     check([64 * 3], [0], [0], 1, 1, 32, 32, change=lambda x: x[3].__setitem__(slice(0, 190), np.linspace(-60, -1e-3, 190)[:, None]))
 
 
+@pytest.mark.parametrize("count", [9, 100])
+def test_decays_above_zero(count):
+    """(The tolerance grows with the state.)"""
+    for change in (lambda x: x[3].fill(0.5), lambda x: x[3].__setitem__(slice(None), 1.0 * (np.arange(count) < 60)[:, None]),
+                   lambda x: x[3].__setitem__(slice(None), np.where(np.arange(count) % 2, 20.0, -20.0)[:, None])):
+        check([count], [0], [0], 1, 2, 64, 64, change=change)
+
+
 @pytest.mark.parametrize("scale", [1.0, 0.0, -3.5])
 def test_a_scale_of_ones_own(scale):
     check([7, 70], [0, -1], [0, 1], 1, 2, 64, 32, scale=scale)

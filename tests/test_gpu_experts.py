@@ -302,3 +302,65 @@ def test_matrices_beyond_2_gib(weight, F, T):
     assert not chosen.any() and np.all(weights == 1.0)
     want, tolerance = mixed(rows, *values, chosen, weights.astype(np.float64))
     assert np.all(np.abs(y - want) <= tolerance), np.max(np.abs(y - want) / tolerance)
+
+
+@pytest.mark.parametrize("T,d,F,E,top", [(1, 64, 32, 8, 2), (3, 65, 33, 8, 2), (12, 1, 40, 6, 2), (40, 63, 24, 8, 2), (100, 128, 72, 8, 2), (100, 65, 33, 8, 2),
+                                         (64, 65, 65, 4, 2), (8, 40, 1064, 64, 4), (16, 39, 1031, 64, 4), (60, 65, 1104, 64, 1)])
+@pytest.mark.parametrize("weight", ["f32", "bf16"])
+@pytest.mark.parametrize("inputs", ["f32", "bf16"])
+def test_numbers_that_are_not_finite_reach_what_they_take_part_in(T, d, F, E, top, weight, inputs):
+    """In a row's and a matrix's first and last entries (which odd widths read twice).  All else is the same to the bit; but where a row
+    goes to other experts the sums of the rows that it leaves or joins may begin elsewhere (by the first row of an expert), and
+    are held to the tolerance."""
+    rng = np.random.default_rng(T + d)
+    arrays = [rng.standard_normal((T, d))] + [rng.standard_normal(s) * s[-1] ** -0.5 for s in ((E, d), (E, F, d), (E, F, d), (E, d, F))]
+    kinds = [inputs] + [weight] * 4
+    clean, values = zip(*[give(a, kind) for a, kind in zip(arrays, kinds)])
+    want = [t.numpy() for t in ct.expert_mixture(*clean, top)]
+    assert all(np.isfinite(a).all() for a in want)
+    chosen = want[1]
+    exact, tolerance = mixed(values[0], *values[2:], *route(values[0], values[1], top, True))
+    counts = np.bincount(chosen.ravel(), minlength=E)
+    busy, idle = int(np.argmax(counts)), int(np.argmin(counts))
+    users = np.any(chosen == busy, -1)
+
+    def with_bad(which, index, value):
+        say(f"case: experts T={T} d={d} F={F} E={E} top={top} {weight} {inputs}: {value} at {index} of {which}")
+        changed = arrays[which].copy()
+        changed[index] = value
+        tensors = [give(changed, kinds[which])[0] if i == which else t for i, t in enumerate(clean)]
+        return [t.numpy() for t in ct.expert_mixture(*tensors, top)]
+
+    for value in (np.nan, np.inf, -np.inf):
+        for last in (0, -1):
+            for which in (2, 3):  # a hidden entry, and by it all outputs of the rows that chose the expert
+                y, now, weights = with_bad(which, (busy, last, last), value)
+                assert not np.isfinite(y[users]).any() and np.array_equal(y[~users], want[0][~users])
+                assert np.array_equal(now, chosen) and np.array_equal(weights, want[2])
+            y, now, _ = with_bad(4, (busy, last, last), value)
+            reached = np.zeros(y.shape, bool)
+            reached[users, last] = True
+            assert not np.isfinite(y[reached]).any() and np.array_equal(y[~reached], want[0][~reached]) and np.array_equal(now, chosen)
+            y, now, weights = with_bad(0, (T // 2, last), value)
+            others = np.arange(T) != T // 2
+            assert not np.isfinite(y[T // 2]).any() and len(set(now[T // 2])) == top and np.all((now >= 0) & (now < E))
+            assert np.array_equal(now[others], chosen[others]) and np.array_equal(weights[others], want[2][others])
+            assert np.all(np.abs(y - exact)[others] <= tolerance[others])
+        if counts[idle] == 0:  # an expert that no row chose
+            for which in (2, 3, 4):
+                assert all(np.array_equal(a, b) for a, b in zip(with_bad(which, (idle, -1, -1), value), want))
+    y, now, weights = with_bad(1, (busy, -1), np.nan)  # the router's
+    assert np.all(now[:, 0] == busy) and not np.isfinite(y).any() and np.isnan(weights).all()
+
+
+def test_a_logit_of_minus_infinity_takes_part_with_nothing():
+    for T in (1, 40):
+        rng = np.random.default_rng(T)
+        arrays = [np.abs(rng.standard_normal((T, 64)))] + [rng.standard_normal(s) * 0.2 for s in ((8, 64), (8, 32, 64), (8, 32, 64), (8, 64, 32))]
+        arrays[1][5] = -1e3  # never chosen, and e^-1000 and less is nothing beside 1
+        tensors = [give(a)[0] for a in arrays]
+        arrays[1][5, 3] = -np.inf
+        for normalise in (True, False):
+            want = ct.expert_mixture(*tensors, 3, normalise)
+            got = ct.expert_mixture(tensors[0], give(arrays[1])[0], *tensors[2:], 3, normalise)
+            assert all(np.array_equal(a.numpy(), b.numpy()) for a, b in zip(got, want))
