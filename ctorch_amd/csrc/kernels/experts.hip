@@ -256,16 +256,17 @@ __device__ __forceinline__ void keep(const dlk_experts_params& p, const Plan& pl
     }
 }
 
-// One chosen expert's products with the rows that chose it, which are the columns here, 16 NT at a time.  16 R rows of its
-// matrices (GATE: of gate and up, and silu(gate) * up of both; else of down) are a wave's own, or, SPLIT, a work-group's whose
-// waves share the sum's index and join their sums in LDS.  A ring of D steps of 64 bytes a row is on its way from memory.
+// One chosen expert's products with the rows that chose it, which are the columns here, 16 at a time.  16 R rows of its
+// matrices (GATE: of gate and up, and silu(gate) * up of both; else of down) are a wave's own, or, SPLIT, 16 a work-group's whose
+// waves share the sum's index and join their sums in LDS.  A ring of D steps of 128 bytes a row is on its way from memory.
 // A work-group stands for expert blockIdx.y, or, where there are fewer pairs than experts, for the expert of pair blockIdx.y
 // if that is its first.
-template <bool GATE, bool F32, int PARTS, int R, int NT, bool SPLIT, bool LOOSE>
+template <bool GATE, bool F32, int PARTS, int R, bool SPLIT, bool LOOSE>
 __global__ __launch_bounds__(SPLIT ? 512 : 256) void experts_rows(const dlk_experts_params p, const Plan plan) {
     constexpr int WAVES = SPLIT ? 8 : 4, THREADS = WAVES * kWave, TILES = GATE ? 2 * R : R;
-    constexpr int ROOM = 15 / (TILES + NT * PARTS), D = SPLIT || ROOM < 2 ? 2 : ROOM > 4 ? 4 : ROOM;
+    constexpr int ROOM = 15 / (TILES + PARTS), D = SPLIT || ROOM < 2 ? 2 : ROOM > 4 ? 4 : ROOM;
     constexpr int SIZE = F32 ? 4 : 2, PAD = 20;
+    static_assert(!SPLIT || R == 1);
     extern __shared__ uint16_t list[];
     __shared__ int counts[WAVES];
     __shared__ float sums[SPLIT ? WAVES : 1][TILES][16][PAD];
@@ -298,7 +299,7 @@ __global__ __launch_bounds__(SPLIT ? 512 : 256) void experts_rows(const dlk_expe
     const int begin = SPLIT ? wave * per : 0, end = min(steps, begin + per);
     const int turn = static_cast<int>((blockIdx.x * WAVES + wave + blockIdx.y * 5u) * 7u % static_cast<uint32_t>(steps));
     struct Held {
-        u32x4 w[TILES][2], x[NT][2][PARTS];
+        u32x4 w[TILES][2], x[2][PARTS];
     };
     // (what lies behind a row's end or the wave's run is read as zero, from beyond the buffer)
     const auto of_step = [&](int step) {
@@ -327,50 +328,35 @@ __global__ __launch_bounds__(SPLIT ? 512 : 256) void experts_rows(const dlk_expe
     for (int d = 0; d < D; ++d) load_weights(begin + d, ring[d]);
     const int count = collect<WAVES>(plan.pick, pairs, e, list, counts);
     if (few && list[0] != blockIdx.y) return;
-    for (int first = 0; first < count; first += 16 * NT) {
-        const int tiles = min(NT, (count - first + 15) / 16); // that hold rows
-        uint32_t x_at[NT];
+    for (int first = 0; first < count; first += 16) {
+        const int own = first + n;
+        const uint32_t x_at = own < count ? static_cast<uint32_t>(GATE ? list[own] / p.top : list[own]) * row_bytes : kBeyond;
+        f32x4 sum[TILES];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const int i = first + 16 * t + n;
-            x_at[t] = i < count ? static_cast<uint32_t>(GATE ? list[i] / p.top : list[i]) * row_bytes : kBeyond;
-        }
-        f32x4 sum[NT][TILES];
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int i = 0; i < TILES; ++i) sum[t][i] = 0.0f;
+        for (int i = 0; i < TILES; ++i) sum[i] = 0.0f;
         const auto load_rows = [&](int step, Held& to) {
             const uint32_t k = of_step(step) + g * 32;
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
-                if (t < tiles)
+            for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
-#pragma unroll
-                        for (int part = 0; part < PARTS; ++part) // (x_at may lie behind the end by itself)
-                            to.x[t][i][part] = __builtin_amdgcn_raw_buffer_load_b128(
-                                x, k + 16 * i < row_bytes ? x_at[t] + part * plane + k + 16 * i : kBeyond, 0, 0);
+                for (int part = 0; part < PARTS; ++part) // (x_at may lie behind the end by itself)
+                    to.x[i][part] = __builtin_amdgcn_raw_buffer_load_b128(x, k + 16 * i < row_bytes ? x_at + part * plane + k + 16 * i : kBeyond, 0, 0);
         };
         const auto multiply = [&](Held& of) {
 #pragma unroll
             for (int i = 0; i < TILES; ++i) exchange(of.w[i]);
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
-                if (t < tiles)
+            for (int i = 0; i < TILES; ++i)
 #pragma unroll
-                    for (int i = 0; i < TILES; ++i)
+                for (int h = 0; h < 2; ++h) {
+                    if constexpr (F32) {
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            if constexpr (F32) {
+                        for (int j = 0; j < 4; ++j) sum[i] = product(__uint_as_float(of.w[i][h][j]), __uint_as_float(of.x[h][0][j]), sum[i]);
+                    } else {
 #pragma unroll
-                                for (int j = 0; j < 4; ++j)
-                                    sum[t][i] = product(__uint_as_float(of.w[i][h][j]), __uint_as_float(of.x[t][h][0][j]), sum[t][i]);
-                            } else {
-#pragma unroll
-                                for (int part = PARTS - 1; part >= 0; --part) sum[t][i] = product(of.w[i][h], of.x[t][h][part], sum[t][i]);
-                            }
-                        }
+                        for (int part = PARTS - 1; part >= 0; --part) sum[i] = product(of.w[i][h], of.x[h][part], sum[i]);
+                    }
+                }
         };
 #pragma unroll
         for (int d = 0; d < D; ++d) {
@@ -384,36 +370,30 @@ __global__ __launch_bounds__(SPLIT ? 512 : 256) void experts_rows(const dlk_expe
                 load_weights(step + D + d, ring[d]);
                 load_rows(step + D + d, ring[d]);
             }
+        if constexpr (SPLIT) {
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            if (t >= tiles) break;
-            if constexpr (SPLIT) {
+            for (int i = 0; i < TILES; ++i) *reinterpret_cast<f32x4*>(&sums[wave][i][n][4 * g]) = sum[i];
+            __syncthreads();
+            for (int i = threadIdx.x; i < 256; i += THREADS) {
+                const int r = i % 16, column = i / 16, row = first_row + r, at = first + column;
+                if (row >= height || at >= count) continue;
+                float v = 0.0f, up = 0.0f;
 #pragma unroll
-                for (int i = 0; i < TILES; ++i) *reinterpret_cast<f32x4*>(&sums[wave][i][n][4 * g]) = sum[t][i];
-                __syncthreads();
-                for (int i = threadIdx.x; i < 256 * R; i += THREADS) {
-                    const int r = i % 16, tile = i / 16 % R, column = i / (16 * R), row = first_row + 16 * tile + r;
-                    const int at = first + 16 * t + column;
-                    if (row >= height || at >= count) continue;
-                    float v = 0.0f, up = 0.0f;
-#pragma unroll
-                    for (int w = 0; w < WAVES; ++w) {
-                        v += sums[w][tile][column][r];
-                        if constexpr (GATE) up += sums[w][R + tile][column][r];
-                    }
-                    keep<GATE>(p, plan, list[at], row, v, up);
+                for (int w = 0; w < WAVES; ++w) {
+                    v += sums[w][0][column][r];
+                    if constexpr (GATE) up += sums[w][1][column][r];
                 }
-                __syncthreads();
-            } else {
-                const int at = first + 16 * t + n;
-#pragma unroll
-                for (int r = 0; r < R; ++r)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int row = first_row + 16 * r + 4 * g + j;
-                        if (row < height && at < count) keep<GATE>(p, plan, list[at], row, sum[t][r][j], GATE ? sum[t][TILES - R + r][j] : 0.0f);
-                    }
+                keep<GATE>(p, plan, list[at], row, v, up);
             }
+            __syncthreads();
+        } else {
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int row = first_row + 16 * r + 4 * g + j;
+                    if (row < height && own < count) keep<GATE>(p, plan, list[own], row, sum[r][j], GATE ? sum[TILES - R + r][j] : 0.0f);
+                }
         }
     }
 }
@@ -807,11 +787,11 @@ Layout layout(const dlk_experts_params& p) {
 template <bool GATE, bool F32, int PARTS, bool LOOSE> void rows_of(const dlk_experts_params& p, const Plan& plan, hipStream_t at) {
     const int pairs = static_cast<int>(p.tokens) * p.top, height = GATE ? p.hidden : p.dim;
     const int active = std::min(pairs, p.experts), tiles = (height + 15) / 16;
-    const auto launch = [&](auto r, auto nt, auto split) {
-        constexpr int R = decltype(r)::value, NT = decltype(nt)::value;
+    const auto launch = [&](auto r, auto split) {
+        constexpr int R = decltype(r)::value;
         constexpr bool SPLIT = decltype(split)::value;
         const int per = R * (SPLIT ? 1 : 4);
-        experts_rows<GATE, F32, PARTS, R, NT, SPLIT, LOOSE><<<dim3((tiles + per - 1) / per, active), SPLIT ? 512 : 256, pairs * 2, at>>>(p, plan);
+        experts_rows<GATE, F32, PARTS, R, SPLIT, LOOSE><<<dim3((tiles + per - 1) / per, active), SPLIT ? 512 : 256, pairs * 2, at>>>(p, plan);
     };
     using std::integral_constant;
     const integral_constant<int, 1> one;
@@ -836,12 +816,12 @@ template <bool GATE, bool F32, int PARTS, bool LOOSE> void rows_of(const dlk_exp
     // where each is made once (16 rows through 4 of 32 experts of 704 x 2047: 129 us a call more with four tiles a wave than through LDS), and
     // f32 rows are twice as long (8 rows through 8 of 64 experts of 1024 x 2048: 255 and 237).
     const int64_t all = static_cast<int64_t>(active) * tiles;
-    if (all < (pairs >= 8 * p.experts ? 512 : 1024)) launch(one, one, split);
+    if (all < (pairs >= 8 * p.experts ? 512 : 1024)) launch(one, split);
     else if (pairs < p.experts || (!LOOSE && !F32 && p.tokens <= 16 && all >= 4096)) {
-        if constexpr (F32) launch(one, one, whole);
-        else if (all < 2048) launch(one, one, whole);
-        else if (all < 4096) launch(two, one, whole);
-        else launch(four, one, whole);
+        if constexpr (F32) launch(one, whole);
+        else if (all < 2048) launch(one, whole);
+        else if (all < 4096) launch(two, whole);
+        else launch(four, whole);
     } else {
         // 6, 8 or 16 tiles a work-group, by what the CU with most of them has (48 tiles of each of 32 experts: 102 us a call with 6, 109 and
         // 142 with the others; 32 of each of 64: 63, 51 and 64; 64 of each of 64: 174, 157 and 148)
