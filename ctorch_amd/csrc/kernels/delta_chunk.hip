@@ -16,8 +16,8 @@
 // triangle.  So entries of the products' right factors that are not finite (R, W, and in the inverse A) go in as zeros, and the
 // tokens' outputs from the first of them on, and the state, become NaN.  (1 to 2 % of a prompt's time.)
 //
-// A bf16 prompt of 8191 tokens through 32 heads of 128 x 128 takes 67 us in the first launch and 290 in the second; 6 f32 ones of 6725
-// in all through 16 heads of 64 x 128 43 and 155.
+// A bf16 prompt of 8191 tokens through 32 heads of 128 x 128 takes 70 us in the first launch and 304 in the second; 6 f32 ones of 6725
+// in all through 16 heads of 64 x 128 45 and 158.
 #include "kernels/parts.h"
 
 #include <algorithm>
@@ -245,7 +245,7 @@ template <int DK, int PARTS> __global__ __launch_bounds__(kThreads, 3) void delt
 
 // ------------------------------------------------------------------------------------------------ chunk after chunk
 // A work-group per request, head and 16 columns of the state.  What counts is how long a chunk takes, not how much there is to
-// do: a prompt's chunks follow one another, and a chunk's three products wait for each other at three barriers, 2.3 us of 128 x 128 (the
+// do: a prompt's chunks follow one another, and a chunk's three products wait for each other at three barriers, 2.4 us of 128 x 128 (the
 // products alone, at the matrix cores' rate, 0.7).  So the waves share it by what waits for what: waves 0 to 3 hold the state (DK / 4
 // rows each; of 32: waves 0 and 1, 16 each) and take it to the next chunk by way of R and W, 16 tokens each, and waves 4 to 7 make
 // the outputs of 16 tokens each beside them.  What the next chunk's products read is asked for as soon as this one's have used theirs

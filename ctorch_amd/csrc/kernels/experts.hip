@@ -1,7 +1,7 @@
 // A layer of experts over few rows (see dlk_experts_params in kernels.h): the router in f64, the hidden entries of the chosen
 // experts, their output entries, and the weighted sum.  Bound by memory: a few rows read each chosen expert's matrices once.  16 rows
-// through 8 of 64 bf16 experts of 1024 x 2048: router 11 us, hidden entries 87 (5.6 TB/s), outputs 48 (5.0 TB/s), sum 4.7; 200 rows
-// through 4 of 32 of 768 x 2048: 8, 46, 31 and 4.7; one row through 2 of 16 of 704 x 1024: 4.5, 4.2, and 3.7 for outputs and sum.
+// through 8 of 64 bf16 experts of 1024 x 2048: router 12 us, hidden entries 90 (5.3 TB/s), outputs 50 (4.8 TB/s), sum 4.8; 200 rows
+// through 4 of 32 of 768 x 2048: 8, 47, 32 and 4.8; one row through 2 of 16 of 704 x 1024: 4.4, 4.3, and 3.8 for outputs and sum.
 //
 // Products keep all bits of an f32: bf16 matrices go into v_mfma_f32_16x16x32_bf16 as they are, rows as three bf16 parts that
 // hold all 24 bits (bf16 rows are one); f32 matrices and rows go into v_mfma_f32_16x16x4_f32.
@@ -823,8 +823,9 @@ template <bool GATE, bool F32, int PARTS, bool LOOSE> void rows_of(const dlk_exp
         else if (all < 4096) launch(two, whole);
         else launch(four, whole);
     } else {
-        // 6, 8 or 16 tiles a work-group, by what the CU with most of them has (48 tiles of each of 32 experts: 102 us a call with 6, 109 and
-        // 142 with the others; 32 of each of 64: 63, 51 and 64; 64 of each of 64: 174, 157 and 148)
+        // 6, 8 or 16 tiles a work-group, by what the CU with most of them has (us a call by what the gates' product
+        // takes: 200 rows through 4 of 32 experts of 768 x 2048, 48 tiles of each, 87 with 6, 90 and 122 with the others; 40 rows through 4 of 64 of
+        // 512 x 1024, 32 of each, 66, 53 and 66; 40 rows through 8 of 64 of 1024 x 2048, 64 of each, 181, 168 and 169)
         const auto most = [&](int rows) { return (static_cast<int64_t>(p.experts) * ((tiles + rows - 1) / rows) + 255) / 256 * rows; };
         if (most(6) < most(16) && most(6) < most(8)) blocks(one, four, six);
         else if (most(8) < most(16)) blocks(one, four, eight);

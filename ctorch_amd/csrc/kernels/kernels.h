@@ -340,7 +340,7 @@ typedef struct dlk_page_pair {
 } dlk_page_pair;
 #define DLK_PAGE_PAIRS 240
 #define DLK_PAGE_POOLS 64
-typedef struct dlk_page_copy_params { /* (an argument block of a launch: below 4 KB) */
+typedef struct dlk_page_copy_params { /* (an argument block of a launch: 3424 bytes, below 4 KB) */
     int pool_count, count;
     int heads, page, row_units; /* a row is row_units * 16 bytes */
     int staged;

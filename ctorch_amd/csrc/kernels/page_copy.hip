@@ -12,6 +12,7 @@ namespace {
 
 constexpr int kThreads = 256, kSteps = 4; // 16 KB a work-group
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+static_assert(sizeof(dlk_page_copy_params) <= 4096, "the arguments of a launch");
 
 // A work-group per piece of (pair, pool).  Of a head's `page` rows the pair's first `rows` are copied: unit i of the pair
 // lies in head i / (rows * units), at unit i % (rows * units) of the head's.

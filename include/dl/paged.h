@@ -110,13 +110,15 @@ DL_API void paged_copy(const nn::PagedKVCache& cache, std::span<const Index> sou
 /// Tables [parents, width] of new requests that go on from position lengths[p] of request p = parents[i] (a row of `tables`
 /// [sequences, width], all of its pages up to there held): the whole pages in front are shared, a partly filled last one is
 /// copied, as far as it is filled, to a page taken from the pool, and the rest of a row is -1.  With too few free pages
-/// the call is refused and the pool stays as it was.
+/// the call is refused and the pool stays as it was.  (Of this cache: in another whose pages the same tables name, paged_copy
+/// copies the last ones.)
 DL_API std::vector<Index> paged_fork(const nn::PagedKVCache& cache, nn::PagePool& pool, std::span<const Index> tables, Index width,
                                      std::span<const Index> lengths, std::span<const Index> parents);
 
 /// Moves the held pages to the front of the pool: those beyond the first n, n the number of held pages, go to the free ones
 /// among them, in ascending order; their ids in `tables` become the new ones.  The tables are all that holds pages: a page
-/// stands in them as often as the pool counts.  Returns how many pages were moved.
+/// stands in them as often as the pool counts.  Returns how many pages were moved.  (It moves this cache's pages: two caches whose
+/// pages share tables and a pool, a draft model's beside the target's, cannot be compacted, since one call renames them for both.)
 DL_API Index paged_compact(const nn::PagedKVCache& cache, nn::PagePool& pool, std::span<Index> tables);
 
 } // namespace dl
